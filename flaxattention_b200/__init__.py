@@ -4,7 +4,9 @@ Export list follows flaxattention/__init__.py:11-22 (without the matplotlib visu
 """
 from .attention import check_status, flax_attention, flax_attention_pallas, math_attention
 from .blockmask import BlockMask, and_masks, create_block_mask, noop_mask, or_masks
+from .paged import PageStep, page_step, paged_attention, rotary_append
 from .pipeline import HostPipeline
+from .rotary import rotary_embedding, rotary_table
 from . import fnp, masks, mods  # noqa: F401
 from typing import Callable
 
@@ -24,6 +26,12 @@ __all__ = [
     "_score_mod_signature",
     "check_status",
     "HostPipeline",
+    "rotary_table",
+    "rotary_embedding",
+    "rotary_append",
+    "PageStep",
+    "page_step",
+    "paged_attention",
     "fnp",
     "masks",
     "mods",

@@ -56,6 +56,35 @@ class FaAttnParams(C.Structure):
     ]
 
 
+class FaRotaryParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("weight_dtype", C.c_int32),
+        ("B", C.c_int32), ("S", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("Dv", C.c_int32),
+        ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float),
+        ("q", FaTensor), ("k", FaTensor), ("q_out", FaTensor), ("k_out", FaTensor),
+        ("table", C.c_void_p), ("table_length", C.c_int64), ("table_stride", C.c_int64),
+        ("positions", C.c_void_p), ("position_bits", C.c_int32),
+        ("position_stride_b", C.c_int64), ("position_stride_s", C.c_int64),
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p),
+        ("v", FaTensor), ("k_pages", FaTensor), ("v_pages", FaTensor),
+        ("num_pages", C.c_int64), ("page_size", C.c_int32),
+        ("slots", C.c_void_p), ("slot_stride_b", C.c_int64), ("slot_stride_s", C.c_int64),
+        ("status", C.c_void_p),
+    ]
+
+
+class FaPagedParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("B", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("Sq", C.c_int32), ("D", C.c_int32), ("Dv", C.c_int32),
+        ("scale", C.c_float), ("b_offset", C.c_int32), ("h_offset", C.c_int32),
+        ("q", FaTensor), ("o", FaTensor), ("k_pages", FaTensor), ("v_pages", FaTensor),
+        ("num_pages", C.c_int64), ("page_size", C.c_int32),
+        ("block_table", C.c_void_p), ("block_table_stride", C.c_int64), ("table_width", C.c_int32),
+        ("lengths", C.c_void_p), ("window", C.c_int32), ("lse", C.c_void_p), ("flags", C.c_int32), ("status", C.c_void_p),
+    ]
+
+
 class FlaxAttnError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"flaxattn error {code}: {msg}")
@@ -74,6 +103,8 @@ EXPORTS = [
     "fa_mask_bits_row_words", "fa_mask_bits", "fa_block_mask_build",
     "fa_snapshot_bytes", "fa_snapshot", "fa_snapshot_holds",
     "fa_fwd_workspace_bytes", "fa_fwd_ws",
+    "fa_rotary", "fa_rotary_bwd_workspace_bytes", "fa_rotary_bwd", "fa_rotary_append",
+    "fa_page_step", "fa_paged_workspace_bytes", "fa_paged", "fa_paged_prepare",
 ]
 
 
@@ -130,6 +161,18 @@ def lib() -> C.CDLL:
     L.fa_snapshot_bytes.argtypes = ranges[1:]
     L.fa_snapshot.argtypes = ranges + [C.c_void_p, C.c_void_p]
     L.fa_snapshot_holds.argtypes = ranges + [C.c_void_p, C.c_void_p, C.c_void_p]
+    L.fa_rotary.argtypes = [C.POINTER(FaRotaryParams), C.c_void_p]
+    L.fa_rotary_bwd_workspace_bytes.restype = C.c_size_t
+    L.fa_rotary_bwd_workspace_bytes.argtypes = [C.POINTER(FaRotaryParams)]
+    L.fa_rotary_bwd.argtypes = [C.POINTER(FaRotaryParams)] + [C.POINTER(FaTensor)] * 4 + [
+        C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+    L.fa_rotary_append.argtypes = [C.POINTER(FaRotaryParams), C.c_void_p]
+    L.fa_page_step.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
+                               C.c_int, C.c_int64] + [C.c_void_p] * 7
+    L.fa_paged_workspace_bytes.restype = C.c_size_t
+    L.fa_paged_workspace_bytes.argtypes = [C.POINTER(FaPagedParams)]
+    L.fa_paged.argtypes = [C.c_void_p, C.POINTER(FaPagedParams), C.c_void_p, C.c_size_t, C.c_void_p]
+    L.fa_paged_prepare.argtypes = [C.c_void_p, C.POINTER(FaPagedParams)]
     L.fa_mask_bits_row_words.restype = C.c_int64
     L.fa_mask_bits_row_words.argtypes = [C.c_int]
     L.fa_mask_bits.argtypes = [C.c_void_p] + [C.c_int] * 6 + [C.c_void_p, C.c_void_p]

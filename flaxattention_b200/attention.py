@@ -97,8 +97,9 @@ def check_status() -> None:
         bits = int(w[0])
         w[0] = 0
         raise _cabi.FlaxAttnError(-3, f"a kernel reported status bits {bits:#x} (bit 0: a bounded barrier wait ran out; "
-                                      "bit 1: a launch configuration the kernel refused); the results of that launch "
-                                      "are incomplete")
+                                      "bit 1: a launch configuration the kernel refused; bit 2: a block table entry that is "
+                                      "no page, or a length beyond the table; bit 3: a position beyond the rotary table; "
+                                      "bit 4: a slot beyond the pages); the results of that launch are incomplete")
 
 
 def _tensor(t: torch.Tensor, layout: str) -> _cabi.FaTensor:

@@ -40,7 +40,8 @@ def is_current() -> bool:
 
 
 def host_sources():
-    srcs = [os.path.join(HERE, "flaxattn.cu"), os.path.join(PKG, "..", "include", "flaxattn.h")]
+    srcs = [os.path.join(HERE, "flaxattn.cu"), os.path.join(HERE, "rotary.cuh"), os.path.join(HERE, "paging.cuh"),
+            os.path.join(PKG, "..", "include", "flaxattn.h")]
     kdir = os.path.join(HERE, "kernels")
     # the templates count too: the library's launch code mirrors their shared-memory maps
     srcs += [os.path.join(kdir, f) for f in sorted(os.listdir(kdir)) if f.endswith((".h", ".cuh"))]

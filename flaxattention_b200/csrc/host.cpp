@@ -21,6 +21,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -613,6 +614,512 @@ PyObject* build_block_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- rotary positions, pages ------------------------------------------------------------------
+// These calls have no Python layer behind them: what is wrong with their arguments is said here.
+const at::Tensor& cuda_tensor(PyObject* o, const char* name) {
+  TORCH_CHECK_TYPE(THPVariable_Check(o), name, ": a tensor is expected, got ", Py_TYPE(o)->tp_name);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  TORCH_CHECK(t.is_cuda() && t.layout() == at::kStrided && t.has_storage(),
+              name, ": flaxattention_b200 runs on CUDA tensors only; there is no CPU path");
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, ": there is no forward-mode derivative");
+  return t;
+}
+// nothing that would look on is on (see watched): a trace or a transform would not see what these calls do
+void check_unwatched() {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::tracer::impl::is_dispatch_enabled() &&
+                                  !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode),
+                              "not under a tracer or a functorch transform");
+}
+int dtype_code(const at::Tensor& t, const char* name) {
+  const auto dt = t.scalar_type();
+  TORCH_CHECK_VALUE(dt == at::kHalf || dt == at::kBFloat16 || dt == at::kFloat, "unsupported dtype ", dt, " of ", name, "; use float16, bfloat16 or float32");
+  return dt == at::kHalf ? FA_F16 : dt == at::kBFloat16 ? FA_BF16 : FA_F32;
+}
+void same_kind(const at::Tensor& t, const at::Tensor& as, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == as.scalar_type(), "Expected ", name, " to have the dtype of the others, but got ", t.scalar_type(), " and ", as.scalar_type());
+  TORCH_CHECK_VALUE(t.device() == as.device(), name, " is on ", t.device(), ", the others on ", as.device());
+}
+void int_kind(const at::Tensor& t, at::ScalarType dt, c10::Device dev, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == dt, name, " must be ", dt, ", got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.device() == dev, name, " is on ", t.device(), ", the others on ", dev);
+}
+void rows_of(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() == 4, "NYI: ", name, " must be a 4D tensor, got ", t.dim(), "D");
+  TORCH_CHECK_VALUE(t.size(3) == 1 || t.stride(3) == 1, name, ": the head dimension must be contiguous");
+  for (int64_t d = 0; d < 4; ++d) TORCH_CHECK_VALUE(t.size(d) <= INT32_MAX, name, ": too large");
+}
+// A tensor that a kernel writes to: every element has a place of its own (as far as strides of 0 tell)
+void writable(const at::Tensor& t, const char* name) {
+  for (int64_t d = 0; d < t.dim(); ++d) TORCH_CHECK_VALUE(t.size(d) <= 1 || t.stride(d) != 0, name, " is written to and must not be an expanded tensor");
+}
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void no_gradient(const at::Tensor& t, const char* name, const char* call) {
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), call, " has no gradient, but ", name, " requires one; call it under torch.no_grad()");
+}
+fa_tensor by_strides(const at::Tensor& t, bool bshd) {
+  fa_tensor r;
+  r.ptr = t.data_ptr();
+  r.stride_b = t.stride(0);
+  r.stride_h = t.stride(bshd ? 2 : 1);
+  r.stride_s = t.stride(bshd ? 1 : 2);
+  return r;
+}
+at::Tensor empty_rows(const at::Tensor& t) {
+  if (t.is_contiguous()) return empty(t.sizes(), t.scalar_type(), t.device());
+  at::Tensor r = at::empty_like(t);
+  return r.size(3) == 1 || r.stride(3) == 1 ? r : empty(t.sizes(), t.scalar_type(), t.device());
+}
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+int64_t integer(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
+  return v != 0;
+}
+
+// What rotary_embedding and rotary_append have in common
+struct Rotary {
+  fa_rotary_params p;
+  bool bshd = false;
+  at::Tensor table, positions, weights[2];
+
+  // rows: any of the tensors that are rotated; tokens from its shape
+  void read(const at::Tensor& rows, PyObject* table_o, PyObject* positions_o, PyObject* const* weights_o, PyObject* eps, PyObject* interleaved) {
+    p.dtype = dtype_code(rows, "the tensors");
+    p.B = (int)rows.size(0);
+    p.S = (int)rows.size(bshd ? 1 : 2);
+    p.D = (int)rows.size(3);
+    p.eps = (float)number(eps);
+    TORCH_CHECK_VALUE(p.eps >= 0.f, "eps must not be negative");
+    p.interleaved = truth(interleaved);
+    p.status = (int32_t*)g_status;
+    const c10::Device dev = rows.device();
+    if (table_o != Py_None) {
+      table = cuda_tensor(table_o, "table");
+      TORCH_CHECK_VALUE(table.dim() == 2 && table.scalar_type() == at::kFloat, "table must be a 2D float32 tensor (see rotary_table)");
+      TORCH_CHECK_VALUE(table.device() == dev, "table is on ", table.device(), ", the others on ", dev);
+      TORCH_CHECK_VALUE(table.size(1) % 2 == 0 && table.size(1) <= p.D, "table has ", table.size(1), " columns; an even number up to the head dim ", p.D, " is expected");
+      TORCH_CHECK_VALUE(table.size(1) <= 1 || table.stride(1) == 1, "the rows of table must be contiguous");
+      no_gradient(table, "table", "the table of rotary positions");
+      p.rotary_dim = (int)table.size(1);
+      p.table = p.rotary_dim > 0 ? (const float*)table.const_data_ptr() : nullptr;
+      p.table_length = table.size(0);
+      p.table_stride = std::max<int64_t>(table.stride(0), table.size(0) == 1 ? table.size(1) : 0);
+      TORCH_CHECK_VALUE(p.table_stride >= p.rotary_dim, "the rows of table must not overlap");
+      TORCH_CHECK_VALUE(p.rotary_dim == 0 || p.table_length > 0, "table has no rows");
+    }
+    if (positions_o != Py_None) {
+      positions = cuda_tensor(positions_o, "positions");
+      TORCH_CHECK_VALUE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, "positions must be int32 or int64, got ", positions.scalar_type());
+      TORCH_CHECK_VALUE(positions.device() == dev, "positions is on ", positions.device(), ", the others on ", dev);
+      const bool per_token = positions.dim() == 2 && positions.size(0) == p.B && positions.size(1) == p.S;
+      TORCH_CHECK_VALUE(per_token || (positions.dim() == 1 && positions.size(0) == p.S), "positions must be [B, S] or [S] = [", p.B, ", ", p.S, "], got ", positions.sizes());
+      p.positions = positions.const_data_ptr();
+      p.position_bits = positions.scalar_type() == at::kInt ? 32 : 64;
+      p.position_stride_b = per_token ? positions.stride(0) : 0;
+      p.position_stride_s = positions.stride(per_token ? 1 : 0);
+    } else {
+      TORCH_CHECK_VALUE(p.rotary_dim == 0 || p.S <= p.table_length, "the table has ", p.table_length, " positions, the tokens need ", p.S);
+    }
+    const void** dst[2] = {&p.q_weight, &p.k_weight};
+    const char* const names[2] = {"query_weight", "key_weight"};
+    p.weight_dtype = p.dtype;
+    for (int i = 0; i < 2; ++i) {
+      if (weights_o[i] == Py_None) continue;
+      const at::Tensor& w = weights[i] = cuda_tensor(weights_o[i], names[i]);
+      TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == p.D && w.is_contiguous(), names[i], " must be a contiguous [", p.D, "] tensor");
+      TORCH_CHECK_VALUE(w.scalar_type() == rows.scalar_type() || w.scalar_type() == at::kFloat, names[i], " must have the dtype of the tensors or float32, got ", w.scalar_type());
+      TORCH_CHECK_VALUE(w.device() == dev, names[i], " is on ", w.device(), ", the others on ", dev);
+      TORCH_CHECK_VALUE(i == 0 || !weights[0].defined() || weights[0].scalar_type() == w.scalar_type(), "query_weight and key_weight must have the same dtype");
+      p.weight_dtype = w.scalar_type() == at::kFloat ? FA_F32 : p.dtype;
+      *dst[i] = w.const_data_ptr();
+    }
+  }
+};
+
+struct RotaryBackward : public torch::autograd::Node {
+  Rotary r;  // (its tensors: the table and the positions)
+  torch::autograd::SavedVariable q_, k_, w_[2], table_, positions_;
+  std::vector<int64_t> sizes[2];
+  bool norm = false;
+
+  std::string name() const override { return "RotaryBackward"; }
+  void release_variables() override {
+    q_.reset_data();
+    k_.reset_data();
+    for (auto& w : w_) w.reset_data();
+    table_.reset_data();
+    positions_.reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const at::Tensor x[2] = {norm ? q_.unpack() : at::Tensor(), norm ? k_.unpack() : at::Tensor()};
+    const at::Tensor w[2] = {w_[0].unpack(), w_[1].unpack()}, table = table_.unpack(), positions = positions_.unpack();
+    // under create_graph: do the gradients depend on something that requires one?
+    bool again = false;
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&grads[0], &grads[1], &x[0], &x[1], &w[0], &w[1]}) again |= at::GradMode::is_enabled() && t->defined() && t->requires_grad();
+    torch::autograd::variable_list out(4);
+    {
+      at::NoGradGuard no_grad;
+      check_status();
+      fa_rotary_params p = r.p;
+      const at::Tensor& some = grads[0].defined() ? grads[0] : grads[1];
+      if (!some.defined()) return out;
+      c10::cuda::OptionalCUDAGuard guard(some.device());
+      const auto type = p.dtype == FA_F16 ? at::kHalf : p.dtype == FA_BF16 ? at::kBFloat16 : at::kFloat;
+      at::Tensor g[2], d[2], dw[2];
+      fa_tensor gt[2], dt[2], unused{};
+      for (int i = 0; i < 2; ++i) {
+        g[i] = grads[i].defined() ? grads[i] : at::zeros(sizes[i], some.options());
+        TORCH_CHECK(g[i].scalar_type() == type && g[i].sizes() == at::IntArrayRef(sizes[i]), "a gradient of another shape or type than the output");
+        if (g[i].size(3) > 1 && g[i].stride(3) != 1) g[i] = g[i].contiguous();
+        const bool want = task_should_compute_output(i), want_w = w[i].defined() && task_should_compute_output(2 + i);
+        (i == 0 ? p.q_weight : p.k_weight) = w[i].defined() ? w[i].const_data_ptr() : nullptr;
+        gt[i] = dt[i] = unused;
+        if (!want && !want_w) {  // nothing of this tensor is asked for
+          (i == 0 ? p.Hq : p.Hkv) = 0;
+          continue;
+        }
+        d[i] = empty_rows(g[i]);
+        if (want_w) dw[i] = empty({p.D}, w[i].scalar_type(), w[i].device());
+        gt[i] = by_strides(g[i], r.bshd);
+        dt[i] = by_strides(d[i], r.bshd);
+        if (norm) {
+          TORCH_CHECK(x[i].scalar_type() == type && x[i].sizes() == at::IntArrayRef(sizes[i]) && x[i].device() == some.device() && (x[i].size(3) == 1 || x[i].stride(3) == 1),
+                      "a saved tensor has come back with another shape, type or device");
+          (i == 0 ? p.q : p.k) = by_strides(x[i], r.bshd);
+        }
+      }
+      p.table = p.rotary_dim > 0 ? (const float*)table.const_data_ptr() : nullptr;
+      p.positions = positions.defined() ? positions.const_data_ptr() : nullptr;
+      const size_t bytes = fa_rotary_bwd_workspace_bytes(&p);
+      at::Tensor ws;
+      if (bytes > 0) ws = empty({(int64_t)bytes}, at::kByte, some.device());
+      void* stream = (void*)c10::cuda::getCurrentCUDAStream(some.device().index()).stream();
+      const int rc = fa_rotary_bwd(&p, &gt[0], &gt[1], &dt[0], &dt[1], dw[0].defined() ? dw[0].mutable_data_ptr() : nullptr,
+                                   dw[1].defined() ? dw[1].mutable_data_ptr() : nullptr, bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, stream);
+      if (rc != FA_OK) raise(rc);
+      for (int i = 0; i < 2; ++i) {
+        if (task_should_compute_output(i)) out[i] = d[i];
+        out[2 + i] = dw[i];
+      }
+    }
+    if (again) {  // (what is derived from these would not know of the way they came about)
+      for (auto& t : out)
+        if (t.defined()) t.requires_grad_(true);
+      auto error = std::make_shared<torch::autograd::DelayedError>("rotary_embedding can be differentiated once", (int64_t)out.size());
+      return (*error)(std::move(out));
+    }
+    return out;
+  }
+};
+
+// rotary(q, k, table, positions, query_weight, key_weight, eps, interleaved, bshd) -> q', k'
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 9, "rotary takes 9 arguments");
+  check_unwatched();
+  const at::Tensor q = cuda_tensor(a[0], "query"), k = cuda_tensor(a[1], "key");
+  rows_of(q, "query");
+  rows_of(k, "key");
+  same_kind(k, q, "key");
+  Rotary r;
+  memset(&r.p, 0, sizeof r.p);
+  r.bshd = truth(a[8]);
+  const int ih = r.bshd ? 2 : 1, is = r.bshd ? 1 : 2;
+  TORCH_CHECK_VALUE(k.size(0) == q.size(0) && k.size(is) == q.size(is) && k.size(3) == q.size(3),
+                    "query and key must have the same batch, sequence and embedding dimensions, but got ", q.sizes(), " and ", k.sizes());
+  r.read(q, a[2], a[3], a + 4, a[6], a[7]);
+  r.p.Hq = (int)q.size(ih);
+  r.p.Hkv = (int)k.size(ih);
+  check_status();
+  at::Tensor qo, ko;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const bool need_grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || (r.weights[0].defined() && r.weights[0].requires_grad()) ||
+                                                          (r.weights[1].defined() && r.weights[1].requires_grad()));
+    c10::cuda::OptionalCUDAGuard guard(q.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    qo = empty_rows(q);
+    ko = empty_rows(k);
+    r.p.q = by_strides(q, r.bshd);
+    r.p.k = by_strides(k, r.bshd);
+    r.p.q_out = by_strides(qo, r.bshd);
+    r.p.k_out = by_strides(ko, r.bshd);
+    const int rc = fa_rotary(&r.p, (void*)c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+    if (rc != FA_OK) raise(rc);
+    if (need_grad) {
+      auto node = std::shared_ptr<RotaryBackward>(new RotaryBackward(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(q, k, r.weights[0], r.weights[1]));
+      node->norm = r.weights[0].defined() || r.weights[1].defined();
+      if (node->norm) {
+        node->q_ = torch::autograd::SavedVariable(q, false);
+        node->k_ = torch::autograd::SavedVariable(k, false);
+      }
+      for (int i = 0; i < 2; ++i) {
+        if (r.weights[i].defined()) node->w_[i] = torch::autograd::SavedVariable(r.weights[i], false);
+        node->sizes[i] = (i == 0 ? q : k).sizes().vec();
+      }
+      if (r.table.defined()) node->table_ = torch::autograd::SavedVariable(r.table, false);
+      if (r.positions.defined()) node->positions_ = torch::autograd::SavedVariable(r.positions, false);
+      node->r.p = r.p;
+      node->r.bshd = r.bshd;
+      torch::autograd::set_history(std::vector<at::Tensor>{qo, ko}, node);
+    }
+  }
+  Ref x(THPVariable_Wrap(qo)), y(THPVariable_Wrap(ko));
+  if (x.p == nullptr || y.p == nullptr) return nullptr;
+  return PyTuple_Pack(2, x.p, y.p);
+  END_HANDLE_TH_ERRORS
+}
+
+// pages as fa_rotary_params and fa_paged_params have them: [pages, heads, tokens of a page, D] by strides
+void read_pages(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& as, int64_t heads, int64_t D, fa_tensor& k, fa_tensor& v, int64_t& n, int32_t& size) {
+  rows_of(kp, "key_pages");
+  rows_of(vp, "value_pages");
+  same_kind(kp, as, "key_pages");
+  same_kind(vp, as, "value_pages");
+  TORCH_CHECK_VALUE(kp.size(1) == heads && kp.size(3) == D, "key_pages must be [pages, ", heads, ", page_size, ", D, "], got ", kp.sizes());
+  TORCH_CHECK_VALUE(vp.size(0) == kp.size(0) && vp.size(1) == kp.size(1) && vp.size(2) == kp.size(2), "value_pages must be the same pages as key_pages, got ", vp.sizes(), " and ", kp.sizes());
+  TORCH_CHECK_VALUE(kp.size(2) > 0, "the pages hold no tokens");
+  k = by_strides(kp, false);
+  v = by_strides(vp, false);
+  n = kp.size(0);
+  size = (int32_t)kp.size(2);
+}
+
+// rotary_append(q or None, k, v, key_pages, value_pages, slots, table, positions, query_weight, key_weight, eps, interleaved, bshd) -> q' or None
+PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 13, "rotary_append takes 13 arguments");
+  check_unwatched();
+  const bool has_q = a[0] != Py_None;
+  const at::Tensor k = cuda_tensor(a[1], "key"), v = cuda_tensor(a[2], "value"), q = has_q ? cuda_tensor(a[0], "query") : at::Tensor();
+  const at::Tensor kp = cuda_tensor(a[3], "key_pages"), vp = cuda_tensor(a[4], "value_pages"), slots = cuda_tensor(a[5], "slots");
+  rows_of(k, "key");
+  rows_of(v, "value");
+  same_kind(v, k, "value");
+  Rotary r;
+  memset(&r.p, 0, sizeof r.p);
+  fa_rotary_params& p = r.p;
+  r.bshd = truth(a[12]);
+  const int ih = r.bshd ? 2 : 1, is = r.bshd ? 1 : 2;
+  TORCH_CHECK_VALUE(v.size(0) == k.size(0) && v.size(1) == k.size(1) && v.size(2) == k.size(2), "key and value must have the same batch, heads and sequence, but got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_VALUE(v.size(3) <= k.size(3), "value embedding dimension must not exceed that of key, got ", v.size(3), " and ", k.size(3));
+  r.read(k, a[6], a[7], a + 8, a[10], a[11]);
+  if (has_q) {
+    rows_of(q, "query");
+    same_kind(q, k, "query");
+    TORCH_CHECK_VALUE(q.size(0) == k.size(0) && q.size(is) == k.size(is) && q.size(3) == k.size(3),
+                      "query and key must have the same batch, sequence and embedding dimensions, but got ", q.sizes(), " and ", k.sizes());
+    no_gradient(q, "query", "rotary_append");
+    p.Hq = (int)q.size(ih);
+  }
+  p.Hkv = (int)k.size(ih);
+  p.Dv = (int)v.size(3);
+  int64_t pages = 0;
+  read_pages(kp, vp, k, p.Hkv, p.D, p.k_pages, p.v_pages, pages, p.page_size);
+  TORCH_CHECK_VALUE(vp.size(3) == p.Dv, "value_pages must have the embedding dimension of value, got ", vp.size(3), " and ", p.Dv);
+  p.num_pages = pages;
+  writable(kp, "key_pages");
+  writable(vp, "value_pages");
+  for (const auto& [t, name] : {std::pair<const at::Tensor&, const char*>{k, "key"}, {v, "value"}, {kp, "key_pages"}, {vp, "value_pages"}}) no_gradient(t, name, "rotary_append");
+  for (int i = 0; i < 2; ++i)
+    if (r.weights[i].defined()) no_gradient(r.weights[i], i == 0 ? "query_weight" : "key_weight", "rotary_append");
+  int_kind(slots, at::kLong, k.device(), "slots");
+  const bool per_token = slots.dim() == 2 && slots.size(0) == p.B && slots.size(1) == p.S;
+  TORCH_CHECK_VALUE(per_token || (slots.dim() == 1 && slots.size(0) == (int64_t)p.B * p.S), "slots must be [B, S] or [B * S] = [", p.B, ", ", p.S, "], got ", slots.sizes());
+  p.slots = (const int64_t*)slots.const_data_ptr();
+  p.slot_stride_b = per_token ? slots.stride(0) : slots.stride(0) * p.S;
+  p.slot_stride_s = per_token ? slots.stride(1) : slots.stride(0);
+  check_status();
+  at::Tensor qo;
+  {
+    pybind11::gil_scoped_release no_gil;
+    c10::cuda::OptionalCUDAGuard guard(k.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (has_q) {
+      qo = empty_rows(q);
+      p.q = by_strides(q, r.bshd);
+      p.q_out = by_strides(qo, r.bshd);
+      if (q.numel() == 0) p.q.ptr = nullptr;
+    }
+    p.k = by_strides(k, r.bshd);
+    p.v = by_strides(v, r.bshd);
+    const int rc = fa_rotary_append(&p, (void*)c10::cuda::getCurrentCUDAStream(k.device().index()).stream());
+    if (rc != FA_OK) raise(rc);
+    written(kp);
+    written(vp);
+  }
+  if (!has_q) Py_RETURN_NONE;
+  return THPVariable_Wrap(qo);
+  END_HANDLE_TH_ERRORS
+}
+
+// page_step(lengths, new_tokens, block_table, free_pages, page_size, num_tokens, taken or None)
+// -> lengths, positions, slots, requests, starts, taken
+PyObject* page_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 7, "page_step takes 7 arguments");
+  check_unwatched();
+  const at::Tensor lengths = cuda_tensor(a[0], "lengths"), fresh = cuda_tensor(a[1], "new_tokens"), table = cuda_tensor(a[2], "block_table"), pool = cuda_tensor(a[3], "free_pages");
+  const at::Tensor taken = a[6] != Py_None ? cuda_tensor(a[6], "taken") : at::Tensor();
+  const int64_t page = integer(a[4]), tokens = integer(a[5]);
+  const c10::Device dev = lengths.device();
+  int_kind(lengths, at::kInt, dev, "lengths");
+  int_kind(fresh, at::kInt, dev, "new_tokens");
+  int_kind(table, at::kInt, dev, "block_table");
+  int_kind(pool, at::kInt, dev, "free_pages");
+  TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.is_contiguous() && lengths.size(0) <= INT32_MAX - 1, "lengths must be a contiguous 1D tensor");
+  const int64_t B = lengths.size(0);
+  TORCH_CHECK_VALUE(fresh.dim() == 1 && fresh.size(0) == B && fresh.is_contiguous(), "new_tokens must be a contiguous [", B, "] tensor, got ", fresh.sizes());
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) == B && (table.size(1) <= 1 || table.stride(1) == 1) && table.size(1) <= INT32_MAX,
+                    "block_table must be [", B, ", pages of a request] with contiguous rows, got ", table.sizes());
+  TORCH_CHECK_VALUE(B <= 1 || table.size(1) == 0 || table.stride(0) >= table.size(1), "the rows of block_table must not overlap");
+  TORCH_CHECK_VALUE(pool.dim() == 1 && pool.is_contiguous(), "free_pages must be a contiguous 1D tensor");
+  TORCH_CHECK_VALUE(page > 0 && page <= INT32_MAX, "page_size must be positive, got ", page);
+  TORCH_CHECK_VALUE(tokens >= 0 && tokens <= INT32_MAX, "num_tokens must be from 0 to 2^31 - 1, got ", tokens);
+  if (taken.defined()) {
+    int_kind(taken, at::kInt, dev, "taken");
+    TORCH_CHECK_VALUE(taken.numel() == 1, "taken must hold one number");
+  }
+  check_status();
+  std::vector<at::Tensor> out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    c10::cuda::OptionalCUDAGuard guard(dev);
+    // one allocation for the tensors of 32 bits, in parts that begin at 16 bytes
+    const auto up = [](int64_t v) { return (v + 3) / 4 * 4; };
+    const int64_t sizes[5] = {B, tokens, tokens, B + 1, 1};
+    int64_t all = 0, off = 0;
+    for (int64_t s : sizes) all += up(s);
+    at::Tensor base = empty({all}, at::kInt, dev);
+    for (int64_t s : sizes) {
+      out.push_back(part(base, off, {s}));
+      off += up(s);
+    }
+    at::Tensor slots = empty({tokens}, at::kLong, dev);
+    const auto at32 = [&](int i) { return (int32_t*)out[i].mutable_data_ptr(); };
+    const int rc = fa_page_step((const int32_t*)lengths.const_data_ptr(), (const int32_t*)fresh.const_data_ptr(), (int)B, (int32_t*)table.data_ptr(), table.stride(0),
+                                (int)table.size(1), (const int32_t*)pool.const_data_ptr(), pool.size(0),
+                                taken.defined() ? (const int32_t*)taken.const_data_ptr() : nullptr, (int)page, tokens, at32(0), at32(1),
+                                (int64_t*)slots.mutable_data_ptr(), at32(2), at32(3), at32(4), (void*)c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+    if (rc != FA_OK) raise(rc);
+    written(table);
+    out.insert(out.begin() + 2, slots);
+  }
+  PyObject* t = PyTuple_New(6);
+  if (t == nullptr) return nullptr;
+  for (int i = 0; i < 6; ++i) {
+    PyObject* o = THPVariable_Wrap(out[i]);
+    if (o == nullptr) {
+      Py_DECREF(t);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(t, i, o);
+  }
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, key_pages, value_pages, block_table, lengths, score_mod, mask_mod, window or None, scale or None, bshd, return_lse, b_offset,
+//                 h_offset, general, module: None or (handle, buffers)) -> out or (out, lse); None: the mods are not known here
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 15, "paged_attention takes 15 arguments");
+  check_unwatched();
+  const at::Tensor q = cuda_tensor(a[0], "query"), kp = cuda_tensor(a[1], "key_pages"), vp = cuda_tensor(a[2], "value_pages"),
+                   table = cuda_tensor(a[3], "block_table"), lengths = cuda_tensor(a[4], "lengths");
+  rows_of(q, "query");
+  fa_paged_params p;
+  memset(&p, 0, sizeof p);
+  const bool bshd = truth(a[9]);
+  const int ih = bshd ? 2 : 1, is = bshd ? 1 : 2;
+  p.dtype = dtype_code(q, "query");
+  p.B = (int)q.size(0); p.Hq = (int)q.size(ih); p.Sq = (int)q.size(is); p.D = (int)q.size(3);
+  TORCH_CHECK_VALUE(kp.dim() == 4 && vp.dim() == 4, "key_pages and value_pages must be [pages, kv heads, page_size, embedding dimension]");
+  p.Hkv = (int)kp.size(1);
+  p.Dv = (int)vp.size(3);
+  read_pages(kp, vp, q, p.Hkv, p.D, p.k_pages, p.v_pages, p.num_pages, p.page_size);
+  TORCH_CHECK_VALUE(p.Hkv > 0 ? p.Hq % p.Hkv == 0 : p.Hq == 0, "Expect number of query heads to be a multiple of kv heads, but got Hq=", p.Hq, " and Hkv=", p.Hkv, ".");
+  TORCH_CHECK_VALUE(p.Dv <= p.D, "value embedding dimension must not exceed that of query and key, got Ev=", p.Dv, " and E=", p.D);
+  int_kind(table, at::kInt, q.device(), "block_table");
+  int_kind(lengths, at::kInt, q.device(), "lengths");
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) == p.B && (table.size(1) <= 1 || table.stride(1) == 1) && table.size(1) <= INT32_MAX,
+                    "block_table must be [", p.B, ", pages of a request] with contiguous rows, got ", table.sizes());
+  TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.size(0) == p.B && lengths.is_contiguous(), "lengths must be a contiguous [", p.B, "] tensor, got ", lengths.sizes());
+  no_gradient(q, "query", "paged_attention");
+  no_gradient(kp, "key_pages", "paged_attention");
+  no_gradient(vp, "value_pages", "paged_attention");
+  p.block_table = (const int32_t*)table.const_data_ptr();
+  p.block_table_stride = table.stride(0);
+  p.table_width = (int)table.size(1);
+  p.lengths = (const int32_t*)lengths.const_data_ptr();
+  p.window = -1;
+  if (a[7] != Py_None) {
+    const int64_t w = integer(a[7]);
+    TORCH_CHECK_VALUE(w >= 0, "window must not be negative, got ", w);
+    p.window = (int)std::min<int64_t>(w, INT32_MAX);
+  }
+  p.scale = a[8] == Py_None ? (float)(1.0 / std::sqrt((double)std::max(p.D, 1))) : (float)number(a[8]);
+  const bool return_lse = truth(a[10]);
+  p.b_offset = (int)integer(a[11]);
+  p.h_offset = (int)integer(a[12]);
+  p.flags = truth(a[13]) ? FA_FLAG_GENERAL_KERNELS : 0;
+  p.status = (int32_t*)g_status;
+  fa_module* module = nullptr;
+  ModsPtr hold;
+  std::vector<at::Tensor> given;
+  const std::vector<at::Tensor>* buffers = &given;
+  if (a[14] != Py_None) {
+    TORCH_CHECK(PyTuple_Check(a[14]) && PyTuple_GET_SIZE(a[14]) == 2, "module: a handle and a tuple of buffers");
+    module = (fa_module*)PyLong_AsVoidPtr(PyTuple_GET_ITEM(a[14], 0));
+    if (PyErr_Occurred()) return nullptr;
+    given = tensors(PyTuple_GET_ITEM(a[14], 1));
+  } else {
+    const auto hit = g_mods->find({a[5] == Py_None || a[5] == g_identity ? nullptr : a[5], a[6] == Py_None || a[6] == g_noop ? nullptr : a[6]});
+    if (hit == g_mods->end()) Py_RETURN_NONE;
+    hold = hit->second;
+    for (const auto& t : hold->buffers)
+      if (t.device() != q.device()) Py_RETURN_NONE;
+    module = hold->module;
+    buffers = &hold->buffers;
+  }
+  check_status();
+  at::Tensor out, lse;
+  {
+    pybind11::gil_scoped_release no_gil;
+    c10::cuda::OptionalCUDAGuard guard(q.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = bshd ? empty({p.B, p.Sq, p.Hq, p.Dv}, q.scalar_type(), q.device()) : empty({p.B, p.Hq, p.Sq, p.Dv}, q.scalar_type(), q.device());
+    if (return_lse) lse = empty({p.B, p.Hq, p.Sq}, at::kFloat, q.device());
+    if (p.B > 0 && p.Hq > 0 && p.Sq > 0) {
+      p.q = by_strides(q, bshd);
+      p.o = by_strides(out, bshd);
+      p.lse = return_lse ? lse.mutable_data_ptr<float>() : nullptr;
+      const size_t bytes = fa_paged_workspace_bytes(&p);
+      const at::Tensor ws = empty({(int64_t)std::max<size_t>(bytes, 16)}, at::kByte, q.device());
+      BuffersLock lock(module, *buffers);
+      const int rc = lock.rc != FA_OK ? lock.rc : fa_paged(module, &p, ws.mutable_data_ptr(), bytes, (void*)c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+      if (rc != FA_OK) raise(rc);
+    }
+  }
+  if (!return_lse) return THPVariable_Wrap(out);
+  Ref o(THPVariable_Wrap(out)), l(THPVariable_Wrap(lse));
+  if (o.p == nullptr || l.p == nullptr) return nullptr;
+  return PyTuple_Pack(2, o.p, l.p);
+  END_HANDLE_TH_ERRORS
+}
+
 // register(score_mod, mask_mod, module, handle, buffers): the module of a pair of mods (None: no mod).
 // The pair is known by identity; the Python layer calls forget when one of the two goes away.
 PyObject* register_mods(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -661,6 +1168,10 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef kMethods[] = {
     {"attention", (PyCFunction)(void*)attention, METH_FASTCALL, nullptr},
     {"build_block_mask", (PyCFunction)(void*)build_block_mask, METH_FASTCALL, nullptr},
+    {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, nullptr},
+    {"rotary_append", (PyCFunction)(void*)rotary_append, METH_FASTCALL, nullptr},
+    {"page_step", (PyCFunction)(void*)page_step, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void*)paged_attention, METH_FASTCALL, nullptr},
     {"register", (PyCFunction)(void*)register_mods, METH_FASTCALL, nullptr},
     {"forget", (PyCFunction)(void*)forget, METH_FASTCALL, nullptr},
     {"setup", (PyCFunction)(void*)setup, METH_FASTCALL, nullptr},

@@ -77,6 +77,32 @@ struct FaParams {
   const unsigned char* beyond[4];
 };
 
+// Attention over pages (fa_paged.cuh)
+struct FaPagedParams {
+  FaTensor q, k, v, o;  // k, v: sb is the stride of a page, ss of a token in it
+  float* lse;           // [B,Hq,Sq] or null
+  const int* table;     // [B, table_stride]: pages of each request
+  long long table_stride;
+  const int* lengths;   // [B] tokens of each request, the Sq newest included
+  float* part_o;        // [2 * workers, rows of a tile, Dv]
+  float* part_ml;       // [2 * workers, rows of a tile, 2] maximum (log2 units) and sum
+  int* plan;            // [B * row_tiles + 1] tiles of the row tiles in front, per kv head
+  int* status;
+  int B, Hq, Hkv, Sq;
+  int num_pages, page_size, max_len;  // max_len: tokens that the table has room for
+  int row_tiles, workers, min_tiles;  // row tiles of a request; CTAs, and the fewest tiles that one gets
+  int window;                         // keys more than this far behind a query are not seen (-1: all are)
+  int b_off, h_off;
+  int box;                            // keys that one look-up in the table gives (1, or the rows of a TMA box)
+  float scale;
+  const void* mod_buf[FA_MAX_MOD_BUFS];
+};
+
+// Status bits that kernels OR into a status word, beside those of the bounded waits (fa_sm100.cuh)
+#define FA_STATUS_BAD_PAGE 4      // a block table entry that is no page, or a length beyond the table
+#define FA_STATUS_BAD_POSITION 8  // a position beyond the rotary table
+#define FA_STATUS_BAD_SLOT 16     // a slot beyond the pages
+
 // Evaluation of mask_mod over a block grid: the class of every block and, optionally, the mask itself as
 // bit matrices.  `B`, `H`: entries evaluated (1 where the mask does not read the batch / head index).
 struct FaMaskParams {

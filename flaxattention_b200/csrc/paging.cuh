@@ -1,0 +1,372 @@
+// Pages of a key / value cache: places for the new tokens of a batch of requests (fa_page_step) and attention over
+// the pages (fa_paged; its kernel is kernels/fa_paged.cuh).  Part of flaxattn.cu.
+namespace {
+
+// ---- block tables, slots and positions of new tokens --------------------------------------
+// Request b has len[b] tokens in its pages and gets n[b] more.  It keeps its ceil(len / P) pages and takes as many free ones
+// as the new length needs; the free list is gone through in the order of the requests.  The new tokens, request after
+// request, are numbered through: token t of the step is token len + (t - start) of its request.
+//
+// One launch: every block runs over all requests, 1024 at a time, adds up their tokens and pages and fills what lies in its own range
+// of tokens (and of new pages, of which there are no more than tokens).  The prefix sums that a block needs are its own, so that
+// no block waits for another.
+constexpr int kStepThreads = 256, kStepItems = 4, kStepChunk = kStepThreads * kStepItems;
+
+struct FaStepParams {
+  const int *len, *count, *free_pages, *taken_in;
+  int* table;
+  long long table_stride, num_free, tokens;
+  int B, width, page;
+  int *out_len, *positions, *requests, *starts, *taken_out;
+  long long* slots;
+};
+
+__global__ void __launch_bounds__(kStepThreads) fa_page_step_kernel(const FaStepParams P) {
+  grid_wait();
+  __shared__ long long start[kStepChunk + 1], page0[kStepChunk + 1];  // tokens and new pages in front of a request
+  __shared__ int len[kStepChunk];
+  __shared__ long long warp_sum[2][kStepThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long lo = (long long)blockIdx.x * kStepChunk, hi = min(lo + kStepChunk, P.tokens);
+  const bool first = blockIdx.x == 0, last = blockIdx.x == gridDim.x - 1;
+  const long long taken = P.taken_in != nullptr ? max(*P.taken_in, 0) : 0;
+  long long tokens = 0, pages = 0;  // of the chunks in front
+  for (int b0 = 0; b0 < P.B; b0 += kStepChunk) {
+    int l[kStepItems], n[kStepItems], g[kStepItems];
+    long long own_t = 0, own_p = 0;
+#pragma unroll
+    for (int i = 0; i < kStepItems; ++i) {
+      const int b = b0 + tid * kStepItems + i;
+      l[i] = b < P.B ? max(P.len[b], 0) : 0;
+      n[i] = b < P.B ? min(max(P.count[b], 0), 0x7fffffff - l[i]) : 0;
+      g[i] = (int)(((unsigned)l[i] + n[i] + P.page - 1u) / P.page - ((unsigned)l[i] + P.page - 1u) / P.page);
+      own_t += n[i];
+      own_p += g[i];
+    }
+    long long sum_t = own_t, sum_p = own_p;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long a = __shfl_up_sync(0xffffffffu, sum_t, off), c = __shfl_up_sync(0xffffffffu, sum_p, off);
+      if (lane >= off) {
+        sum_t += a;
+        sum_p += c;
+      }
+    }
+    __syncthreads();  // (the chunk in front has been read)
+    if (lane == 31) {
+      warp_sum[0][warp] = sum_t;
+      warp_sum[1][warp] = sum_p;
+    }
+    __syncthreads();
+    long long at_t = tokens + sum_t - own_t, at_p = pages + sum_p - own_p;
+    for (int w = 0; w < kStepThreads / 32; ++w) {
+      if (w < warp) {
+        at_t += warp_sum[0][w];
+        at_p += warp_sum[1][w];
+      }
+      tokens += warp_sum[0][w];
+      pages += warp_sum[1][w];
+    }
+#pragma unroll
+    for (int i = 0; i < kStepItems; ++i) {
+      const int k = tid * kStepItems + i, b = b0 + k;
+      start[k] = at_t;
+      page0[k] = at_p;
+      len[k] = l[i];
+      if (first && b < P.B) {
+        P.out_len[b] = l[i] + n[i];
+        P.starts[b] = (int)min(at_t, 0x7fffffffll);
+      }
+      at_t += n[i];
+      at_p += g[i];
+    }
+    if (tid == kStepThreads - 1) {
+      start[kStepChunk] = at_t;
+      page0[kStepChunk] = at_p;
+    }
+    __syncthreads();
+    // the request whose range holds x: the last one that begins at or in front of it
+    const auto find = [&](const long long* from, long long x) {
+      int a = 0, c = kStepChunk;
+      while (c - a > 1) {
+        const int m = (a + c) >> 1;
+        if (from[m] <= x) a = m;
+        else c = m;
+      }
+      return a;
+    };
+    const auto fresh = [&](long long nth) {  // the nth new page
+      const long long at = taken + nth;
+      return at < P.num_free ? max(P.free_pages[at], -1) : -1;
+    };
+    for (long long t = max(lo, start[0]) + tid; t < min(hi, start[kStepChunk]); t += kStepThreads) {
+      const int k = find(start, t), b = b0 + k;
+      const int pos = len[k] + (int)(t - start[k]), col = pos / P.page, had = (int)(((unsigned)len[k] + P.page - 1u) / P.page);
+      int page = -1;
+      if (col < P.width) page = col < had ? P.table[b * P.table_stride + col] : fresh(page0[k] + (col - had));
+      P.positions[t] = pos;
+      P.requests[t] = b;
+      P.slots[t] = page < 0 ? -1ll : (long long)page * P.page + (pos - col * P.page);
+    }
+    // (new pages: there may be more of them than the call has tokens for, which the last block takes)
+    for (long long q = max(lo, page0[0]) + tid; q < (last ? page0[kStepChunk] : min(lo + kStepChunk, page0[kStepChunk])); q += kStepThreads) {
+      const int k = find(page0, q);
+      const long long col = ((unsigned)len[k] + P.page - 1u) / P.page + (q - page0[k]);
+      if (col < P.width) P.table[(long long)(b0 + k) * P.table_stride + col] = fresh(q);
+    }
+  }
+  if (first && tid == 0) {
+    P.starts[P.B] = (int)min(tokens, 0x7fffffffll);
+    *P.taken_out = (int)min(taken + pages, 0x7fffffffll);
+  }
+  for (long long t = max(lo, tokens) + tid; t < hi; t += kStepThreads) {  // no tokens
+    P.positions[t] = 0;
+    P.requests[t] = -1;
+    P.slots[t] = -1;
+  }
+}
+
+// ---- attention: the parts of segments that several workers share ---------------------------
+// WARPS warps per query row, which take the row's parts in turn.
+template <int DT, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) fa_paged_combine_kernel(const __grid_constant__ FaPagedParams p, int BM, int Dv, int n_rows) {
+  grid_wait();
+  constexpr int U = 4;
+  __shared__ float4 sums[WARPS == 1 ? 1 : WARPS][64];
+  __shared__ float totals[WARPS];
+  const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
+  const int row = WARPS == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= n_rows) return;
+  // row: request, kv head, row among the G * Sq of the head
+  const int G = p.Hq / p.Hkv, per_head = G * p.Sq;
+  const int bh = row / per_head, r = row - bh * per_head, b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const int rt = r / BM, item = b * p.row_tiles + rt, items = p.B * p.row_tiles;
+  const int before = p.plan[item], n = p.plan[item + 1] - before, total = p.plan[items] * p.Hkv;
+  const int per = max(p.min_tiles, (total + p.workers - 1) / p.workers);
+  const int begin = before * p.Hkv + hk * n, c0 = begin / per, c1 = (begin + n - 1) / per;
+  if (c0 == c1) return;  // (one worker's: written by it)
+  const int q = r / G, h = hk * G + r - q * G;
+  // part of worker c: its first part, but for the first worker's, which begins inside the run
+  const auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && begin != c0 * per ? 1 : 0)) * BM + (r - rt * BM); };
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[at(c) * 2]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  const float m_use = m == -INFINITY ? 0.f : m;
+  const bool second = lane * 4 + 128 < Dv, active = lane * 4 < Dv;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), acc2 = acc;
+  float l = 0.f;
+  for (int c = c0 + warp; c <= c1; c += WARPS * U) {
+    float2 ml[U];
+    float4 x[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = c + u * WARPS <= c1;
+      const long long a = in ? at(c + u * WARPS) : 0;
+      ml[u] = in ? *(const float2*)(p.part_ml + a * 2) : make_float2(-INFINITY, 0.f);
+      x[u] = in && active ? *(const float4*)(p.part_o + a * Dv + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      y[u] = in && second ? *(const float4*)(p.part_o + a * Dv + lane * 4 + 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // (a part that has seen nothing counts for nothing; one whose sum is no number stays so)
+      const float w = ml[u].y == 0.f ? 0.f : exp2f(ml[u].x - m_use);
+      if (w == 0.f) continue;
+      l += w * ml[u].y;
+      acc.x += w * x[u].x; acc.y += w * x[u].y; acc.z += w * x[u].z; acc.w += w * x[u].w;
+      acc2.x += w * y[u].x; acc2.y += w * y[u].y; acc2.z += w * y[u].z; acc2.w += w * y[u].w;
+    }
+  }
+  if (WARPS > 1) {
+    sums[WARPS == 1 ? 0 : warp][lane] = acc;
+    sums[WARPS == 1 ? 0 : warp][lane + 32] = acc2;
+    if (lane == 0) totals[warp] = l;
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) {
+      const float4 x = sums[WARPS == 1 ? 0 : w][lane], y = sums[WARPS == 1 ? 0 : w][lane + 32];
+      acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+      acc2.x += y.x; acc2.y += y.y; acc2.z += y.z; acc2.w += y.w;
+      l += totals[w];
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : l;  // (0 and no number stay)
+  char* og = (char*)p.o.ptr + ((long long)b * p.o.sb + (long long)h * p.o.sh + (long long)q * p.o.ss) * (DT == FA_F32 ? 4 : 2);
+  const auto put = [&](int col, const float4& v) {
+    const float f[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rot_put<DT>(og, col + i, f[i]);
+  };
+  if (active) put(lane * 4, acc);
+  if (second) put(lane * 4 + 128, acc2);
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[((long long)b * p.Hq + h) * p.Sq + q] = l == 0.f ? -INFINITY : (m_use + log2f(l)) * 0.6931471805599453f;
+}
+
+// ---- host --------------------------------------------------------------------------------
+struct FaPagedLaunchHost {
+  FaPagedParams p;
+  FaTensorMapHost tk, tv;
+};
+struct PagedCfg {
+  int RG, WN, stages, smem, per_sm, box;
+  bool tma;
+};
+int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
+
+// Tiles, buffers and CTAs per SM (the map of fa_paged.cuh).  Rows: one warp takes 16.  Registers allow eight warps per SM at 255
+// each; the buffers are as many as fill the shared memory of that many CTAs, two at least.
+void pick_paged(const fa_paged_params* p, PagedCfg& c) {
+  const long long rows = (long long)(p->Hq / p->Hkv) * p->Sq;
+  const bool f32 = p->dtype == FA_F32;
+  const int es = esize(p->dtype);
+  c.RG = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  c.WN = f32 && p->D > 64 ? 16 : 32;
+  c.box = gcd(p->page_size, c.WN);
+  c.tma = !f32 && p->D % 64 == 0 && p->Dv % 64 == 0 && c.box >= 8 && p->num_pages > 0 && !(p->flags & FA_FLAG_GENERAL_KERNELS);
+  if (!c.tma) c.box = 1;
+  const int stage = c.tma ? c.WN * (p->D + p->Dv) * es : c.WN * (pitch(p->D, es) + pitch(p->Dv, es));
+  const int fixed = f32 ? c.RG * 16 * (pitch(p->D, 4) + pitch(c.WN, 4)) : 0;
+  const int most = 8 / c.RG;
+  c.stages = std::min(std::max((226 * 1024 / most - 2048 - fixed) / stage, 2), 4);
+  c.smem = c.stages * stage + fixed + (c.tma ? c.stages * 16 + 16 + 1024 : 0);
+  c.per_sm = std::max(1, std::min(most, 227 * 1024 / (c.smem + 1024)));
+}
+int paged_row_tiles(const fa_paged_params* p, const PagedCfg& c) {
+  return (int)(((long long)(p->Hq / p->Hkv) * p->Sq + c.RG * 16 - 1) / (c.RG * 16));
+}
+int paged_workers(const PagedCfg& c) { return c.per_sm * device_sm_count(); }
+
+int get_paged_kernel(fa_module* m, const fa_paged_params* p, const PagedCfg& c, Kernel** k) {
+  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.stages, 3}, {c.tma ? 1 : 0, 1}}), "fa_paged.cuh",
+                    [&] { return defs({{"FA_DTYPE", p->dtype}, {"FA_D", p->D}, {"FA_DV", p->Dv}, {"FA_RG", c.RG}, {"FA_WN", c.WN},
+                                       {"FA_STAGES", c.stages}, {"FA_TMA", c.tma ? 1 : 0}}); },
+                    "fa_paged_kernel", c.smem, k);
+}
+
+int paged_check(fa_module* m, const fa_paged_params* p) {
+  if (!m) return fail(FA_EINVAL, "module is null");
+  if (!p) return fail(FA_EINVAL, "params is null");
+  if (p->dtype < FA_F16 || p->dtype > FA_F32) return fail(FA_EINVAL, "unknown dtype");
+  if (p->B <= 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Sq <= 0) return fail(FA_EINVAL, "B, Hq, Hkv and Sq must be positive");
+  if (p->Hq % p->Hkv) return fail(FA_EINVAL, "Hq must be a multiple of Hkv");
+  if (p->D <= 0 || p->D % 16 || p->Dv <= 0 || p->Dv % 16) return fail(FA_EUNSUPPORTED, "head dims must be positive multiples of 16");
+  if (p->Dv > p->D) return fail(FA_EINVAL, "value head dim must not exceed the query/key head dim");
+  if (p->D > 256) return fail(FA_EUNSUPPORTED, "head dim above 256 is not supported");
+  if (p->Sq > 1 << 20) return fail(FA_EUNSUPPORTED, "Sq must not exceed 2^20");
+  if (p->page_size <= 0 || p->num_pages < 0 || p->table_width < 0) return fail(FA_EINVAL, "page_size must be positive, num_pages and table_width not negative");
+  if (p->num_pages > 0x7fffffffll) return fail(FA_EUNSUPPORTED, "num_pages must stay below 2^31");
+  if (!p->lengths) return fail(FA_EINVAL, "lengths is null");
+  if (p->table_width > 0 && !p->block_table) return fail(FA_EINVAL, "block_table is null");
+  const int es = esize(p->dtype);
+  if (int rc = check_tensor(p->q, "q", es)) return rc;
+  if (int rc = check_tensor(p->o, "o", es)) return rc;
+  if (int rc = check_tensor(p->k_pages, "k_pages", es, p->num_pages > 0)) return rc;
+  if (int rc = check_tensor(p->v_pages, "v_pages", es, p->num_pages > 0)) return rc;
+  PagedCfg c;
+  pick_paged(p, c);
+  if ((long long)p->B * p->Hq * p->Sq > 0x7fffffffll - 1024) return fail(FA_EUNSUPPORTED, "B * Hq * Sq must stay below 2^31");
+  const long long longest = std::min<long long>((long long)p->table_width * p->page_size, 0x7fffffffll);
+  if ((double)p->B * paged_row_tiles(p, c) * p->Hkv * (double)(longest / c.WN + 2) > 2e9) return fail(FA_EUNSUPPORTED, "more than 2e9 tiles of keys");
+  return FA_OK;
+}
+
+size_t paged_up(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" {
+
+int fa_page_step(const int32_t* lengths, const int32_t* new_tokens, int B, int32_t* block_table, int64_t block_table_stride, int table_width,
+                 const int32_t* free_pages, int64_t num_free, const int32_t* taken, int page_size, int64_t num_tokens,
+                 int32_t* out_lengths, int32_t* positions, int64_t* slots, int32_t* requests, int32_t* starts, int32_t* out_taken, void* stream) {
+  if (B < 0 || table_width < 0 || num_free < 0 || num_tokens < 0 || page_size <= 0)
+    return fail(FA_EINVAL, "B, table_width, num_free and num_tokens must not be negative, page_size must be positive");
+  if (B > 0 && (!lengths || !new_tokens || !out_lengths)) return fail(FA_EINVAL, "lengths, new_tokens or out_lengths is null");
+  if (!starts || !out_taken) return fail(FA_EINVAL, "starts or out_taken is null");
+  if (num_tokens > 0 && (!positions || !slots || !requests)) return fail(FA_EINVAL, "positions, slots or requests is null");
+  if ((B > 0 && table_width > 0 && !block_table) || (num_free > 0 && !free_pages)) return fail(FA_EINVAL, "block_table or free_pages is null");
+  if (num_tokens > 0x7fffffffll) return fail(FA_EUNSUPPORTED, "num_tokens must stay below 2^31");
+  prof_reset();
+  FaStepParams k{};
+  k.len = lengths; k.count = new_tokens; k.free_pages = free_pages; k.taken_in = taken;
+  k.table = block_table; k.table_stride = block_table_stride; k.num_free = num_free; k.tokens = num_tokens;
+  k.B = B; k.width = table_width; k.page = page_size;
+  k.out_len = out_lengths; k.positions = positions; k.requests = requests; k.starts = starts; k.taken_out = out_taken;
+  k.slots = (long long*)slots;
+  const unsigned blocks = (unsigned)std::max<long long>(1, (num_tokens + kStepChunk - 1) / kStepChunk);
+  return launch_here("fa_page_step_kernel", fa_page_step_kernel, dim3(blocks), dim3(kStepThreads), stream, k);
+}
+
+size_t fa_paged_workspace_bytes(const fa_paged_params* p) {
+  if (!p || p->Hkv <= 0 || p->Hq <= 0 || p->Sq <= 0 || p->D <= 0 || p->Dv <= 0 || p->page_size <= 0 || p->B <= 0) return 0;
+  PagedCfg c;
+  pick_paged(p, c);
+  const size_t rows = 2 * (size_t)paged_workers(c) * c.RG * 16;
+  return paged_up(rows * p->Dv * 4) + paged_up(rows * 8) + paged_up(((size_t)p->B * paged_row_tiles(p, c) + 1) * 4);
+}
+
+int fa_paged_prepare(fa_module* m, const fa_paged_params* p) {
+  if (!m || !p) return fail(FA_EINVAL, "module or params is null");
+  if (p->dtype < FA_F16 || p->dtype > FA_F32 || p->Hkv <= 0 || p->Hq <= 0 || p->Hq % p->Hkv || p->Sq <= 0 || p->page_size <= 0 || p->D <= 0 || p->D > 256 ||
+      p->D % 16 || p->Dv <= 0 || p->Dv > p->D || p->Dv % 16)
+    return fail(FA_EINVAL, "type, heads, head dims or sizes that fa_paged does not take");
+  PagedCfg c;
+  pick_paged(p, c);
+  Kernel* kernel = nullptr;
+  return get_paged_kernel(m, p, c, &kernel);
+}
+
+int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = paged_check(m, p)) return rc;
+  if (!workspace || workspace_bytes < fa_paged_workspace_bytes(p)) return fail(FA_EWORKSPACE, "paged attention workspace too small");
+  if ((uintptr_t)workspace & 15) return fail(FA_EINVAL, "workspace must be 16-byte aligned");
+  prof_reset();
+  PagedCfg c;
+  pick_paged(p, c);
+  FaPagedLaunchHost L;
+  memset(&L, 0, sizeof L);
+  FaPagedParams& k = L.p;
+  fill_buffers(m, k.mod_buf);
+  k.q = cvt(p->q); k.k = cvt(p->k_pages); k.v = cvt(p->v_pages); k.o = cvt(p->o);
+  k.lse = p->lse; k.table = p->block_table; k.table_stride = p->block_table_stride; k.lengths = p->lengths; k.status = p->status;
+  k.B = p->B; k.Hq = p->Hq; k.Hkv = p->Hkv; k.Sq = p->Sq;
+  k.num_pages = (int)p->num_pages; k.page_size = p->page_size;
+  k.max_len = (int)std::min<long long>((long long)p->table_width * p->page_size, 0x7fffffffll - 64);
+  k.row_tiles = paged_row_tiles(p, c); k.workers = paged_workers(c); k.min_tiles = 1;
+  k.window = p->window < 0 ? -1 : std::min(p->window, 1 << 30);
+  k.b_off = p->b_offset; k.h_off = p->h_offset; k.scale = p->scale;
+  const size_t rows = 2 * (size_t)k.workers * c.RG * 16;
+  k.part_o = (float*)workspace;
+  k.part_ml = (float*)((char*)workspace + paged_up(rows * p->Dv * 4));
+  k.plan = (int*)((char*)k.part_ml + paged_up(rows * 8));
+  if (c.tma) {
+    // (strides that no tensor map takes: 16-byte pieces)
+    if (make_map(&L.tk, p->dtype, p->k_pages, p->D, p->page_size, p->Hkv, (int)p->num_pages, c.box) != FA_OK ||
+        make_map(&L.tv, p->dtype, p->v_pages, p->Dv, p->page_size, p->Hkv, (int)p->num_pages, c.box) != FA_OK) {
+      fa_paged_params q = *p;
+      q.flags |= FA_FLAG_GENERAL_KERNELS;
+      PagedCfg g;
+      pick_paged(&q, g);
+      g.per_sm = std::min(g.per_sm, c.per_sm);  // (the workspace is the other's)
+      c = g;
+      k.workers = paged_workers(c);
+    }
+  }
+  k.box = c.box;
+  Kernel* kernel = nullptr;
+  if (int rc = get_paged_kernel(m, p, c, &kernel)) return rc;
+  if (int rc = launch(kernel, dim3((unsigned)k.workers), dim3(c.RG * 32), &L, stream)) return rc;
+  // Few segments for the workers: many parts each, and eight warps add up a row's.
+  const long long segments = (long long)p->B * k.row_tiles * p->Hkv;
+  const int n_rows = p->B * p->Hq * p->Sq;
+  const bool wide = k.workers / segments >= 16;
+  return rot_dispatch(p->dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    return wide ? launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 8>, dim3((unsigned)n_rows), dim3(256), stream, k, c.RG * 16, p->Dv, n_rows)
+                : launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 1>, dim3((unsigned)((n_rows + 3) / 4)), dim3(128), stream, k, c.RG * 16, p->Dv, n_rows);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,652 @@
+// Rotary positions of queries and keys, with an optional RMS norm per head in the same pass (fa_rotary,
+// fa_rotary_bwd), and the same for new tokens whose keys and values go into the pages of a cache
+// (fa_rotary_append).  Part of flaxattn.cu.
+//
+//   y = x * rsqrt(mean(x^2) + eps) * w                    (with weights)
+//   (a, b) -> (a cos - b sin, b cos + a sin)              pairs of the first R values of y: i and i + R / 2, or
+//                                                         neighbours; the others stay as they are
+// and backward, with g the gradient behind the rotation turned back by the same angles (the transposed map) and
+// u = x * rsqrt(..):   dw = sum over rows of g u,   dx = rsqrt(..) (g w - u mean(g w u)).
+//
+// All sums are in fp32, and a result is rounded once, when it is written.  Memory sets the pace: every value is read
+// and written once, with a few operations in between.
+namespace {
+
+constexpr int kRotThreads = 256;
+
+struct FaRotTensor {
+  char* ptr;
+  long long sb, sh, ss;  // byte strides of batch, head and token (pages: of page, head and token in a page)
+};
+struct FaRotParams {
+  FaRotTensor x[3], y[3];  // q, k, v: where they come from and go (backward: dy of q and k, and dx)
+  FaRotTensor in[2];       // backward: q and k
+  const void* w[2];        // norm weights or null
+  float* dw[2];            // backward: partial sums [parts, D] or null
+  const float* table;      // [table_len] rows of cos[R / 2] | sin[R / 2]
+  long long table_stride, table_len;
+  const void* pos;         // null: the token's number in its sequence
+  long long pos_sb, pos_ss;
+  const long long* slots;  // null: y[1] and y[2] are tensors like y[0]
+  long long slot_sb, slot_ss, num_slots;
+  int page_size;
+  int pos64, w_f32, interleaved;
+  int tokens, S, heads[3], D, Dv, R;
+  int groups[3], per_group;  // groups of heads of each tensor, heads of a group
+  int lane_shift;            // log2 of the lanes that share a row
+  float eps, sign;           // sign of sin: -1 turns back
+  int* status;
+};
+
+template <int DT>
+__device__ __forceinline__ float rot_get(const void* p, long long i) {
+  if (DT == FA_F32) return ((const float*)p)[i];
+  if (DT == FA_F16) return __half2float(((const __half*)p)[i]);
+  return __bfloat162float(((const __nv_bfloat16*)p)[i]);
+}
+template <int DT>
+__device__ __forceinline__ void rot_put(void* p, long long i, float v) {
+  if (DT == FA_F32) ((float*)p)[i] = v;
+  else if (DT == FA_F16) ((__half*)p)[i] = __float2half_rn(v);
+  else ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
+}
+template <int DT>
+constexpr int kRotVec = DT == FA_F32 ? 4 : 8;  // values of 16 bytes
+template <int DT>
+__device__ __forceinline__ void rot_unpack(const uint4& u, float (&f)[kRotVec<DT>]) {
+  const unsigned v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == FA_F32) {
+      f[i] = __uint_as_float(v[i]);
+    } else if constexpr (DT == FA_F16) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    } else {
+      f[2 * i] = __uint_as_float(v[i] << 16);
+      f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ uint4 rot_pack(const float (&f)[kRotVec<DT>]) {
+  unsigned v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == FA_F32) {
+      v[i] = __float_as_uint(f[i]);
+    } else if constexpr (DT == FA_F16) {
+      const __half2 t = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      v[i] = *reinterpret_cast<const unsigned*>(&t);
+    } else {
+      const __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      v[i] = *reinterpret_cast<const unsigned*>(&t);
+    }
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+template <int DT>
+__device__ __forceinline__ void rot_weights(const FaRotParams& P, int kind, int chunk, bool have, float (&w)[kRotVec<DT>]) {
+  constexpr int V = kRotVec<DT>;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    w[i] = !have ? 0.f : P.w_f32 ? ((const float*)P.w[kind])[chunk * V + i] : rot_get<DT>(P.w[kind], chunk * V + i);
+}
+
+// row of the table for token s of sequence b; -1 (and the status bit) for a position that it does not reach
+__device__ __forceinline__ long long rot_position(const FaRotParams& P, int b, int s) {
+  long long pos = s;
+  if (P.pos != nullptr) {
+    const long long at = b * P.pos_sb + s * P.pos_ss;
+    pos = P.pos64 ? ((const long long*)P.pos)[at] : ((const int*)P.pos)[at];
+  }
+  if (pos >= 0 && pos < P.table_len) return pos;
+  if (P.status != nullptr) atomicOr(P.status, FA_STATUS_BAD_POSITION);
+  return -1;
+}
+// byte offset of token (b, s) in the destination; -1: it has none (keys and values of a slot below 0 or, with the
+// status bit, beyond the pages)
+__device__ __forceinline__ long long rot_destination(const FaRotParams& P, int kind, int b, int s) {
+  const FaRotTensor& y = P.y[kind];
+  if (P.slots == nullptr || kind == 0) return b * y.sb + s * y.ss;
+  const long long slot = P.slots[b * P.slot_sb + s * P.slot_ss];
+  if (slot < 0) return -1;
+  if (slot >= P.num_slots) {
+    if (P.status != nullptr) atomicOr(P.status, FA_STATUS_BAD_SLOT);
+    return -1;
+  }
+  long long page, at;
+  if (P.num_slots <= 0x7fffffffll) {
+    page = (unsigned)slot / (unsigned)P.page_size;
+    at = (unsigned)slot % (unsigned)P.page_size;
+  } else {
+    page = slot / P.page_size;
+    at = slot % P.page_size;
+  }
+  return page * y.sb + at * y.ss;
+}
+
+// This thread's place in the grid: a lane of the `1 << lane_shift` that share a row, a token, a tensor and its heads.
+struct RotPlace {
+  int lane, token, kind, h0, h1;
+  __device__ __forceinline__ RotPlace(const FaRotParams& P) {
+    lane = threadIdx.x & ((1 << P.lane_shift) - 1);
+    token = (int)(blockIdx.x * (kRotThreads >> P.lane_shift) + (threadIdx.x >> P.lane_shift));
+    int group = blockIdx.y;
+    kind = 0;
+    while (kind < 2 && group >= P.groups[kind]) group -= P.groups[kind++];
+    h0 = group * P.per_group;
+    h1 = min(h0 + P.per_group, P.heads[kind]);
+  }
+};
+template <class T>
+__device__ __forceinline__ T rot_sum(T v, int lane_shift) {
+  for (int off = 1 << lane_shift >> 1; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+
+// cos and sin of the pairs `lane * V ..` of a token
+template <int V>
+__device__ __forceinline__ void rot_angles(const FaRotParams& P, long long pos, int lane, bool turns, float (&c)[V], float (&s)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; i += 4) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (turns && pos >= 0) {
+      const float* row = P.table + pos * P.table_stride + lane * V + i;
+      a = *(const float4*)row;
+      b = *(const float4*)(row + P.R / 2);
+    }
+    c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
+    s[i] = P.sign * b.x; s[i + 1] = P.sign * b.y; s[i + 2] = P.sign * b.z; s[i + 3] = P.sign * b.w;
+  }
+}
+template <int V, bool INTERLEAVED>
+__device__ __forceinline__ void rot_turn(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float& u = INTERLEAVED ? (2 * i < V ? a[(2 * i) % V] : b[(2 * i) % V]) : a[i];
+    float& v = INTERLEAVED ? (2 * i < V ? a[(2 * i + 1) % V] : b[(2 * i + 1) % V]) : b[i];
+    const float x = u, y = v;
+    u = x * c[i] - y * s[i];
+    v = y * c[i] + x * s[i];
+  }
+}
+
+// Two 16-byte pieces of a row per lane: the two that hold its pairs.  A thread keeps the angles of its token in
+// registers for all heads of its group, and the lanes of a warp beside each other are tokens beside each other.
+template <int DT, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotThreads) fa_rotary_kernel(const __grid_constant__ FaRotParams P) {
+  grid_wait();
+  constexpr int V = kRotVec<DT>, U = 4;
+  const RotPlace at(P);
+  const bool live = at.token < P.tokens;
+  const int b = live ? at.token / P.S : 0, s = live ? at.token - b * P.S : 0;
+  const int kind = at.kind, chunks = (kind == 2 ? P.Dv : P.D) / V, pairs = kind == 2 ? 0 : P.R / (2 * V);
+  const bool turns = at.lane < pairs;
+  const int ca = turns && !INTERLEAVED ? at.lane : turns ? 2 * at.lane : 2 * pairs + 2 * (at.lane - pairs);
+  const int cb = turns && !INTERLEAVED ? at.lane + pairs : ca + 1;
+  const long long to = live ? rot_destination(P, kind, b, s) : -1;
+  const bool have_a = live && to >= 0 && ca < chunks, have_b = live && to >= 0 && cb < chunks;
+  const bool norm = kind < 2 && P.w[kind < 2 ? kind : 0] != nullptr;
+  float c[V], sn[V], wa[V], wb[V];
+  rot_angles<V>(P, turns && live ? rot_position(P, b, s) : -1, at.lane, turns, c, sn);
+  if (norm) {
+    rot_weights<DT>(P, kind, ca, ca < chunks, wa);
+    rot_weights<DT>(P, kind, cb, cb < chunks, wb);
+  }
+  const char* src = P.x[kind].ptr + b * P.x[kind].sb + s * P.x[kind].ss;
+  char* dst = P.y[kind].ptr + to;
+  for (int h = at.h0; h < at.h1; h += U) {
+    uint4 ra[U], rb[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const char* row = src + (h + u) * P.x[kind].sh;
+      const bool in = h + u < at.h1;
+      ra[u] = in && have_a ? *(const uint4*)(row + ca * 16) : make_uint4(0, 0, 0, 0);
+      rb[u] = in && have_b ? *(const uint4*)(row + cb * 16) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (h + u >= at.h1) break;
+      if (norm || turns) {
+        float a[V], d[V];
+        rot_unpack<DT>(ra[u], a);
+        rot_unpack<DT>(rb[u], d);
+        if (norm) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < V; ++i) ss += a[i] * a[i] + d[i] * d[i];
+          const float r = rsqrtf(rot_sum(ss, P.lane_shift) / P.D + P.eps);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            a[i] *= r * wa[i];
+            d[i] *= r * wb[i];
+          }
+        }
+        if (turns) rot_turn<V, INTERLEAVED>(a, d, c, sn);
+        ra[u] = rot_pack<DT>(a);
+        rb[u] = rot_pack<DT>(d);
+      }
+      char* row = dst + (h + u) * P.y[kind].sh;
+      if (have_a) *(uint4*)(row + ca * 16) = ra[u];
+      if (have_b) *(uint4*)(row + cb * 16) = rb[u];
+    }
+  }
+}
+
+// The backward with norm weights: blocks go through the tokens in steps of the grid and keep the sums for dw in
+// registers; what a block has goes to one row of partial sums, which fa_rotary_dw_kernel adds up in order.
+template <int DT, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotThreads) fa_rotary_bwd_kernel(const __grid_constant__ FaRotParams P) {
+  grid_wait();
+  constexpr int V = kRotVec<DT>;
+  __shared__ float sums[kRotThreads / 32][256];
+  const RotPlace at(P);
+  const int kind = at.kind, chunks = P.D / V, pairs = P.R / (2 * V);
+  const bool turns = at.lane < pairs;
+  const int ca = turns && !INTERLEAVED ? at.lane : turns ? 2 * at.lane : 2 * pairs + 2 * (at.lane - pairs);
+  const int cb = turns && !INTERLEAVED ? at.lane + pairs : ca + 1;
+  const bool norm = P.w[kind] != nullptr;
+  float wa[V], wb[V], da[V], db[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) da[i] = db[i] = 0.f;
+  if (norm) {
+    rot_weights<DT>(P, kind, ca, ca < chunks, wa);
+    rot_weights<DT>(P, kind, cb, cb < chunks, wb);
+  }
+  const int step = gridDim.x * (kRotThreads >> P.lane_shift);
+  // (every thread goes round as often as the first of its block: the shuffles are the warp's)
+  for (int t0 = blockIdx.x * (kRotThreads >> P.lane_shift); t0 < P.tokens; t0 += step) {
+    const int t = t0 + (threadIdx.x >> P.lane_shift);
+    const bool live = t < P.tokens, have_a = live && ca < chunks, have_b = live && cb < chunks;
+    const int b = live ? t / P.S : 0, s = live ? t - b * P.S : 0;
+    float c[V], sn[V];
+    rot_angles<V>(P, turns && live ? rot_position(P, b, s) : -1, at.lane, turns, c, sn);
+    const char* gs = P.x[kind].ptr + b * P.x[kind].sb + s * P.x[kind].ss;
+    const char* xs = norm ? P.in[kind].ptr + b * P.in[kind].sb + s * P.in[kind].ss : gs;
+    char* ds = P.y[kind].ptr + b * P.y[kind].sb + s * P.y[kind].ss;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll 2
+    for (int h = at.h0; h < at.h1; ++h) {
+      const uint4 ga = have_a ? *(const uint4*)(gs + h * P.x[kind].sh + ca * 16) : zero;
+      const uint4 gb = have_b ? *(const uint4*)(gs + h * P.x[kind].sh + cb * 16) : zero;
+      float a[V], d[V];
+      rot_unpack<DT>(ga, a);
+      rot_unpack<DT>(gb, d);
+      if (turns) rot_turn<V, INTERLEAVED>(a, d, c, sn);
+      if (norm) {
+        const uint4 xa = have_a ? *(const uint4*)(xs + h * P.in[kind].sh + ca * 16) : zero;
+        const uint4 xb = have_b ? *(const uint4*)(xs + h * P.in[kind].sh + cb * 16) : zero;
+        float u[V], v[V], ss = 0.f, gx = 0.f;
+        rot_unpack<DT>(xa, u);
+        rot_unpack<DT>(xb, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          ss += u[i] * u[i] + v[i] * v[i];
+          gx += a[i] * wa[i] * u[i] + d[i] * wb[i] * v[i];
+        }
+        const float r = rsqrtf(rot_sum(ss, P.lane_shift) / P.D + P.eps);
+        const float m = rot_sum(gx, P.lane_shift) * r / P.D;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float p = u[i] * r, q = v[i] * r;
+          da[i] += a[i] * p;
+          db[i] += d[i] * q;
+          a[i] = r * (a[i] * wa[i] - p * m);
+          d[i] = r * (d[i] * wb[i] - q * m);
+        }
+      }
+      if (have_a) *(uint4*)(ds + h * P.y[kind].sh + ca * 16) = rot_pack<DT>(a);
+      if (have_b) *(uint4*)(ds + h * P.y[kind].sh + cb * 16) = rot_pack<DT>(d);
+    }
+  }
+  if (P.dw[kind] == nullptr) return;
+  // rows of a warp, then warps of the block
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    for (int off = 1 << P.lane_shift; off < 32; off <<= 1) {
+      da[i] += __shfl_xor_sync(0xffffffffu, da[i], off);
+      db[i] += __shfl_xor_sync(0xffffffffu, db[i], off);
+    }
+  if ((threadIdx.x & 31) == at.lane) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (ca < chunks) sums[threadIdx.x >> 5][ca * V + i] = da[i];
+      if (cb < chunks) sums[threadIdx.x >> 5][cb * V + i] = db[i];
+    }
+  }
+  __syncthreads();
+  const long long part = (long long)blockIdx.x * P.groups[kind] + at.h0 / P.per_group;
+  for (int i = threadIdx.x; i < P.D; i += kRotThreads) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRotThreads / 32; ++k) v += sums[k][i];
+    P.dw[kind][part * P.D + i] = v;
+  }
+}
+
+// What no 16-byte pieces fit: a warp per row, value by value.  Backward (BACK): the same with dy, as above.
+template <int DT, bool BACK>
+__global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid_constant__ FaRotParams P) {
+  grid_wait();
+  __shared__ float sums[BACK ? kRotThreads / 32 : 1][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kind = blockIdx.y;
+  const int D = kind == 2 ? P.Dv : P.D, half = kind == 2 ? 0 : P.R / 2, H = P.heads[kind];
+  const bool norm = kind < 2 && P.w[kind < 2 ? kind : 0] != nullptr;
+  if (BACK) {
+    for (int i = lane; i < D; i += 32) sums[warp][i] = 0.f;
+    __syncwarp();
+  }
+  const auto weight = [&](int i) { return P.w_f32 ? ((const float*)P.w[kind])[i] : rot_get<DT>(P.w[kind], i); };
+  const long long rows = (long long)P.tokens * H;
+  for (long long row = (long long)blockIdx.x * (kRotThreads / 32) + warp; row < rows; row += (long long)gridDim.x * (kRotThreads / 32)) {
+    const int t = (int)(row / H), h = (int)(row - (long long)t * H), b = t / P.S, s = t - b * P.S;
+    const long long to = rot_destination(P, kind, b, s);
+    if (to < 0) continue;
+    const char* x = P.x[kind].ptr + b * P.x[kind].sb + s * P.x[kind].ss + h * P.x[kind].sh;
+    char* y = P.y[kind].ptr + to + h * P.y[kind].sh;
+    const long long pos = half > 0 ? rot_position(P, b, s) : -1;
+    const float* angles = P.table + (pos < 0 ? 0 : pos) * P.table_stride;
+    const char* in = BACK && norm ? P.in[kind].ptr + b * P.in[kind].sb + s * P.in[kind].ss + h * P.in[kind].sh : x;
+    // (backward: in 64 bits, since with few values in a row the terms of dx nearly cancel)
+    using Real = std::conditional_t<BACK, double, float>;
+    Real r = 1, m = 0;
+    if (norm) {
+      Real ss = 0;
+      for (int i = lane; i < D; i += 32) {
+        const Real v = rot_get<DT>(in, i);
+        ss += v * v;
+      }
+      ss = rot_sum(ss, 5) / D + P.eps;
+      if constexpr (BACK) r = rsqrt(ss);
+      else r = rsqrtf(ss);
+    }
+    // pairs, then the values that stay: `first` and `second` of a unit (second < 0: there is none)
+    const auto unit = [&](int k, int& i, int& j, float& c, float& sn) {
+      const bool turns = k < half;
+      i = turns ? (P.interleaved ? 2 * k : k) : 2 * half + (k - half);
+      j = turns ? (P.interleaved ? 2 * k + 1 : k + half) : -1;
+      c = !turns ? 1.f : pos < 0 ? 0.f : angles[k];
+      sn = !turns || pos < 0 ? 0.f : P.sign * angles[half + k];
+    };
+    const int units = D - half;
+    if (BACK && norm) {
+      for (int k = lane; k < units; k += 32) {
+        int i, j;
+        float c, sn;
+        unit(k, i, j, c, sn);
+        const float a = rot_get<DT>(x, i), d = j >= 0 ? rot_get<DT>(x, j) : 0.f;
+        m += (Real)(a * c - d * sn) * weight(i) * rot_get<DT>(in, i);
+        if (j >= 0) m += (Real)(d * c + a * sn) * weight(j) * rot_get<DT>(in, j);
+      }
+      m = rot_sum(m, 5) * r / D;
+    }
+    for (int k = lane; k < units; k += 32) {
+      int i, j;
+      float c, sn;
+      unit(k, i, j, c, sn);
+      float a = rot_get<DT>(x, i), d = j >= 0 ? rot_get<DT>(x, j) : 0.f;
+      if (!BACK && norm) {
+        a *= r * weight(i);
+        if (j >= 0) d *= r * weight(j);
+      }
+      float p = a * c - d * sn, q = d * c + a * sn;
+      if (BACK && norm) {
+        const Real u = rot_get<DT>(in, i) * r, v = j >= 0 ? rot_get<DT>(in, j) * r : 0;
+        sums[warp][i] += p * (float)u;
+        if (j >= 0) sums[warp][j] += q * (float)v;
+        p = (float)(r * ((Real)p * weight(i) - u * m));
+        if (j >= 0) q = (float)(r * ((Real)q * weight(j) - v * m));
+      }
+      rot_put<DT>(y, i, p);
+      if (j >= 0) rot_put<DT>(y, j, q);
+    }
+  }
+  if (!BACK || P.dw[kind < 2 ? kind : 0] == nullptr) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < D; i += kRotThreads) {
+    float v = 0.f;
+    for (int k = 0; k < kRotThreads / 32; ++k) v += sums[BACK ? k : 0][i];
+    P.dw[kind][(long long)blockIdx.x * D + i] = v;
+  }
+}
+
+// dw from the partial sums of the blocks: 32 columns per block, 32 rows of threads, always in the same order
+struct FaRotDw {
+  const float* part[2];
+  void* dw[2];
+  int parts[2];
+  int D;
+};
+template <int DT>
+__global__ void __launch_bounds__(1024) fa_rotary_dw_kernel(const __grid_constant__ FaRotDw P) {
+  grid_wait();
+  __shared__ float sums[32][33];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5, kind = blockIdx.y;
+  if (P.dw[kind] == nullptr) return;
+  float v = 0.f;
+  if (col < P.D) {
+#pragma unroll 8
+    for (int i = slice; i < P.parts[kind]; i += 32) v += P.part[kind][(long long)i * P.D + col];
+  }
+  sums[slice][threadIdx.x & 31] = v;
+  __syncthreads();
+  v = sums[threadIdx.x & 31][slice];
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  const int mine = blockIdx.x * 32 + slice;
+  if ((threadIdx.x & 31) == 0 && mine < P.D) rot_put<DT>(P.dw[kind], mine, v);
+}
+
+// ---- host --------------------------------------------------------------------------------
+FaRotTensor rot_tensor(const fa_tensor& t, int es) { return {(char*)t.ptr, t.stride_b * es, t.stride_h * es, t.stride_s * es}; }
+bool rot_aligned(const FaRotTensor& t) { return (((uintptr_t)t.ptr | (uintptr_t)t.sb | (uintptr_t)t.sh | (uintptr_t)t.ss) & 15) == 0; }
+
+int rot_check(const fa_rotary_params* p) {
+  if (!p) return fail(FA_EINVAL, "params is null");
+  if (p->dtype < FA_F16 || p->dtype > FA_F32) return fail(FA_EINVAL, "unknown dtype");
+  if (p->weight_dtype != p->dtype && p->weight_dtype != FA_F32) return fail(FA_EINVAL, "norm weights have the type of the tensors or fp32");
+  if (p->B < 0 || p->S < 0 || p->Hq < 0 || p->Hkv < 0) return fail(FA_EINVAL, "B, S, Hq and Hkv must not be negative");
+  if ((long long)p->B * p->S > 0x7fffffffll - 256) return fail(FA_EUNSUPPORTED, "B * S must stay below 2^31");
+  if ((long long)p->Hq + 2LL * p->Hkv > 65535) return fail(FA_EUNSUPPORTED, "Hq + 2 Hkv must not exceed 65535");
+  if (p->D <= 0 || p->D > 256) return fail(FA_EUNSUPPORTED, "head dims from 1 to 256");
+  if (p->rotary_dim < 0 || p->rotary_dim > p->D || p->rotary_dim % 2) return fail(FA_EINVAL, "rotary_dim must be even and at most the head dim");
+  if (p->rotary_dim > 0 && !p->table) return fail(FA_EINVAL, "the table is null");
+  if (p->table && (p->table_length <= 0 || p->table_stride < p->rotary_dim)) return fail(FA_EINVAL, "the table needs rows of at least rotary_dim values");
+  if (p->positions && p->position_bits != 32 && p->position_bits != 64) return fail(FA_EINVAL, "positions of 32 or 64 bits");
+  if (!(p->eps >= 0.f)) return fail(FA_EINVAL, "eps must not be negative");
+  return FA_OK;
+}
+
+// Everything but the tensors; `heads`: of q, k and v (0: not there)
+void rot_fill(const fa_rotary_params* p, int hq, int hk, int hv, FaRotParams& k) {
+  memset(&k, 0, sizeof k);
+  k.w[0] = p->q_weight;
+  k.w[1] = p->k_weight;
+  k.table = p->table; k.table_stride = p->table_stride; k.table_len = p->table_length;
+  k.pos = p->positions; k.pos64 = p->position_bits == 64;
+  k.pos_sb = p->position_stride_b; k.pos_ss = p->position_stride_s;
+  k.w_f32 = p->weight_dtype == FA_F32;
+  k.interleaved = p->interleaved != 0;
+  k.tokens = p->B * p->S; k.S = p->S;
+  k.heads[0] = hq; k.heads[1] = hk; k.heads[2] = hv;
+  k.D = p->D; k.Dv = p->Dv; k.R = p->rotary_dim;
+  k.eps = p->eps; k.sign = 1.f;
+  k.status = p->status;
+}
+// Whether all rows can be taken in 16-byte pieces, two per lane; fills the lanes of a row.
+bool rot_by_pieces(const FaRotParams& k, int dtype, int* lane_shift) {
+  const int v = dtype == FA_F32 ? 4 : 8;
+  if (k.D % (2 * v) || k.R % (2 * v) || k.Dv % v || k.Dv > k.D) return false;
+  if (k.R > 0 && ((uintptr_t)k.table % 16 || k.table_stride % 4)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (k.heads[i] > 0 && !(rot_aligned(k.x[i]) && rot_aligned(k.y[i]) && (i == 2 || k.in[i].ptr == nullptr || rot_aligned(k.in[i])))) return false;
+  int shift = 0;
+  while ((1 << shift) < k.D / (2 * v)) ++shift;
+  *lane_shift = shift;
+  return shift <= 5;
+}
+// Heads that a thread goes through.  Up to 8, so that the angles are read seldom; fewer while the grid would leave SMs
+// with less than four blocks.
+void rot_groups(FaRotParams& k, long long token_blocks) {
+  int per = 8;
+  const auto blocks = [&](int n) {
+    long long g = 0;
+    for (int i = 0; i < 3; ++i) g += (k.heads[i] + n - 1) / n;
+    return g * token_blocks;
+  };
+  while (per > 1 && blocks(per) < 4LL * device_sm_count()) per /= 2;
+  k.per_group = per;
+  for (int i = 0; i < 3; ++i) k.groups[i] = (k.heads[i] + per - 1) / per;
+}
+
+template <class F>
+int rot_dispatch(int dtype, F&& f) {
+  if (dtype == FA_F16) return f(std::integral_constant<int, FA_F16>{});
+  if (dtype == FA_BF16) return f(std::integral_constant<int, FA_BF16>{});
+  return f(std::integral_constant<int, FA_F32>{});
+}
+
+// x -> y of the tensors that `k` describes
+int rot_launch(FaRotParams& k, int dtype, void* stream) {
+  const int heads = k.heads[0] + k.heads[1] + k.heads[2];
+  if (k.tokens == 0 || heads == 0) return FA_OK;
+  if (rot_by_pieces(k, dtype, &k.lane_shift)) {
+    const long long token_blocks = ((long long)k.tokens + (kRotThreads >> k.lane_shift) - 1) / (kRotThreads >> k.lane_shift);
+    rot_groups(k, token_blocks);
+    const dim3 grid((unsigned)token_blocks, (unsigned)(k.groups[0] + k.groups[1] + k.groups[2]));
+    return rot_dispatch(dtype, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      return launch_here("fa_rotary_kernel", k.interleaved ? fa_rotary_kernel<DT, true> : fa_rotary_kernel<DT, false>, grid,
+                         dim3(kRotThreads), stream, k);
+    });
+  }
+  const long long rows = (long long)k.tokens * std::max(k.heads[0], std::max(k.heads[1], k.heads[2]));
+  const dim3 grid((unsigned)std::min<long long>((rows + kRotThreads / 32 - 1) / (kRotThreads / 32), 1 << 20), k.heads[2] > 0 ? 3 : 2);
+  return rot_dispatch(dtype, [&](auto dt) {
+    return launch_here("fa_rotary_any_kernel", fa_rotary_any_kernel<decltype(dt)::value, false>, grid, dim3(kRotThreads), stream, k);
+  });
+}
+
+// blocks along the tokens of the backward with norm weights: about four per SM in all
+int rot_bwd_blocks(const fa_rotary_params* p) { return std::max(1, 4 * device_sm_count() / std::max(1, (p->Hq + 3) / 4 + (p->Hkv + 3) / 4)); }
+constexpr int kRotBwdHeads = 4;  // heads of a group there
+long long rot_bwd_parts(const fa_rotary_params* p, int heads) {
+  return std::max<long long>((long long)rot_bwd_blocks(p) * ((heads + kRotBwdHeads - 1) / kRotBwdHeads), 2LL * device_sm_count());
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa_rotary(const fa_rotary_params* p, void* stream) {
+  if (int rc = rot_check(p)) return rc;
+  prof_reset();
+  FaRotParams k;
+  rot_fill(p, p->Hq, p->Hkv, 0, k);
+  const int es = esize(p->dtype);
+  const fa_tensor* from[2] = {&p->q, &p->k};
+  const fa_tensor* to[2] = {&p->q_out, &p->k_out};
+  for (int i = 0; i < 2; ++i) {
+    if (k.heads[i] > 0 && k.tokens > 0 && (!from[i]->ptr || !to[i]->ptr)) return fail(FA_EINVAL, "a tensor is null");
+    k.x[i] = rot_tensor(*from[i], es);
+    k.y[i] = rot_tensor(*to[i], es);
+  }
+  return rot_launch(k, p->dtype, stream);
+}
+
+size_t fa_rotary_bwd_workspace_bytes(const fa_rotary_params* p) {
+  if (!p || !(p->q_weight || p->k_weight) || p->Hq < 0 || p->Hkv < 0 || p->D <= 0) return 0;
+  return (size_t)(rot_bwd_parts(p, p->Hq) + rot_bwd_parts(p, p->Hkv)) * p->D * sizeof(float);
+}
+
+int fa_rotary_bwd(const fa_rotary_params* p, const fa_tensor* dq_out, const fa_tensor* dk_out, const fa_tensor* dq, const fa_tensor* dk,
+                  void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = rot_check(p)) return rc;
+  if (!dq_out || !dk_out || !dq || !dk) return fail(FA_EINVAL, "a gradient is null");
+  if ((dq_weight && !p->q_weight) || (dk_weight && !p->k_weight)) return fail(FA_EINVAL, "a gradient of weights that are not there");
+  prof_reset();
+  FaRotParams k;
+  rot_fill(p, p->Hq, p->Hkv, 0, k);
+  const int es = esize(p->dtype);
+  const fa_tensor *from[2] = {dq_out, dk_out}, *to[2] = {dq, dk}, *in[2] = {&p->q, &p->k};
+  void* dw[2] = {dq_weight, dk_weight};
+  for (int i = 0; i < 2; ++i) {
+    if (k.heads[i] > 0 && k.tokens > 0 && (!from[i]->ptr || !to[i]->ptr || (k.w[i] && !in[i]->ptr))) return fail(FA_EINVAL, "a tensor is null");
+    k.x[i] = rot_tensor(*from[i], es);
+    k.y[i] = rot_tensor(*to[i], es);
+    if (k.w[i]) k.in[i] = rot_tensor(*in[i], es);
+  }
+  k.sign = -1.f;
+  // (no norm: nothing but the rotation, which needs no inputs)
+  if (!k.w[0] && !k.w[1]) return rot_launch(k, p->dtype, stream);
+  const size_t need = fa_rotary_bwd_workspace_bytes(p);
+  if (!workspace || workspace_bytes < need) return fail(FA_EWORKSPACE, "rotary backward workspace too small");
+  if ((uintptr_t)workspace & 15) return fail(FA_EINVAL, "workspace must be 16-byte aligned");
+  FaRotDw sum;
+  memset(&sum, 0, sizeof sum);
+  sum.D = p->D;
+  float* part[2] = {(float*)workspace, (float*)workspace + rot_bwd_parts(p, p->Hq) * p->D};
+  for (int i = 0; i < 2; ++i) {
+    k.dw[i] = dw[i] ? part[i] : nullptr;
+    sum.part[i] = part[i];
+    sum.dw[i] = dw[i];
+  }
+  if (k.tokens > 0) {
+    int rc;
+    if (rot_by_pieces(k, p->dtype, &k.lane_shift)) {
+      const long long token_blocks = ((long long)k.tokens + (kRotThreads >> k.lane_shift) - 1) / (kRotThreads >> k.lane_shift);
+      const unsigned blocks = (unsigned)std::min<long long>(token_blocks, rot_bwd_blocks(p));
+      k.per_group = kRotBwdHeads;
+      for (int i = 0; i < 2; ++i) {
+        k.groups[i] = (k.heads[i] + kRotBwdHeads - 1) / kRotBwdHeads;
+        sum.parts[i] = (int)blocks * k.groups[i];
+      }
+      rc = rot_dispatch(p->dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        return launch_here("fa_rotary_bwd_kernel", k.interleaved ? fa_rotary_bwd_kernel<DT, true> : fa_rotary_bwd_kernel<DT, false>,
+                           dim3(blocks, (unsigned)(k.groups[0] + k.groups[1])), dim3(kRotThreads), stream, k);
+      });
+    } else {
+      const long long rows = (long long)k.tokens * std::max(k.heads[0], k.heads[1]);
+      const unsigned blocks = (unsigned)std::min<long long>((rows + kRotThreads / 32 - 1) / (kRotThreads / 32), 2LL * device_sm_count());
+      sum.parts[0] = sum.parts[1] = (int)blocks;
+      rc = rot_dispatch(p->dtype, [&](auto dt) {
+        return launch_here("fa_rotary_any_kernel", fa_rotary_any_kernel<decltype(dt)::value, true>, dim3(blocks, 2), dim3(kRotThreads), stream, k);
+      });
+    }
+    if (rc) return rc;
+  }
+  if (!dw[0] && !dw[1]) return FA_OK;
+  return rot_dispatch(p->weight_dtype, [&](auto dt) {
+    return launch_here("fa_rotary_dw_kernel", fa_rotary_dw_kernel<decltype(dt)::value>, dim3((unsigned)((p->D + 31) / 32), 2), dim3(1024), stream, sum);
+  });
+}
+
+int fa_rotary_append(const fa_rotary_params* p, void* stream) {
+  if (int rc = rot_check(p)) return rc;
+  if (p->Hkv > 0 && (p->Dv <= 0 || p->Dv > 256)) return fail(FA_EUNSUPPORTED, "head dims from 1 to 256");
+  if (p->page_size <= 0 || p->num_pages < 0) return fail(FA_EINVAL, "page_size must be positive, num_pages not negative");
+  if (p->num_pages > (1ll << 62) / p->page_size) return fail(FA_EINVAL, "too many pages");
+  prof_reset();
+  FaRotParams k;
+  rot_fill(p, p->q.ptr ? p->Hq : 0, p->Hkv, p->Hkv, k);
+  if (k.tokens == 0) return FA_OK;
+  if (k.heads[1] > 0 && (!p->k.ptr || !p->v.ptr || !p->slots)) return fail(FA_EINVAL, "a tensor is null");
+  if (k.heads[1] > 0 && p->num_pages > 0 && (!p->k_pages.ptr || !p->v_pages.ptr)) return fail(FA_EINVAL, "a tensor is null");
+  if (k.heads[0] > 0 && !p->q_out.ptr) return fail(FA_EINVAL, "a tensor is null");
+  const int es = esize(p->dtype);
+  const fa_tensor *from[3] = {&p->q, &p->k, &p->v}, *to[3] = {&p->q_out, &p->k_pages, &p->v_pages};
+  for (int i = 0; i < 3; ++i) {
+    k.x[i] = rot_tensor(*from[i], es);
+    k.y[i] = rot_tensor(*to[i], es);
+  }
+  k.slots = (const long long*)p->slots;
+  k.slot_sb = p->slot_stride_b; k.slot_ss = p->slot_stride_s;
+  k.page_size = p->page_size;
+  k.num_slots = p->num_pages * p->page_size;
+  return rot_launch(k, p->dtype, stream);
+}
+
+}  // extern "C"

@@ -257,6 +257,91 @@ int fa_snapshot_holds(const void* const* src, const size_t* bytes, int n, const 
 int fa_mask_bits(fa_module* m, int B, int H, int Q_LEN, int KV_LEN, int b_offset, int h_offset, uint32_t* bits,
                  void* stream);
 
+/* ---- Rotary positions, norms of queries and keys (no counterpart in the reference) ------------
+ *
+ *   y = x * rsqrt(mean(x^2) + eps) * weight          where a weight [D] is given, per row of a head
+ *   (a, b) -> (a cos - b sin, b cos + a sin)         for the pairs of the first rotary_dim values of y
+ *
+ * in one pass, in fp32, rounded once.  Pairs are i and i + rotary_dim / 2, or neighbours (interleaved).  Any strides with a
+ * contiguous head dimension are taken; 16-byte aligned ones whose head and rotary dims are multiples of 32 bytes are fast. */
+typedef struct fa_rotary_params {
+  int32_t dtype;        /* of all tensors */
+  int32_t weight_dtype; /* of the norm weights and their gradients: dtype or FA_F32 */
+  int32_t B, S, Hq, Hkv, D, Dv; /* Dv: fa_rotary_append only.  B * S may be 0 */
+  int32_t rotary_dim;   /* even, at most D; 0: no rotation */
+  int32_t interleaved;
+  float eps;
+  fa_tensor q, k;          /* [B, H, S, D] by strides */
+  fa_tensor q_out, k_out;  /* fa_rotary (q_out: fa_rotary_append too) */
+  const float* table;      /* [table_length, table_stride]: a row holds cos of the rotary_dim / 2 pairs, then sin */
+  int64_t table_length, table_stride;
+  const void* positions;   /* row of the table for each token, position_bits wide, element strides; NULL: 0 .. S - 1 */
+  int32_t position_bits;
+  int64_t position_stride_b, position_stride_s;
+  const void *q_weight, *k_weight; /* [D] or NULL: no norm */
+  /* fa_rotary_append */
+  fa_tensor v;
+  fa_tensor k_pages, v_pages; /* stride_b: of a page, stride_h: of a kv head, stride_s: of a token in a page */
+  int64_t num_pages;
+  int32_t page_size;
+  const int64_t* slots;       /* page * page_size + token of the page, for each token; below 0: k and v go nowhere */
+  int64_t slot_stride_b, slot_stride_s;
+  int32_t* status; /* optional status word: 8 = a position beyond the table (its pairs become 0), 16 = a slot beyond the pages (not written) */
+} fa_rotary_params;
+
+int fa_rotary(const fa_rotary_params* p, void* stream);
+
+/* Gradients: dq, dk from those of the outputs (q and k of p are read where weights are given), and of the weights where
+ * dq_weight / dk_weight are not NULL (sums in a fixed order).  The workspace is 0 without weights. */
+size_t fa_rotary_bwd_workspace_bytes(const fa_rotary_params* p);
+int fa_rotary_bwd(const fa_rotary_params* p, const fa_tensor* dq_out, const fa_tensor* dk_out, const fa_tensor* dq,
+                  const fa_tensor* dk, void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* For new tokens of a key / value cache in pages: q goes to q_out (q.ptr NULL: there are no queries), k to the slots of k_pages, both
+ * as above, and v as it is to those of v_pages.  One launch. */
+int fa_rotary_append(const fa_rotary_params* p, void* stream);
+
+/* ---- Pages of a key / value cache (no counterpart in the reference) -----------------------------
+ *
+ * Request b has lengths[b] tokens in its pages and gets new_tokens[b] more (below 0 counts as 0).  block_table
+ * [B, block_table_stride] lists its pages; the entries of the pages that it needs in addition are filled in, from
+ * free_pages[taken] on, request after request (-1 where the list has come to its end).  The new tokens are numbered through, request
+ * after request; positions, slots and requests [num_tokens] say for each its place in its request, its place in the pages
+ * (-1: the list or the table has no room) and its request, starts [B + 1] where the tokens of a request begin.  Beyond the last new
+ * token positions are 0, slots and requests -1.  out_taken: how many of the list are taken then (more than there are, where
+ * it was too short).  The call may be repeated: it changes block_table only, to the same values.  One launch. */
+int fa_page_step(const int32_t* lengths, const int32_t* new_tokens, int B, int32_t* block_table, int64_t block_table_stride, int table_width,
+                 const int32_t* free_pages, int64_t num_free, const int32_t* taken /* NULL: 0 */, int page_size, int64_t num_tokens,
+                 int32_t* out_lengths, int32_t* positions, int64_t* slots, int32_t* requests, int32_t* starts, int32_t* out_taken,
+                 void* stream);
+
+/* Attention of the Sq newest tokens of each request over its pages.  Query i is token lengths[b] - Sq + i, sees the keys up to
+ * itself, at most `window` behind it, and those that mask_mod keeps; that token's number is the q index of the mods.  A row that sees
+ * nothing is 0 with an lse of -inf.  The work is split over the requests' lengths on the device: the launches depend on none of them. */
+typedef struct fa_paged_params {
+  int32_t dtype;
+  int32_t B, Hq, Hkv, Sq, D, Dv;
+  float scale;
+  int32_t b_offset, h_offset;
+  fa_tensor q, o;
+  fa_tensor k_pages, v_pages; /* stride_b: of a page, stride_h: of a kv head, stride_s: of a token in a page */
+  int64_t num_pages;
+  int32_t page_size;
+  const int32_t* block_table; /* [B, block_table_stride]; entries behind a request's length are not read */
+  int64_t block_table_stride;
+  int32_t table_width;
+  const int32_t* lengths;     /* [B], the new tokens included */
+  int32_t window;             /* below 0: no window */
+  float* lse;                 /* [B,Hq,Sq] natural-log logsumexp or NULL */
+  int32_t flags;              /* FA_FLAG_GENERAL_KERNELS: K and V in 16-byte pieces instead of by TMA */
+  int32_t* status;            /* optional status word: 4 = a block table entry that is no page, or a length that is
+                                 negative or beyond the table (such keys are left out) */
+} fa_paged_params;
+size_t fa_paged_workspace_bytes(const fa_paged_params* p);
+int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t workspace_bytes, void* stream);
+/* Compiles (or fetches from the cache) the kernel that a call of these sizes, type, page_size and flags runs.  Needs no GPU. */
+int fa_paged_prepare(fa_module* m, const fa_paged_params* p);
+
 #ifdef __cplusplus
 }
 #endif
