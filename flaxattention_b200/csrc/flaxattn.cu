@@ -389,12 +389,16 @@ int launch(Kernel* k, dim3 grid, dim3 block, void* params, void* stream, int clu
 }
 // the same for the kernels of this file
 template <class... P, class... A>
-int launch_here(const char* name, void (*fn)(P...), dim3 grid, dim3 block, void* stream, A... args) {
+int launch_here_smem(const char* name, void (*fn)(P...), dim3 grid, dim3 block, int smem, void* stream, A... args) {
   ProfScope prof(name, stream);
   cudaLaunchAttribute attr;
-  const cudaLaunchConfig_t cfg = launch_config(grid, block, 0, stream, &attr);
+  const cudaLaunchConfig_t cfg = launch_config(grid, block, smem, stream, &attr);
   FA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fn, P(args)...));
   return FA_OK;
+}
+template <class... P, class... A>
+int launch_here(const char* name, void (*fn)(P...), dim3 grid, dim3 block, void* stream, A... args) {
+  return launch_here_smem(name, fn, grid, block, 0, stream, args...);
 }
 
 // ---- configuration ---------------------------------------------------------------------

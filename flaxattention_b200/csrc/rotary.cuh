@@ -13,6 +13,8 @@
 namespace {
 
 constexpr int kRotThreads = 256;
+constexpr int kRotStages = 3;  // rows of a thread's ring in the backward
+constexpr int kRotHeads = 16;  // most heads that a thread goes through
 
 struct FaRotTensor {
   char* ptr;
@@ -52,35 +54,69 @@ __device__ __forceinline__ void rot_put(void* p, long long i, float v) {
 }
 template <int DT>
 constexpr int kRotVec = DT == FA_F32 ? 4 : 8;  // values of 16 bytes
+// Two fp32 values in a register pair: products and sums of both in one instruction
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void f2_get(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 swapped(F2 a) {
+  float x, y;
+  f2_get(a, x, y);
+  return f2(y, x);
+}
+__device__ __forceinline__ float both(F2 a) {
+  float x, y;
+  f2_get(a, x, y);
+  return x + y;
+}
 template <int DT>
-__device__ __forceinline__ void rot_unpack(const uint4& u, float (&f)[kRotVec<DT>]) {
+constexpr int kRotPairs = kRotVec<DT> / 2;
+template <int DT>
+__device__ __forceinline__ void rot_unpack(const uint4& u, F2 (&f)[kRotPairs<DT>]) {
   const unsigned v[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (DT == FA_F32) {
-      f[i] = __uint_as_float(v[i]);
+      if (i & 1) f[i / 2] = f2(__uint_as_float(v[i - 1]), __uint_as_float(v[i]));
     } else if constexpr (DT == FA_F16) {
       const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
+      f[i] = f2(t.x, t.y);
     } else {
-      f[2 * i] = __uint_as_float(v[i] << 16);
-      f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+      f[i] = f2(__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xffff0000u));
     }
   }
 }
 template <int DT>
-__device__ __forceinline__ uint4 rot_pack(const float (&f)[kRotVec<DT>]) {
+__device__ __forceinline__ uint4 rot_pack(const F2 (&f)[kRotPairs<DT>]) {
   unsigned v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    float x, y;
     if constexpr (DT == FA_F32) {
-      v[i] = __float_as_uint(f[i]);
+      f2_get(f[i / 2], x, y);
+      v[i] = __float_as_uint(i & 1 ? y : x);
     } else if constexpr (DT == FA_F16) {
-      const __half2 t = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      f2_get(f[i], x, y);
+      const __half2 t = __floats2half2_rn(x, y);
       v[i] = *reinterpret_cast<const unsigned*>(&t);
     } else {
-      const __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      f2_get(f[i], x, y);
+      const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
       v[i] = *reinterpret_cast<const unsigned*>(&t);
     }
   }
@@ -141,8 +177,9 @@ struct RotPlace {
   }
 };
 template <class T>
-__device__ __forceinline__ T rot_sum(T v, int lane_shift) {
-  for (int off = 1 << lane_shift >> 1; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+__device__ __forceinline__ T rot_sum(T v) {  // over a warp
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
   return v;
 }
 
@@ -161,24 +198,61 @@ __device__ __forceinline__ void rot_angles(const FaRotParams& P, long long pos, 
     s[i] = P.sign * b.x; s[i + 1] = P.sign * b.y; s[i + 2] = P.sign * b.z; s[i + 3] = P.sign * b.w;
   }
 }
+// The rotation of a lane's two pieces a and b as a' = a p + (b or a with its neighbours exchanged) q, and b' with its own p and q: the
+// factors, with the weights of the values that they multiply (1: none).  A lane whose values stay has the weights and 0.
+template <int V>
+struct RotFactors {
+  F2 pa[V / 2], qa[V / 2], pb[V / 2], qb[V / 2];
+};
 template <int V, bool INTERLEAVED>
-__device__ __forceinline__ void rot_turn(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V]) {
+__device__ __forceinline__ void rot_factors(RotFactors<V>& f, bool turns, const float (&c)[V], const float (&s)[V], const float (&wa)[V], const float (&wb)[V]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float& u = INTERLEAVED ? (2 * i < V ? a[(2 * i) % V] : b[(2 * i) % V]) : a[i];
-    float& v = INTERLEAVED ? (2 * i < V ? a[(2 * i + 1) % V] : b[(2 * i + 1) % V]) : b[i];
-    const float x = u, y = v;
-    u = x * c[i] - y * s[i];
-    v = y * c[i] + x * s[i];
+  for (int i = 0; i < V / 2; ++i) {
+    const int x = 2 * i, y = 2 * i + 1;
+    if (INTERLEAVED) {  // pairs i of piece a, V / 2 + i of piece b
+      const float ca = turns ? c[i] : 1.f, cb = turns ? c[V / 2 + i] : 1.f, sa = turns ? s[i] : 0.f, sb = turns ? s[V / 2 + i] : 0.f;
+      f.pa[i] = f2(wa[x] * ca, wa[y] * ca);
+      f.qa[i] = f2(-wa[y] * sa, wa[x] * sa);
+      f.pb[i] = f2(wb[x] * cb, wb[y] * cb);
+      f.qb[i] = f2(-wb[y] * sb, wb[x] * sb);
+    } else {
+      const float cx = turns ? c[x] : 1.f, cy = turns ? c[y] : 1.f, sx = turns ? s[x] : 0.f, sy = turns ? s[y] : 0.f;
+      f.pa[i] = f2(wa[x] * cx, wa[y] * cy);
+      f.qa[i] = f2(-wb[x] * sx, -wb[y] * sy);
+      f.pb[i] = f2(wb[x] * cx, wb[y] * cy);
+      f.qb[i] = f2(wa[x] * sx, wa[y] * sy);
+    }
+  }
+}
+template <int V, bool INTERLEAVED>
+__device__ __forceinline__ void rot_turn(F2 (&a)[V / 2], F2 (&b)[V / 2], const RotFactors<V>& f) {
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    const F2 u = a[i], v = b[i];
+    a[i] = fma(INTERLEAVED ? swapped(u) : v, f.qa[i], u * f.pa[i]);
+    b[i] = fma(INTERLEAVED ? swapped(v) : u, f.qb[i], v * f.pb[i]);
+  }
+}
+// the sums of N values over the lanes of a row each
+template <int N>
+__device__ __forceinline__ void rot_sums(float (&v)[N], int lane_shift) {
+  for (int off = 1 << lane_shift >> 1; off > 0; off >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
   }
 }
 
-// Two 16-byte pieces of a row per lane: the two that hold its pairs.  A thread keeps the angles of its token in
-// registers for all heads of its group, and the lanes of a warp beside each other are tokens beside each other.
+// Two 16-byte pieces of a row per lane: the two that hold its pairs.  A thread keeps the angles of its token, times the weights, in
+// registers for all heads of its group, and the lanes of a warp beside each other are tokens beside each other.  Four rows are computed
+// while the next four are on their way.
+//
+// B4 H32/8 S4096 D128 bf16 with norms: 55 us for 335 MB, 6.1 TB/s.  In single values, with an angle and a weight multiplied per value and each group
+// of rows asked for when the one before was written, it was bound by the instructions' issue: 79 us; 65 with two values per instruction
+// and the weights in the angles.  Two rows at a time 61, more blocks per SM (fewer registers) 85 and more.
 template <int DT, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotThreads) fa_rotary_kernel(const __grid_constant__ FaRotParams P) {
+__global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_constant__ FaRotParams P) {
   grid_wait();
-  constexpr int V = kRotVec<DT>, U = 4;
+  constexpr int V = kRotVec<DT>, N = V / 2, U = 4;
   const RotPlace at(P);
   const bool live = at.token < P.tokens;
   const int b = live ? at.token / P.S : 0, s = live ? at.token - b * P.S : 0;
@@ -189,44 +263,77 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_kernel(const __grid_con
   const long long to = live ? rot_destination(P, kind, b, s) : -1;
   const bool have_a = live && to >= 0 && ca < chunks, have_b = live && to >= 0 && cb < chunks;
   const bool norm = kind < 2 && P.w[kind < 2 ? kind : 0] != nullptr;
-  float c[V], sn[V], wa[V], wb[V];
-  rot_angles<V>(P, turns && live ? rot_position(P, b, s) : -1, at.lane, turns, c, sn);
-  if (norm) {
-    rot_weights<DT>(P, kind, ca, ca < chunks, wa);
-    rot_weights<DT>(P, kind, cb, cb < chunks, wb);
-  }
+  // (the first rows are asked for before the angles, which come over the positions)
   const char* src = P.x[kind].ptr + b * P.x[kind].sb + s * P.x[kind].ss;
-  char* dst = P.y[kind].ptr + to;
-  for (int h = at.h0; h < at.h1; h += U) {
-    uint4 ra[U], rb[U];
+  uint4 na[U], nb[U];
+  const auto load = [&](int h) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const char* row = src + (h + u) * P.x[kind].sh;
       const bool in = h + u < at.h1;
-      ra[u] = in && have_a ? *(const uint4*)(row + ca * 16) : make_uint4(0, 0, 0, 0);
-      rb[u] = in && have_b ? *(const uint4*)(row + cb * 16) : make_uint4(0, 0, 0, 0);
+      na[u] = in && have_a ? *(const uint4*)(row + ca * 16) : make_uint4(0, 0, 0, 0);
+      nb[u] = in && have_b ? *(const uint4*)(row + cb * 16) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  load(at.h0);
+  RotFactors<V> f;
+  {
+    float c[V], sn[V], wa[V], wb[V];
+    rot_angles<V>(P, turns && live ? rot_position(P, b, s) : -1, at.lane, turns, c, sn);
+#pragma unroll
+    for (int i = 0; i < V; ++i) wa[i] = wb[i] = 1.f;
+    if (norm) {
+      rot_weights<DT>(P, kind, ca, ca < chunks, wa);
+      rot_weights<DT>(P, kind, cb, cb < chunks, wb);
+    }
+    rot_factors<V, INTERLEAVED>(f, turns, c, sn, wa, wb);
+  }
+  char* dst = P.y[kind].ptr + to;
+  const float per_value = 1.f / P.D;
+  for (int h = at.h0; h < at.h1; h += U) {
+    uint4 ra[U], rb[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ra[u] = na[u];
+      rb[u] = nb[u];
+    }
+    if (h + U < at.h1) load(h + U);  // (on their way while these are computed)
+    float ss[U];
+    if (norm) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        F2 x[N], y[N];
+        rot_unpack<DT>(ra[u], x);
+        rot_unpack<DT>(rb[u], y);
+        F2 sum = x[0] * x[0];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (i > 0) sum = fma(x[i], x[i], sum);
+          sum = fma(y[i], y[i], sum);
+        }
+        ss[u] = both(sum);
+      }
+      rot_sums(ss, P.lane_shift);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (h + u >= at.h1) break;
       if (norm || turns) {
-        float a[V], d[V];
-        rot_unpack<DT>(ra[u], a);
-        rot_unpack<DT>(rb[u], d);
+        F2 x[N], y[N];
+        rot_unpack<DT>(ra[u], x);
+        rot_unpack<DT>(rb[u], y);
         if (norm) {
-          float ss = 0.f;
+          const float r = rsqrtf(ss[u] * per_value + P.eps);
+          const F2 rr = f2(r, r);
 #pragma unroll
-          for (int i = 0; i < V; ++i) ss += a[i] * a[i] + d[i] * d[i];
-          const float r = rsqrtf(rot_sum(ss, P.lane_shift) / P.D + P.eps);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            a[i] *= r * wa[i];
-            d[i] *= r * wb[i];
+          for (int i = 0; i < N; ++i) {
+            x[i] = x[i] * rr;
+            y[i] = y[i] * rr;
           }
         }
-        if (turns) rot_turn<V, INTERLEAVED>(a, d, c, sn);
-        ra[u] = rot_pack<DT>(a);
-        rb[u] = rot_pack<DT>(d);
+        rot_turn<V, INTERLEAVED>(x, y, f);
+        ra[u] = rot_pack<DT>(x);
+        rb[u] = rot_pack<DT>(y);
       }
       char* row = dst + (h + u) * P.y[kind].sh;
       if (have_a) *(uint4*)(row + ca * 16) = ra[u];
@@ -235,12 +342,20 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_kernel(const __grid_con
   }
 }
 
+__device__ __forceinline__ void rot_copy16(void* shared, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(shared)), "l"(from) : "memory");
+}
+
 // The backward with norm weights: blocks go through the tokens in steps of the grid and keep the sums for dw in
 // registers; what a block has goes to one row of partial sums, which fa_rotary_dw_kernel adds up in order.
+//
+// B4 H32/8 S4096 D128 bf16: 82 us for the 503 MB that have to move, 6.1 TB/s.  What it took: two values per instruction
+// (fma.rn.f32x2), 157 us to 107, and rows on their way through shared memory instead of one row ahead in registers, which has
+// twice as many bytes in flight, 107 to 83.
 template <int DT, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotThreads) fa_rotary_bwd_kernel(const __grid_constant__ FaRotParams P) {
+__global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_bwd_kernel(const __grid_constant__ FaRotParams P) {
   grid_wait();
-  constexpr int V = kRotVec<DT>;
+  constexpr int V = kRotVec<DT>, N = V / 2;
   __shared__ float sums[kRotThreads / 32][256];
   const RotPlace at(P);
   const int kind = at.kind, chunks = P.D / V, pairs = P.R / (2 * V);
@@ -248,72 +363,125 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_bwd_kernel(const __grid
   const int ca = turns && !INTERLEAVED ? at.lane : turns ? 2 * at.lane : 2 * pairs + 2 * (at.lane - pairs);
   const int cb = turns && !INTERLEAVED ? at.lane + pairs : ca + 1;
   const bool norm = P.w[kind] != nullptr;
-  float wa[V], wb[V], da[V], db[V];
+  F2 wa[N], wb[N], da[N], db[N];
+  {
+    float x[V], y[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) da[i] = db[i] = 0.f;
-  if (norm) {
-    rot_weights<DT>(P, kind, ca, ca < chunks, wa);
-    rot_weights<DT>(P, kind, cb, cb < chunks, wb);
-  }
-  const int step = gridDim.x * (kRotThreads >> P.lane_shift);
-  // (every thread goes round as often as the first of its block: the shuffles are the warp's)
-  for (int t0 = blockIdx.x * (kRotThreads >> P.lane_shift); t0 < P.tokens; t0 += step) {
-    const int t = t0 + (threadIdx.x >> P.lane_shift);
-    const bool live = t < P.tokens, have_a = live && ca < chunks, have_b = live && cb < chunks;
-    const int b = live ? t / P.S : 0, s = live ? t - b * P.S : 0;
-    float c[V], sn[V];
-    rot_angles<V>(P, turns && live ? rot_position(P, b, s) : -1, at.lane, turns, c, sn);
-    const char* gs = P.x[kind].ptr + b * P.x[kind].sb + s * P.x[kind].ss;
-    const char* xs = norm ? P.in[kind].ptr + b * P.in[kind].sb + s * P.in[kind].ss : gs;
-    char* ds = P.y[kind].ptr + b * P.y[kind].sb + s * P.y[kind].ss;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 2
-    for (int h = at.h0; h < at.h1; ++h) {
-      const uint4 ga = have_a ? *(const uint4*)(gs + h * P.x[kind].sh + ca * 16) : zero;
-      const uint4 gb = have_b ? *(const uint4*)(gs + h * P.x[kind].sh + cb * 16) : zero;
-      float a[V], d[V];
-      rot_unpack<DT>(ga, a);
-      rot_unpack<DT>(gb, d);
-      if (turns) rot_turn<V, INTERLEAVED>(a, d, c, sn);
-      if (norm) {
-        const uint4 xa = have_a ? *(const uint4*)(xs + h * P.in[kind].sh + ca * 16) : zero;
-        const uint4 xb = have_b ? *(const uint4*)(xs + h * P.in[kind].sh + cb * 16) : zero;
-        float u[V], v[V], ss = 0.f, gx = 0.f;
-        rot_unpack<DT>(xa, u);
-        rot_unpack<DT>(xb, v);
+    for (int i = 0; i < V; ++i) x[i] = y[i] = 0.f;
+    if (norm) {
+      rot_weights<DT>(P, kind, ca, ca < chunks, x);
+      rot_weights<DT>(P, kind, cb, cb < chunks, y);
+    }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          ss += u[i] * u[i] + v[i] * v[i];
-          gx += a[i] * wa[i] * u[i] + d[i] * wb[i] * v[i];
-        }
-        const float r = rsqrtf(rot_sum(ss, P.lane_shift) / P.D + P.eps);
-        const float m = rot_sum(gx, P.lane_shift) * r / P.D;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float p = u[i] * r, q = v[i] * r;
-          da[i] += a[i] * p;
-          db[i] += d[i] * q;
-          a[i] = r * (a[i] * wa[i] - p * m);
-          d[i] = r * (d[i] * wb[i] - q * m);
-        }
-      }
-      if (have_a) *(uint4*)(ds + h * P.y[kind].sh + ca * 16) = rot_pack<DT>(a);
-      if (have_b) *(uint4*)(ds + h * P.y[kind].sh + cb * 16) = rot_pack<DT>(d);
+    for (int i = 0; i < N; ++i) {
+      wa[i] = f2(x[2 * i], x[2 * i + 1]);
+      wb[i] = f2(y[2 * i], y[2 * i + 1]);
+      da[i] = db[i] = f2(0.f, 0.f);
     }
   }
+  const float per_value = 1.f / P.D;
+  const int block_tokens = kRotThreads >> P.lane_shift, step = gridDim.x * block_tokens, heads = at.h1 - at.h0;
+  // Rows come through shared memory, kRotStages - 1 of them on their way: every thread has 16-byte places of its own for its pieces of dy
+  // and x (no barriers).  The rows of a thread are those of its heads of its first token, then of its next, ..; every thread goes round as
+  // often as the first of its block, since the shuffles are the warp's.
+  extern __shared__ uint4 ring[];  // [kRotStages][4][kRotThreads]
+  const int t_first = blockIdx.x * block_tokens, rounds = t_first < P.tokens ? (P.tokens - 1 - t_first) / step + 1 : 0, rows = rounds * heads;
+  int next = 0, next_h = at.h0, next_t = t_first + (threadIdx.x >> P.lane_shift);  // the row that is asked for next
+  const char *next_g = nullptr, *next_x = nullptr;
+  const auto ask = [&]() {
+    if (next < rows && next_t < P.tokens) {
+      if (next_h == at.h0) {
+        const int b = next_t / P.S, s = next_t - b * P.S;
+        next_g = P.x[kind].ptr + b * P.x[kind].sb + s * P.x[kind].ss + at.h0 * P.x[kind].sh;
+        if (norm) next_x = P.in[kind].ptr + b * P.in[kind].sb + s * P.in[kind].ss + at.h0 * P.in[kind].sh;
+      }
+      uint4* place = ring + (next % kRotStages) * 4 * kRotThreads + threadIdx.x;
+      if (ca < chunks) rot_copy16(place, next_g + ca * 16);
+      if (cb < chunks) rot_copy16(place + kRotThreads, next_g + cb * 16);
+      if (norm && ca < chunks) rot_copy16(place + 2 * kRotThreads, next_x + ca * 16);
+      if (norm && cb < chunks) rot_copy16(place + 3 * kRotThreads, next_x + cb * 16);
+      next_g += P.x[kind].sh;
+      if (norm) next_x += P.in[kind].sh;
+    }
+    ++next;
+    if (++next_h == at.h1) {
+      next_h = at.h0;
+      next_t += step;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kRotStages - 1; ++i) ask();
+  int row = 0;
+  for (int round = 0; round < rounds; ++round) {
+    const int t = t_first + round * step + (threadIdx.x >> P.lane_shift);
+    const bool live = t < P.tokens, have_a = live && ca < chunks, have_b = live && cb < chunks;
+    const int b = live ? t / P.S : 0, s = live ? t - b * P.S : 0;
+    RotFactors<V> f;
+    {
+      float c[V], sn[V], one[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) one[i] = 1.f;
+      rot_angles<V>(P, turns && live ? rot_position(P, b, s) : -1, at.lane, turns, c, sn);
+      rot_factors<V, INTERLEAVED>(f, turns, c, sn, one, one);
+    }
+    char* ds = P.y[kind].ptr + b * P.y[kind].sb + s * P.y[kind].ss + at.h0 * P.y[kind].sh;
+    for (int h = 0; h < heads; ++h, ++row) {
+      ask();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRotStages - 1) : "memory");
+      const uint4* place = ring + (row % kRotStages) * 4 * kRotThreads + threadIdx.x;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      F2 a[N], d[N], u[N], v[N];
+      rot_unpack<DT>(have_a ? place[0] : zero, a);
+      rot_unpack<DT>(have_b ? place[kRotThreads] : zero, d);
+      if (turns) rot_turn<V, INTERLEAVED>(a, d, f);
+      if (norm) {
+        rot_unpack<DT>(have_a ? place[2 * kRotThreads] : zero, u);
+        rot_unpack<DT>(have_b ? place[3 * kRotThreads] : zero, v);
+        F2 ss = u[0] * u[0], gx = f2(0.f, 0.f), tu[N], tv[N];  // g w
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (i > 0) ss = fma(u[i], u[i], ss);
+          ss = fma(v[i], v[i], ss);
+          tu[i] = a[i] * wa[i];
+          tv[i] = d[i] * wb[i];
+          gx = fma(tu[i], u[i], gx);
+          gx = fma(tv[i], v[i], gx);
+        }
+        float sum[2] = {both(ss), both(gx)};
+        rot_sums(sum, P.lane_shift);
+        const float r = rsqrtf(sum[0] * per_value + P.eps), m = -(sum[1] * r * per_value);
+        const F2 rr = f2(r, r), mm = f2(m, m);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          u[i] = u[i] * rr;  // x rsqrt(..)
+          v[i] = v[i] * rr;
+          da[i] = fma(a[i], u[i], da[i]);
+          db[i] = fma(d[i], v[i], db[i]);
+          a[i] = fma(u[i], mm, tu[i]) * rr;
+          d[i] = fma(v[i], mm, tv[i]) * rr;
+        }
+      }
+      if (have_a) *(uint4*)(ds + ca * 16) = rot_pack<DT>(a);
+      if (have_b) *(uint4*)(ds + cb * 16) = rot_pack<DT>(d);
+      ds += P.y[kind].sh;
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (P.dw[kind] == nullptr) return;
   // rows of a warp, then warps of the block
 #pragma unroll
-  for (int i = 0; i < V; ++i)
+  for (int i = 0; i < N; ++i) {
+    float v[4];
+    f2_get(da[i], v[0], v[1]);
+    f2_get(db[i], v[2], v[3]);
     for (int off = 1 << P.lane_shift; off < 32; off <<= 1) {
-      da[i] += __shfl_xor_sync(0xffffffffu, da[i], off);
-      db[i] += __shfl_xor_sync(0xffffffffu, db[i], off);
-    }
-  if ((threadIdx.x & 31) == at.lane) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (ca < chunks) sums[threadIdx.x >> 5][ca * V + i] = da[i];
-      if (cb < chunks) sums[threadIdx.x >> 5][cb * V + i] = db[i];
+      for (int k = 0; k < 4; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+    }
+    if ((threadIdx.x & 31) == at.lane) {
+      if (ca < chunks) *(float2*)&sums[threadIdx.x >> 5][ca * V + 2 * i] = make_float2(v[0], v[1]);
+      if (cb < chunks) *(float2*)&sums[threadIdx.x >> 5][cb * V + 2 * i] = make_float2(v[2], v[3]);
     }
   }
   __syncthreads();
@@ -358,7 +526,7 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid
         const Real v = rot_get<DT>(in, i);
         ss += v * v;
       }
-      ss = rot_sum(ss, 5) / D + P.eps;
+      ss = rot_sum(ss) / D + P.eps;
       if constexpr (BACK) r = rsqrt(ss);
       else r = rsqrtf(ss);
     }
@@ -380,7 +548,7 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid
         m += (Real)(a * c - d * sn) * weight(i) * rot_get<DT>(in, i);
         if (j >= 0) m += (Real)(d * c + a * sn) * weight(j) * rot_get<DT>(in, j);
       }
-      m = rot_sum(m, 5) * r / D;
+      m = rot_sum(m) * r / D;
     }
     for (int k = lane; k < units; k += 32) {
       int i, j;
@@ -412,7 +580,8 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid
   }
 }
 
-// dw from the partial sums of the blocks: 32 columns per block, 32 rows of threads, always in the same order
+// dw from the partial sums of the blocks: 8 columns per block, 128 rows of threads, always in the same order.  (32 columns and 32 rows, 8 blocks
+// at D 128: 6.0 us for 472 + 118 parts.)
 struct FaRotDw {
   const float* part[2];
   void* dw[2];
@@ -422,21 +591,23 @@ struct FaRotDw {
 template <int DT>
 __global__ void __launch_bounds__(1024) fa_rotary_dw_kernel(const __grid_constant__ FaRotDw P) {
   grid_wait();
-  __shared__ float sums[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5, kind = blockIdx.y;
+  __shared__ float sums[32][8];
+  const int col = blockIdx.x * 8 + (threadIdx.x & 7), slice = threadIdx.x >> 3, kind = blockIdx.y;
   if (P.dw[kind] == nullptr) return;
   float v = 0.f;
   if (col < P.D) {
-#pragma unroll 8
-    for (int i = slice; i < P.parts[kind]; i += 32) v += P.part[kind][(long long)i * P.D + col];
+#pragma unroll 4
+    for (int i = slice; i < P.parts[kind]; i += 128) v += P.part[kind][(long long)i * P.D + col];
   }
-  sums[slice][threadIdx.x & 31] = v;
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  v += __shfl_xor_sync(0xffffffffu, v, 16);
+  if ((threadIdx.x & 31) < 8) sums[threadIdx.x >> 5][threadIdx.x & 7] = v;
   __syncthreads();
-  v = sums[threadIdx.x & 31][slice];
+  if (threadIdx.x >= 8 || col >= P.D) return;
+  v = 0.f;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  const int mine = blockIdx.x * 32 + slice;
-  if ((threadIdx.x & 31) == 0 && mine < P.D) rot_put<DT>(P.dw[kind], mine, v);
+  for (int i = 0; i < 32; ++i) v += sums[i][threadIdx.x];
+  rot_put<DT>(P.dw[kind], col, v);
 }
 
 // ---- host --------------------------------------------------------------------------------
@@ -487,10 +658,10 @@ bool rot_by_pieces(const FaRotParams& k, int dtype, int* lane_shift) {
   *lane_shift = shift;
   return shift <= 5;
 }
-// Heads that a thread goes through.  Up to 8, so that the angles are read seldom; fewer while the grid would leave SMs
-// with less than four blocks.
+// Heads that a thread goes through.  Up to 16, so that the angles are read seldom (B4 H32/8 S4096 D128 bf16 with norms, us, 4 / 8 / 16 heads: forward
+// 68 / 56 / 55; 16384 tokens appended 81 / 72 / 70); fewer while the grid would leave SMs with less than four blocks.
 void rot_groups(FaRotParams& k, long long token_blocks) {
-  int per = 8;
+  int per = kRotHeads;
   const auto blocks = [&](int n) {
     long long g = 0;
     for (int i = 0; i < 3; ++i) g += (k.heads[i] + n - 1) / n;
@@ -506,6 +677,21 @@ int rot_dispatch(int dtype, F&& f) {
   if (dtype == FA_F16) return f(std::integral_constant<int, FA_F16>{});
   if (dtype == FA_BF16) return f(std::integral_constant<int, FA_BF16>{});
   return f(std::integral_constant<int, FA_F32>{});
+}
+
+// Leave for more than 48 KB of dynamic shared memory, asked for once per kernel and device
+int allow_smem(const void* fn, int smem) {
+  static std::mutex mu;
+  static std::map<const void*, unsigned long long> known;
+  int dev = 0;
+  FA_CUDA_CHECK(cudaGetDevice(&dev));
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  std::lock_guard<std::mutex> lk(mu);
+  unsigned long long& have = known[fn];
+  if (bit != 0 && (have & bit)) return FA_OK;
+  FA_CUDA_CHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  have |= bit;
+  return FA_OK;
 }
 
 // x -> y of the tensors that `k` describes
@@ -529,12 +715,16 @@ int rot_launch(FaRotParams& k, int dtype, void* stream) {
   });
 }
 
-// blocks along the tokens of the backward with norm weights: about four per SM in all
-int rot_bwd_blocks(const fa_rotary_params* p) { return std::max(1, 4 * device_sm_count() / std::max(1, (p->Hq + 3) / 4 + (p->Hkv + 3) / 4)); }
-constexpr int kRotBwdHeads = 4;  // heads of a group there
-long long rot_bwd_parts(const fa_rotary_params* p, int heads) {
-  return std::max<long long>((long long)rot_bwd_blocks(p) * ((heads + kRotBwdHeads - 1) / kRotBwdHeads), 2LL * device_sm_count());
+#ifndef ROT_BH
+#define ROT_BH 8
+#endif
+constexpr int kRotBwdHeads = ROT_BH;  // heads of a group there
+// Blocks along the tokens of the backward with norm weights: about four per SM in all, two of which it holds at once.
+unsigned rot_bwd_blocks(const FaRotParams& k, long long token_blocks) {
+  return (unsigned)std::min<long long>(token_blocks, std::max(1, 4 * device_sm_count() / (k.groups[0] + k.groups[1])));
 }
+// no more partial sums than that of a tensor, whichever kernel runs
+long long rot_bwd_parts(int heads) { return 4LL * device_sm_count() + heads; }
 
 }  // namespace
 
@@ -558,7 +748,7 @@ int fa_rotary(const fa_rotary_params* p, void* stream) {
 
 size_t fa_rotary_bwd_workspace_bytes(const fa_rotary_params* p) {
   if (!p || !(p->q_weight || p->k_weight) || p->Hq < 0 || p->Hkv < 0 || p->D <= 0) return 0;
-  return (size_t)(rot_bwd_parts(p, p->Hq) + rot_bwd_parts(p, p->Hkv)) * p->D * sizeof(float);
+  return (size_t)(rot_bwd_parts(p->Hq) + rot_bwd_parts(p->Hkv)) * p->D * sizeof(float);
 }
 
 int fa_rotary_bwd(const fa_rotary_params* p, const fa_tensor* dq_out, const fa_tensor* dk_out, const fa_tensor* dq, const fa_tensor* dk,
@@ -587,26 +777,25 @@ int fa_rotary_bwd(const fa_rotary_params* p, const fa_tensor* dq_out, const fa_t
   FaRotDw sum;
   memset(&sum, 0, sizeof sum);
   sum.D = p->D;
-  float* part[2] = {(float*)workspace, (float*)workspace + rot_bwd_parts(p, p->Hq) * p->D};
+  float* part[2] = {(float*)workspace, (float*)workspace + rot_bwd_parts(p->Hq) * p->D};
   for (int i = 0; i < 2; ++i) {
     k.dw[i] = dw[i] ? part[i] : nullptr;
     sum.part[i] = part[i];
     sum.dw[i] = dw[i];
   }
-  if (k.tokens > 0) {
+  if (k.tokens > 0 && k.heads[0] + k.heads[1] > 0) {
     int rc;
     if (rot_by_pieces(k, p->dtype, &k.lane_shift)) {
       const long long token_blocks = ((long long)k.tokens + (kRotThreads >> k.lane_shift) - 1) / (kRotThreads >> k.lane_shift);
-      const unsigned blocks = (unsigned)std::min<long long>(token_blocks, rot_bwd_blocks(p));
-      k.per_group = kRotBwdHeads;
-      for (int i = 0; i < 2; ++i) {
-        k.groups[i] = (k.heads[i] + kRotBwdHeads - 1) / kRotBwdHeads;
-        sum.parts[i] = (int)blocks * k.groups[i];
-      }
+      rot_groups(k, token_blocks);
+      const unsigned blocks = rot_bwd_blocks(k, token_blocks);
+      for (int i = 0; i < 2; ++i) sum.parts[i] = (int)blocks * k.groups[i];
       rc = rot_dispatch(p->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        return launch_here("fa_rotary_bwd_kernel", k.interleaved ? fa_rotary_bwd_kernel<DT, true> : fa_rotary_bwd_kernel<DT, false>,
-                           dim3(blocks, (unsigned)(k.groups[0] + k.groups[1])), dim3(kRotThreads), stream, k);
+        const auto fn = k.interleaved ? fa_rotary_bwd_kernel<DT, true> : fa_rotary_bwd_kernel<DT, false>;
+        constexpr int smem = kRotStages * 4 * kRotThreads * 16;
+        if (int e = allow_smem((const void*)fn, smem)) return e;
+        return launch_here_smem("fa_rotary_bwd_kernel", fn, dim3(blocks, (unsigned)(k.groups[0] + k.groups[1])), dim3(kRotThreads), smem, stream, k);
       });
     } else {
       const long long rows = (long long)k.tokens * std::max(k.heads[0], k.heads[1]);
@@ -620,7 +809,7 @@ int fa_rotary_bwd(const fa_rotary_params* p, const fa_tensor* dq_out, const fa_t
   }
   if (!dw[0] && !dw[1]) return FA_OK;
   return rot_dispatch(p->weight_dtype, [&](auto dt) {
-    return launch_here("fa_rotary_dw_kernel", fa_rotary_dw_kernel<decltype(dt)::value>, dim3((unsigned)((p->D + 31) / 32), 2), dim3(1024), stream, sum);
+    return launch_here("fa_rotary_dw_kernel", fa_rotary_dw_kernel<decltype(dt)::value>, dim3((unsigned)((p->D + 7) / 8), 2), dim3(1024), stream, sum);
   });
 }
 
