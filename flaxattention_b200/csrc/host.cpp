@@ -1107,9 +1107,10 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.o = by_strides(out, bshd);
       p.lse = return_lse ? lse.mutable_data_ptr<float>() : nullptr;
       const size_t bytes = fa_paged_workspace_bytes(&p);
-      const at::Tensor ws = empty({(int64_t)std::max<size_t>(bytes, 16)}, at::kByte, q.device());
+      at::Tensor ws;
+      if (bytes > 0) ws = empty({(int64_t)bytes}, at::kByte, q.device());
       BuffersLock lock(module, *buffers);
-      const int rc = lock.rc != FA_OK ? lock.rc : fa_paged(module, &p, ws.mutable_data_ptr(), bytes, (void*)c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+      const int rc = lock.rc != FA_OK ? lock.rc : fa_paged(module, &p, bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, (void*)c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
       if (rc != FA_OK) raise(rc);
     }
   }

@@ -90,6 +90,7 @@ struct FaPagedParams {
   int* status;
   int B, Hq, Hkv, Sq;
   int num_pages, page_size, max_len;  // max_len: tokens that the table has room for
+  int page_shift;                     // log2 of page_size, or -1
   int row_tiles, workers, min_tiles;  // row tiles of a request; CTAs, and the fewest tiles that one gets
   int window;                         // keys more than this far behind a query are not seen (-1: all are)
   int b_off, h_off;

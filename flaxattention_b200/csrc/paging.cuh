@@ -1,5 +1,11 @@
 // Pages of a key / value cache: places for the new tokens of a batch of requests (fa_page_step) and attention over
 // the pages (fa_paged; its kernel is kernels/fa_paged.cuh).  Part of flaxattn.cu.
+#ifndef PAGED_SHORT_TILES
+#define PAGED_SHORT_TILES 32
+#endif
+#ifndef PAGED_SHORT_SEGMENTS
+#define PAGED_SHORT_SEGMENTS 2
+#endif
 namespace {
 
 // ---- block tables, slots and positions of new tokens --------------------------------------
@@ -210,27 +216,51 @@ struct FaPagedLaunchHost {
   FaTensorMapHost tk, tv;
 };
 struct PagedCfg {
-  int RG, WN, stages, smem, per_sm, box;
+  int RG, WN, stages, smem, per_sm, box, few, fr, nw;
   bool tma;
 };
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
 
-// Tiles, buffers and CTAs per SM (the map of fa_paged.cuh).  Rows: one warp takes 16.  Registers allow eight warps per SM at 255
-// each; the buffers are as many as fill the shared memory of that many CTAs, two at least.
+// Warps of a CTA that has a segment for itself, or 0: segments are cut.  Where the table has room for few tiles, and where all segments are
+// resident at once.
+int paged_short_warps(const fa_paged_params* p, const PagedCfg& c) {
+  const long long segments = (long long)p->B * p->Hkv;
+  long long keys = (long long)p->table_width * p->page_size;
+  if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + p->Sq + c.WN);
+  const long long tiles = (keys + c.WN - 1) / c.WN;
+  if (c.RG != 1 || tiles > PAGED_SHORT_TILES || segments > PAGED_SHORT_SEGMENTS * (long long)device_sm_count()) return 0;
+  return tiles <= 8 ? 4 : 8;
+}
+
+// Tiles, buffers and CTAs per SM (the map of fa_paged.cuh).
+//   * Rows: a warp takes 16, of 16-bit types up to 8 in the way made for few; fp32 rounds up to a power of two.
+//   * Keys of a tile: 32; fp32 fewer for wide heads, so that a tile of K and V stays at 16 KB and an SM has room for as many of them.
+//   * Registers allow eight warps per SM at 255 each.  The buffers are as many as fill the shared memory of that many CTAs, two at least.
+//   * Tables with room for few tiles: a CTA per segment (nw warps, two buffers each).
 void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   const long long rows = (long long)(p->Hq / p->Hkv) * p->Sq;
   const bool f32 = p->dtype == FA_F32;
   const int es = esize(p->dtype);
   c.RG = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  c.WN = f32 && p->D > 64 ? 16 : 32;
+  c.WN = !f32 || p->D <= 64 ? 32 : p->D <= 128 ? 16 : 8;
+  c.few = !f32 && rows <= 8;
+  c.fr = 0;
+  if (f32)
+    for (c.fr = 1; c.fr < std::min<long long>(rows, 16);) c.fr *= 2;
   c.box = gcd(p->page_size, c.WN);
   c.tma = !f32 && p->D % 64 == 0 && p->Dv % 64 == 0 && c.box >= 8 && p->num_pages > 0 && !(p->flags & FA_FLAG_GENERAL_KERNELS);
   if (!c.tma) c.box = 1;
   const int stage = c.tma ? c.WN * (p->D + p->Dv) * es : c.WN * (pitch(p->D, es) + pitch(p->Dv, es));
-  const int fixed = f32 ? c.RG * 16 * (pitch(p->D, 4) + pitch(c.WN, 4)) : 0;
   const int most = 8 / c.RG;
-  c.stages = std::min(std::max((226 * 1024 / most - 2048 - fixed) / stage, 2), 4);
-  c.smem = c.stages * stage + fixed + (c.tma ? c.stages * 16 + 16 + 1024 : 0);
+  const auto fixed = [&](int warps) { return f32 ? (c.RG == 1 ? c.fr : c.RG * 16) * p->D * 4 + warps * c.fr * c.WN * 4 : 0; };
+  for (c.nw = paged_short_warps(p, c); c.nw > 0; c.nw /= 2) {
+    c.stages = 2;
+    c.smem = c.nw * 2 * stage + fixed(c.nw) + (c.tma ? c.nw * 2 * 16 + 16 + 1024 : 0);
+    c.per_sm = 1;
+    if (c.smem <= kMaxSmem) return;
+  }
+  c.stages = std::min(std::max((226 * 1024 / most - 2048 - fixed(c.RG)) / stage, 2), 4);
+  c.smem = c.stages * stage + fixed(c.RG) + (c.tma ? c.stages * 16 + 16 + 1024 : 0);
   c.per_sm = std::max(1, std::min(most, 227 * 1024 / (c.smem + 1024)));
 }
 int paged_row_tiles(const fa_paged_params* p, const PagedCfg& c) {
@@ -239,9 +269,9 @@ int paged_row_tiles(const fa_paged_params* p, const PagedCfg& c) {
 int paged_workers(const PagedCfg& c) { return c.per_sm * device_sm_count(); }
 
 int get_paged_kernel(fa_module* m, const fa_paged_params* p, const PagedCfg& c, Kernel** k) {
-  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.stages, 3}, {c.tma ? 1 : 0, 1}}), "fa_paged.cuh",
+  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.stages, 3}, {c.tma ? 1 : 0, 1}, {c.few, 1}, {c.fr, 5}, {c.nw, 4}}), "fa_paged.cuh",
                     [&] { return defs({{"FA_DTYPE", p->dtype}, {"FA_D", p->D}, {"FA_DV", p->Dv}, {"FA_RG", c.RG}, {"FA_WN", c.WN},
-                                       {"FA_STAGES", c.stages}, {"FA_TMA", c.tma ? 1 : 0}}); },
+                                       {"FA_STAGES", c.stages}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_NW", c.nw}}); },
                     "fa_paged_kernel", c.smem, k);
 }
 
@@ -301,10 +331,17 @@ int fa_page_step(const int32_t* lengths, const int32_t* new_tokens, int B, int32
 
 size_t fa_paged_workspace_bytes(const fa_paged_params* p) {
   if (!p || p->Hkv <= 0 || p->Hq <= 0 || p->Sq <= 0 || p->D <= 0 || p->Dv <= 0 || p->page_size <= 0 || p->B <= 0) return 0;
-  PagedCfg c;
-  pick_paged(p, c);
-  const size_t rows = 2 * (size_t)paged_workers(c) * c.RG * 16;
-  return paged_up(rows * p->Dv * 4) + paged_up(rows * 8) + paged_up(((size_t)p->B * paged_row_tiles(p, c) + 1) * 4);
+  size_t most = 0;
+  for (int flags : {p->flags, p->flags | FA_FLAG_GENERAL_KERNELS}) {  // (what runs where no tensor map takes the strides)
+    fa_paged_params q = *p;
+    q.flags = flags;
+    PagedCfg c;
+    pick_paged(&q, c);
+    if (c.nw > 0) continue;
+    const size_t rows = 2 * (size_t)paged_workers(c) * c.RG * 16;
+    most = std::max(most, paged_up(rows * p->Dv * 4) + paged_up(rows * 8) + paged_up(((size_t)p->B * paged_row_tiles(p, c) + 1) * 4));
+  }
+  return most;
 }
 
 int fa_paged_prepare(fa_module* m, const fa_paged_params* p) {
@@ -320,7 +357,8 @@ int fa_paged_prepare(fa_module* m, const fa_paged_params* p) {
 
 int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = paged_check(m, p)) return rc;
-  if (!workspace || workspace_bytes < fa_paged_workspace_bytes(p)) return fail(FA_EWORKSPACE, "paged attention workspace too small");
+  const size_t need = fa_paged_workspace_bytes(p);
+  if (need && (!workspace || workspace_bytes < need)) return fail(FA_EWORKSPACE, "paged attention workspace too small");
   if ((uintptr_t)workspace & 15) return fail(FA_EINVAL, "workspace must be 16-byte aligned");
   prof_reset();
   PagedCfg c;
@@ -333,30 +371,32 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
   k.lse = p->lse; k.table = p->block_table; k.table_stride = p->block_table_stride; k.lengths = p->lengths; k.status = p->status;
   k.B = p->B; k.Hq = p->Hq; k.Hkv = p->Hkv; k.Sq = p->Sq;
   k.num_pages = (int)p->num_pages; k.page_size = p->page_size;
+  k.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p->page_size == 1 << i) k.page_shift = i;
   k.max_len = (int)std::min<long long>((long long)p->table_width * p->page_size, 0x7fffffffll - 64);
-  k.row_tiles = paged_row_tiles(p, c); k.workers = paged_workers(c); k.min_tiles = 1;
   k.window = p->window < 0 ? -1 : std::min(p->window, 1 << 30);
   k.b_off = p->b_offset; k.h_off = p->h_offset; k.scale = p->scale;
-  const size_t rows = 2 * (size_t)k.workers * c.RG * 16;
-  k.part_o = (float*)workspace;
-  k.part_ml = (float*)((char*)workspace + paged_up(rows * p->Dv * 4));
-  k.plan = (int*)((char*)k.part_ml + paged_up(rows * 8));
   if (c.tma) {
     // (strides that no tensor map takes: 16-byte pieces)
     if (make_map(&L.tk, p->dtype, p->k_pages, p->D, p->page_size, p->Hkv, (int)p->num_pages, c.box) != FA_OK ||
         make_map(&L.tv, p->dtype, p->v_pages, p->Dv, p->page_size, p->Hkv, (int)p->num_pages, c.box) != FA_OK) {
       fa_paged_params q = *p;
       q.flags |= FA_FLAG_GENERAL_KERNELS;
-      PagedCfg g;
-      pick_paged(&q, g);
-      g.per_sm = std::min(g.per_sm, c.per_sm);  // (the workspace is the other's)
-      c = g;
-      k.workers = paged_workers(c);
+      pick_paged(&q, c);
     }
   }
+  k.row_tiles = paged_row_tiles(p, c);
+  k.workers = paged_workers(c);
+  k.min_tiles = 1;
+  const size_t rows = 2 * (size_t)k.workers * c.RG * 16;
+  k.part_o = (float*)workspace;
+  k.part_ml = (float*)((char*)workspace + paged_up(rows * p->Dv * 4));
+  k.plan = (int*)((char*)k.part_ml + paged_up(rows * 8));
   k.box = c.box;
   Kernel* kernel = nullptr;
   if (int rc = get_paged_kernel(m, p, c, &kernel)) return rc;
+  if (c.nw > 0) return launch(kernel, dim3((unsigned)((long long)p->B * k.row_tiles * p->Hkv)), dim3(c.nw * 32), &L, stream);
   if (int rc = launch(kernel, dim3((unsigned)k.workers), dim3(c.RG * 32), &L, stream)) return rc;
   // Few segments for the workers: many parts each, and eight warps add up a row's.
   const long long segments = (long long)p->B * k.row_tiles * p->Hkv;

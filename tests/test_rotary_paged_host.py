@@ -82,7 +82,7 @@ def test_paged_arguments(kw, code):
 def test_paged_workspace_and_module():
     L = _cabi.lib()
     m = _cabi.Module(None)
-    p = paged()
+    p = paged(table_width=4096)
     need = L.fa_paged_workspace_bytes(C.byref(p))
     assert need >= 148 * 2 * 16 * (64 + 2) * 4 + 3 * 4
     assert L.fa_paged(m.handle, C.byref(p), 0x8000, need - 1, None) == -5
