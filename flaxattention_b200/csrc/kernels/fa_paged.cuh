@@ -12,22 +12,24 @@
 //
 // Who takes which tiles:
 //   * Lengths are known on the device only and differ, so the work is cut there: the tiles of all segments, one behind the other, are
-//     dealt out evenly to the CTAs ("workers") of a grid that is resident at once.  A worker keeps the running (max, sum, O) of one
-//     segment, over whose end its loads run on into the next.  A segment that lies in one worker's run is written out; of others the
-//     workers leave parts (O not divided, max, sum), which fa_paged_combine_kernel merges.
-//   * FA_SHORT, for tables that have room for a few tiles only: a CTA per segment, whose warps take every FA_NW-th tile and merge
-//     in shared memory; one launch, and no sums over the lengths in front.
+//     dealt out evenly to the CTAs ("workers") of a grid that is resident at once.  A worker goes through the segments of its run; its key
+//     groups take every FA_CG-th tile, each with a running (max, sum, O) of its own, and merge through shared memory where a segment
+//     ends, while the loads of the next are on their way.  A segment that lies in one worker's run is written out; of others the workers leave
+//     parts (O not divided, max, sum), which fa_paged_combine_kernel merges.
+//   * FA_SHORT, for tables that have room for a few tiles only: a CTA per segment; one launch, and no sums over the lengths in front.
 //
-// The warps of a worker (FA_RG; FA_SHORT: each on its own) have 16 query rows each and share the tiles of K and V, which come by TMA
-// (FA_TMA: pages that hold whole boxes of 8 keys and more, head dims of whole 128-byte columns) or in 16-byte cp.async pieces.
+// CTA = FA_CG key groups of FA_RG warps with 16 query rows each.  The warps of a key group share its tiles of K and V, which come by TMA
+// (FA_TMA: pages that hold whole boxes of 8 keys and more, head dims of whole 128-byte columns) or in 16-byte cp.async pieces.  That the groups
+// of a CTA read beside each other counts: with a run for each warp DRAM gave 6.1 to 6.2 TB/s (B32 H8 D64, 16384 keys in pages of 64).
 // Three ways to multiply:
-//   * FA_FEW, up to 8 rows, which is what one new token has: S' = K Q' and O' = V' P', so that keys and columns fill the 16 rows of an
-//     mma.sync and the queries its 8 columns: half the instructions of the next way, of which the queries would fill half.
-//   * 16-bit, more rows: S = Q K', O = P V, 16 rows per warp.
+//   * FA_FEW groups of 8 rows, by one warp: S' = K Q' and O' = V' P', so that keys and columns fill the 16 rows of an mma.sync and the
+//     queries its 8 columns.  For up to 8 rows, which is what one new token has, half the instructions of the next way, of which the
+//     queries would fill half; for 17 to 24, three quarters, and no second warp to wait for.
+//   * 16-bit, other rows: S = Q K', O = P V, 16 rows per warp.
 //   * fp32: on the FMA pipes, in fp32 throughout; a lane has a key (and a part of the head dim) for the scores, columns for the values.
 //
-// Compile-time parameters (macros): FA_DTYPE, FA_D, FA_DV, FA_RG (1, 2, 4), FA_WN (keys of a tile: 32; fp32: 32, 16, 8), FA_STAGES, FA_TMA,
-// FA_FEW, FA_FR (fp32: rows of a warp), FA_NW (FA_SHORT: warps of a CTA).
+// Compile-time parameters (macros): FA_DTYPE, FA_D, FA_DV, FA_RG (1, 2, 4), FA_WN (keys of a tile: 32 or 16; fp32: 32, 16, 8), FA_SLOTS, FA_TMA,
+// FA_FEW (0: the other way), FA_FR (fp32: rows of a warp), FA_CG, FA_SHORT.
 #pragma once
 #include "fa_sm100.cuh"
 
@@ -43,38 +45,42 @@ namespace fa_pg {
 constexpr int DT = FA_DTYPE;
 constexpr bool F32 = DT == FA_DT_F32;
 constexpr bool FEW = FA_FEW != 0;
-constexpr bool SHORT = FA_NW > 0;
+constexpr bool SHORT = FA_SHORT != 0;
 constexpr bool TMA = FA_TMA != 0;
 constexpr int D = FA_D;
 constexpr int DV = FA_DV;
 constexpr int RG = FA_RG;
-constexpr int NW = SHORT ? FA_NW : RG;  // warps of the CTA
+constexpr int CG = FA_CG;
+constexpr int NW = CG * RG;  // warps of the CTA
 constexpr int NT = NW * 32;
-constexpr int BM = RG * 16;             // rows of a row tile
+constexpr int NQ = FA_FEW;               // groups of 8 rows
+constexpr int BM = FEW ? NQ * 8 : RG * 16;  // rows of a row tile
 constexpr int WN = FA_WN;
-constexpr int STAGES = FA_STAGES;
+constexpr int SLOTS = FA_SLOTS;
 constexpr int ES = F32 ? 4 : 2;
 constexpr int PK = TMA ? D * ES : FaTile<D, ES>::PITCH;
 constexpr int PV = TMA ? DV * ES : FaTile<DV, ES>::PITCH;
 constexpr int ATOMS_K = D / 64, ATOMS_V = DV / 64;  // 128-byte column groups of a row (TMA)
-constexpr int K_BYTES = WN * PK, V_BYTES = WN * PV;
-constexpr int PIPE_BYTES = STAGES * (K_BYTES + V_BYTES);  // of a worker
-constexpr int WORKERS = SHORT ? NW : 1;                   // of a CTA
+// A key group's buffers are a ring of slots that take a tile of K or of V: K, V, K of the next, ..; what was in a slot has been used up, and the
+// tile half a ring ahead is asked for.  Eight warps per SM, two for each of its schedulers, so that one's products run under the other's
+// softmax (D 128, up to 8 rows: a warp alone takes 1.5 us per tile, and four per SM with any number of slots 187 us where eight take 180).
+constexpr int SLOT_BYTES = WN * (PK > PV ? PK : PV);
+constexpr int PIPE_BYTES = SLOTS * SLOT_BYTES;  // of a key group
+constexpr bool ODD = SLOTS % 2 != 0;
+constexpr int AHEAD = (SLOTS + 1) / 2;  // tiles that are known before the first is computed
 constexpr int FR = FA_FR;
 // fp32: the query rows, and per warp the probabilities of a tile
 constexpr int PQ = D * 4, QROWS = RG == 1 ? FR : BM;
 constexpr int Q_BYTES = F32 ? QROWS * PQ + NW * FR * WN * 4 : 0;
-constexpr int BAR_BYTES = TMA ? WORKERS * STAGES * 16 + 16 : 0;
-constexpr int SMEM_BYTES = WORKERS * PIPE_BYTES + Q_BYTES + BAR_BYTES + (TMA ? 1024 : 0);
+// where the key groups merge: 32 columns of their rows at a time, and the rows' max and sum
+constexpr int MROWS = F32 && RG == 1 ? FR : BM, MPITCH = 36;
+constexpr int MERGE_BYTES = CG > 1 ? CG * MROWS * (MPITCH + 2) * 4 : 0;
+constexpr int BAR_BYTES = TMA ? CG * SLOTS * 8 + 16 : 0;
+constexpr int SMEM_BYTES = CG * PIPE_BYTES + Q_BYTES + MERGE_BYTES + BAR_BYTES + (TMA ? 1024 : 0);
 constexpr fa_u32 ALL = WN == 32 ? 0xffffffffu : (1u << (WN & 31)) - 1u;  // every key of a tile
-// rows that the warps of a CTA merge (SHORT), in a warp's own part of the buffers
-constexpr int MROWS = F32 ? FR : (FEW ? 8 : 16), MPITCH = DV + 4;
-
 static_assert(!TMA || (!F32 && D % 64 == 0 && DV % 64 == 0), "TMA: 16-bit types, whole column groups");
-static_assert(F32 || WN == 32, "tiles of 32 keys");
+static_assert(F32 || WN == 32 || WN == 16, "tiles of 16 or 32 keys");
 static_assert(!FEW || (RG == 1 && !F32), "few rows: one warp, 16-bit types");
-static_assert(!SHORT || RG == 1, "a CTA per segment: up to 16 rows");
-static_assert(MROWS * MPITCH * 4 <= PIPE_BYTES, "the merge of the warps fits into their buffers");
 
 // A segment, and the tile of it that is next.
 struct Seg {
@@ -102,16 +108,17 @@ __device__ __forceinline__ int seg_tiles(const FaPagedParams& p, int item) {
   seg_open(p, item, s);
   return s.last - s.tile;
 }
-__device__ __forceinline__ void seg_next(const FaPagedParams& p, Seg& s) {
-  if (SHORT) {
-    s.tile += NW;
-    return;
+// n tiles on, over the ends of segments
+__device__ __forceinline__ void seg_advance(const FaPagedParams& p, Seg& s, int n) {
+  s.tile += n;
+  while (!SHORT && s.tile >= s.last) {
+    const int over = s.tile - s.last;
+    const bool wrap = s.hk + 1 == p.Hkv;
+    s.hk = wrap ? 0 : s.hk + 1;
+    if (wrap && s.item + 1 == p.B * p.row_tiles) return;  // (behind the last tile of all)
+    seg_open(p, wrap ? s.item + 1 : s.item, s);
+    s.tile += over;
   }
-  if (++s.tile < s.last) return;
-  const bool wrap = s.hk + 1 == p.Hkv;
-  s.hk = wrap ? 0 : s.hk + 1;
-  if (wrap && s.item + 1 == p.B * p.row_tiles) return;  // (behind the last tile of all)
-  seg_open(p, wrap ? s.item + 1 : s.item, s);
 }
 
 // K and V of a tile on their way: where its keys are.  Every lane of every warp has the same but for its own key (TMA: box).
@@ -126,7 +133,7 @@ struct Load {
 // The rows of a tile in 16-byte pieces, those that are not there as zeros
 template <int COLS, int PITCH>
 __device__ __forceinline__ void load_pieces(const FaTensor& t, fa_u32 dst, const Load& n, int tid) {
-  constexpr int CPR = COLS * ES / 16, NL = SHORT ? 32 : NT;  // (NL threads share a tile)
+  constexpr int CPR = COLS * ES / 16, NL = RG * 32;  // (the threads of a key group)
   const long long at = n.page >= 0 ? (n.page * t.sb + n.hk * t.sh + n.row * t.ss) * ES : -1;
 #pragma unroll 4
   for (int i = tid; i < (WN * CPR + 31) / 32 * 32; i += NL) {  // (whole warps: the shuffle)
@@ -162,10 +169,11 @@ struct Rows {
   __device__ __forceinline__ int row(int h) const { return first_row + h; }
   __device__ __forceinline__ bool idle(int h, int rows) const { return first_row + h >= rows; }
   template <class F>
-  static __device__ __forceinline__ float over_keys(float v, F f) {
+  static __device__ __forceinline__ void over_keys(float (&v)[HR], F f) {
 #pragma unroll
-    for (int off = WN / 2; off > 0; off >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, off));
-    return v;
+    for (int off = WN / 2; off > 0; off >>= 1)
+#pragma unroll
+      for (int h = 0; h < HR; ++h) v[h] = f(v[h], __shfl_xor_sync(0xffffffffu, v[h], off));
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -219,82 +227,98 @@ struct Rows {
       }
     }
   }
-  // f(h, column, value) for every value of this thread
+  // f(h, column, value) for every value of this thread in columns 32 i ..
   template <class F>
-  __device__ __forceinline__ void each(F f) {
+  __device__ __forceinline__ void each(int i, F f) {
 #pragma unroll
     for (int h = 0; h < HR; ++h)
-#pragma unroll
-      for (int i = 0; i < NC; ++i)
-        if (lane + 32 * i < DV) f(h, lane + 32 * i, o[h][i]);
+      if (lane + 32 * i < DV) f(h, lane + 32 * i, o[h][i]);
   }
   __device__ __forceinline__ bool speaks() const { return lane == 0; }  // writes a row's max and sum
 };
 #elif FA_FEW
-constexpr int HR = 2, NS = WN / 8;
+constexpr int HR = 2 * NQ, NS = WN / 8;
 struct Rows {
-  float s[WN / 16][4], o[DV / 16][4], m[2], l[2];
-  fa_u32 qf[D / 16][2];
+  float s[WN / 16][NQ][4], o[DV / 16][NQ][4], m[HR], l[HR];
+  fa_u32 qf[D / 16][NQ][2];
   int lane;
-  __device__ __forceinline__ float& score(int h, int j) { return s[j >> 1][(j & 1) * 2 + h]; }
+  __device__ __forceinline__ float& score(int h, int j) { return s[j >> 1][h >> 1][(j & 1) * 2 + (h & 1)]; }
   __device__ __forceinline__ int key(int j) const { return (lane >> 2) + j * 8; }
-  __device__ __forceinline__ int row(int h) const { return (lane & 3) * 2 + h; }
-  __device__ __forceinline__ bool idle(int h, int rows) const { return h >= rows; }
+  __device__ __forceinline__ int row(int h) const { return (h >> 1) * 8 + (lane & 3) * 2 + (h & 1); }
+  __device__ __forceinline__ bool idle(int h, int rows) const { return (h >> 1) * 8 + (h & 1) >= rows; }
   template <class F>
-  static __device__ __forceinline__ float over_keys(float v, F f) {
+  static __device__ __forceinline__ void over_keys(float (&v)[HR], F f) {
 #pragma unroll
-    for (int off = 4; off < 32; off <<= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, off));
-    return v;
+    for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+      for (int h = 0; h < HR; ++h) v[h] = f(v[h], __shfl_xor_sync(0xffffffffu, v[h], off));
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < DV / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int i = 0; i < DV / 16; ++i)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o[i][q][0] = o[i][q][1] = o[i][q][2] = o[i][q][3] = 0.f;
   }
   __device__ __forceinline__ void rescale(int h, float c) {
 #pragma unroll
     for (int i = 0; i < DV / 16; ++i) {
-      o[i][h] *= c;
-      o[i][2 + h] *= c;
+      o[i][h >> 1][h & 1] *= c;
+      o[i][h >> 1][2 + (h & 1)] *= c;
     }
   }
   __device__ __forceinline__ void scores(const unsigned char*, fa_u32 tile, int) {
 #pragma unroll
-    for (int i = 0; i < WN / 16; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int i = 0; i < WN / 16; ++i)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) s[i][q][0] = s[i][q][1] = s[i][q][2] = s[i][q][3] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
       for (int i = 0; i < WN / 16; ++i) {
         fa_u32 a[4];
         fa_ldsm_x4(chunk_at<PK>(tile, i * 16 + (lane & 15), kk * 2 + (lane >> 4)), a[0], a[1], a[2], a[3]);
-        fa_mma16816<DT>(s[i], a, qf[kk][0], qf[kk][1]);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) fa_mma16816<DT>(s[i][q], a, qf[kk][q][0], qf[kk][q][1]);
       }
     }
   }
-  // The probabilities go in as two parts, rounded and what the rounding left: with one, bf16 results were 2.3e-3 off in place of the 1.7e-3
-  // that rounding the output takes (D 128, 16384 keys).
+  // Up to 8 rows the probabilities go in as two parts, rounded and what the rounding left: with one, bf16 results were 2.3e-3 off in place of the
+  // 1.7e-3 that rounding the output takes (D 128, 16384 keys).  With more rows the products would cost time.
   __device__ __forceinline__ void values(const unsigned char*, fa_u32 tile, int) {
+    constexpr bool TWO = NQ == 1;
 #pragma unroll
     for (int kj = 0; kj < WN / 16; ++kj) {
-      float r[4];
-      fa_rest2<DT>(s[kj][0], s[kj][1], r[0], r[1]);
-      fa_rest2<DT>(s[kj][2], s[kj][3], r[2], r[3]);
-      const fa_u32 b0 = transposed(fa_pack2<DT>(s[kj][0], s[kj][1])), b1 = transposed(fa_pack2<DT>(s[kj][2], s[kj][3]));
-      const fa_u32 c0 = transposed(fa_pack2<DT>(r[0], r[1])), c1 = transposed(fa_pack2<DT>(r[2], r[3]));
+      fa_u32 b[NQ][2], rest[2];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) b[q][e] = transposed(fa_pack2<DT>(s[kj][q][2 * e], s[kj][q][2 * e + 1]));
+      if (TWO) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float r0, r1;
+          fa_rest2<DT>(s[kj][0][2 * e], s[kj][0][2 * e + 1], r0, r1);
+          rest[e] = transposed(fa_pack2<DT>(r0, r1));
+        }
+      }
 #pragma unroll
       for (int i = 0; i < DV / 16; ++i) {
         fa_u32 a[4];
         fa_ldsm_x4_t(chunk_at<PV>(tile, kj * 16 + (lane >> 4) * 8 + (lane & 7), i * 2 + ((lane >> 3) & 1)), a[0], a[1], a[2], a[3]);
-        fa_mma16816<DT>(o[i], a, b0, b1);
-        fa_mma16816<DT>(o[i], a, c0, c1);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) fa_mma16816<DT>(o[i][q], a, b[q][0], b[q][1]);
+        if (TWO) fa_mma16816<DT>(o[i][0], a, rest[0], rest[1]);
       }
     }
   }
   template <class F>
-  __device__ __forceinline__ void each(F f) {
+  __device__ __forceinline__ void each(int b, F f) {
 #pragma unroll
-    for (int i = 0; i < DV / 16; ++i)
+    for (int i = 2 * b; i < 2 * b + 2 && i < DV / 16; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f(e & 1, i * 16 + (lane >> 2) + (e >> 1) * 8, o[i][e]);
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f(2 * q + (e & 1), i * 16 + (lane >> 2) + (e >> 1) * 8, o[i][q][e]);
   }
   __device__ __forceinline__ bool speaks() const { return lane < 4; }
 };
@@ -309,9 +333,11 @@ struct Rows {
   __device__ __forceinline__ int row(int h) const { return first_row + h * 8 + (lane >> 2); }
   __device__ __forceinline__ bool idle(int h, int rows) const { return first_row + h * 8 >= rows; }
   template <class F>
-  static __device__ __forceinline__ float over_keys(float v, F f) {
-    v = f(v, __shfl_xor_sync(0xffffffffu, v, 1));
-    return f(v, __shfl_xor_sync(0xffffffffu, v, 2));
+  static __device__ __forceinline__ void over_keys(float (&v)[HR], F f) {
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1)
+#pragma unroll
+      for (int h = 0; h < HR; ++h) v[h] = f(v[h], __shfl_xor_sync(0xffffffffu, v[h], off));
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -359,9 +385,9 @@ struct Rows {
     }
   }
   template <class F>
-  __device__ __forceinline__ void each(F f) {
+  __device__ __forceinline__ void each(int b, F f) {
 #pragma unroll
-    for (int j = 0; j < DV / 8; ++j)
+    for (int j = 4 * b; j < 4 * b + 4 && j < DV / 8; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) f(e >> 1, j * 8 + (lane & 3) * 2 + (e & 1), o[j][e]);
   }
@@ -376,7 +402,12 @@ struct Sum {
   __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
 };
 
-// two values of an output row beside each other
+// a value of an output row
+__device__ __forceinline__ void put1(char* row, int c, float x) {
+  if (F32) *(float*)(row + c * 4) = x;
+  else *(fa_u16*)(row + c * 2) = (fa_u16)fa_pack2<DT>(x, 0.f);
+}
+// two beside each other
 __device__ __forceinline__ void put2(char* row, int c, float x, float y) {
   if (F32) *(float2*)(row + c * 4) = make_float2(x, y);
   else *(fa_u32*)(row + c * 2) = fa_pack2<DT>(x, y);
@@ -384,6 +415,23 @@ __device__ __forceinline__ void put2(char* row, int c, float x, float y) {
 // 1 / sum; 0 of a row that has seen nothing, no number of a sum that is none
 __device__ __forceinline__ float inverse(float l) { return l > 0.f ? 1.f / l : l; }
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? FA_NEG_INF : (m + log2f(l)) * FA_LN2; }
+
+// The warps of a key group wait for one another; true where any of their threads says so.
+__device__ __forceinline__ bool group_sync(int cg, bool v) {
+  if (RG == 1) {
+    __syncwarp();
+    return v;
+  }
+  if (CG == 1) return __syncthreads_or(v) != 0;
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred a, b;\n\t"
+      "setp.ne.s32 a, %1, 0;\n\t"
+      "barrier.cta.red.or.pred b, %2, %3, a;\n\t"
+      "selp.s32 %0, 1, 0, b;\n\t}"
+      : "=r"(r) : "r"((int)v), "r"(cg + 1), "n"(RG * 32) : "memory");
+  return r != 0;
+}
 
 }  // namespace fa_pg
 
@@ -397,17 +445,20 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
   }
   unsigned char* const base = TMA ? smem_raw + ((1024u - (fa_smem_u32(smem_raw) & 1023u)) & 1023u) : smem_raw;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // this worker's buffers: K, V
-  unsigned char* const bufs = base + (SHORT ? warp * PIPE_BYTES : 0);
-  const fa_u32 sK = fa_smem_u32(bufs), sV = sK + STAGES * K_BYTES;
-  [[maybe_unused]] unsigned char* const q_tile = base + WORKERS * PIPE_BYTES;
-  const int row0 = SHORT ? 0 : warp * 16;  // first row of this warp
+  const int rg = warp % RG, cg = warp / RG;
+  // [rings of the key groups | fp32: queries, probabilities | merge | barriers]
+  unsigned char* const bufs = base + cg * PIPE_BYTES;
+  const fa_u32 ring = fa_smem_u32(bufs);
+  [[maybe_unused]] unsigned char* const q_tile = base + CG * PIPE_BYTES;
+  [[maybe_unused]] float* const merge = (float*)(base + CG * PIPE_BYTES + Q_BYTES);  // [CG][MROWS][MPITCH]
+  [[maybe_unused]] float2* const merge_ml = (float2*)(merge + CG * MROWS * MPITCH);  // [CG][MROWS]
+  const int row0 = rg * 16;  // first row of this warp
 #if FA_TMA
-  const fa_u32 all_bars = fa_smem_u32(base) + WORKERS * PIPE_BYTES;
-  const fa_u32 bars = all_bars + (SHORT ? warp * STAGES * 16 : 0);  // K 0 .. STAGES - 1, V 0 .. STAGES - 1
-  volatile int* abort_flag = (volatile int*)(base + WORKERS * (PIPE_BYTES + STAGES * 16));
+  const fa_u32 all_bars = fa_smem_u32(base) + CG * PIPE_BYTES + Q_BYTES + MERGE_BYTES;
+  const fa_u32 bars = all_bars + cg * SLOTS * 8;  // one per slot
+  volatile int* abort_flag = (volatile int*)(base + CG * (PIPE_BYTES + SLOTS * 8) + Q_BYTES + MERGE_BYTES);
   if (tid == 0) {
-    for (int i = 0; i < WORKERS * 2 * STAGES; ++i) fa_mbar_init(all_bars + i * 8, 1);
+    for (int i = 0; i < CG * SLOTS; ++i) fa_mbar_init(all_bars + i * 8, 1);
     fa_mbar_init_fence();
     *abort_flag = 0;
   }
@@ -424,8 +475,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
     seg.hk = blockIdx.x % p.Hkv;
     seg_open(p, blockIdx.x / p.Hkv, seg);
     t0 = 0;
-    t1 = max(seg.last - seg.tile - warp + NW - 1, 0) / NW;
-    seg.tile += warp;
+    t1 = seg.last - seg.tile;
     if (tid == 0 && seg.hk == 0 && (p.lengths[seg.b] > p.max_len || p.lengths[seg.b] < 0) && p.status != nullptr) atomicOr(p.status, FA_STATUS_BAD_PAGE);
   } else {
     // every lane counts a run of items, then the lanes are added up
@@ -467,11 +517,11 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
     seg.hk = off / n;
     seg.tile += off - seg.hk * n;
   }
-  [[maybe_unused]] const int seg_first = seg.tile;  // where the first segment's part begins
 
   // ---- loads -----------------------------------------------------------------------------
-  Seg ahead = seg;     // of the tile that is asked for next
-  int to_load = t1 - t0;
+  Seg ahead = seg;  // of the tile that is asked for next: every CG-th of the run
+  int to_load = max(t1 - t0 - cg + CG - 1, 0) / CG;
+  if (to_load > 0) seg_advance(p, ahead, cg);
   // looks the next tile's pages up
   auto look_up = [&](Load& n) {
     n.any = to_load > 0;
@@ -488,8 +538,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
     // (the keys that are there go along; those whose page is none are taken out when the entry has come)
     const int left = ahead.end - ahead.tile * WN;
     n.keep = left >= WN ? ALL : left > 0 ? (1u << left) - 1u : 0u;
-    --to_load;
-    seg_next(p, ahead);
+    if (--to_load > 0) seg_advance(p, ahead, CG);
   };
   // takes keys out whose page is none
   auto settle = [&](Load& n) {
@@ -507,7 +556,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
   };
 #if FA_TMA
   auto load = [&](const FaTensorMap* map, fa_u32 dst, fa_u32 bar, int atoms, const Load& n) {
-    if (!SHORT && warp != 0) return;
+    if (rg != 0) return;
     const fa_u32 boxes = __ballot_sync(0xffffffffu, n.page >= 0);
     if (lane == 0) fa_mbar_expect_tx(bar, __popc(boxes) * p.box * 128 * atoms);
     __syncwarp();
@@ -516,33 +565,38 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
         fa_tma_load_4d(dst + a * (WN * 128) + lane * p.box * 128, map, bar, a * 64, n.row, n.hk, n.page);
     }
   };
-  auto load_k = [&](int stage, const Load& n) { load(&L.tk, sK + stage * K_BYTES, bars + stage * 8, ATOMS_K, n); };
-  auto load_v = [&](int stage, const Load& n) { load(&L.tv, sV + stage * V_BYTES, bars + (STAGES + stage) * 8, ATOMS_V, n); };
+  auto load_k = [&](int slot, const Load& n) { load(&L.tk, ring + slot * SLOT_BYTES, bars + slot * 8, ATOMS_K, n); };
+  auto load_v = [&](int slot, const Load& n) { load(&L.tv, ring + slot * SLOT_BYTES, bars + slot * 8, ATOMS_V, n); };
 #else
-  const int loader = SHORT ? lane : tid;
-  auto load_k = [&](int stage, const Load& n) { load_pieces<D, PK>(p.k, sK + stage * K_BYTES, n, loader); };
-  auto load_v = [&](int stage, const Load& n) { load_pieces<DV, PV>(p.v, sV + stage * V_BYTES, n, loader); };
+  const int loader = rg * 32 + lane;
+  auto load_k = [&](int slot, const Load& n) { load_pieces<D, PK>(p.k, ring + slot * SLOT_BYTES, n, loader); };
+  auto load_v = [&](int slot, const Load& n) { load_pieces<DV, PV>(p.v, ring + slot * SLOT_BYTES, n, loader); };
 #endif
 
-  fa_u32 keep[STAGES];
+  fa_u32 keep[AHEAD];
+  Load pending, next, after;  // the tile whose V is asked for next, the one whose K is, and the one behind that
+  pending.any = next.any = after.any = false;
+  int asked = 0;  // slots asked for
 #pragma unroll
-  for (int st = 0; st < STAGES; ++st) {
-    Load n;
-    look_up(n);
+  for (int st = 0; st < AHEAD; ++st) {
+    look_up(next);
     keep[st] = 0;
-    if (n.any) {
-      settle(n);
-      keep[st] = n.keep;
-      load_k(st, n);
+    if (next.any) {
+      settle(next);
+      keep[st] = next.keep;
+      load_k(2 * st, next);
     }
     fa_cp_commit();
-    if (n.any) load_v(st, n);
-    fa_cp_commit();
+    if (2 * st + 1 < SLOTS) {
+      if (next.any) load_v(2 * st + 1, next);
+      fa_cp_commit();
+    }
+    asked += next.any ? (2 * st + 1 < SLOTS ? 2 : 1) : 0;
   }
-  Load next, after;  // the tile STAGES ahead of the one that is computed, and the one behind it
+  pending = next;
   look_up(next);
 
-  // ---- the tiles -------------------------------------------------------------------------
+  // ---- the segments ----------------------------------------------------------------------
   Rows R;
   R.lane = lane;
 #if FA_DTYPE == FA_DT_F32
@@ -552,18 +606,35 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
 #elif !FA_FEW
   R.first_row = row0;
 #endif
-  int qpos[HR], head[HR];  // of this thread's rows: position (-1: no row), query head
   const float sc2 = p.scale * FA_LOG2E;
-  bool open = false, failed = false;
-  [[maybe_unused]] bool k_again = false;  // K of the tile STAGES ahead has been asked for, V not yet
-  int cur = 0, rows = 0;                  // buffer of this tile; rows of the row tile
+  bool failed = false;
+  int slot = 0;  // that is used next
   [[maybe_unused]] fa_u32 phase = 0;
-  bool first_part = true;  // of this worker
-  // (a warp of a CTA with a segment of its own has to take part in its end even if it has no tile)
-  auto begin_rows = [&]() {
-    const int rt = seg.item - seg.b * p.row_tiles;
-    rows = min(G * p.Sq - rt * BM, BM);
-    const char* qb = (const char*)p.q.ptr + seg.b * p.q.sb * ES;
+  [[maybe_unused]] int n_used = 0;  // slots
+  // a slot's tile has come: its number; then it is used up, and the next is looked at
+  auto arrived = [&]() {
+#if FA_TMA
+    failed = !fa_mbar_wait_all(bars + slot * 8, phase, abort_flag);
+#else
+    fa_cp_wait<SLOTS - 1>();
+    group_sync(cg, false);
+#endif
+    return slot;
+  };
+  auto used = [&]() {
+    failed = group_sync(cg, failed);
+    if (++slot == SLOTS) {
+      slot = 0;
+      phase ^= 1u;
+    }
+    ++n_used;
+  };
+
+  for (int t = t0; t < t1;) {
+    // this worker's part of the segment: tiles seg.tile .. part_end - 1
+    const int part_end = min(seg.last, seg.tile + (t1 - t)), rt = seg.item - seg.b * p.row_tiles;
+    const int rows = min(G * p.Sq - rt * BM, BM);
+    int qpos[HR], head[HR];  // of this thread's rows: position (-1: no row), query head
 #pragma unroll
     for (int h = 0; h < HR; ++h) {
       const int row = rt * BM + R.row(h), i = row / G;
@@ -573,254 +644,249 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
       R.l[h] = 0.f;
     }
     R.clear();
+    const char* qb = (const char*)p.q.ptr + seg.b * p.q.sb * ES;
 #if FA_DTYPE == FA_DT_F32
-    if (RG == 1 && !SHORT) __syncwarp();
-    else __syncthreads();  // (the tile before has been read)
+    __syncthreads();  // (the rows of the segment before have been read)
     for (int i = tid; i < QROWS * (D / 4); i += NT) {
       const int r = i / (D / 4), c = i - r * (D / 4), row = rt * BM + r, qi = row / G;
       const float* src = (const float*)(qb + (qi * p.q.ss + (long long)(seg.hk * G + row - qi * G) * p.q.sh) * ES) + c * 4;
       *(float4*)(q_tile + r * PQ + c * 16) = qi < p.Sq ? *(const float4*)src : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    if (RG == 1 && !SHORT) __syncwarp();
-    else __syncthreads();
+    __syncthreads();
 #else
-    constexpr int NR = FEW ? 1 : 2;  // fragments of rows g and, where there are as many, g + 8
+    // (rows g, g + 8, .. of the row tile, g = lane / 4)
 #pragma unroll
-    for (int hh = 0; hh < NR; ++hh) {
-      const int row = rt * BM + row0 + hh * 8 + (lane >> 2), i = row / G;
+    for (int q = 0; q < (FEW ? NQ : 2); ++q) {
+      const int row = rt * BM + row0 + q * 8 + (lane >> 2), i = row / G;
       const fa_u32* src = (const fa_u32*)(qb + (i * p.q.ss + (long long)(seg.hk * G + row - i * G) * p.q.sh) * ES) + (lane & 3);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        R.qf[kk][hh] = i < p.Sq ? src[kk * 8] : 0u;
-        R.qf[kk][NR + hh] = i < p.Sq ? src[kk * 8 + 4] : 0u;
-      }
-    }
-#endif
-  };
-  if (SHORT) begin_rows();
-
-  [[maybe_unused]] int t_now = t0;
-  for (int t = t0; t < t1; ++t) {
-    t_now = t;
-    if (!SHORT && !open) {
-      open = true;
-      begin_rows();
-    }
-    // ---- scores
-#if FA_TMA
-    failed = !fa_mbar_wait_all(bars + cur * 8, phase, abort_flag);
+        const fa_u32 lo = i < p.Sq ? src[kk * 8] : 0u, hi = i < p.Sq ? src[kk * 8 + 4] : 0u;
+#if FA_FEW
+        R.qf[kk][q][0] = lo;
+        R.qf[kk][q][1] = hi;
 #else
-    fa_cp_wait<2 * STAGES - 1>();
-    if (RG == 1) __syncwarp();
-    else __syncthreads();
+        R.qf[kk][q] = lo;
+        R.qf[kk][2 + q] = hi;
 #endif
-    R.scores(bufs + cur * K_BYTES, sK + cur * K_BYTES, rows);
-    // K's buffer is free
-    if (RG == 1) __syncwarp();
-    else failed = __syncthreads_or(failed) != 0;
-    if (failed) break;
-    if (next.any) {
-      settle(next);
-      load_k(cur, next);
-      k_again = true;
+      }
     }
-    fa_cp_commit();
-    look_up(after);
-
-    const int n0 = seg.tile * WN;
-    const fa_u32 kept = keep[0];
-    // does any row of the tile have to look at the positions?
-    const bool edge = n0 + WN - 1 > seg.pos || (p.window >= 0 && n0 < seg.end - 1 - p.window) || kept != ALL;
-    const int gb = seg.b + p.b_off;
-#pragma unroll
-    for (int h = 0; h < HR; ++h) {
-      if (R.idle(h, rows)) {  // (the rows of all lanes)
-#pragma unroll
-        for (int j = 0; j < NS; ++j) R.score(h, j) = 0.f;
-        continue;
-      }
-      [[maybe_unused]] const int qp = max(qpos[h], 0), gh = head[h] + p.h_off;
-#pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        [[maybe_unused]] const int kv = n0 + R.key(j);
-        float x = R.score(h, j);
-#if FA_HAS_SCORE_MOD && defined(FA_SCORE_AFFINE)
-        x = fmaf(x, fa_score_mul(0.f, gb, gh, qp, kv) * sc2, fa_score_add2(0.f, gb, gh, qp, kv));
-#elif FA_HAS_SCORE_MOD
-        x = fa_score_mod(x * p.scale, gb, gh, qp, kv) * FA_LOG2E;
-#else
-        x *= sc2;
 #endif
-        R.score(h, j) = x;
+
+    // ---- the tiles of this key group (a group whose wait has run out leaves them out, but takes part in the merges)
+    for (int tile = seg.tile + (CG - (t - t0) % CG + cg) % CG; tile < part_end && !failed; tile += CG) {
+      int at = arrived();
+      R.scores(bufs + at * SLOT_BYTES, ring + at * SLOT_BYTES, rows);
+      used();
+      if (failed) break;
+      // the slot takes what is SLOTS behind: V of the tile whose K is on its way (odd rings), or K of the next
+      if (ODD) {
+        if (pending.any) load_v(at, pending);
+        asked += pending.any;
+      } else {
+        if (next.any) {
+          settle(next);
+          load_k(at, next);
+        }
+        asked += next.any;
       }
-      if (edge || FA_HAS_MASK_MOD) {
+      fa_cp_commit();
+      look_up(after);
+
+      const int n0 = tile * WN;
+      const fa_u32 kept = keep[0];
+      // does any row of the tile have to look at the positions?
+      const bool edge = n0 + WN - 1 > seg.pos || (p.window >= 0 && n0 < seg.end - 1 - p.window) || kept != ALL;
+      const int gb = seg.b + p.b_off;
+      float mx[HR];
+#pragma unroll
+      for (int h = 0; h < HR; ++h) {
+        mx[h] = FA_NEG_INF;
+        if (R.idle(h, rows)) continue;  // (the rows of all lanes)
+        [[maybe_unused]] const int qp = max(qpos[h], 0), gh = head[h] + p.h_off;
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-          const int kv = n0 + R.key(j);
-          bool see = kv <= qpos[h] && (p.window < 0 || qpos[h] - kv <= p.window) && ((kept >> R.key(j)) & 1u);
-#if FA_HAS_MASK_MOD
-          see = see && fa_mask_mod(gb, gh, qp, kv);
-#endif
-          if (!see) R.score(h, j) = FA_NEG_INF;
-        }
-      }
-      float mx = FA_NEG_INF;
-#pragma unroll
-      for (int j = 0; j < NS; ++j) mx = fmaxf(mx, R.score(h, j));
-      mx = Rows::over_keys(mx, Max());
-      const float m_new = fmaxf(R.m[h], mx);
-      const float m_use = (m_new == FA_NEG_INF) ? 0.f : m_new;
-      const float corr = fa_ex2(R.m[h] - m_use);
-      R.m[h] = m_new;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        const float e = fa_ex2(R.score(h, j) - m_use);
-        R.score(h, j) = e;
-        sum += e;
-      }
-      R.l[h] = R.l[h] * corr + sum;
-      // (after the first tiles the maximum seldom moves)
-      if (__any_sync(0xffffffffu, corr != 1.f)) R.rescale(h, corr);
-    }
-    // ---- values
-#if FA_TMA
-    failed = !fa_mbar_wait_all(bars + (STAGES + cur) * 8, phase, abort_flag);
-    // Rows of keys that are not there hold whatever was in the page or the buffer, perhaps no number: 0, since a weight of 0
-    // does not take that out of the product.  (Each warp for itself; all write the same.)
-    if (kept != ALL) {
-      for (int i = lane; i < WN * ATOMS_V * 8; i += 32) {
-        const int r = (i >> 3) % WN;
-        if (!((kept >> r) & 1u)) *(uint4*)(bufs + STAGES * K_BYTES + cur * V_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before TMA writes the buffer again)
-      __syncwarp();
-    }
+          [[maybe_unused]] const int kv = n0 + R.key(j);
+          float x = R.score(h, j);
+#if FA_HAS_SCORE_MOD && defined(FA_SCORE_AFFINE)
+          x = fmaf(x, fa_score_mul(0.f, gb, gh, qp, kv) * sc2, fa_score_add2(0.f, gb, gh, qp, kv));
+#elif FA_HAS_SCORE_MOD
+          x = fa_score_mod(x * p.scale, gb, gh, qp, kv) * FA_LOG2E;
 #else
-    fa_cp_wait<2 * STAGES - 1>();
-    if (RG == 1) __syncwarp();
-    else __syncthreads();
+          x *= sc2;
 #endif
-    R.values(bufs + STAGES * K_BYTES + cur * V_BYTES, sV + cur * V_BYTES, rows);
-    if (RG == 1) __syncwarp();
-    else failed = __syncthreads_or(failed) != 0;
-    if (failed) break;
-    if (next.any) load_v(cur, next);
-    fa_cp_commit();
-    k_again = false;
+          R.score(h, j) = x;
+        }
+        if (edge || FA_HAS_MASK_MOD) {
 #pragma unroll
-    for (int i = 0; i + 1 < STAGES; ++i) keep[i] = keep[i + 1];
-    keep[STAGES - 1] = next.any ? next.keep : 0u;
-    next = after;
-    if (++cur == STAGES) {
-      cur = 0;
-      phase ^= 1u;
+          for (int j = 0; j < NS; ++j) {
+            const int kv = n0 + R.key(j);
+            bool see = kv <= qpos[h] && (p.window < 0 || qpos[h] - kv <= p.window) && ((kept >> R.key(j)) & 1u);
+#if FA_HAS_MASK_MOD
+            see = see && fa_mask_mod(gb, gh, qp, kv);
+#endif
+            if (!see) R.score(h, j) = FA_NEG_INF;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NS; ++j) mx[h] = fmaxf(mx[h], R.score(h, j));
+      }
+      Rows::over_keys(mx, Max());
+      float corr[HR];
+      bool moved = false;
+#pragma unroll
+      for (int h = 0; h < HR; ++h) {
+        const float m_new = fmaxf(R.m[h], mx[h]);
+        mx[h] = m_new == FA_NEG_INF ? 0.f : m_new;
+        corr[h] = fa_ex2(R.m[h] - mx[h]);
+        R.m[h] = m_new;
+        moved |= corr[h] != 1.f && !R.idle(h, rows);
+      }
+#pragma unroll
+      for (int h = 0; h < HR; ++h) {
+        if (R.idle(h, rows)) {
+#pragma unroll
+          for (int j = 0; j < NS; ++j) R.score(h, j) = 0.f;
+          continue;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          const float e = fa_ex2(R.score(h, j) - mx[h]);
+          R.score(h, j) = e;
+          sum += e;
+        }
+        R.l[h] = R.l[h] * corr[h] + sum;
+      }
+      // (after the first tiles the maximum seldom moves)
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int h = 0; h < HR; ++h) R.rescale(h, corr[h]);
+      }
+
+      at = arrived();
+#if FA_TMA
+      // Rows of keys that are not there hold whatever was in the page or the buffer, perhaps no number: 0, since a weight of 0
+      // does not take that out of the product.  (Each warp for itself; all write the same.)
+      if (kept != ALL) {
+        for (int i = lane; i < WN * ATOMS_V * 8; i += 32) {
+          const int r = (i >> 3) % WN;
+          if (!((kept >> r) & 1u)) *(uint4*)(bufs + at * SLOT_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before TMA writes the buffer again)
+        __syncwarp();
+      }
+#endif
+      R.values(bufs + at * SLOT_BYTES, ring + at * SLOT_BYTES, rows);
+      used();
+      if (failed) break;
+      if (ODD) {
+        if (next.any) {
+          settle(next);
+          load_k(at, next);
+        }
+        asked += next.any;
+        pending = next;
+      } else {
+        if (next.any) load_v(at, next);
+        asked += next.any;
+      }
+      fa_cp_commit();
+#pragma unroll
+      for (int i = 0; i + 1 < AHEAD; ++i) keep[i] = keep[i + 1];
+      keep[AHEAD - 1] = next.any ? next.keep : 0u;
+      next = after;
     }
 
-    // ---- the end of the segment, or of this worker's part of it
-    const bool ends = seg.tile + 1 == seg.last;
-    if (!SHORT && (ends || t + 1 == t1)) {
-      open = false;
-      const int rt = seg.item - seg.b * p.row_tiles;
-      // whole: the part begins where the segment does
+    // ---- the end of the segment, or of this worker's part of it: written out if the part is the segment
+    bool whole = true;
+    if (!SHORT) {
       Seg x;
       seg_open(p, seg.item, x);
-      const bool whole = ends && (!first_part || seg_first == x.tile);
-      const int slot = (int)blockIdx.x * 2 + (first_part ? 0 : 1);
-      first_part = false;
-      float l[HR];
-#pragma unroll
-      for (int h = 0; h < HR; ++h) l[h] = F32 ? Rows::over_keys(R.l[h], Sum()) : Rows::over_keys(R.l[h], Sum());
-      if (whole) {
-        char* out[HR];
-#pragma unroll
-        for (int h = 0; h < HR; ++h) {
-          const int row = rt * BM + R.row(h), i = row / G;
-          out[h] = R.row(h) < rows ? (char*)p.o.ptr + (seg.b * p.o.sb + head[h] * p.o.sh + i * p.o.ss) * ES : nullptr;
-          if (out[h] != nullptr && R.speaks() && p.lse != nullptr) p.lse[((long long)seg.b * p.Hq + head[h]) * p.Sq + i] = log_sum(R.m[h], l[h]);
-          l[h] = inverse(l[h]);
-        }
-#if FA_DTYPE != FA_DT_F32 && FA_FEW
-        // (transposed back: lane / 4 is the row then, and a lane has two columns beside each other)
-        const int r = lane >> 2, i = (rt * BM + r) / G, hd = seg.hk * G + rt * BM + r - i * G;
-        char* og = (char*)p.o.ptr + (seg.b * p.o.sb + hd * p.o.sh + i * p.o.ss) * ES;
-#pragma unroll
-        for (int c = 0; c < DV / 8; ++c) {
-          const fa_u32 v = transposed(fa_pack2<DT>(R.o[c >> 1][(c & 1) * 2] * l[0], R.o[c >> 1][(c & 1) * 2 + 1] * l[1]));
-          if (r < rows) *(fa_u32*)(og + (c * 8 + (lane & 3) * 2) * 2) = v;
-        }
-#elif FA_DTYPE == FA_DT_F32
-        R.each([&](int h, int c, float v) {
-          if (out[h] != nullptr) *(float*)(out[h] + c * 4) = v * l[h];
-        });
-#else
-#pragma unroll
-        for (int j = 0; j < DV / 8; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (out[h] != nullptr) put2(out[h], j * 8 + (lane & 3) * 2, R.o[j][h * 2] * l[h], R.o[j][h * 2 + 1] * l[h]);
-#endif
-      } else {
-        R.each([&](int h, int c, float v) {
-          if (R.row(h) < rows) p.part_o[((long long)slot * BM + R.row(h)) * DV + c] = v;
-        });
-#pragma unroll
-        for (int h = 0; h < HR; ++h)
-          if (R.row(h) < rows && R.speaks()) *(float2*)(p.part_ml + ((long long)slot * BM + R.row(h)) * 2) = make_float2(R.m[h], l[h]);
-      }
+      whole = seg.tile == x.tile && part_end == seg.last;
     }
-    seg_next(p, seg);
+    const int part = (int)blockIdx.x * 2 + (t == t0 ? 0 : 1);
+    float* const part_o = p.part_o + (long long)part * BM * DV;
+    float* const part_ml = p.part_ml + (long long)part * BM * 2;
+    Rows::over_keys(R.l, Sum());
+    if (CG > 1) {
+#pragma unroll
+      for (int h = 0; h < HR; ++h)
+        if (R.speaks()) merge_ml[cg * MROWS + R.row(h)] = make_float2(R.m[h], R.l[h]);
+#pragma unroll
+      for (int blk = 0; blk < (DV + 31) / 32; ++blk) {
+        if (blk > 0) __syncthreads();  // (the columns before have been read)
+        R.each(blk, [&](int h, int c, float v) { merge[(cg * MROWS + R.row(h)) * MPITCH + c - blk * 32] = v; });
+        __syncthreads();
+        constexpr int PAIRS = DV < 32 ? DV / 2 : 16;
+        for (int i = tid; i < rows * PAIRS; i += NT) {
+          const int r = i / PAIRS, c = (i - r * PAIRS) * 2;
+          if (blk * 32 + c >= DV) continue;
+          float2 ml[CG];
+          float m = FA_NEG_INF;
+#pragma unroll
+          for (int g = 0; g < CG; ++g) {
+            ml[g] = merge_ml[g * MROWS + r];
+            m = fmaxf(m, ml[g].x);
+          }
+          const float m_use = m == FA_NEG_INF ? 0.f : m;
+          float x = 0.f, y = 0.f, l = 0.f;
+#pragma unroll
+          for (int g = 0; g < CG; ++g) {
+            const float2 v = *(const float2*)(merge + (g * MROWS + r) * MPITCH + c);
+            const float f = ml[g].y == 0.f ? 0.f : exp2f(ml[g].x - m_use);  // (a group that has seen nothing counts for nothing)
+            l += f * ml[g].y;
+            x += f * v.x;
+            y += f * v.y;
+          }
+          if (whole) {
+            const int qi = (rt * BM + r) / G, hd = seg.hk * G + rt * BM + r - qi * G;
+            const float inv = inverse(l);
+            put2((char*)p.o.ptr + (seg.b * p.o.sb + hd * p.o.sh + qi * p.o.ss) * ES, blk * 32 + c, x * inv, y * inv);
+            if (blk == 0 && c == 0 && p.lse != nullptr) p.lse[((long long)seg.b * p.Hq + hd) * p.Sq + qi] = log_sum(m_use, l);
+          } else {
+            *(float2*)(part_o + r * DV + blk * 32 + c) = make_float2(x, y);
+            if (blk == 0 && c == 0) *(float2*)(part_ml + r * 2) = make_float2(m, l);
+          }
+        }
+      }
+      __syncthreads();  // (before the next segment's sums)
+    } else {
+      char* out[HR];
+      float inv[HR];
+#pragma unroll
+      for (int h = 0; h < HR; ++h) {
+        const int i = (rt * BM + R.row(h)) / G;
+        out[h] = (char*)p.o.ptr + (seg.b * p.o.sb + head[h] * p.o.sh + i * p.o.ss) * ES;
+        inv[h] = inverse(R.l[h]);
+        if (R.row(h) >= rows || !R.speaks()) continue;
+        if (!whole) *(float2*)(part_ml + R.row(h) * 2) = make_float2(R.m[h], R.l[h]);
+        else if (p.lse != nullptr) p.lse[((long long)seg.b * p.Hq + head[h]) * p.Sq + i] = log_sum(R.m[h], R.l[h]);
+      }
+#pragma unroll
+      for (int blk = 0; blk < (DV + 31) / 32; ++blk)
+        R.each(blk, [&](int h, int c, float v) {
+          if (R.row(h) >= rows) return;
+          if (whole) put1(out[h], c, v * inv[h]);
+          else part_o[R.row(h) * DV + c] = v;
+        });
+    }
+    t += part_end - seg.tile;
+    if (t < t1) seg_advance(p, seg, part_end - seg.tile);
   }
   fa_grid_release();
   fa_cp_wait<0>();
 #if FA_TMA
   if (failed) {
-    // The copies in flight have to land before the shared memory goes to another CTA or is used again (with a limit of its own: the flag
-    // is up).  Buffers from `cur` on hold the tiles up to the end of the ring, those before it the next round's.
-    if (SHORT ? lane == 0 : tid == 0) {
+    // The copies in flight have to land before the shared memory goes to another CTA (with a limit of its own: the flag is up).
+    if (rg == 0 && lane == 0) {
       const fa_u64 start = fa_globaltimer();
-      for (int i = 0; i < 2 * STAGES; ++i) {
-        const int st = i < STAGES ? i : i - STAGES, ahead_by = st >= cur ? st - cur : st - cur + STAGES;
-        const bool again = i == cur && k_again;
-        if (t_now + ahead_by + (again ? STAGES : 0) >= t1) continue;  // (nothing was asked for)
-        while (!fa_mbar_try(bars + i * 8, phase ^ (st < cur || again ? 1u : 0u)) && fa_globaltimer() - start <= FA_WAIT_LIMIT_NS / 4) {
+      for (int i = n_used; i < asked; ++i) {
+        while (!fa_mbar_try(bars + (i % SLOTS) * 8, (i / SLOTS) & 1) && fa_globaltimer() - start <= FA_WAIT_LIMIT_NS / 4) {
         }
       }
     }
     if (lane == 0 && p.status != nullptr) atomicOr(p.status, FA_STATUS_WAIT_TIMEOUT);
-    __syncwarp();
   }
 #endif
-  if (SHORT) {
-    // ---- merge the warps: each leaves its rows in its own buffers, [MROWS][O | max, sum]
-    float* const mine = (float*)bufs;
-    __syncwarp();
-    R.each([&](int h, int c, float v) { mine[R.row(h) * MPITCH + c] = v; });
-#pragma unroll
-    for (int h = 0; h < HR; ++h) {
-      const float l = Rows::over_keys(R.l[h], Sum());
-      if (R.speaks()) *(float2*)(mine + R.row(h) * MPITCH + DV) = make_float2(R.m[h], l);
-    }
-    __syncthreads();
-    for (int i = tid; i < rows * (DV / 2); i += NT) {
-      const int r = i / (DV / 2), c = (i - r * (DV / 2)) * 2, qi = r / G, h = seg.hk * G + r - qi * G;
-      float m = FA_NEG_INF;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) m = fmaxf(m, ((const float*)(base + w * PIPE_BYTES))[r * MPITCH + DV]);
-      const float m_use = m == FA_NEG_INF ? 0.f : m;
-      float x = 0.f, y = 0.f, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float* part = (const float*)(base + w * PIPE_BYTES) + r * MPITCH;
-        const float2 ml = *(const float2*)(part + DV), v = *(const float2*)(part + c);
-        const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - m_use);  // (a warp that has seen nothing counts for nothing)
-        l += f * ml.y;
-        x += f * v.x;
-        y += f * v.y;
-      }
-      const float inv = inverse(l);
-      put2((char*)p.o.ptr + (seg.b * p.o.sb + h * p.o.sh + qi * p.o.ss) * ES, c, x * inv, y * inv);
-      if (c == 0 && p.lse != nullptr) p.lse[((long long)seg.b * p.Hq + h) * p.Sq + qi] = log_sum(m_use, l);
-    }
-  }
 }

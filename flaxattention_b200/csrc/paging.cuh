@@ -1,10 +1,16 @@
 // Pages of a key / value cache: places for the new tokens of a batch of requests (fa_page_step) and attention over
 // the pages (fa_paged; its kernel is kernels/fa_paged.cuh).  Part of flaxattn.cu.
+#ifndef PAGED_BOX
+#define PAGED_BOX 32
+#endif
 #ifndef PAGED_SHORT_TILES
 #define PAGED_SHORT_TILES 32
 #endif
 #ifndef PAGED_SHORT_SEGMENTS
 #define PAGED_SHORT_SEGMENTS 2
+#endif
+#ifndef PAGED_WARPS
+#define PAGED_WARPS 4
 #endif
 namespace {
 
@@ -139,7 +145,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) fa_paged_combin
   grid_wait();
   constexpr int U = 4;
   __shared__ float4 sums[WARPS == 1 ? 1 : WARPS][64];
-  __shared__ float totals[WARPS];
+  __shared__ float2 totals[WARPS];
   const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
   const int row = WARPS == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= n_rows) return;
@@ -154,49 +160,55 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) fa_paged_combin
   const int q = r / G, h = hk * G + r - q * G;
   // part of worker c: its first part, but for the first worker's, which begins inside the run
   const auto at = [&](int c) { return ((long long)c * 2 + (c == c0 && begin != c0 * per ? 1 : 0)) * BM + (r - rt * BM); };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[at(c) * 2]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  const float m_use = m == -INFINITY ? 0.f : m;
   const bool second = lane * 4 + 128 < Dv, active = lane * 4 < Dv;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), acc2 = acc;
-  float l = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const auto scale = [&](float f) {
+    l *= f;
+    acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+    acc2.x *= f; acc2.y *= f; acc2.z *= f; acc2.w *= f;
+  };
+  const auto add = [&](float f, float sum, const float4& x, const float4& y) {
+    l += f * sum;
+    acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+    acc2.x += f * y.x; acc2.y += f * y.y; acc2.z += f * y.z; acc2.w += f * y.w;
+  };
+  // (a part that has seen nothing counts for nothing; one whose sum is no number stays so)
+  const auto weight = [](float2 ml, float top) { return ml.y == 0.f ? 0.f : exp2f(ml.x - (top == -INFINITY ? 0.f : top)); };
   for (int c = c0 + warp; c <= c1; c += WARPS * U) {
     float2 ml[U];
     float4 x[U], y[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u) {  // (all of them on their way at once)
       const bool in = c + u * WARPS <= c1;
       const long long a = in ? at(c + u * WARPS) : 0;
       ml[u] = in ? *(const float2*)(p.part_ml + a * 2) : make_float2(-INFINITY, 0.f);
       x[u] = in && active ? *(const float4*)(p.part_o + a * Dv + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
       y[u] = in && second ? *(const float4*)(p.part_o + a * Dv + lane * 4 + 128) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+    float top = m;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // (a part that has seen nothing counts for nothing; one whose sum is no number stays so)
-      const float w = ml[u].y == 0.f ? 0.f : exp2f(ml[u].x - m_use);
-      if (w == 0.f) continue;
-      l += w * ml[u].y;
-      acc.x += w * x[u].x; acc.y += w * x[u].y; acc.z += w * x[u].z; acc.w += w * x[u].w;
-      acc2.x += w * y[u].x; acc2.y += w * y[u].y; acc2.z += w * y[u].z; acc2.w += w * y[u].w;
-    }
+    for (int u = 0; u < U; ++u) top = fmaxf(top, ml[u].x);
+    scale(weight(make_float2(m, l), top));
+    m = top;
+#pragma unroll
+    for (int u = 0; u < U; ++u) add(weight(ml[u], top), ml[u].y, x[u], y[u]);
   }
   if (WARPS > 1) {
     sums[WARPS == 1 ? 0 : warp][lane] = acc;
     sums[WARPS == 1 ? 0 : warp][lane + 32] = acc2;
-    if (lane == 0) totals[warp] = l;
+    if (lane == 0) totals[warp] = make_float2(m, l);
     __syncthreads();
     if (warp != 0) return;
+    float top = m;
 #pragma unroll
-    for (int w = 1; w < WARPS; ++w) {
-      const float4 x = sums[WARPS == 1 ? 0 : w][lane], y = sums[WARPS == 1 ? 0 : w][lane + 32];
-      acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
-      acc2.x += y.x; acc2.y += y.y; acc2.z += y.z; acc2.w += y.w;
-      l += totals[w];
-    }
+    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, totals[w].x);
+    scale(weight(make_float2(m, l), top));
+    m = top;
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) add(weight(totals[w], top), totals[w].y, sums[WARPS == 1 ? 0 : w][lane], sums[WARPS == 1 ? 0 : w][lane + 32]);
   }
+  const float m_use = m == -INFINITY ? 0.f : m;
   const float inv = l > 0.f ? 1.f / l : l;  // (0 and no number stay)
   char* og = (char*)p.o.ptr + ((long long)b * p.o.sb + (long long)h * p.o.sh + (long long)q * p.o.ss) * (DT == FA_F32 ? 4 : 2);
   const auto put = [&](int col, const float4& v) {
@@ -216,14 +228,14 @@ struct FaPagedLaunchHost {
   FaTensorMapHost tk, tv;
 };
 struct PagedCfg {
-  int RG, WN, stages, smem, per_sm, box, few, fr, nw;
-  bool tma;
+  int RG, CG, BM, WN, slots, smem, per_sm, box, few, fr;
+  bool tma, one_each;  // one_each: a CTA per segment (FA_SHORT)
 };
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
 
-// Warps of a CTA that has a segment for itself, or 0: segments are cut.  Where the table has room for few tiles, and where all segments are
+// Key groups of a CTA that has a segment for itself, or 0: segments are cut.  Where the table has room for few tiles, and where all segments are
 // resident at once.
-int paged_short_warps(const fa_paged_params* p, const PagedCfg& c) {
+int paged_short_groups(const fa_paged_params* p, const PagedCfg& c) {
   const long long segments = (long long)p->B * p->Hkv;
   long long keys = (long long)p->table_width * p->page_size;
   if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + p->Sq + c.WN);
@@ -233,45 +245,58 @@ int paged_short_warps(const fa_paged_params* p, const PagedCfg& c) {
 }
 
 // Tiles, buffers and CTAs per SM (the map of fa_paged.cuh).
-//   * Rows: a warp takes 16, of 16-bit types up to 8 in the way made for few; fp32 rounds up to a power of two.
-//   * Keys of a tile: 32; fp32 fewer for wide heads, so that a tile of K and V stays at 16 KB and an SM has room for as many of them.
-//   * Registers allow eight warps per SM at 255 each.  The buffers are as many as fill the shared memory of that many CTAs, two at least.
-//   * Tables with room for few tiles: a CTA per segment (nw warps, two buffers each).
+//   * Rows: a warp takes 16; of 16-bit types up to 8, and 17 to 24 where the registers allow it, in the way made for few (`few` groups of 8);
+//     fp32 rounds up to a power of two.
+//   * Keys of a tile: 32; fewer for wide heads, so that a tile of K or V stays at 8 KB and an SM has room for as many of them.
+//   * CTAs of four warps, two per SM: registers allow eight warps at 255 each, two for each scheduler.  The rings of slots (a tile of K or V) fill
+//     the shared memory; where three slots do not fit, one CTA per SM.
+//   * Tables with room for few tiles: a CTA per segment, four slots for each key group.
 void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   const long long rows = (long long)(p->Hq / p->Hkv) * p->Sq;
   const bool f32 = p->dtype == FA_F32;
   const int es = esize(p->dtype);
-  c.RG = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  c.WN = !f32 || p->D <= 64 ? 32 : p->D <= 128 ? 16 : 8;
-  c.few = !f32 && rows <= 8;
+  c.few = f32 ? 0 : rows <= 8 ? 1 : rows > 16 && rows <= 24 && p->D <= 128 ? 3 : 0;
+  c.RG = rows <= 16 || c.few > 0 ? 1 : rows <= 32 ? 2 : 4;
+  c.BM = c.few > 0 ? c.few * 8 : c.RG * 16;
+  c.WN = !f32 ? (p->D <= 128 ? 32 : 16) : p->D <= 64 ? 32 : p->D <= 128 ? 16 : 8;
   c.fr = 0;
   if (f32)
     for (c.fr = 1; c.fr < std::min<long long>(rows, 16);) c.fr *= 2;
-  c.box = gcd(p->page_size, c.WN);
+  c.box = gcd(p->page_size, std::min(c.WN, PAGED_BOX));
   c.tma = !f32 && p->D % 64 == 0 && p->Dv % 64 == 0 && c.box >= 8 && p->num_pages > 0 && !(p->flags & FA_FLAG_GENERAL_KERNELS);
   if (!c.tma) c.box = 1;
-  const int stage = c.tma ? c.WN * (p->D + p->Dv) * es : c.WN * (pitch(p->D, es) + pitch(p->Dv, es));
-  const int most = 8 / c.RG;
-  const auto fixed = [&](int warps) { return f32 ? (c.RG == 1 ? c.fr : c.RG * 16) * p->D * 4 + warps * c.fr * c.WN * 4 : 0; };
-  for (c.nw = paged_short_warps(p, c); c.nw > 0; c.nw /= 2) {
-    c.stages = 2;
-    c.smem = c.nw * 2 * stage + fixed(c.nw) + (c.tma ? c.nw * 2 * 16 + 16 + 1024 : 0);
-    c.per_sm = 1;
+  const int slot = c.WN * (c.tma ? p->D * es : pitch(p->D, es));  // (K's: the value dim is no larger)
+  const int mrows = f32 && c.RG == 1 ? c.fr : c.BM;
+  const auto smem = [&](int slots) {
+    const int q = f32 ? (c.RG == 1 ? c.fr : c.RG * 16) * p->D * 4 + c.CG * c.RG * c.fr * c.WN * 4 : 0;
+    return c.CG * slots * slot + q + (c.CG > 1 ? c.CG * mrows * 38 * 4 : 0) + (c.tma ? c.CG * slots * 8 + 16 + 1024 : 0);
+  };
+  c.one_each = true;
+  c.per_sm = 1;
+  c.slots = 4;
+  for (c.CG = paged_short_groups(p, c); c.CG > 0; c.CG /= 2) {
+    c.smem = smem(c.slots);
     if (c.smem <= kMaxSmem) return;
   }
-  c.stages = std::min(std::max((226 * 1024 / most - 2048 - fixed(c.RG)) / stage, 2), 4);
-  c.smem = c.stages * stage + fixed(c.RG) + (c.tma ? c.stages * 16 + 16 + 1024 : 0);
-  c.per_sm = std::max(1, std::min(most, 227 * 1024 / (c.smem + 1024)));
+  c.one_each = false;
+  c.CG = std::max(PAGED_WARPS / c.RG, 1);
+  for (c.per_sm = 8 / (c.CG * c.RG);; c.per_sm /= 2) {
+    const int room = std::min(227 * 1024 / c.per_sm - 1024, kMaxSmem);
+    for (c.slots = 8; c.slots > 2 && smem(c.slots) > room;) --c.slots;
+    if (c.slots >= 3 || c.per_sm == 1) break;
+  }
+  c.smem = smem(c.slots);
 }
 int paged_row_tiles(const fa_paged_params* p, const PagedCfg& c) {
-  return (int)(((long long)(p->Hq / p->Hkv) * p->Sq + c.RG * 16 - 1) / (c.RG * 16));
+  return (int)(((long long)(p->Hq / p->Hkv) * p->Sq + c.BM - 1) / c.BM);
 }
 int paged_workers(const PagedCfg& c) { return c.per_sm * device_sm_count(); }
 
 int get_paged_kernel(fa_module* m, const fa_paged_params* p, const PagedCfg& c, Kernel** k) {
-  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.stages, 3}, {c.tma ? 1 : 0, 1}, {c.few, 1}, {c.fr, 5}, {c.nw, 4}}), "fa_paged.cuh",
-                    [&] { return defs({{"FA_DTYPE", p->dtype}, {"FA_D", p->D}, {"FA_DV", p->Dv}, {"FA_RG", c.RG}, {"FA_WN", c.WN},
-                                       {"FA_STAGES", c.stages}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_NW", c.nw}}); },
+  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.slots, 4}, {c.tma ? 1 : 0, 1}, {c.few, 2}, {c.fr, 5}, {c.CG, 4}, {c.one_each ? 1 : 0, 1}}), "fa_paged.cuh",
+                    [&] { return std::string(p->dtype == FA_F32 ? "" : "#include \"fa_tanh.cuh\"\n") +
+                                defs({{"FA_DTYPE", p->dtype}, {"FA_D", p->D}, {"FA_DV", p->Dv}, {"FA_RG", c.RG}, {"FA_WN", c.WN},
+                                       {"FA_SLOTS", c.slots}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_CG", c.CG}, {"FA_SHORT", c.one_each ? 1 : 0}}); },
                     "fa_paged_kernel", c.smem, k);
 }
 
@@ -337,8 +362,8 @@ size_t fa_paged_workspace_bytes(const fa_paged_params* p) {
     q.flags = flags;
     PagedCfg c;
     pick_paged(&q, c);
-    if (c.nw > 0) continue;
-    const size_t rows = 2 * (size_t)paged_workers(c) * c.RG * 16;
+    if (c.one_each) continue;
+    const size_t rows = 2 * (size_t)paged_workers(c) * c.BM;
     most = std::max(most, paged_up(rows * p->Dv * 4) + paged_up(rows * 8) + paged_up(((size_t)p->B * paged_row_tiles(p, c) + 1) * 4));
   }
   return most;
@@ -389,23 +414,24 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
   k.row_tiles = paged_row_tiles(p, c);
   k.workers = paged_workers(c);
   k.min_tiles = 1;
-  const size_t rows = 2 * (size_t)k.workers * c.RG * 16;
+  const size_t rows = 2 * (size_t)k.workers * c.BM;
   k.part_o = (float*)workspace;
   k.part_ml = (float*)((char*)workspace + paged_up(rows * p->Dv * 4));
   k.plan = (int*)((char*)k.part_ml + paged_up(rows * 8));
   k.box = c.box;
   Kernel* kernel = nullptr;
   if (int rc = get_paged_kernel(m, p, c, &kernel)) return rc;
-  if (c.nw > 0) return launch(kernel, dim3((unsigned)((long long)p->B * k.row_tiles * p->Hkv)), dim3(c.nw * 32), &L, stream);
-  if (int rc = launch(kernel, dim3((unsigned)k.workers), dim3(c.RG * 32), &L, stream)) return rc;
+  const dim3 block((unsigned)(c.CG * c.RG * 32));
+  if (c.one_each) return launch(kernel, dim3((unsigned)((long long)p->B * k.row_tiles * p->Hkv)), block, &L, stream);
+  if (int rc = launch(kernel, dim3((unsigned)k.workers), block, &L, stream)) return rc;
   // Few segments for the workers: many parts each, and eight warps add up a row's.
   const long long segments = (long long)p->B * k.row_tiles * p->Hkv;
   const int n_rows = p->B * p->Hq * p->Sq;
   const bool wide = k.workers / segments >= 16;
   return rot_dispatch(p->dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    return wide ? launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 8>, dim3((unsigned)n_rows), dim3(256), stream, k, c.RG * 16, p->Dv, n_rows)
-                : launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 1>, dim3((unsigned)((n_rows + 3) / 4)), dim3(128), stream, k, c.RG * 16, p->Dv, n_rows);
+    return wide ? launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 8>, dim3((unsigned)n_rows), dim3(256), stream, k, c.BM, p->Dv, n_rows)
+                : launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 1>, dim3((unsigned)((n_rows + 3) / 4)), dim3(128), stream, k, c.BM, p->Dv, n_rows);
   });
 }
 
