@@ -77,6 +77,7 @@ constexpr int MROWS = F32 && RG == 1 ? FR : BM, MPITCH = 36;
 constexpr int MERGE_BYTES = CG > 1 ? CG * MROWS * (MPITCH + 2) * 4 : 0;
 constexpr int BAR_BYTES = TMA ? CG * SLOTS * 8 + 16 : 0;
 constexpr int SMEM_BYTES = CG * PIPE_BYTES + Q_BYTES + MERGE_BYTES + BAR_BYTES + (TMA ? 1024 : 0);
+constexpr float RISE = 8.f;  // (log2 units) what scores may rise before a row's maximum is looked for again
 constexpr fa_u32 ALL = WN == 32 ? 0xffffffffu : (1u << (WN & 31)) - 1u;  // every key of a tile
 static_assert(!TMA || (!F32 && D % 64 == 0 && DV % 64 == 0), "TMA: 16-bit types, whole column groups");
 static_assert(F32 || WN == 32 || WN == 16, "tiles of 16 or 32 keys");
@@ -89,10 +90,12 @@ struct Seg {
   int pos;
   int end;    // keys from here on are behind every row
   int tile, last;  // tiles of WN keys, first and one beyond the last
+  const int* pages;  // row of the block table
 };
 __device__ __forceinline__ void seg_open(const FaPagedParams& p, int item, Seg& s) {
   s.item = item;
   s.b = p.row_tiles == 1 ? item : item / p.row_tiles;
+  s.pages = p.table + s.b * p.table_stride;
   const int rt = item - s.b * p.row_tiles, G = p.Hq / p.Hkv;
   const int len = min(max(p.lengths[s.b], 0), p.max_len);
   s.first = rt * BM / G;
@@ -128,6 +131,7 @@ struct Load {
   int page;     // this lane's, or -1: no such key, or no such page
   int row;      // token in it
   fa_u32 keep;  // keys of the tile that are there, bit by bit
+  fa_u32 boxes; // lanes with a page
 };
 
 // The rows of a tile in 16-byte pieces, those that are not there as zeros
@@ -533,7 +537,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
     if (there) {
       const int slot = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
       n.row = key - slot * p.page_size;
-      n.page = p.table[ahead.b * p.table_stride + slot];
+      n.page = ahead.pages[slot];
     }
     // (the keys that are there go along; those whose page is none are taken out when the entry has come)
     const int left = ahead.end - ahead.tile * WN;
@@ -545,6 +549,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
     const bool there = lane * p.box < WN && ((n.keep >> (lane * p.box)) & 1u);
     const bool bad = there && (n.page < 0 || n.page >= p.num_pages);
     if (bad) n.page = -1;
+    n.boxes = __ballot_sync(0xffffffffu, n.page >= 0);
     fa_u32 out = __ballot_sync(0xffffffffu, bad);
     if (out != 0) {
       if (lane == 0 && p.status != nullptr) atomicOr(p.status, FA_STATUS_BAD_PAGE);
@@ -557,8 +562,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
 #if FA_TMA
   auto load = [&](const FaTensorMap* map, fa_u32 dst, fa_u32 bar, int atoms, const Load& n) {
     if (rg != 0) return;
-    const fa_u32 boxes = __ballot_sync(0xffffffffu, n.page >= 0);
-    if (lane == 0) fa_mbar_expect_tx(bar, __popc(boxes) * p.box * 128 * atoms);
+    if (lane == 0) fa_mbar_expect_tx(bar, __popc(n.boxes) * p.box * 128 * atoms);
     __syncwarp();
     if (n.page >= 0) {
       for (int a = 0; a < atoms; ++a)
@@ -675,6 +679,8 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
 
     // ---- the tiles of this key group (a group whose wait has run out leaves them out, but takes part in the merges)
     for (int tile = seg.tile + (CG - (t - t0) % CG + cg) % CG; tile < part_end && !failed; tile += CG) {
+      // (its pages were looked up a tile ago; here, so that nothing waits for them when a slot is free)
+      if (next.any) settle(next);
       int at = arrived();
       R.scores(bufs + at * SLOT_BYTES, ring + at * SLOT_BYTES, rows);
       used();
@@ -684,10 +690,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
         if (pending.any) load_v(at, pending);
         asked += pending.any;
       } else {
-        if (next.any) {
-          settle(next);
-          load_k(at, next);
-        }
+        if (next.any) load_k(at, next);
         asked += next.any;
       }
       fa_cp_commit();
@@ -698,10 +701,14 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
       // does any row of the tile have to look at the positions?
       const bool edge = n0 + WN - 1 > seg.pos || (p.window >= 0 && n0 < seg.end - 1 - p.window) || kept != ALL;
       const int gb = seg.b + p.b_off;
-      float mx[HR];
+      // Scores are taken relative to a maximum that need not be the present one: as long as none is more than 2^RISE times what a row's
+      // maximum was when it was last looked for, probabilities stay in range, and one vote takes the place of the lanes' search for it (and of
+      // the correction of O), which a warp would wait for in every tile.
+      float top[HR];
+      bool rises = false;
 #pragma unroll
       for (int h = 0; h < HR; ++h) {
-        mx[h] = FA_NEG_INF;
+        top[h] = FA_NEG_INF;
         if (R.idle(h, rows)) continue;  // (the rows of all lanes)
         [[maybe_unused]] const int qp = max(qpos[h], 0), gh = head[h] + p.h_off;
 #pragma unroll
@@ -729,18 +736,19 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
           }
         }
 #pragma unroll
-        for (int j = 0; j < NS; ++j) mx[h] = fmaxf(mx[h], R.score(h, j));
+        for (int j = 0; j < NS; ++j) top[h] = fmaxf(top[h], R.score(h, j));
+        rises |= top[h] > R.m[h] + RISE;
       }
-      Rows::over_keys(mx, Max());
-      float corr[HR];
-      bool moved = false;
+      if (__any_sync(0xffffffffu, rises)) {
+        Rows::over_keys(top, Max());
 #pragma unroll
-      for (int h = 0; h < HR; ++h) {
-        const float m_new = fmaxf(R.m[h], mx[h]);
-        mx[h] = m_new == FA_NEG_INF ? 0.f : m_new;
-        corr[h] = fa_ex2(R.m[h] - mx[h]);
-        R.m[h] = m_new;
-        moved |= corr[h] != 1.f && !R.idle(h, rows);
+        for (int h = 0; h < HR; ++h) {
+          const float m_new = fmaxf(R.m[h], top[h]);
+          const float corr = fa_ex2(R.m[h] - (m_new == FA_NEG_INF ? 0.f : m_new));
+          R.m[h] = m_new;
+          R.l[h] *= corr;
+          R.rescale(h, corr);
+        }
       }
 #pragma unroll
       for (int h = 0; h < HR; ++h) {
@@ -749,19 +757,15 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
           for (int j = 0; j < NS; ++j) R.score(h, j) = 0.f;
           continue;
         }
+        const float m = R.m[h] == FA_NEG_INF ? 0.f : R.m[h];
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-          const float e = fa_ex2(R.score(h, j) - mx[h]);
+          const float e = fa_ex2(R.score(h, j) - m);
           R.score(h, j) = e;
           sum += e;
         }
-        R.l[h] = R.l[h] * corr[h] + sum;
-      }
-      // (after the first tiles the maximum seldom moves)
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int h = 0; h < HR; ++h) R.rescale(h, corr[h]);
+        R.l[h] += sum;
       }
 
       at = arrived();
@@ -781,10 +785,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
       used();
       if (failed) break;
       if (ODD) {
-        if (next.any) {
-          settle(next);
-          load_k(at, next);
-        }
+        if (next.any) load_k(at, next);
         asked += next.any;
         pending = next;
       } else {
