@@ -498,13 +498,14 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// A tensor over a part of `base`'s storage, contiguous, starting `offset` elements in.
-at::Tensor part(const at::Tensor& base, int64_t offset, at::IntArrayRef sizes) {
-  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), base.dtype());
+// A tensor over a part of `base`'s storage, contiguous, starting `offset` elements (of its own type) in.
+at::Tensor part(const at::Tensor& base, int64_t offset, at::IntArrayRef sizes, caffe2::TypeMeta type) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), type);
   impl->set_sizes_contiguous(sizes);
   impl->set_storage_offset(offset);
   return at::Tensor(std::move(impl));
 }
+at::Tensor part(const at::Tensor& base, int64_t offset, at::IntArrayRef sizes) { return part(base, offset, sizes, base.dtype()); }
 
 // The tensors of a tuple (at most 8)
 std::vector<at::Tensor> tensors(PyObject* o) {
@@ -997,25 +998,24 @@ PyObject* page_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release no_gil;
     c10::cuda::OptionalCUDAGuard guard(dev);
-    // one allocation for the tensors of 32 bits, in parts that begin at 16 bytes
-    const auto up = [](int64_t v) { return (v + 3) / 4 * 4; };
-    const int64_t sizes[5] = {B, tokens, tokens, B + 1, 1};
+    // one allocation, in parts that begin at 16 bytes
+    const int64_t sizes[6] = {B, tokens, tokens, tokens, B + 1, 1};
     int64_t all = 0, off = 0;
-    for (int64_t s : sizes) all += up(s);
-    at::Tensor base = empty({all}, at::kInt, dev);
-    for (int64_t s : sizes) {
-      out.push_back(part(base, off, {s}));
-      off += up(s);
+    for (int i = 0; i < 6; ++i) all += (sizes[i] * (i == 2 ? 8 : 4) + 15) / 16 * 16;
+    const at::Tensor base = empty({all}, at::kByte, dev);
+    void* ptr[6];
+    for (int i = 0; i < 6; ++i) {
+      const int64_t bytes = i == 2 ? 8 : 4;
+      out.push_back(part(base, off / bytes, {sizes[i]}, i == 2 ? caffe2::TypeMeta::Make<int64_t>() : caffe2::TypeMeta::Make<int32_t>()));
+      ptr[i] = (char*)base.mutable_data_ptr() + off;
+      off += (sizes[i] * bytes + 15) / 16 * 16;
     }
-    at::Tensor slots = empty({tokens}, at::kLong, dev);
-    const auto at32 = [&](int i) { return (int32_t*)out[i].mutable_data_ptr(); };
     const int rc = fa_page_step((const int32_t*)lengths.const_data_ptr(), (const int32_t*)fresh.const_data_ptr(), (int)B, (int32_t*)table.data_ptr(), table.stride(0),
                                 (int)table.size(1), (const int32_t*)pool.const_data_ptr(), pool.size(0),
-                                taken.defined() ? (const int32_t*)taken.const_data_ptr() : nullptr, (int)page, tokens, at32(0), at32(1),
-                                (int64_t*)slots.mutable_data_ptr(), at32(2), at32(3), at32(4), (void*)c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+                                taken.defined() ? (const int32_t*)taken.const_data_ptr() : nullptr, (int)page, tokens, (int32_t*)ptr[0], (int32_t*)ptr[1],
+                                (int64_t*)ptr[2], (int32_t*)ptr[3], (int32_t*)ptr[4], (int32_t*)ptr[5], (void*)c10::cuda::getCurrentCUDAStream(dev.index()).stream());
     if (rc != FA_OK) raise(rc);
     written(table);
-    out.insert(out.begin() + 2, slots);
   }
   PyObject* t = PyTuple_New(6);
   if (t == nullptr) return nullptr;
