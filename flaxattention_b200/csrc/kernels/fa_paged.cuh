@@ -36,7 +36,7 @@
 struct FaPagedLaunch {
   FaPagedParams p;
 #if FA_TMA
-  FaTensorMap tk, tv;  // 4-d maps (D, token in page, head, page), box 64 x p.box x 1 x 1, 128-byte swizzle
+  FaTensorMap tk, tv;  // 4-d maps (D, token in page, head, page), box 128 bytes x p.box x 1 x 1, 128-byte swizzle
 #endif
 };
 
@@ -60,7 +60,7 @@ constexpr int SLOTS = FA_SLOTS;
 constexpr int ES = F32 ? 4 : 2;
 constexpr int PK = TMA ? D * ES : FaTile<D, ES>::PITCH;
 constexpr int PV = TMA ? DV * ES : FaTile<DV, ES>::PITCH;
-constexpr int ATOMS_K = D / 64, ATOMS_V = DV / 64;  // 128-byte column groups of a row (TMA)
+constexpr int ATOMS_K = D * ES / 128, ATOMS_V = DV * ES / 128;  // 128-byte column groups of a row (TMA)
 // A key group's buffers are a ring of slots that take a tile of K or of V: K, V, K of the next, ..; what was in a slot has been used up, and the
 // tile half a ring ahead is asked for.  Eight warps per SM, two for each of its schedulers, so that one's products run under the other's
 // softmax (D 128, up to 8 rows: a warp alone takes 1.5 us per tile, and four per SM with any number of slots 187 us where eight take 180).
@@ -79,7 +79,7 @@ constexpr int BAR_BYTES = TMA ? CG * SLOTS * 8 + 16 : 0;
 constexpr int SMEM_BYTES = CG * PIPE_BYTES + Q_BYTES + MERGE_BYTES + BAR_BYTES + (TMA ? 1024 : 0);
 constexpr float RISE = 8.f;  // (log2 units) what scores may rise before a row's maximum is looked for again
 constexpr fa_u32 ALL = WN == 32 ? 0xffffffffu : (1u << (WN & 31)) - 1u;  // every key of a tile
-static_assert(!TMA || (!F32 && D % 64 == 0 && DV % 64 == 0), "TMA: 16-bit types, whole column groups");
+static_assert(!TMA || (D * ES % 128 == 0 && DV * ES % 128 == 0), "TMA: whole column groups");
 static_assert(F32 || WN == 32 || WN == 16, "tiles of 16 or 32 keys");
 static_assert(!FEW || (RG == 1 && !F32), "few rows: one warp, 16-bit types");
 
@@ -190,24 +190,34 @@ struct Rows {
     for (int i = 0; i < NC; ++i) o[h][i] *= c;
   }
   __device__ __forceinline__ void scores(const unsigned char* tile, fa_u32, int rows) {
-    const unsigned char* k = tile + (lane % WN) * PK + (lane / WN) * (D / PARTS * 4);
+    // (four sums for a product, two to an instruction: a chain of D / PARTS additions would be waited for)
     const float* qp = q + (lane / WN) * (D / PARTS);
+    const int r = lane % WN, c0 = (lane / WN) * (D / PARTS / 4);
+    fa_u64 acc[HR][2];
 #pragma unroll
-    for (int h = 0; h < HR; ++h) s[h] = 0.f;
+    for (int h = 0; h < HR; ++h) acc[h][0] = acc[h][1] = 0ull;
 #pragma unroll 4
     for (int c = 0; c < D / PARTS / 4; ++c) {
-      const float4 x = *(const float4*)(k + c * 16);
+      const ulonglong2 x = *(const ulonglong2*)(tile + chunk_at<PK>(0, r, c0 + c));
 #pragma unroll
       for (int h = 0; h < HR; ++h) {
         if (HR > 4 && idle(h, rows)) break;
-        const float4 y = *(const float4*)(qp + h * D + c * 4);
-        s[h] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[h]))));
+        const ulonglong2 y = *(const ulonglong2*)(qp + h * D + c * 4);
+        acc[h][0] = fa_fma2(x.x, y.x, acc[h][0]);
+        acc[h][1] = fa_fma2(x.y, y.y, acc[h][1]);
       }
     }
 #pragma unroll
-    for (int h = 0; h < HR; ++h)
+    for (int h = 0; h < HR; ++h) {
+      float x0, x1, x2, x3;
+      fa_f2_unpack(acc[h][0], x0, x1);
+      fa_f2_unpack(acc[h][1], x2, x3);
+      s[h] = (x0 + x1) + (x2 + x3);
+    }
 #pragma unroll
-      for (int off = WN; off < 32; off <<= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], off);
+    for (int off = WN; off < 32; off <<= 1)
+#pragma unroll
+      for (int h = 0; h < HR; ++h) s[h] += __shfl_xor_sync(0xffffffffu, s[h], off);
   }
   __device__ __forceinline__ void values(const unsigned char* tile, fa_u32, int rows) {
     __syncwarp();
@@ -215,20 +225,48 @@ struct Rows {
     for (int h = 0; h < HR; ++h)
       if (lane < WN) probs[h * WN + lane] = s[h];
     __syncwarp();
+    // (few rows: even and odd keys apart, two to an instruction)
+    constexpr bool APART = HR * NC <= 16;
+    fa_u64 acc[APART ? HR : 1][APART ? NC : 1];
+    if (APART) {
+#pragma unroll
+      for (int h = 0; h < (APART ? HR : 1); ++h)
+#pragma unroll
+        for (int i = 0; i < (APART ? NC : 1); ++i) acc[h][i] = 0ull;
+    }
 #pragma unroll 2
     for (int j = 0; j < WN; j += 4) {
       float v[4][NC];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 0; i < NC; ++i) v[e][i] = lane + 32 * i < DV ? *(const float*)(tile + (j + e) * PV + (lane + 32 * i) * 4) : 0.f;
+        for (int i = 0; i < NC; ++i) {
+          const int c = lane + 32 * i;
+          v[e][i] = c < DV ? *(const float*)(tile + chunk_at<PV>(0, j + e, c >> 2) + (c & 3) * 4) : 0.f;
+        }
 #pragma unroll
       for (int h = 0; h < HR; ++h) {
         if (HR > 4 && idle(h, rows)) break;
-        const float4 x = *(const float4*)(probs + h * WN + j);
+        if constexpr (APART) {
+          const ulonglong2 x = *(const ulonglong2*)(probs + h * WN + j);
 #pragma unroll
-        for (int i = 0; i < NC; ++i) o[h][i] = fmaf(x.x, v[0][i], fmaf(x.y, v[1][i], fmaf(x.z, v[2][i], fmaf(x.w, v[3][i], o[h][i]))));
+          for (int i = 0; i < NC; ++i) acc[h][i] = fa_fma2(x.y, fa_f2(v[2][i], v[3][i]), fa_fma2(x.x, fa_f2(v[0][i], v[1][i]), acc[h][i]));
+        } else {
+          const float4 x = *(const float4*)(probs + h * WN + j);
+#pragma unroll
+          for (int i = 0; i < NC; ++i) o[h][i] = fmaf(x.x, v[0][i], fmaf(x.y, v[1][i], fmaf(x.z, v[2][i], fmaf(x.w, v[3][i], o[h][i]))));
+        }
       }
+    }
+    if constexpr (APART) {
+#pragma unroll
+      for (int h = 0; h < HR; ++h)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          float x, y;
+          fa_f2_unpack(acc[h][i], x, y);
+          o[h][i] += x + y;
+        }
     }
   }
   // f(h, column, value) for every value of this thread in columns 32 i ..
@@ -566,7 +604,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __
     __syncwarp();
     if (n.page >= 0) {
       for (int a = 0; a < atoms; ++a)
-        fa_tma_load_4d(dst + a * (WN * 128) + lane * p.box * 128, map, bar, a * 64, n.row, n.hk, n.page);
+        fa_tma_load_4d(dst + a * (WN * 128) + lane * p.box * 128, map, bar, a * (128 / ES), n.row, n.hk, n.page);
     }
   };
   auto load_k = [&](int slot, const Load& n) { load(&L.tk, ring + slot * SLOT_BYTES, bars + slot * 8, ATOMS_K, n); };

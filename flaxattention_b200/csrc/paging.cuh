@@ -1,17 +1,5 @@
 // Pages of a key / value cache: places for the new tokens of a batch of requests (fa_page_step) and attention over
 // the pages (fa_paged; its kernel is kernels/fa_paged.cuh).  Part of flaxattn.cu.
-#ifndef PAGED_BOX
-#define PAGED_BOX 32
-#endif
-#ifndef PAGED_SHORT_TILES
-#define PAGED_SHORT_TILES 32
-#endif
-#ifndef PAGED_SHORT_SEGMENTS
-#define PAGED_SHORT_SEGMENTS 2
-#endif
-#ifndef PAGED_WARPS
-#define PAGED_WARPS 4
-#endif
 namespace {
 
 // ---- block tables, slots and positions of new tokens --------------------------------------
@@ -285,24 +273,15 @@ struct PagedCfg {
 };
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
 
-// Key groups of a CTA that has a segment for itself, or 0: segments are cut.  Where the table has room for few tiles, and where all segments are
-// resident at once.
-int paged_short_groups(const fa_paged_params* p, const PagedCfg& c) {
-  const long long segments = (long long)p->B * p->Hkv;
-  long long keys = (long long)p->table_width * p->page_size;
-  if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + p->Sq + c.WN);
-  const long long tiles = (keys + c.WN - 1) / c.WN;
-  if (c.RG != 1 || tiles > PAGED_SHORT_TILES || segments > PAGED_SHORT_SEGMENTS * (long long)device_sm_count()) return 0;
-  return tiles <= 8 ? 4 : 8;
-}
-
 // Tiles, buffers and CTAs per SM (the map of fa_paged.cuh).
 //   * Rows: a warp takes 16; of 16-bit types up to 8, and 17 to 24 where the registers allow it, in the way made for few (`few` groups of 8);
 //     fp32 rounds up to a power of two.
 //   * Keys of a tile: 32; fewer for wide heads, so that a tile of K or V stays at 8 KB and an SM has room for as many of them.
 //   * CTAs of four warps, two per SM: registers allow eight warps at 255 each, two for each scheduler.  The rings of slots (a tile of K or V) fill
 //     the shared memory; where three slots do not fit, one CTA per SM.
-//   * Tables with room for few tiles: a CTA per segment, four slots for each key group.
+//   * No more segments than SMs and tables with room for four tiles per key group (or as many as are resident at once and one tile): a CTA per segment. (us on the
+//     GPU, cut / a CTA each: 64 segments of 32 tiles, D 64, eight groups 12.1 / 8.7; D 128, four groups, 8 tiles 9.3 / 7.0, 16 10.2 / 9.8, 32 14.6 /
+//     15.5; 256 segments of 8 tiles 14.2 / 13.1, of 16 16.6 / 18.8.  One launch instead of two also saves the host 2.5 us.)
 void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   const long long rows = (long long)(p->Hq / p->Hkv) * p->Sq;
   const bool f32 = p->dtype == FA_F32;
@@ -314,8 +293,8 @@ void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   c.fr = 0;
   if (f32)
     for (c.fr = 1; c.fr < std::min<long long>(rows, 16);) c.fr *= 2;
-  c.box = gcd(p->page_size, std::min(c.WN, PAGED_BOX));
-  c.tma = !f32 && p->D % 64 == 0 && p->Dv % 64 == 0 && c.box >= 8 && p->num_pages > 0 && !(p->flags & FA_FLAG_GENERAL_KERNELS);
+  c.box = gcd(p->page_size, c.WN);
+  c.tma = p->D * es % 128 == 0 && p->Dv * es % 128 == 0 && c.box >= 8 && p->num_pages > 0 && !(p->flags & FA_FLAG_GENERAL_KERNELS);
   if (!c.tma) c.box = 1;
   const int slot = c.WN * (c.tma ? p->D * es : pitch(p->D, es));  // (K's: the value dim is no larger)
   const int mrows = f32 && c.RG == 1 ? c.fr : c.BM;
@@ -323,15 +302,22 @@ void pick_paged(const fa_paged_params* p, PagedCfg& c) {
     const int q = f32 ? (c.RG == 1 ? c.fr : c.RG * 16) * p->D * 4 + c.CG * c.RG * c.fr * c.WN * 4 : 0;
     return c.CG * slots * slot + q + (c.CG > 1 ? c.CG * mrows * 38 * 4 : 0) + (c.tma ? c.CG * slots * 8 + 16 + 1024 : 0);
   };
+  long long keys = (long long)p->table_width * p->page_size;
+  if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + p->Sq + c.WN);
+  const long long segments = (long long)p->B * p->Hkv;
   c.one_each = true;
   c.per_sm = 1;
   c.slots = 4;
-  for (c.CG = paged_short_groups(p, c); c.CG > 0; c.CG /= 2) {
+  for (c.CG = 8; c.RG == 1 && c.CG >= 4 && segments <= device_sm_count(); c.CG /= 2) {
     c.smem = smem(c.slots);
-    if (c.smem <= kMaxSmem) return;
+    if (c.smem <= kMaxSmem && keys <= 4LL * c.CG * c.WN) return;
   }
+  c.CG = 4;
+  c.slots = 2;  // (a tile for each group at most: nothing to ask for ahead)
+  c.smem = smem(c.slots);
+  if (c.RG == 1 && keys <= (long long)c.CG * c.WN && c.smem <= kMaxSmem && segments <= (long long)device_sm_count() * (227 * 1024 / (c.smem + 1024))) return;
   c.one_each = false;
-  c.CG = std::max(PAGED_WARPS / c.RG, 1);
+  c.CG = 4 / c.RG;
   for (c.per_sm = 8 / (c.CG * c.RG);; c.per_sm /= 2) {
     const int room = std::min(227 * 1024 / c.per_sm - 1024, kMaxSmem);
     for (c.slots = 8; c.slots > 2 && smem(c.slots) > room;) --c.slots;
