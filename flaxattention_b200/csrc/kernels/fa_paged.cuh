@@ -477,7 +477,7 @@ __device__ __forceinline__ bool group_sync(int cg, bool v) {
 
 }  // namespace fa_pg
 
-extern "C" __global__ void __launch_bounds__(fa_pg::NT) fa_paged_kernel(const __grid_constant__ FaPagedLaunch L) {
+extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel(const __grid_constant__ FaPagedLaunch L) {
   using namespace fa_pg;
   const FaPagedParams& p = L.p;
   extern __shared__ __align__(128) unsigned char smem_raw[];

@@ -277,11 +277,16 @@ int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
 //   * Rows: a warp takes 16; of 16-bit types up to 8, and 17 to 24 where the registers allow it, in the way made for few (`few` groups of 8);
 //     fp32 rounds up to a power of two.
 //   * Keys of a tile: 32; fewer for wide heads, so that a tile of K or V stays at 8 KB and an SM has room for as many of them.
-//   * CTAs of four warps, two per SM: registers allow eight warps at 255 each, two for each scheduler.  The rings of slots (a tile of K or V) fill
-//     the shared memory; where three slots do not fit, one CTA per SM.
-//   * No more segments than SMs and tables with room for four tiles per key group (or as many as are resident at once and one tile): a CTA per segment. (us on the
-//     GPU, cut / a CTA each: 64 segments of 32 tiles, D 64, eight groups 12.1 / 8.7; D 128, four groups, 8 tiles 9.3 / 7.0, 16 10.2 / 9.8, 32 14.6 /
-//     15.5; 256 segments of 8 tiles 14.2 / 13.1, of 16 16.6 / 18.8.  One launch instead of two also saves the host 2.5 us.)
+//   * CTAs of four warps, as many per SM as hold two slots (a tile of K and one of V) for each key group, up to four: that many warps hide each
+//     other's waits, and more slots for fewer do not (us, two CTAs with three or more slots / three or four with two: 32 requests of up to 16384 keys D 128
+//     191 / 182, one of 131072 88 / 84, 300 of up to 700 D 64 78 / 58, D 96 105 / 87, fp32 D 64 103 / 99).  Two where registers are short: more than 8
+//     rows of wide heads (D 128, 12 rows 37 / 41), two and four row groups.
+//   * A CTA per segment, one launch and no parts, instead of cut segments:
+//     - no more segments than SMs, and tables with room for four tiles per key group: as many groups as fit, four slots each.  (us on the GPU, cut / a
+//       CTA each: 64 segments of 32 tiles, D 64, eight groups 12.1 / 8.7; D 128, four groups, 8 tiles 9.3 / 7.0, 16 10.2 / 9.8, 32 14.6 / 15.5.)
+//     - more segments, and tables with room for 64 tiles (32 while they would not fill the SMs one and a half times): four groups.  The SMs take a
+//       segment when they have done one, while a cut run ends and begins inside segments.  (1024 segments of up to 64 tiles, D 128 108 / 95, 512 of 16, D 64
+//       30 / 9.4, 256 of 4 13 / 4.4; of up to 256 tiles 98 / 114: the longest is waited for.)
 void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   const long long rows = (long long)(p->Hq / p->Hkv) * p->Sq;
   const bool f32 = p->dtype == FA_F32;
@@ -304,25 +309,29 @@ void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   };
   long long keys = (long long)p->table_width * p->page_size;
   if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + p->Sq + c.WN);
-  const long long segments = (long long)p->B * p->Hkv;
+  const long long segments = (long long)p->B * p->Hkv, sms = device_sm_count();
+  const int most = c.RG > 1 || (f32 ? c.fr > 8 : c.few != 1 && p->D > 64) ? 2 : c.few == 1 || f32 ? 4 : 3;  // CTAs of an SM
+  // as many as there is room for with `slots`
+  const auto fit = [&](int slots) {
+    for (c.per_sm = most; c.per_sm > 1 && smem(slots) > 227 * 1024 / c.per_sm - 1024;) --c.per_sm;
+  };
   c.one_each = true;
-  c.per_sm = 1;
-  c.slots = 4;
-  for (c.CG = 8; c.RG == 1 && c.CG >= 4 && segments <= device_sm_count(); c.CG /= 2) {
-    c.smem = smem(c.slots);
-    if (c.smem <= kMaxSmem && keys <= 4LL * c.CG * c.WN) return;
+  if (c.RG == 1 && segments <= sms) {
+    c.per_sm = 1;
+    c.slots = 4;
+    for (c.CG = 8; c.CG >= 4; c.CG /= 2) {
+      c.smem = smem(c.slots);
+      if (c.smem <= kMaxSmem && keys <= 4LL * c.CG * c.WN) return;
+    }
   }
-  c.CG = 4;
-  c.slots = 2;  // (a tile for each group at most: nothing to ask for ahead)
-  c.smem = smem(c.slots);
-  if (c.RG == 1 && keys <= (long long)c.CG * c.WN && c.smem <= kMaxSmem && segments <= (long long)device_sm_count() * (227 * 1024 / (c.smem + 1024))) return;
-  c.one_each = false;
   c.CG = 4 / c.RG;
-  for (c.per_sm = 8 / (c.CG * c.RG);; c.per_sm /= 2) {
-    const int room = std::min(227 * 1024 / c.per_sm - 1024, kMaxSmem);
-    for (c.slots = 8; c.slots > 2 && smem(c.slots) > room;) --c.slots;
-    if (c.slots >= 3 || c.per_sm == 1) break;
-  }
+  c.slots = 2;
+  fit(c.slots);
+  c.smem = smem(c.slots);
+  if (c.RG == 1 && segments > sms && keys <= (2 * segments > 3 * sms ? 64LL : 32LL) * c.WN) return;
+  c.one_each = false;
+  const int room = std::min(227 * 1024 / c.per_sm - 1024, kMaxSmem);
+  while (c.slots < 8 && smem(c.slots + 1) <= room) ++c.slots;
   c.smem = smem(c.slots);
 }
 int paged_row_tiles(const fa_paged_params* p, const PagedCfg& c) {
@@ -333,10 +342,10 @@ int paged_workers(const PagedCfg& c) { return c.per_sm * device_sm_count(); }
 // 16-bit types: a score_mod's divisions to two units in the last place of fp32, without the branches of exact ones (a score of 30 is then off by 4e-6,
 // its probability by as much in proportion, where the rounding of results to fp16 takes 5e-4).
 int get_paged_kernel(fa_module* m, const fa_paged_params* p, const PagedCfg& c, Kernel** k) {
-  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.slots, 4}, {c.tma ? 1 : 0, 1}, {c.few, 2}, {c.fr, 5}, {c.CG, 4}, {c.one_each ? 1 : 0, 1}}), "fa_paged.cuh",
+  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.slots, 4}, {c.tma ? 1 : 0, 1}, {c.few, 2}, {c.fr, 5}, {c.CG, 4}, {c.one_each ? 1 : 0, 1}, {c.per_sm, 3}}), "fa_paged.cuh",
                     [&] { return std::string(p->dtype == FA_F32 ? "" : "#include \"fa_tanh.cuh\"\n") +
                                 defs({{"FA_DTYPE", p->dtype}, {"FA_D", p->D}, {"FA_DV", p->Dv}, {"FA_RG", c.RG}, {"FA_WN", c.WN},
-                                       {"FA_SLOTS", c.slots}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_CG", c.CG}, {"FA_SHORT", c.one_each ? 1 : 0}}); },
+                                       {"FA_SLOTS", c.slots}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_CG", c.CG}, {"FA_SHORT", c.one_each ? 1 : 0}, {"FA_CTAS", c.per_sm}}); },
                     "fa_paged_kernel", c.smem, k, p->dtype == FA_F32 ? nullptr : "--prec-div=false");
 }
 
