@@ -660,11 +660,13 @@ void no_gradient(const at::Tensor& t, const char* name, const char* call) {
   TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), call, " has no gradient, but ", name, " requires one; call it under torch.no_grad()");
 }
 fa_tensor by_strides(const at::Tensor& t, bool bshd) {
+  // (the stride of a dimension of one entry can be anything, and says nothing)
+  const auto stride = [&](int d) { return t.size(d) == 1 ? t.size(3) : t.stride(d); };
   fa_tensor r;
   r.ptr = t.data_ptr();
-  r.stride_b = t.stride(0);
-  r.stride_h = t.stride(bshd ? 2 : 1);
-  r.stride_s = t.stride(bshd ? 1 : 2);
+  r.stride_b = stride(0);
+  r.stride_h = stride(bshd ? 2 : 1);
+  r.stride_s = stride(bshd ? 1 : 2);
   return r;
 }
 at::Tensor empty_rows(const at::Tensor& t) {

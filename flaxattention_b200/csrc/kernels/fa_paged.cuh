@@ -88,7 +88,7 @@ struct Seg {
   int item, hk, b;
   int first;  // first query of the row tile, and its position among the request's tokens
   int pos;
-  int end;    // keys from here on are behind every row
+  int begin, end;  // keys in front of begin are out of every row's window, those from end on are behind every row
   int tile, last;  // tiles of WN keys, first and one beyond the last
   const int* pages;  // row of the block table
 };
@@ -102,7 +102,8 @@ __device__ __forceinline__ void seg_open(const FaPagedParams& p, int item, Seg& 
   const int final = min(p.Sq, ((rt + 1) * BM - 1) / G + 1) - 1;  // its last query
   s.pos = len - p.Sq + s.first;
   s.end = max(len - p.Sq + final + 1, 0);
-  s.tile = (p.window < 0 ? 0 : max(s.pos - p.window, 0)) / WN;
+  s.begin = p.window < 0 ? 0 : max(s.pos - p.window, 0);
+  s.tile = s.begin / WN;
   s.last = max((s.end + WN - 1) / WN, s.tile + 1);  // (at least one: somebody has to write a row that sees nothing)
 }
 // tiles of item `item`'s segments
@@ -127,6 +128,7 @@ __device__ __forceinline__ void seg_advance(const FaPagedParams& p, Seg& s, int 
 // K and V of a tile on their way: where its keys are.  Every lane of every warp has the same but for its own key (TMA: box).
 struct Load {
   bool any;     // there is a tile
+  bool looked;  // this lane has a page to look at
   int hk;
   int page;     // this lane's, or -1: no such key, or no such page
   int row;      // token in it
@@ -532,7 +534,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
       if (lane >= off) upto += v;
     }
     const int total = __shfl_sync(0xffffffffu, upto, 31) * p.Hkv;
-    const int per = max(p.min_tiles, (total + p.workers - 1) / p.workers);
+    const int per = (total + p.workers - 1) / p.workers;
     if (blockIdx.x == 0 && warp == 0) {  // for the kernel that merges
       int at = upto - own;
       for (int i = i0; i < i1; ++i) {
@@ -568,10 +570,12 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
   auto look_up = [&](Load& n) {
     n.any = to_load > 0;
     n.page = -1;
+    n.looked = false;
     if (!n.any) return;
     const int key = ahead.tile * WN + lane * p.box;  // (box: 1 without TMA)
-    const bool there = lane * p.box < WN && key < ahead.end;
+    const bool there = lane * p.box < WN && key < ahead.end && key + p.box > ahead.begin;  // (pages out of the window may be gone)
     n.hk = ahead.hk;
+    n.looked = there;
     if (there) {
       const int slot = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
       n.row = key - slot * p.page_size;
@@ -580,12 +584,13 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     // (the keys that are there go along; those whose page is none are taken out when the entry has come)
     const int left = ahead.end - ahead.tile * WN;
     n.keep = left >= WN ? ALL : left > 0 ? (1u << left) - 1u : 0u;
+    const int gone = ahead.begin - ahead.tile * WN;  // (below WN)
+    if (gone > 0) n.keep &= ALL << gone;
     if (--to_load > 0) seg_advance(p, ahead, CG);
   };
   // takes keys out whose page is none
   auto settle = [&](Load& n) {
-    const bool there = lane * p.box < WN && ((n.keep >> (lane * p.box)) & 1u);
-    const bool bad = there && (n.page < 0 || n.page >= p.num_pages);
+    const bool bad = n.looked && (n.page < 0 || n.page >= p.num_pages);
     if (bad) n.page = -1;
     n.boxes = __ballot_sync(0xffffffffu, n.page >= 0);
     fa_u32 out = __ballot_sync(0xffffffffu, bad);

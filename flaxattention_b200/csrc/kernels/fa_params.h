@@ -91,7 +91,7 @@ struct FaPagedParams {
   int B, Hq, Hkv, Sq;
   int num_pages, page_size, max_len;  // max_len: tokens that the table has room for
   int page_shift;                     // log2 of page_size, or -1
-  int row_tiles, workers, min_tiles;  // row tiles of a request; CTAs, and the fewest tiles that one gets
+  int row_tiles, workers;             // row tiles of a request; CTAs
   int window;                         // keys more than this far behind a query are not seen (-1: all are)
   int b_off, h_off;
   int box;                            // keys that one look-up in the table gives (1, or the rows of a TMA box)

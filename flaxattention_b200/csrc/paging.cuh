@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) fa_paged_combin
   const int bh = row / per_head, r = row - bh * per_head, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int rt = r / BM, item = b * p.row_tiles + rt, items = p.B * p.row_tiles;
   const int before = p.plan[item], n = p.plan[item + 1] - before, total = p.plan[items] * p.Hkv;
-  const int per = max(p.min_tiles, (total + p.workers - 1) / p.workers);
+  const int per = (total + p.workers - 1) / p.workers;
   const int begin = before * p.Hkv + hk * n, c0 = begin / per, c1 = (begin + n - 1) / per;
   if (c0 == c1) return;  // (one worker's: written by it)
   const int q = r / G, h = hk * G + r - q * G;
@@ -465,7 +465,6 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
   }
   k.row_tiles = paged_row_tiles(p, c);
   k.workers = paged_workers(c);
-  k.min_tiles = 1;
   const size_t rows = 2 * (size_t)k.workers * c.BM;
   k.part_o = (float*)workspace;
   k.part_ml = (float*)((char*)workspace + paged_up(rows * p->Dv * 4));

@@ -75,8 +75,9 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, score_m
     logsumexp ``[B, Hq, Sq]`` in float32.
 
     Scores, softmax and sums are in fp32; 16-bit probabilities are rounded to the dtype for the product with the values.  Cached values of keys
-    that are masked, but lie within a request's length, must be finite.  A table entry that is no page, or a length beyond the table,
-    leaves the keys out, and the next call raises ``FlaxAttnError`` (``check_status``).  Meant for a few tokens per request; there is no
+    that ``mask_mod`` takes out must be finite; what lies behind a request's length or out of the window is not looked at, so that pages which the window
+    has left may be given back.  A table entry that is no page, or a length beyond the table, leaves the keys out, and the next call raises
+    ``FlaxAttnError`` (``check_status``).  Meant for a few tokens per request; there is no
     gradient.  ``kernel_options``: ``{"kernels": "general"}`` takes keys and values in 16-byte pieces where TMA would do.
     """
     general = kernel_options is not None and kernel_options.get("kernels") == "general"

@@ -108,6 +108,46 @@ def test_window_of_row_tiles():
     run(7, [300, 40], 4, 2, 90, 64, 16, "f16", window=50)
 
 
+@pytest.mark.parametrize("D,page", [(64, 16), (64, 8), (64, 64), (48, 16), (48, 3)])
+@pytest.mark.parametrize("Sq", [1, 3])
+def test_pages_that_the_window_has_left(D, page, Sq):
+    """Their table entries are none any more, and what else lies in front of the window is no number."""
+    for dtype in ("f16", "f32"):
+        dt, window, lengths = DTYPES[dtype], 70, [1, 71, 72, 75, 130, 333, 1000]
+        c = Cache(24, lengths, 2, D, page, dt)
+        for b, n in enumerate(lengths):
+            first = max(n - Sq - window, 0)  # the first key that any of the queries sees
+            for i in range(first // page):
+                c.table[b, i] = -1
+            p = c.table[b, first // page].long()
+            c.k_pages[p, :, : first % page] = math.nan
+            c.v_pages[p, :, : first % page] = math.inf
+        q = normal(np.random.default_rng(25), len(lengths), 4, Sq, D, dtype=dt)
+        for table in (c.table, torch.cat([c.table, torch.full((len(lengths), 6000), -1, dtype=torch.int32, device="cuda")], 1)):  # a CTA per segment, cut segments
+            out, lse = fa.paged_attention(q.cuda(), c.k_pages, c.v_pages, table, c.lengths, window=window, return_lse=True)
+            check_attention(out, lse, attend(q, c.keys, c.values, window=window), dt)
+        torch.cuda.synchronize()
+        fa.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("Hq,Hkv,Sq", [(4, 2, 1), (12, 2, 2), (6, 2, 7), (8, 1, 5)])
+def test_the_same_for_wide_tables(dtype, Hq, Hkv, Sq):
+    """Tables with room for much more than there is: the work is cut on the device, with the same results."""
+    for D, page, lengths in ((64, 16, [0, 1, 33, 700, 64]), (48, 5, [0, 1, 33, 700, 64]), (128, 64, [3000, 1]), (64, 16, list(range(0, 160)))):
+        run(26, lengths, Hq, Hkv, Sq, D, page, dtype, width=20000 // page)
+        run(26, lengths, Hq, Hkv, Sq, D, page, dtype, score=distance, mask=parity, window=100, width=20000 // page)
+
+
+def test_strides_of_single_entries():
+    """The stride of a dimension of one entry says nothing."""
+    c = Cache(27, [100], 1, 64, 16, torch.float16)
+    q = normal(np.random.default_rng(28), 1, 1, 1, 64, dtype=torch.float16).cuda()
+    odd = lambda t: t.as_strided(t.shape, [t.stride(i) if n > 1 else 1 for i, n in enumerate(t.shape)])  # noqa: E731
+    a = fa.paged_attention(q, c.k_pages, c.v_pages, c.table, c.lengths)
+    assert torch.equal(a, fa.paged_attention(odd(q), odd(c.k_pages), odd(c.v_pages), c.table, c.lengths))
+
+
 def test_captured_tensors():
     """Mods over tensors: document ids by position, a bias per head; a tensor on the CPU as well."""
     ids = torch.randint(0, 3, (600,), generator=torch.Generator().manual_seed(0))
