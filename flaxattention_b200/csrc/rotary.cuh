@@ -198,18 +198,26 @@ __device__ __forceinline__ void rot_angles(const FaRotParams& P, long long pos, 
     s[i] = P.sign * b.x; s[i + 1] = P.sign * b.y; s[i + 2] = P.sign * b.z; s[i + 3] = P.sign * b.w;
   }
 }
+// How a lane finds the other value of a pair.
+//   kHalves         pairs i and i + R / 2, R / 2 whole pieces: a lane has both pieces
+//   kNeighbours     neighbouring values, R whole pairs of pieces: they are in the piece
+//   kNeighboursAny  neighbouring values, any even R
+//   kAny            pairs i and i + R / 2, any even R: the pieces of a row lie side by side in the lanes, and the other values come
+//                   through shared memory.  B4 H32/8 S2048 D128 bf16 with norms, R 20: forward and backward 86 and 88 us (value by value 219 and 633), R 128 28 and 45.
+enum RotMode { kHalves, kNeighbours, kNeighboursAny, kAny };
+
 // The rotation of a lane's two pieces a and b as a' = a p + (b or a with its neighbours exchanged) q, and b' with its own p and q: the
 // factors, with the weights of the values that they multiply (1: none).  A lane whose values stay has the weights and 0.
 template <int V>
 struct RotFactors {
   F2 pa[V / 2], qa[V / 2], pb[V / 2], qb[V / 2];
 };
-template <int V, bool INTERLEAVED>
+template <int V, RotMode MODE>
 __device__ __forceinline__ void rot_factors(RotFactors<V>& f, bool turns, const float (&c)[V], const float (&s)[V], const float (&wa)[V], const float (&wb)[V]) {
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) {
     const int x = 2 * i, y = 2 * i + 1;
-    if (INTERLEAVED) {  // pairs i of piece a, V / 2 + i of piece b
+    if (MODE == kNeighbours) {  // pairs i of piece a, V / 2 + i of piece b
       const float ca = turns ? c[i] : 1.f, cb = turns ? c[V / 2 + i] : 1.f, sa = turns ? s[i] : 0.f, sb = turns ? s[V / 2 + i] : 0.f;
       f.pa[i] = f2(wa[x] * ca, wa[y] * ca);
       f.qa[i] = f2(-wa[y] * sa, wa[x] * sa);
@@ -224,15 +232,111 @@ __device__ __forceinline__ void rot_factors(RotFactors<V>& f, bool turns, const 
     }
   }
 }
-template <int V, bool INTERLEAVED>
+template <int V, RotMode MODE>
 __device__ __forceinline__ void rot_turn(F2 (&a)[V / 2], F2 (&b)[V / 2], const RotFactors<V>& f) {
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) {
     const F2 u = a[i], v = b[i];
-    a[i] = fma(INTERLEAVED ? swapped(u) : v, f.qa[i], u * f.pa[i]);
-    b[i] = fma(INTERLEAVED ? swapped(v) : u, f.qb[i], v * f.pb[i]);
+    a[i] = fma(MODE == kHalves ? v : swapped(u), f.qa[i], u * f.pa[i]);
+    b[i] = fma(MODE == kHalves ? u : swapped(v), f.qb[i], v * f.pb[i]);
   }
 }
+// any R: value e of a row, its pair's number, the other value's place and whether e is the pair's first
+struct RotPair {
+  int pair, other;
+  bool first;
+  __device__ __forceinline__ RotPair(const FaRotParams& P, bool halves, int e) {
+    const int half = P.R / 2;
+    first = halves ? e < half : (e & 1) == 0;
+    pair = !halves ? e >> 1 : first ? e : e - half;
+    other = !halves ? e ^ 1 : first ? e + half : e - half;
+  }
+};
+// Factors for values V * chunk .. (no such chunk: it holds zeros)
+template <int DT>
+__device__ __forceinline__ void rot_factors_any(const FaRotParams& P, bool halves, long long pos, int kind, int chunk, bool have, bool weighted, F2 (&p)[kRotPairs<DT>],
+                                                F2 (&q)[kRotPairs<DT>]) {
+  constexpr int V = kRotVec<DT>;
+  const auto weight = [&](int i) { return !weighted ? 1.f : P.w_f32 ? ((const float*)P.w[kind])[i] : rot_get<DT>(P.w[kind], i); };
+  float f[V], g[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = chunk * V + i;
+    f[i] = have ? weight(e) : 0.f;
+    g[i] = 0.f;
+    if (have && e < P.R) {
+      const RotPair t(P, halves, e);
+      const float c = pos < 0 ? 0.f : P.table[pos * P.table_stride + t.pair], s = pos < 0 ? 0.f : P.sign * P.table[pos * P.table_stride + P.R / 2 + t.pair];
+      f[i] *= c;
+      g[i] = weight(t.other) * (t.first ? -s : s);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    p[i] = f2(f[2 * i], f[2 * i + 1]);
+    q[i] = f2(g[2 * i], g[2 * i + 1]);
+  }
+}
+// kAny: the other values of those of a chunk; 0 for values that stay.  The row's even and odd pieces lie in two planes, a piece per lane from
+// `lane0` on.
+template <int DT>
+__device__ __forceinline__ void rot_others(const FaRotParams& P, const uint4* planes, int plane, int lane0, int chunk, F2 (&y)[kRotPairs<DT>]) {
+  constexpr int V = kRotVec<DT>;
+  const int half = P.R / 2;
+  const auto place = [&](int o) { return planes + ((o / V) & 1) * plane + lane0 + o / V / 2; };
+  if ((half & 1) == 0) {  // two others lie beside each other
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const int e = chunk * V + 2 * i, o = e < half ? e + half : e - half;
+      y[i] = f2(0.f, 0.f);
+      if (e < P.R) {
+        if constexpr (DT == FA_F32) {
+          const float2 t = ((const float2*)place(o))[(o % V) / 2];
+          y[i] = f2(t.x, t.y);
+        } else {
+          const unsigned t = ((const unsigned*)place(o))[(o % V) / 2];
+          if constexpr (DT == FA_F16) {
+            const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&t));
+            y[i] = f2(u.x, u.y);
+          } else {
+            y[i] = f2(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u));
+          }
+        }
+      }
+    }
+    return;
+  }
+  float f[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = chunk * V + i, o = e < half ? e + half : e - half;
+    f[i] = e < P.R ? rot_get<DT>(place(o), o % V) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) y[i] = f2(f[2 * i], f[2 * i + 1]);
+}
+// any R, without a norm: the values of a piece that stay as they came (a NaN loses its payload on the way through fp32)
+template <int DT>
+__device__ __forceinline__ uint4 rot_keep(const FaRotParams& P, int chunk, uint4 to, const uint4& from) {
+  constexpr int V = kRotVec<DT>;
+  const int stays = P.R - chunk * V;  // from here on
+  if (0 >= stays) to.x = from.x;
+  if (V / 4 >= stays) to.y = from.y;
+  if (V / 2 >= stays) to.z = from.z;
+  if (3 * V / 4 >= stays) to.w = from.w;
+  return to;
+}
+// kNeighboursAny: the pairs of a piece, those that turn
+template <int V>
+__device__ __forceinline__ void rot_turn_any(const FaRotParams& P, int chunk, F2 (&a)[V / 2], const F2 (&p)[V / 2], const F2 (&q)[V / 2]) {
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    const F2 u = a[i];
+    a[i] = u * p[i];
+    if (chunk * V + 2 * i < P.R) a[i] = fma(swapped(u), q[i], a[i]);  // (0 times what stays may be no number)
+  }
+}
+
 // the sums of N values over the lanes of a row each
 template <int N>
 __device__ __forceinline__ void rot_sums(float (&v)[N], int lane_shift) {
@@ -249,17 +353,18 @@ __device__ __forceinline__ void rot_sums(float (&v)[N], int lane_shift) {
 // B4 H32/8 S4096 D128 bf16 with norms: 55 us for 335 MB, 6.1 TB/s.  In single values, with an angle and a weight multiplied per value and each group
 // of rows asked for when the one before was written, it was bound by the instructions' issue: 79 us; 65 with two values per instruction
 // and the weights in the angles.  Two rows at a time 61, more blocks per SM (fewer registers) 85 and more.
-template <int DT, bool INTERLEAVED>
+template <int DT, RotMode MODE>
 __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_constant__ FaRotParams P) {
   grid_wait();
   constexpr int V = kRotVec<DT>, N = V / 2, U = 4;
+  __shared__ uint4 planes[MODE == kAny ? kRotThreads / 32 : 1][64];  // kAny: the pieces of a warp's rows, even ones and odd ones
   const RotPlace at(P);
   const bool live = at.token < P.tokens;
   const int b = live ? at.token / P.S : 0, s = live ? at.token - b * P.S : 0;
   const int kind = at.kind, chunks = (kind == 2 ? P.Dv : P.D) / V, pairs = kind == 2 ? 0 : P.R / (2 * V);
-  const bool turns = at.lane < pairs;
-  const int ca = turns && !INTERLEAVED ? at.lane : turns ? 2 * at.lane : 2 * pairs + 2 * (at.lane - pairs);
-  const int cb = turns && !INTERLEAVED ? at.lane + pairs : ca + 1;
+  const bool turns = MODE >= kNeighboursAny ? kind < 2 && 2 * at.lane * V < P.R : at.lane < pairs;
+  const int ca = MODE == kHalves ? (turns ? at.lane : 2 * pairs + 2 * (at.lane - pairs)) : 2 * at.lane;
+  const int cb = MODE == kHalves && turns ? at.lane + pairs : ca + 1;
   const long long to = live ? rot_destination(P, kind, b, s) : -1;
   const bool have_a = live && to >= 0 && ca < chunks, have_b = live && to >= 0 && cb < chunks;
   const bool norm = kind < 2 && P.w[kind < 2 ? kind : 0] != nullptr;
@@ -277,7 +382,11 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
   };
   load(at.h0);
   RotFactors<V> f;
-  {
+  if constexpr (MODE >= kNeighboursAny) {
+    const long long pos = turns && live ? rot_position(P, b, s) : -1;
+    rot_factors_any<DT>(P, MODE == kAny, pos, kind, ca, ca < chunks, norm, f.pa, f.qa);
+    rot_factors_any<DT>(P, MODE == kAny, pos, kind, cb, cb < chunks, norm, f.pb, f.qb);
+  } else {
     float c[V], sn[V], wa[V], wb[V];
     rot_angles<V>(P, turns && live ? rot_position(P, b, s) : -1, at.lane, turns, c, sn);
 #pragma unroll
@@ -286,7 +395,7 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
       rot_weights<DT>(P, kind, ca, ca < chunks, wa);
       rot_weights<DT>(P, kind, cb, cb < chunks, wb);
     }
-    rot_factors<V, INTERLEAVED>(f, turns, c, sn, wa, wb);
+    rot_factors<V, MODE>(f, turns, c, sn, wa, wb);
   }
   char* dst = P.y[kind].ptr + to;
   const float per_value = 1.f / P.D;
@@ -318,12 +427,25 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (h + u >= at.h1) break;
+      F2 ox[N], oy[N];
+      if constexpr (MODE == kAny) {
+        uint4* const mine = planes[threadIdx.x >> 5];
+        __syncwarp();  // (the row before has been read)
+        mine[threadIdx.x & 31] = ra[u];
+        mine[32 + (threadIdx.x & 31)] = rb[u];
+        __syncwarp();
+        const int lane0 = (threadIdx.x & 31) - at.lane;
+        if (turns) {
+          rot_others<DT>(P, mine, 32, lane0, ca, ox);
+          rot_others<DT>(P, mine, 32, lane0, cb, oy);
+        }
+      }
       if (norm || turns) {
         F2 x[N], y[N];
         rot_unpack<DT>(ra[u], x);
         rot_unpack<DT>(rb[u], y);
+        const float r = norm ? rsqrtf(ss[u] * per_value + P.eps) : 1.f;
         if (norm) {
-          const float r = rsqrtf(ss[u] * per_value + P.eps);
           const F2 rr = f2(r, r);
 #pragma unroll
           for (int i = 0; i < N; ++i) {
@@ -331,9 +453,25 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
             y[i] = y[i] * rr;
           }
         }
-        rot_turn<V, INTERLEAVED>(x, y, f);
-        ra[u] = rot_pack<DT>(x);
-        rb[u] = rot_pack<DT>(y);
+        if constexpr (MODE == kAny) {
+          const F2 rr = f2(r, r);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            x[i] = x[i] * f.pa[i];
+            y[i] = y[i] * f.pb[i];
+            if (!turns) continue;
+            x[i] = fma(ox[i] * rr, f.qa[i], x[i]);
+            y[i] = fma(oy[i] * rr, f.qb[i], y[i]);
+          }
+        } else if constexpr (MODE == kNeighboursAny) {
+          rot_turn_any<V>(P, ca, x, f.pa, f.qa);
+          rot_turn_any<V>(P, cb, y, f.pb, f.qb);
+        } else {
+          rot_turn<V, MODE>(x, y, f);
+        }
+        const uint4 pa = rot_pack<DT>(x), pb = rot_pack<DT>(y);
+        ra[u] = MODE >= kNeighboursAny && !norm ? rot_keep<DT>(P, ca, pa, ra[u]) : pa;
+        rb[u] = MODE >= kNeighboursAny && !norm ? rot_keep<DT>(P, cb, pb, rb[u]) : pb;
       }
       char* row = dst + (h + u) * P.y[kind].sh;
       if (have_a) *(uint4*)(row + ca * 16) = ra[u];
@@ -352,16 +490,16 @@ __device__ __forceinline__ void rot_copy16(void* shared, const void* from) {
 // B4 H32/8 S4096 D128 bf16: 82 us for the 503 MB that have to move, 6.1 TB/s.  What it took: two values per instruction
 // (fma.rn.f32x2), 157 us to 107, and rows on their way through shared memory instead of one row ahead in registers, which has
 // twice as many bytes in flight, 107 to 83.
-template <int DT, bool INTERLEAVED>
+template <int DT, RotMode MODE>
 __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_bwd_kernel(const __grid_constant__ FaRotParams P) {
   grid_wait();
   constexpr int V = kRotVec<DT>, N = V / 2;
   __shared__ float sums[kRotThreads / 32][256];
   const RotPlace at(P);
   const int kind = at.kind, chunks = P.D / V, pairs = P.R / (2 * V);
-  const bool turns = at.lane < pairs;
-  const int ca = turns && !INTERLEAVED ? at.lane : turns ? 2 * at.lane : 2 * pairs + 2 * (at.lane - pairs);
-  const int cb = turns && !INTERLEAVED ? at.lane + pairs : ca + 1;
+  const bool turns = MODE >= kNeighboursAny ? 2 * at.lane * V < P.R : at.lane < pairs;
+  const int ca = MODE == kHalves ? (turns ? at.lane : 2 * pairs + 2 * (at.lane - pairs)) : 2 * at.lane;
+  const int cb = MODE == kHalves && turns ? at.lane + pairs : ca + 1;
   const bool norm = P.w[kind] != nullptr;
   F2 wa[N], wb[N], da[N], db[N];
   {
@@ -418,12 +556,16 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_bwd_kernel(const __g
     const bool live = t < P.tokens, have_a = live && ca < chunks, have_b = live && cb < chunks;
     const int b = live ? t / P.S : 0, s = live ? t - b * P.S : 0;
     RotFactors<V> f;
-    {
+    if constexpr (MODE >= kNeighboursAny) {
+      const long long pos = turns && live ? rot_position(P, b, s) : -1;
+      rot_factors_any<DT>(P, MODE == kAny, pos, kind, ca, ca < chunks, false, f.pa, f.qa);
+      rot_factors_any<DT>(P, MODE == kAny, pos, kind, cb, cb < chunks, false, f.pb, f.qb);
+    } else {
       float c[V], sn[V], one[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) one[i] = 1.f;
       rot_angles<V>(P, turns && live ? rot_position(P, b, s) : -1, at.lane, turns, c, sn);
-      rot_factors<V, INTERLEAVED>(f, turns, c, sn, one, one);
+      rot_factors<V, MODE>(f, turns, c, sn, one, one);
     }
     char* ds = P.y[kind].ptr + b * P.y[kind].sb + s * P.y[kind].ss + at.h0 * P.y[kind].sh;
     for (int h = 0; h < heads; ++h, ++row) {
@@ -434,7 +576,28 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_bwd_kernel(const __g
       F2 a[N], d[N], u[N], v[N];
       rot_unpack<DT>(have_a ? place[0] : zero, a);
       rot_unpack<DT>(have_b ? place[kRotThreads] : zero, d);
-      if (turns) rot_turn<V, INTERLEAVED>(a, d, f);
+      if constexpr (MODE == kAny) {
+        __syncwarp();  // (the other lanes' pieces)
+        if (turns && live) {
+          F2 oa[N], od[N];
+          const int lane0 = threadIdx.x - at.lane;
+          rot_others<DT>(P, place - threadIdx.x, kRotThreads, lane0, ca, oa);
+          rot_others<DT>(P, place - threadIdx.x, kRotThreads, lane0, cb, od);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            a[i] = fma(oa[i], f.qa[i], a[i] * f.pa[i]);
+            d[i] = fma(od[i], f.qb[i], d[i] * f.pb[i]);
+          }
+        }
+        __syncwarp();  // (before the place takes another row)
+      } else if constexpr (MODE == kNeighboursAny) {
+        if (turns) {
+          rot_turn_any<V>(P, ca, a, f.pa, f.qa);
+          rot_turn_any<V>(P, cb, d, f.pb, f.qb);
+        }
+      } else {
+        if (turns) rot_turn<V, MODE>(a, d, f);
+      }
       if (norm) {
         rot_unpack<DT>(have_a ? place[2 * kRotThreads] : zero, u);
         rot_unpack<DT>(have_b ? place[3 * kRotThreads] : zero, v);
@@ -494,7 +657,7 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_bwd_kernel(const __g
   }
 }
 
-// What no 16-byte pieces fit: a warp per row, value by value.  Backward (BACK): the same with dy, as above.
+// What no 16-byte pieces fit (head dims, strides, addresses): a warp per row, value by value.  Backward (BACK): the same with dy, as above.
 template <int DT, bool BACK>
 __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid_constant__ FaRotParams P) {
   grid_wait();
@@ -554,6 +717,11 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid
       int i, j;
       float c, sn;
       unit(k, i, j, c, sn);
+      if (j < 0 && !norm) {  // (as it is)
+        if (DT == FA_F32) ((unsigned*)y)[i] = ((const unsigned*)x)[i];
+        else ((unsigned short*)y)[i] = ((const unsigned short*)x)[i];
+        continue;
+      }
       float a = rot_get<DT>(x, i), d = j >= 0 ? rot_get<DT>(x, j) : 0.f;
       if (!BACK && norm) {
         a *= r * weight(i);
@@ -649,14 +817,18 @@ void rot_fill(const fa_rotary_params* p, int hq, int hk, int hv, FaRotParams& k)
 // Whether all rows can be taken in 16-byte pieces, two per lane; fills the lanes of a row.
 bool rot_by_pieces(const FaRotParams& k, int dtype, int* lane_shift) {
   const int v = dtype == FA_F32 ? 4 : 8;
-  if (k.D % (2 * v) || k.R % (2 * v) || k.Dv % v || k.Dv > k.D) return false;
-  if (k.R > 0 && ((uintptr_t)k.table % 16 || k.table_stride % 4)) return false;
+  if (k.D % v || k.Dv % v || k.Dv > k.D) return false;
   for (int i = 0; i < 3; ++i)
     if (k.heads[i] > 0 && !(rot_aligned(k.x[i]) && rot_aligned(k.y[i]) && (i == 2 || k.in[i].ptr == nullptr || rot_aligned(k.in[i])))) return false;
   int shift = 0;
-  while ((1 << shift) < k.D / (2 * v)) ++shift;
+  while ((1 << shift) < (k.D + 2 * v - 1) / (2 * v)) ++shift;
   *lane_shift = shift;
   return shift <= 5;
+}
+// (angles are read 16 bytes at a time, but for any R)
+RotMode rot_mode(const FaRotParams& k, int dtype) {
+  const bool whole = k.R % (dtype == FA_F32 ? 8 : 16) == 0 && (k.R == 0 || ((uintptr_t)k.table % 16 == 0 && k.table_stride % 4 == 0));
+  return k.interleaved ? (whole ? kNeighbours : kNeighboursAny) : whole ? kHalves : kAny;
 }
 // Heads that a thread goes through.  Up to 16, so that the angles are read seldom (B4 H32/8 S4096 D128 bf16 with norms, us, 4 / 8 / 16 heads: forward
 // 68 / 56 / 55; 16384 tokens appended 81 / 72 / 70); fewer while the grid would leave SMs with less than four blocks.
@@ -704,8 +876,8 @@ int rot_launch(FaRotParams& k, int dtype, void* stream) {
     const dim3 grid((unsigned)token_blocks, (unsigned)(k.groups[0] + k.groups[1] + k.groups[2]));
     return rot_dispatch(dtype, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
-      return launch_here("fa_rotary_kernel", k.interleaved ? fa_rotary_kernel<DT, true> : fa_rotary_kernel<DT, false>, grid,
-                         dim3(kRotThreads), stream, k);
+      void (*const of_mode[])(FaRotParams) = {fa_rotary_kernel<DT, kHalves>, fa_rotary_kernel<DT, kNeighbours>, fa_rotary_kernel<DT, kNeighboursAny>, fa_rotary_kernel<DT, kAny>};
+      return launch_here("fa_rotary_kernel", of_mode[rot_mode(k, dtype)], grid, dim3(kRotThreads), stream, k);
     });
   }
   const long long rows = (long long)k.tokens * std::max(k.heads[0], std::max(k.heads[1], k.heads[2]));
@@ -792,7 +964,9 @@ int fa_rotary_bwd(const fa_rotary_params* p, const fa_tensor* dq_out, const fa_t
       for (int i = 0; i < 2; ++i) sum.parts[i] = (int)blocks * k.groups[i];
       rc = rot_dispatch(p->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        const auto fn = k.interleaved ? fa_rotary_bwd_kernel<DT, true> : fa_rotary_bwd_kernel<DT, false>;
+        void (*const of_mode[])(FaRotParams) = {fa_rotary_bwd_kernel<DT, kHalves>, fa_rotary_bwd_kernel<DT, kNeighbours>, fa_rotary_bwd_kernel<DT, kNeighboursAny>,
+                                                fa_rotary_bwd_kernel<DT, kAny>};
+        const auto fn = of_mode[rot_mode(k, DT)];
         constexpr int smem = kRotStages * 4 * kRotThreads * 16;
         if (int e = allow_smem((const void*)fn, smem)) return e;
         return launch_here_smem("fa_rotary_bwd_kernel", fn, dim3(blocks, (unsigned)(k.groups[0] + k.groups[1])), dim3(kRotThreads), smem, stream, k);

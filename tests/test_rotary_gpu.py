@@ -105,6 +105,19 @@ def test_positions(kind, per_request):
     run(3, 4, 2, 41, 30, 20, "f16", False, True, positions=pos)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan, 6e4])
+def test_values_that_stay_are_copied(interleaved, value):
+    """What lies behind the rotated part is passed on bit by bit, whatever it is, and does not touch what is rotated."""
+    for D, R in ((64, 20), (64, 22), (64, 32), (24, 6), (20, 6), (128, 128 - 2)):
+        q, k, *_ = case(4, 1, 2, 1, 5, D, "f16", False)
+        q[..., R:] = value
+        q[..., R] = 1.0
+        oq, _ = fa.rotary_embedding(q.cuda(), k.cuda(), fa.rotary_table(5, R).cuda(), interleaved=interleaved)
+        assert torch.equal(oq[..., R:].cpu().view(torch.int16), q[..., R:].view(torch.int16))
+        assert torch.isfinite(oq[..., :R]).all()
+
+
 def test_weights_in_fp32_and_of_one_side():
     run(2, 4, 2, 50, 128, 64, "bf16", True, wdtype=torch.float32)
     for which in ((0,), (1,)):
