@@ -16,11 +16,17 @@
 //     groups take every FA_CG-th tile, each with a running (max, sum, O) of its own, and merge through shared memory where a segment
 //     ends, while the loads of the next are on their way.  A segment that lies in one worker's run is written out; of others the workers leave
 //     parts (O not divided, max, sum), which fa_paged_combine_kernel merges.
-//   * FA_SHORT, for tables that have room for a few tiles only: a CTA per segment; one launch, and no sums over the lengths in front.
+//   * FA_SHORT: a CTA per segment; one launch, no parts and no sums over the lengths in front.  For tables with room for a few tiles, and for
+//     many segments of middling length, where the SMs take the next segment when they have done one (the host's rule has both sides' times).
+//
+// Measured (us on the GPU, bf16, up to 8 rows; of the bytes of K and V): 32 requests of 1640 to 16384 keys in pages of 64, 32 / 8 heads, D 128, 1.21 GB,
+// 182, 6.7 TB/s; one of 131072, 0.54 GB, 84 and 4 for the merge, 6.1 TB/s: DRAM, and 5.5 in front of the first product (the launch, the lengths,
+// the table, the first tiles) and behind the last.  64 requests of 16 keys 6.3: that chain alone.  20 rows and a score_mod 41: the chains of products
+// and exponentials of 8 warps per SM, more than which 255 registers a thread do not allow.
 //
 // CTA = FA_CG key groups of FA_RG warps with 16 query rows each.  The warps of a key group share its tiles of K and V, which come by TMA
 // (FA_TMA: pages that hold whole boxes of 8 keys and more, head dims of whole 128-byte columns) or in 16-byte cp.async pieces.  That the groups
-// of a CTA read beside each other counts: with a run for each warp DRAM gave 6.1 to 6.2 TB/s (B32 H8 D64, 16384 keys in pages of 64).
+// of a CTA read beside each other counts (B32 H8 D64, 16384 keys in pages of 64: 6.6 TB/s; with a run for each warp 6.1 to 6.2).
 // Three ways to multiply:
 //   * FA_FEW groups of 8 rows, by one warp: S' = K Q' and O' = V' P', so that keys and columns fill the 16 rows of an mma.sync and the
 //     queries its 8 columns.  For up to 8 rows, which is what one new token has, half the instructions of the next way, of which the
@@ -62,8 +68,8 @@ constexpr int PK = TMA ? D * ES : FaTile<D, ES>::PITCH;
 constexpr int PV = TMA ? DV * ES : FaTile<DV, ES>::PITCH;
 constexpr int ATOMS_K = D * ES / 128, ATOMS_V = DV * ES / 128;  // 128-byte column groups of a row (TMA)
 // A key group's buffers are a ring of slots that take a tile of K or of V: K, V, K of the next, ..; what was in a slot has been used up, and the
-// tile half a ring ahead is asked for.  Eight warps per SM, two for each of its schedulers, so that one's products run under the other's
-// softmax (D 128, up to 8 rows: a warp alone takes 1.5 us per tile, and four per SM with any number of slots 187 us where eight take 180).
+// tile half a ring ahead is asked for.  Two slots and as many warps per SM as fit, so that one's products run under the
+// others' softmax: a warp alone takes 1.5 us per tile (D 128, up to 8 rows), and fewer warps with more slots are slower (the host's rule).
 constexpr int SLOT_BYTES = WN * (PK > PV ? PK : PV);
 constexpr int PIPE_BYTES = SLOTS * SLOT_BYTES;  // of a key group
 constexpr bool ODD = SLOTS % 2 != 0;

@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(kStepThreads) fa_page_step_kernel(const __grid
 }
 
 // ---- attention: the parts of segments that several workers share ---------------------------
-// WARPS warps per query row, which take the row's parts in turn.
+// WARPS warps per query row, which take the row's parts in turn: eight where a row may have many (one request of 131072 keys, 444 workers, 32 rows: 4.4 us,
+// a chain of plan, parts and sums), else one (3.4).
 template <int DT, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) fa_paged_combine_kernel(const __grid_constant__ FaPagedParams p, int BM, int Dv, int n_rows) {
   grid_wait();

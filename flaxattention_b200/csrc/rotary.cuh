@@ -353,6 +353,8 @@ __device__ __forceinline__ void rot_sums(float (&v)[N], int lane_shift) {
 // B4 H32/8 S4096 D128 bf16 with norms: 55 us for 335 MB, 6.1 TB/s.  In single values, with an angle and a weight multiplied per value and each group
 // of rows asked for when the one before was written, it was bound by the instructions' issue: 79 us; 65 with two values per instruction
 // and the weights in the angles.  Two rows at a time 61, more blocks per SM (fewer registers) 85 and more.
+// 16384 tokens appended to pages (H32/8 D128 bf16): 70 us for 411 MB, 5.8 TB/s: the values only change place, and keys and values are written
+// in runs of a row (256 bytes).  One token of 32 requests: 3.9 us, the launch, the slot and the row one behind the other.
 template <int DT, RotMode MODE>
 __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_constant__ FaRotParams P) {
   grid_wait();
