@@ -89,6 +89,8 @@ static_assert(!TMA || (D * ES % 128 == 0 && DV * ES % 128 == 0), "TMA: whole col
 static_assert(F32 || WN == 32 || WN == 16, "tiles of 16 or 32 keys");
 static_assert(!FEW || (RG == 1 && !F32), "few rows: one warp, 16-bit types");
 
+__device__ __forceinline__ int divided(int n, const FaDiv& d) { return d.shift < 0 ? n : (int)(__umulhi((fa_u32)n, d.mul) >> d.shift); }
+
 // A segment, and the tile of it that is next.
 struct Seg {
   int item, hk, b;
@@ -100,12 +102,12 @@ struct Seg {
 };
 __device__ __forceinline__ void seg_open(const FaPagedParams& p, int item, Seg& s) {
   s.item = item;
-  s.b = p.row_tiles == 1 ? item : item / p.row_tiles;
+  s.b = divided(item, p.by_tiles);
   s.pages = p.table + s.b * p.table_stride;
-  const int rt = item - s.b * p.row_tiles, G = p.Hq / p.Hkv;
+  const int rt = item - s.b * p.row_tiles;
   const int len = min(max(p.lengths[s.b], 0), p.max_len);
-  s.first = rt * BM / G;
-  const int final = min(p.Sq, ((rt + 1) * BM - 1) / G + 1) - 1;  // its last query
+  s.first = divided(rt * BM, p.by_group);
+  const int final = min(p.Sq, divided((rt + 1) * BM - 1, p.by_group) + 1) - 1;  // its last query
   s.pos = len - p.Sq + s.first;
   s.end = max(len - p.Sq + final + 1, 0);
   s.begin = p.window < 0 ? 0 : max(s.pos - p.window, 0);
@@ -121,12 +123,16 @@ __device__ __forceinline__ int seg_tiles(const FaPagedParams& p, int item) {
 // n tiles on, over the ends of segments
 __device__ __forceinline__ void seg_advance(const FaPagedParams& p, Seg& s, int n) {
   s.tile += n;
+#pragma unroll 1
   while (!SHORT && s.tile >= s.last) {
     const int over = s.tile - s.last;
-    const bool wrap = s.hk + 1 == p.Hkv;
-    s.hk = wrap ? 0 : s.hk + 1;
-    if (wrap && s.item + 1 == p.B * p.row_tiles) return;  // (behind the last tile of all)
-    seg_open(p, wrap ? s.item + 1 : s.item, s);
+    if (++s.hk == p.Hkv) {
+      s.hk = 0;
+      if (s.item + 1 == p.B * p.row_tiles) return;  // (behind the last tile of all)
+      seg_open(p, s.item + 1, s);
+    } else {
+      s.tile = s.begin / WN;
+    }
     s.tile += over;
   }
 }
@@ -501,7 +507,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
   const fa_u32 ring = fa_smem_u32(bufs);
   [[maybe_unused]] unsigned char* const q_tile = base + CG * PIPE_BYTES;
   [[maybe_unused]] float* const merge = (float*)(base + CG * PIPE_BYTES + Q_BYTES);  // [CG][MROWS][MPITCH]
-  [[maybe_unused]] float2* const merge_ml = (float2*)(merge + CG * MROWS * MPITCH);  // [CG][MROWS]
+  [[maybe_unused]] float2* const merge_ml = (float2*)(merge + CG * MROWS * MPITCH);  // [MROWS][CG]
   const int row0 = rg * 16;  // first row of this warp
 #if FA_TMA
   const fa_u32 all_bars = fa_smem_u32(base) + CG * PIPE_BYTES + Q_BYTES + MERGE_BYTES;
@@ -543,6 +549,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     const int per = (total + p.workers - 1) / p.workers;
     if (blockIdx.x == 0 && warp == 0) {  // for the kernel that merges
       int at = upto - own;
+#pragma unroll 1
       for (int i = i0; i < i1; ++i) {
         p.plan[i] = at;
         at += seg_tiles(p, i);
@@ -550,6 +557,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
       if (lane == 31) p.plan[items] = upto;
       // a length that the table has no room for
       bool beyond = false;
+#pragma unroll 1
       for (int i = lane; i < p.B; i += 32) beyond |= p.lengths[i] > p.max_len || p.lengths[i] < 0;
       if (beyond && p.status != nullptr) atomicOr(p.status, FA_STATUS_BAD_PAGE);
     }
@@ -559,6 +567,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     const int from = __popc(__ballot_sync(0xffffffffu, (long long)upto * p.Hkv <= t0));  // the lane whose run has tile t0
     int item = __shfl_sync(0xffffffffu, i0, from), before = __shfl_sync(0xffffffffu, upto - own, from);
     seg_open(p, item, seg);
+#pragma unroll 1
     while (t0 >= (before + seg.last - seg.tile) * p.Hkv) {
       before += seg.last - seg.tile;
       seg_open(p, ++item, seg);
@@ -583,7 +592,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     n.hk = ahead.hk;
     n.looked = there;
     if (there) {
-      const int slot = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+      const int slot = divided(key, p.by_page);
       n.row = key - slot * p.page_size;
       n.page = ahead.pages[slot];
     }
@@ -602,6 +611,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     fa_u32 out = __ballot_sync(0xffffffffu, bad);
     if (out != 0) {
       if (lane == 0 && p.status != nullptr) atomicOr(p.status, FA_STATUS_BAD_PAGE);
+#pragma unroll 1
       for (; out != 0; out &= out - 1) {
         const int first = (__ffs(out) - 1) * p.box;
         n.keep &= ~((p.box >= 32 ? 0xffffffffu : (1u << p.box) - 1u) << first);
@@ -630,13 +640,16 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
   Load pending, next, after;  // the tile whose V is asked for next, the one whose K is, and the one behind that
   pending.any = next.any = after.any = false;
   int asked = 0;  // slots asked for
-#pragma unroll
-  for (int st = 0; st < AHEAD; ++st) {
+#pragma unroll 1
+  for (int st = 0;; ++st) {  // (not unrolled: its instructions come from memory before the first tile does)
     look_up(next);
-    keep[st] = 0;
+    if (st == AHEAD) break;
+#pragma unroll
+    for (int i = 0; i + 1 < AHEAD; ++i) keep[i] = keep[i + 1];
+    keep[AHEAD - 1] = 0;
     if (next.any) {
       settle(next);
-      keep[st] = next.keep;
+      keep[AHEAD - 1] = next.keep;
       load_k(2 * st, next);
     }
     fa_cp_commit();
@@ -645,9 +658,8 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
       fa_cp_commit();
     }
     asked += next.any ? (2 * st + 1 < SLOTS ? 2 : 1) : 0;
+    pending = next;
   }
-  pending = next;
-  look_up(next);
 
   // ---- the segments ----------------------------------------------------------------------
   Rows R;
@@ -683,6 +695,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     ++n_used;
   };
 
+#pragma unroll 1
   for (int t = t0; t < t1;) {
     // this worker's part of the segment: tiles seg.tile .. part_end - 1
     const int part_end = min(seg.last, seg.tile + (t1 - t)), rt = seg.item - seg.b * p.row_tiles;
@@ -690,7 +703,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     int qpos[HR], head[HR];  // of this thread's rows: position (-1: no row), query head
 #pragma unroll
     for (int h = 0; h < HR; ++h) {
-      const int row = rt * BM + R.row(h), i = row / G;
+      const int row = rt * BM + R.row(h), i = divided(row, p.by_group);
       head[h] = seg.hk * G + row - i * G;
       qpos[h] = i < p.Sq ? seg.pos - seg.first + i : -1;
       R.m[h] = FA_NEG_INF;
@@ -701,7 +714,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #if FA_DTYPE == FA_DT_F32
     __syncthreads();  // (the rows of the segment before have been read)
     for (int i = tid; i < QROWS * (D / 4); i += NT) {
-      const int r = i / (D / 4), c = i - r * (D / 4), row = rt * BM + r, qi = row / G;
+      const int r = i / (D / 4), c = i - r * (D / 4), row = rt * BM + r, qi = divided(row, p.by_group);
       const float* src = (const float*)(qb + (qi * p.q.ss + (long long)(seg.hk * G + row - qi * G) * p.q.sh) * ES) + c * 4;
       *(float4*)(q_tile + r * PQ + c * 16) = qi < p.Sq ? *(const float4*)src : make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -710,7 +723,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     // (rows g, g + 8, .. of the row tile, g = lane / 4)
 #pragma unroll
     for (int q = 0; q < (FEW ? NQ : 2); ++q) {
-      const int row = rt * BM + row0 + q * 8 + (lane >> 2), i = row / G;
+      const int row = rt * BM + row0 + q * 8 + (lane >> 2), i = divided(row, p.by_group);
       const fa_u32* src = (const fa_u32*)(qb + (i * p.q.ss + (long long)(seg.hk * G + row - i * G) * p.q.sh) * ES) + (lane & 3);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
@@ -727,6 +740,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #endif
 
     // ---- the tiles of this key group (a group whose wait has run out leaves them out, but takes part in the merges)
+#pragma unroll 1
     for (int tile = seg.tile + (CG - (t - t0) % CG + cg) % CG; tile < part_end && !failed; tile += CG) {
       // (its pages were looked up a tile ago; here, so that nothing waits for them when a slot is free)
       if (next.any) settle(next);
@@ -862,41 +876,60 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     if (CG > 1) {
 #pragma unroll
       for (int h = 0; h < HR; ++h)
-        if (R.speaks()) merge_ml[cg * MROWS + R.row(h)] = make_float2(R.m[h], R.l[h]);
-#pragma unroll
+        if (R.speaks()) merge_ml[R.row(h) * CG + cg] = make_float2(R.m[h], R.l[h]);
+#pragma unroll 1
       for (int blk = 0; blk < (DV + 31) / 32; ++blk) {
         if (blk > 0) __syncthreads();  // (the columns before have been read)
-        R.each(blk, [&](int h, int c, float v) { merge[(cg * MROWS + R.row(h)) * MPITCH + c - blk * 32] = v; });
+#pragma unroll
+        for (int b = 0; b < (DV + 31) / 32; ++b)
+          if (b == blk) R.each(b, [&](int h, int c, float v) { merge[(cg * MROWS + R.row(h)) * MPITCH + c - b * 32] = v; });
         __syncthreads();
+        if (blk == 0) {
+          // what a group's values of a row count for, once for all columns; the groups of a row are lanes beside each other
+          for (int i = tid; i < (rows * CG + 31) / 32 * 32; i += NT) {
+            const bool in = i < rows * CG;
+            const int r = i / CG;
+            const float2 ml = in ? merge_ml[i] : make_float2(FA_NEG_INF, 0.f);
+            float m = ml.x;
+#pragma unroll
+            for (int off = 1; off < CG; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+            const float m_use = m == FA_NEG_INF ? 0.f : m;
+            float f = ml.y == 0.f ? 0.f : exp2f(ml.x - m_use);  // (a group that has seen nothing counts for nothing)
+            float l = f * ml.y;
+#pragma unroll
+            for (int off = 1; off < CG; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+            if (!in) continue;
+            if (whole) {
+              f *= inverse(l);
+              if (i % CG == 0 && p.lse != nullptr) {
+                const int qi = divided(rt * BM + r, p.by_group), hd = seg.hk * G + rt * BM + r - qi * G;
+                p.lse[((long long)seg.b * p.Hq + hd) * p.Sq + qi] = log_sum(m_use, l);
+              }
+            } else if (i % CG == 0) {
+              *(float2*)(part_ml + r * 2) = make_float2(m, l);
+            }
+            merge_ml[i].x = f;
+          }
+          __syncthreads();
+        }
         constexpr int PAIRS = DV < 32 ? DV / 2 : 16;
+#pragma unroll 1
         for (int i = tid; i < rows * PAIRS; i += NT) {
           const int r = i / PAIRS, c = (i - r * PAIRS) * 2;
           if (blk * 32 + c >= DV) continue;
-          float2 ml[CG];
-          float m = FA_NEG_INF;
-#pragma unroll
-          for (int g = 0; g < CG; ++g) {
-            ml[g] = merge_ml[g * MROWS + r];
-            m = fmaxf(m, ml[g].x);
-          }
-          const float m_use = m == FA_NEG_INF ? 0.f : m;
-          float x = 0.f, y = 0.f, l = 0.f;
+          float x = 0.f, y = 0.f;
 #pragma unroll
           for (int g = 0; g < CG; ++g) {
             const float2 v = *(const float2*)(merge + (g * MROWS + r) * MPITCH + c);
-            const float f = ml[g].y == 0.f ? 0.f : exp2f(ml[g].x - m_use);  // (a group that has seen nothing counts for nothing)
-            l += f * ml[g].y;
+            const float f = merge_ml[r * CG + g].x;
             x += f * v.x;
             y += f * v.y;
           }
           if (whole) {
-            const int qi = (rt * BM + r) / G, hd = seg.hk * G + rt * BM + r - qi * G;
-            const float inv = inverse(l);
-            put2((char*)p.o.ptr + (seg.b * p.o.sb + hd * p.o.sh + qi * p.o.ss) * ES, blk * 32 + c, x * inv, y * inv);
-            if (blk == 0 && c == 0 && p.lse != nullptr) p.lse[((long long)seg.b * p.Hq + hd) * p.Sq + qi] = log_sum(m_use, l);
+            const int qi = divided(rt * BM + r, p.by_group), hd = seg.hk * G + rt * BM + r - qi * G;
+            put2((char*)p.o.ptr + (seg.b * p.o.sb + hd * p.o.sh + qi * p.o.ss) * ES, blk * 32 + c, x, y);
           } else {
             *(float2*)(part_o + r * DV + blk * 32 + c) = make_float2(x, y);
-            if (blk == 0 && c == 0) *(float2*)(part_ml + r * 2) = make_float2(m, l);
           }
         }
       }
@@ -906,7 +939,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
       float inv[HR];
 #pragma unroll
       for (int h = 0; h < HR; ++h) {
-        const int i = (rt * BM + R.row(h)) / G;
+        const int i = divided(rt * BM + R.row(h), p.by_group);
         out[h] = (char*)p.o.ptr + (seg.b * p.o.sb + head[h] * p.o.sh + i * p.o.ss) * ES;
         inv[h] = inverse(R.l[h]);
         if (R.row(h) >= rows || !R.speaks()) continue;
@@ -931,6 +964,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     // The copies in flight have to land before the shared memory goes to another CTA (with a limit of its own: the flag is up).
     if (rg == 0 && lane == 0) {
       const fa_u64 start = fa_globaltimer();
+#pragma unroll 1
       for (int i = n_used; i < asked; ++i) {
         while (!fa_mbar_try(bars + (i % SLOTS) * 8, (i / SLOTS) & 1) && fa_globaltimer() - start <= FA_WAIT_LIMIT_NS / 4) {
         }

@@ -77,6 +77,13 @@ struct FaParams {
   const unsigned char* beyond[4];
 };
 
+// n / d of 0 <= n < 2^31 in one multiplication: floor(n (floor(2^(32 + shift) / d) + 1) / 2^(32 + shift)) with 2^shift < d <= 2^(shift + 1),
+// so that the multiplier's error, at most 1 in 2^(32 + shift), stays below 1 / d times n's largest.  (shift -1: d is 1.)
+struct FaDiv {
+  unsigned mul;
+  int shift;
+};
+
 // Attention over pages (fa_paged.cuh)
 struct FaPagedParams {
   FaTensor q, k, v, o;  // k, v: sb is the stride of a page, ss of a token in it
@@ -90,7 +97,7 @@ struct FaPagedParams {
   int* status;
   int B, Hq, Hkv, Sq;
   int num_pages, page_size, max_len;  // max_len: tokens that the table has room for
-  int page_shift;                     // log2 of page_size, or -1
+  FaDiv by_page, by_group, by_tiles;  // by page_size, Hq / Hkv, row_tiles
   int row_tiles, workers;             // row tiles of a request; CTAs
   int window;                         // keys more than this far behind a query are not seen (-1: all are)
   int b_off, h_off;

@@ -273,6 +273,12 @@ struct PagedCfg {
   bool tma, one_each;  // one_each: a CTA per segment (FA_SHORT)
 };
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
+FaDiv divide_by(int d) {
+  FaDiv r{0, -1};
+  while (d > 1 && (d - 1) >> (r.shift + 1) != 0) ++r.shift;  // 2^shift < d <= 2^(shift + 1)
+  if (d > 1) r.mul = (unsigned)((1ull << (32 + r.shift)) / (unsigned)d + 1);
+  return r;
+}
 
 // Tiles, buffers and CTAs per SM (the map of fa_paged.cuh).
 //   * Rows: a warp takes 16; of 16-bit types up to 8, and 17 to 24 where the registers allow it, in the way made for few (`few` groups of 8);
@@ -449,9 +455,8 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
   k.lse = p->lse; k.table = p->block_table; k.table_stride = p->block_table_stride; k.lengths = p->lengths; k.status = p->status;
   k.B = p->B; k.Hq = p->Hq; k.Hkv = p->Hkv; k.Sq = p->Sq;
   k.num_pages = (int)p->num_pages; k.page_size = p->page_size;
-  k.page_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if (p->page_size == 1 << i) k.page_shift = i;
+  k.by_page = divide_by(p->page_size);
+  k.by_group = divide_by(p->Hq / p->Hkv);
   k.max_len = (int)std::min<long long>((long long)p->table_width * p->page_size, 0x7fffffffll - 64);
   k.window = p->window < 0 ? -1 : std::min(p->window, 1 << 30);
   k.b_off = p->b_offset; k.h_off = p->h_offset; k.scale = p->scale;
@@ -465,6 +470,7 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
     }
   }
   k.row_tiles = paged_row_tiles(p, c);
+  k.by_tiles = divide_by(k.row_tiles);
   k.workers = paged_workers(c);
   const size_t rows = 2 * (size_t)k.workers * c.BM;
   k.part_o = (float*)workspace;
