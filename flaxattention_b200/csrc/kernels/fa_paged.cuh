@@ -695,32 +695,11 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     ++n_used;
   };
 
-#pragma unroll 1
-  for (int t = t0; t < t1;) {
-    // this worker's part of the segment: tiles seg.tile .. part_end - 1
-    const int part_end = min(seg.last, seg.tile + (t1 - t)), rt = seg.item - seg.b * p.row_tiles;
-    const int rows = min(G * p.Sq - rt * BM, BM);
-    int qpos[HR], head[HR];  // of this thread's rows: position (-1: no row), query head
-#pragma unroll
-    for (int h = 0; h < HR; ++h) {
-      const int row = rt * BM + R.row(h), i = divided(row, p.by_group);
-      head[h] = seg.hk * G + row - i * G;
-      qpos[h] = i < p.Sq ? seg.pos - seg.first + i : -1;
-      R.m[h] = FA_NEG_INF;
-      R.l[h] = 0.f;
-    }
-    R.clear();
+#if FA_DTYPE != FA_DT_F32
+  // the queries of a segment: rows g, g + 8, .. of the row tile, g = lane / 4
+  auto load_q = [&]() {
+    const int rt = seg.item - seg.b * p.row_tiles;
     const char* qb = (const char*)p.q.ptr + seg.b * p.q.sb * ES;
-#if FA_DTYPE == FA_DT_F32
-    __syncthreads();  // (the rows of the segment before have been read)
-    for (int i = tid; i < QROWS * (D / 4); i += NT) {
-      const int r = i / (D / 4), c = i - r * (D / 4), row = rt * BM + r, qi = divided(row, p.by_group);
-      const float* src = (const float*)(qb + (qi * p.q.ss + (long long)(seg.hk * G + row - qi * G) * p.q.sh) * ES) + c * 4;
-      *(float4*)(q_tile + r * PQ + c * 16) = qi < p.Sq ? *(const float4*)src : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    __syncthreads();
-#else
-    // (rows g, g + 8, .. of the row tile, g = lane / 4)
 #pragma unroll
     for (int q = 0; q < (FEW ? NQ : 2); ++q) {
       const int row = rt * BM + row0 + q * 8 + (lane >> 2), i = divided(row, p.by_group);
@@ -737,6 +716,34 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #endif
       }
     }
+  };
+  load_q();
+#endif
+
+#pragma unroll 1
+  for (int t = t0; t < t1;) {
+    // this worker's part of the segment: tiles seg.tile .. part_end - 1
+    const int part_end = min(seg.last, seg.tile + (t1 - t)), rt = seg.item - seg.b * p.row_tiles;
+    const int rows = min(G * p.Sq - rt * BM, BM);
+    int qpos[HR], head[HR];  // of this thread's rows: position (-1: no row), query head
+#pragma unroll
+    for (int h = 0; h < HR; ++h) {
+      const int row = rt * BM + R.row(h), i = divided(row, p.by_group);
+      head[h] = seg.hk * G + row - i * G;
+      qpos[h] = i < p.Sq ? seg.pos - seg.first + i : -1;
+      R.m[h] = FA_NEG_INF;
+      R.l[h] = 0.f;
+    }
+    R.clear();
+#if FA_DTYPE == FA_DT_F32
+    const char* qb = (const char*)p.q.ptr + seg.b * p.q.sb * ES;
+    __syncthreads();  // (the rows of the segment before have been read)
+    for (int i = tid; i < QROWS * (D / 4); i += NT) {
+      const int r = i / (D / 4), c = i - r * (D / 4), row = rt * BM + r, qi = divided(row, p.by_group);
+      const float* src = (const float*)(qb + (qi * p.q.ss + (long long)(seg.hk * G + row - qi * G) * p.q.sh) * ES) + c * 4;
+      *(float4*)(q_tile + r * PQ + c * 16) = qi < p.Sq ? *(const float4*)src : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __syncthreads();
 #endif
 
     // ---- the tiles of this key group (a group whose wait has run out leaves them out, but takes part in the merges)
@@ -863,13 +870,15 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     }
 
     // ---- the end of the segment, or of this worker's part of it: written out if the part is the segment
-    bool whole = true;
-    if (!SHORT) {
-      Seg x;
-      seg_open(p, seg.item, x);
-      whole = seg.tile == x.tile && part_end == seg.last;
+    const bool whole = SHORT || (seg.tile == seg.begin / WN && part_end == seg.last);
+    const int part = (int)blockIdx.x * 2 + (t == t0 ? 0 : 1), b = seg.b, hk = seg.hk;
+    t += part_end - seg.tile;
+    if (t < t1) {
+      seg_advance(p, seg, part_end - seg.tile);
+#if FA_DTYPE != FA_DT_F32
+      load_q();  // (on their way during the merge)
+#endif
     }
-    const int part = (int)blockIdx.x * 2 + (t == t0 ? 0 : 1);
     float* const part_o = p.part_o + (long long)part * BM * DV;
     float* const part_ml = p.part_ml + (long long)part * BM * 2;
     Rows::over_keys(R.l, Sum());
@@ -902,8 +911,8 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
             if (whole) {
               f *= inverse(l);
               if (i % CG == 0 && p.lse != nullptr) {
-                const int qi = divided(rt * BM + r, p.by_group), hd = seg.hk * G + rt * BM + r - qi * G;
-                p.lse[((long long)seg.b * p.Hq + hd) * p.Sq + qi] = log_sum(m_use, l);
+                const int qi = divided(rt * BM + r, p.by_group), hd = hk * G + rt * BM + r - qi * G;
+                p.lse[((long long)b * p.Hq + hd) * p.Sq + qi] = log_sum(m_use, l);
               }
             } else if (i % CG == 0) {
               *(float2*)(part_ml + r * 2) = make_float2(m, l);
@@ -926,8 +935,8 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
             y += f * v.y;
           }
           if (whole) {
-            const int qi = divided(rt * BM + r, p.by_group), hd = seg.hk * G + rt * BM + r - qi * G;
-            put2((char*)p.o.ptr + (seg.b * p.o.sb + hd * p.o.sh + qi * p.o.ss) * ES, blk * 32 + c, x, y);
+            const int qi = divided(rt * BM + r, p.by_group), hd = hk * G + rt * BM + r - qi * G;
+            put2((char*)p.o.ptr + (b * p.o.sb + hd * p.o.sh + qi * p.o.ss) * ES, blk * 32 + c, x, y);
           } else {
             *(float2*)(part_o + r * DV + blk * 32 + c) = make_float2(x, y);
           }
@@ -940,11 +949,11 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #pragma unroll
       for (int h = 0; h < HR; ++h) {
         const int i = divided(rt * BM + R.row(h), p.by_group);
-        out[h] = (char*)p.o.ptr + (seg.b * p.o.sb + head[h] * p.o.sh + i * p.o.ss) * ES;
+        out[h] = (char*)p.o.ptr + (b * p.o.sb + head[h] * p.o.sh + i * p.o.ss) * ES;
         inv[h] = inverse(R.l[h]);
         if (R.row(h) >= rows || !R.speaks()) continue;
         if (!whole) *(float2*)(part_ml + R.row(h) * 2) = make_float2(R.m[h], R.l[h]);
-        else if (p.lse != nullptr) p.lse[((long long)seg.b * p.Hq + head[h]) * p.Sq + i] = log_sum(R.m[h], R.l[h]);
+        else if (p.lse != nullptr) p.lse[((long long)b * p.Hq + head[h]) * p.Sq + i] = log_sum(R.m[h], R.l[h]);
       }
 #pragma unroll
       for (int blk = 0; blk < (DV + 31) / 32; ++blk)
@@ -954,8 +963,6 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
           else part_o[R.row(h) * DV + c] = v;
         });
     }
-    t += part_end - seg.tile;
-    if (t < t1) seg_advance(p, seg, part_end - seg.tile);
   }
   fa_grid_release();
   fa_cp_wait<0>();
