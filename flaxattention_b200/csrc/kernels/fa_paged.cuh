@@ -695,6 +695,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     ++n_used;
   };
 
+  if (SHORT) fa_grid_release();
 #if FA_DTYPE != FA_DT_F32
   // the queries of a segment: rows g, g + 8, .. of the row tile, g = lane / 4
   auto load_q = [&]() {
@@ -964,7 +965,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
         });
     }
   }
-  fa_grid_release();
+  if (!SHORT) fa_grid_release();
   fa_cp_wait<0>();
 #if FA_TMA
   if (failed) {

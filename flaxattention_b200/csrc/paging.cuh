@@ -356,7 +356,7 @@ int get_paged_kernel(fa_module* m, const fa_paged_params* p, const PagedCfg& c, 
                     "fa_paged_kernel", c.smem, k, p->dtype == FA_F32 ? nullptr : "--prec-div=false");
 }
 
-int paged_check(fa_module* m, const fa_paged_params* p) {
+int paged_check(fa_module* m, const fa_paged_params* p, PagedCfg& c) {
   if (!m) return fail(FA_EINVAL, "module is null");
   if (!p) return fail(FA_EINVAL, "params is null");
   if (p->dtype < FA_F16 || p->dtype > FA_F32) return fail(FA_EINVAL, "unknown dtype");
@@ -375,7 +375,6 @@ int paged_check(fa_module* m, const fa_paged_params* p) {
   if (int rc = check_tensor(p->o, "o", es)) return rc;
   if (int rc = check_tensor(p->k_pages, "k_pages", es, p->num_pages > 0)) return rc;
   if (int rc = check_tensor(p->v_pages, "v_pages", es, p->num_pages > 0)) return rc;
-  PagedCfg c;
   pick_paged(p, c);
   if ((long long)p->B * p->Hq * p->Sq > 0x7fffffffll - 1024) return fail(FA_EUNSUPPORTED, "B * Hq * Sq must stay below 2^31");
   const long long longest = std::min<long long>((long long)p->table_width * p->page_size, 0x7fffffffll);
@@ -384,6 +383,11 @@ int paged_check(fa_module* m, const fa_paged_params* p) {
 }
 
 size_t paged_up(size_t n) { return (n + 255) / 256 * 256; }
+size_t paged_bytes(const fa_paged_params* p, const PagedCfg& c) {
+  if (c.one_each) return 0;
+  const size_t rows = 2 * (size_t)paged_workers(c) * c.BM;
+  return paged_up(rows * p->Dv * 4) + paged_up(rows * 8) + paged_up(((size_t)p->B * paged_row_tiles(p, c) + 1) * 4);
+}
 
 }  // namespace
 
@@ -415,15 +419,14 @@ int fa_page_step(const int32_t* lengths, const int32_t* new_tokens, int B, int32
 
 size_t fa_paged_workspace_bytes(const fa_paged_params* p) {
   if (!p || p->Hkv <= 0 || p->Hq <= 0 || p->Sq <= 0 || p->D <= 0 || p->Dv <= 0 || p->page_size <= 0 || p->B <= 0) return 0;
-  size_t most = 0;
-  for (int flags : {p->flags, p->flags | FA_FLAG_GENERAL_KERNELS}) {  // (what runs where no tensor map takes the strides)
+  PagedCfg c;
+  pick_paged(p, c);
+  size_t most = paged_bytes(p, c);
+  if (c.tma) {  // (what runs where no tensor map takes the strides)
     fa_paged_params q = *p;
-    q.flags = flags;
-    PagedCfg c;
+    q.flags |= FA_FLAG_GENERAL_KERNELS;
     pick_paged(&q, c);
-    if (c.one_each) continue;
-    const size_t rows = 2 * (size_t)paged_workers(c) * c.BM;
-    most = std::max(most, paged_up(rows * p->Dv * 4) + paged_up(rows * 8) + paged_up(((size_t)p->B * paged_row_tiles(p, c) + 1) * 4));
+    most = std::max(most, paged_bytes(&q, c));
   }
   return most;
 }
@@ -440,13 +443,10 @@ int fa_paged_prepare(fa_module* m, const fa_paged_params* p) {
 }
 
 int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t workspace_bytes, void* stream) {
-  if (int rc = paged_check(m, p)) return rc;
-  const size_t need = fa_paged_workspace_bytes(p);
-  if (need && (!workspace || workspace_bytes < need)) return fail(FA_EWORKSPACE, "paged attention workspace too small");
+  PagedCfg c;
+  if (int rc = paged_check(m, p, c)) return rc;
   if ((uintptr_t)workspace & 15) return fail(FA_EINVAL, "workspace must be 16-byte aligned");
   prof_reset();
-  PagedCfg c;
-  pick_paged(p, c);
   FaPagedLaunchHost L;
   memset(&L, 0, sizeof L);
   FaPagedParams& k = L.p;
@@ -469,6 +469,8 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
       pick_paged(&q, c);
     }
   }
+  const size_t need = paged_bytes(p, c);
+  if (need && (!workspace || workspace_bytes < need)) return fail(FA_EWORKSPACE, "paged attention workspace too small");
   k.row_tiles = paged_row_tiles(p, c);
   k.by_tiles = divide_by(k.row_tiles);
   k.workers = paged_workers(c);
