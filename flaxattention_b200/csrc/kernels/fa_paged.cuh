@@ -203,7 +203,60 @@ struct Rows {
 #pragma unroll
     for (int i = 0; i < NC; ++i) o[h][i] *= c;
   }
+  // Eight rows and more: what a lane reads of shared memory sets the pace (16 bytes of each lane take four cycles, also where lanes read the same), so a lane
+  // takes eight rows and four keys at a time, 12 reads for 64 two-value products where one key takes 17 for 32, of 1 in 128 / WN pieces of the
+  // head dim; then the lanes of a key swap and add what they have.  (64 segments of 4096 keys, D 128, one key / four: 8 rows 99 / 66 us, 16 rows 171 / 117,
+  // 28 rows 319 / 221; D 64, 8 rows 58 / 41; D 256, 16 rows 383 / 268.)  Not unrolled: twice is slower at D 256, 268 / 297, and the same elsewhere.
+  __device__ __forceinline__ void scores_by_four(const unsigned char* tile, int rows) {
+    constexpr int B4 = WN / 4, P = 32 / B4;
+    const int p0 = lane / B4, r = lane % B4;
+    // (the pieces of the lanes that are served together lie in different banks)
+    const int p = P == 4 ? p0 : P == 8 ? (p0 & 1) * 4 + (p0 >> 1) : (p0 & 3) * 2 + ((p0 >> 2) & 1) + (p0 & 8);
+#pragma unroll
+    for (int h0 = 0; h0 < HR; h0 += 8) {
+      fa_u64 acc[8][4];
+#pragma unroll
+      for (int h = 0; h < 8; ++h) acc[h][0] = acc[h][1] = acc[h][2] = acc[h][3] = 0ull;
+      if (!idle(h0, rows)) {
+        const bool all = !idle(h0 + 4, rows);
+#pragma unroll 1
+        for (int c = p; c < D / 4; c += P) {
+          ulonglong2 x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] = *(const ulonglong2*)(tile + chunk_at<PK>(0, r + k * B4, c));
+#pragma unroll
+          for (int h = 0; h < 8; ++h) {
+            if (h == 4 && !all) break;
+            const ulonglong2 y = *(const ulonglong2*)(q + (h0 + h) * D + c * 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[h][k] = fa_fma2(x[k].y, y.y, fa_fma2(x[k].x, y.x, acc[h][k]));
+          }
+        }
+        __syncwarp();
+      }
+      const bool upper = (lane & (WN / 2)) != 0, odd = (lane & B4) != 0;
+#pragma unroll
+      for (int h = 0; h < 8; ++h) {
+        float t[4], u[2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float e, o2;
+          fa_f2_unpack(acc[h][k], e, o2);
+          t[k] = e + o2;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) u[k] = (upper ? t[k + 2] : t[k]) + __shfl_xor_sync(0xffffffffu, upper ? t[k] : t[k + 2], WN / 2);
+        s[h0 + h] = (odd ? u[1] : u[0]) + __shfl_xor_sync(0xffffffffu, odd ? u[0] : u[1], B4);
+#pragma unroll
+        for (int off = WN; off < 32; off <<= 1) s[h0 + h] += __shfl_xor_sync(0xffffffffu, s[h0 + h], off);
+      }
+    }
+  }
   __device__ __forceinline__ void scores(const unsigned char* tile, fa_u32, int rows) {
+    if constexpr (HR >= 8) {
+      scores_by_four(tile, rows);
+      return;
+    }
     // (four sums for a product, two to an instruction: a chain of D / PARTS additions would be waited for)
     const float* qp = q + (lane / WN) * (D / PARTS);
     const int r = lane % WN, c0 = (lane / WN) * (D / PARTS / 4);
