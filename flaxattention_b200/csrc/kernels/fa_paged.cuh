@@ -21,7 +21,7 @@
 //
 // Measured (us on the GPU, bf16, up to 8 rows; of the bytes of K and V): 32 requests of 1640 to 16384 keys in pages of 64, 32 / 8 heads, D 128, 1.21 GB,
 // 182, 6.7 TB/s; one of 131072, 0.54 GB, 84 and 4 for the merge, 6.1 TB/s: DRAM, and 5.5 in front of the first product (the launch, the lengths,
-// the table, the first tiles) and behind the last.  64 requests of 16 keys 6.3: that chain alone.  20 rows and a score_mod 41: the chains of products
+// the table, the first tiles) and behind the last.  64 requests of 16 keys 6.3: that chain alone.  20 rows and a score_mod 40: the chains of products
 // and exponentials of 8 warps per SM, more than which 255 registers a thread do not allow.
 //
 // CTA = FA_CG key groups of FA_RG warps with 16 query rows each.  The warps of a key group share its tiles of K and V, which come by TMA
@@ -32,7 +32,8 @@
 //     queries its 8 columns.  For up to 8 rows, which is what one new token has, half the instructions of the next way, of which the
 //     queries would fill half; for 17 to 24, three quarters, and no second warp to wait for.
 //   * 16-bit, other rows: S = Q K', O = P V, 16 rows per warp.
-//   * fp32: on the FMA pipes, in fp32 throughout; a lane has a key (and a part of the head dim) for the scores, columns for the values.
+//   * fp32: on the FMA pipes, in fp32 throughout; a lane has a key, or from 8 rows on four keys of eight rows, and a part of the head dim for the
+//     scores, columns for the values.
 //
 // Compile-time parameters (macros): FA_DTYPE, FA_D, FA_DV, FA_RG (1, 2, 4), FA_WN (keys of a tile: 32 or 16; fp32: 32, 16, 8), FA_SLOTS, FA_TMA,
 // FA_FEW (0: the other way), FA_FR (fp32: rows of a warp), FA_CG, FA_SHORT.
