@@ -26,7 +26,7 @@ struct FaStepParams {
 // Where the things (tokens, pages) that a block fills lie among those of the requests of a chunk: `from[k]` is the first one of request k,
 // relative to the block's first.
 struct FaStepRange {
-  int from[kStepChunk + 1];
+  int from[kStepChunk];
   int lo, hi;  // the requests that hold the block's first and last
   static __device__ __forceinline__ int clamp(long long v) { return (int)max(min(v, 0x7fffffffll), -0x7fffffffll); }
   // the requests whose ranges hold x[..]: the last that begin at or in front of them.  Looked for together, in as many steps as the block's
@@ -99,9 +99,10 @@ __global__ void __launch_bounds__(kStepThreads) fa_page_step_kernel(const __grid
       tokens += warp_sum[0][w];
       pages += warp_sum[1][w];
     }
-    // what this block fills of the chunk's, relative to its range
-    const int t_lo = (int)max(tokens0 - lo, 0ll), t_hi = (int)max(min(hi, tokens) - lo, 0ll);
-    const int p_lo = (int)max(min(pages0 - page_lo, (long long)P.pages_per_block), 0ll), p_hi = (int)max(min(pages - page_lo, (long long)P.pages_per_block), 0ll);
+    // what this block fills of the chunk's, relative to its range (in 64 bits up to there: the requests may ask for more than 2^31 tokens in all)
+    const auto within = [](long long v, long long n) { return (int)max(min(v, n), 0ll); };
+    const int t_lo = within(tokens0 - lo, hi - lo), t_hi = within(tokens - lo, hi - lo);
+    const int p_lo = within(pages0 - page_lo, P.pages_per_block), p_hi = within(pages - page_lo, P.pages_per_block);
 #pragma unroll
     for (int i = 0; i < kStepItems; ++i) {
       const int k = tid * kStepItems + i, b = b0 + k;
@@ -113,7 +114,6 @@ __global__ void __launch_bounds__(kStepThreads) fa_page_step_kernel(const __grid
       if (t_lo < t_hi && ta < t_hi && t_hi <= tb) tok.hi = k;
       if (p_lo < p_hi && pa <= p_lo && p_lo < pb) pag.lo = k;
       if (p_lo < p_hi && pa < p_hi && p_hi <= pb) pag.hi = k;
-      if (k == kStepChunk - 1) pag.from[kStepChunk] = FaStepRange::clamp(pb);
       if (first && b < P.B) {
         P.out_len[b] = l[i] + n[i];
         P.starts[b] = (int)min(at_t, 0x7fffffffll);
@@ -161,9 +161,11 @@ __global__ void __launch_bounds__(kStepThreads) fa_page_step_kernel(const __grid
     }
     if (last && pages - page_lo > P.pages_per_block) {  // more new pages than the call has tokens for: request by request
       for (int k = warp; k < kStepChunk && b0 + k < P.B; k += kStepThreads / 32) {
-        const int had = had_of(k), skip = max(P.pages_per_block - pag.from[k], 0);
-        for (int i = skip + lane; i < pag.from[k + 1] - pag.from[k] && had + i < P.width; i += 32)
-          P.table[(long long)(b0 + k) * P.table_stride + had + i] = fresh(page_lo + pag.from[k] + (long long)i);
+        // (a request that begins 2^31 pages on has its place clamped: its number of pages is counted again, and the list has come to its end there)
+        const long long had = had_of(k), need = ((long long)len[k] + min(max(P.count[b0 + k], 0), 0x7fffffff - len[k]) + P.page - 1) / P.page;
+        const long long from = pag.from[k], end = min(need, (long long)P.width);
+        for (long long c = had + max(P.pages_per_block - from, 0ll) + lane; c < end; c += 32)
+          P.table[(b0 + k) * P.table_stride + c] = fresh(page_lo + from + c - had);
       }
     }
   }
@@ -406,7 +408,8 @@ int fa_page_step(const int32_t* lengths, const int32_t* new_tokens, int B, int32
   prof_reset();
   FaStepParams k{};
   k.len = lengths; k.count = new_tokens; k.free_pages = free_pages; k.taken_in = taken;
-  k.table = block_table; k.table_stride = block_table_stride; k.num_free = num_free; k.tokens = num_tokens;
+  k.table = block_table; k.table_stride = block_table_stride; k.tokens = num_tokens;
+  k.num_free = std::min<int64_t>(num_free, 0x7fffffffll);  // (no more pages have a number)
   k.B = B; k.width = table_width; k.page = page_size;
   k.out_len = out_lengths; k.positions = positions; k.requests = requests; k.starts = starts; k.taken_out = out_taken;
   k.slots = (long long*)slots;
