@@ -696,6 +696,20 @@ struct Rotary {
   bool bshd = false;
   at::Tensor table, positions, weights[2];
 
+  // where table and positions lie
+  static void place(fa_rotary_params& p, const at::Tensor& table, const at::Tensor& positions) {
+    if (table.defined()) {
+      p.table = p.rotary_dim > 0 ? (const float*)table.const_data_ptr() : nullptr;
+      p.table_stride = std::max<int64_t>(table.stride(0), table.size(0) == 1 ? table.size(1) : 0);
+    }
+    if (positions.defined()) {
+      const bool per_token = positions.dim() == 2;
+      p.positions = positions.const_data_ptr();
+      p.position_stride_b = per_token ? positions.stride(0) : 0;
+      p.position_stride_s = positions.stride(per_token ? 1 : 0);
+    }
+  }
+
   // rows: any of the tensors that are rotated; tokens from its shape
   void read(const at::Tensor& rows, PyObject* table_o, PyObject* positions_o, PyObject* const* weights_o, PyObject* eps, PyObject* interleaved) {
     p.dtype = dtype_code(rows, "the tensors");
@@ -715,9 +729,8 @@ struct Rotary {
       TORCH_CHECK_VALUE(table.size(1) <= 1 || table.stride(1) == 1, "the rows of table must be contiguous");
       no_gradient(table, "table", "the table of rotary positions");
       p.rotary_dim = (int)table.size(1);
-      p.table = p.rotary_dim > 0 ? (const float*)table.const_data_ptr() : nullptr;
       p.table_length = table.size(0);
-      p.table_stride = std::max<int64_t>(table.stride(0), table.size(0) == 1 ? table.size(1) : 0);
+      place(p, table, {});
       TORCH_CHECK_VALUE(p.table_stride >= p.rotary_dim, "the rows of table must not overlap");
       TORCH_CHECK_VALUE(p.rotary_dim == 0 || p.table_length > 0, "table has no rows");
     }
@@ -727,10 +740,8 @@ struct Rotary {
       TORCH_CHECK_VALUE(positions.device() == dev, "positions is on ", positions.device(), ", the others on ", dev);
       const bool per_token = positions.dim() == 2 && positions.size(0) == p.B && positions.size(1) == p.S;
       TORCH_CHECK_VALUE(per_token || (positions.dim() == 1 && positions.size(0) == p.S), "positions must be [B, S] or [S] = [", p.B, ", ", p.S, "], got ", positions.sizes());
-      p.positions = positions.const_data_ptr();
       p.position_bits = positions.scalar_type() == at::kInt ? 32 : 64;
-      p.position_stride_b = per_token ? positions.stride(0) : 0;
-      p.position_stride_s = positions.stride(per_token ? 1 : 0);
+      place(p, {}, positions);
     } else {
       TORCH_CHECK_VALUE(p.rotary_dim == 0 || p.S <= p.table_length, "the table has ", p.table_length, " positions, the tokens need ", p.S);
     }
@@ -749,6 +760,8 @@ struct Rotary {
     }
   }
 };
+
+constexpr const char* kGivenBack = "a saved tensor has come back with another shape, type or device";
 
 struct RotaryBackward : public torch::autograd::Node {
   Rotary r;  // (its tensors: the table and the positions)
@@ -779,6 +792,15 @@ struct RotaryBackward : public torch::autograd::Node {
       if (!some.defined()) return out;
       c10::cuda::OptionalCUDAGuard guard(some.device());
       const auto type = p.dtype == FA_F16 ? at::kHalf : p.dtype == FA_BF16 ? at::kBFloat16 : at::kFloat;
+      // (a saved-tensor hook may have given back something else than it was given, or the same with other strides)
+      const auto same = [&](const at::Tensor& t, at::ScalarType of) { return t.device() == some.device() && t.scalar_type() == of; };
+      for (int i = 0; i < 2; ++i)
+        TORCH_CHECK(!w[i].defined() || (same(w[i], p.weight_dtype == FA_F32 ? at::kFloat : type) && w[i].sizes() == at::IntArrayRef({p.D}) && w[i].is_contiguous()), kGivenBack);
+      TORCH_CHECK(!table.defined() || (same(table, at::kFloat) && table.sizes() == at::IntArrayRef({p.table_length, p.rotary_dim}) && (p.rotary_dim <= 1 || table.stride(1) == 1)), kGivenBack);
+      TORCH_CHECK(!positions.defined() || (same(positions, p.position_bits == 32 ? at::kInt : at::kLong) &&
+                                           (positions.sizes() == at::IntArrayRef({p.B, p.S}) || positions.sizes() == at::IntArrayRef({p.S}))),
+                  kGivenBack);
+      Rotary::place(p, table, positions);
       at::Tensor g[2], d[2], dw[2];
       fa_tensor gt[2], dt[2], unused{};
       for (int i = 0; i < 2; ++i) {
@@ -798,12 +820,10 @@ struct RotaryBackward : public torch::autograd::Node {
         dt[i] = by_strides(d[i], r.bshd);
         if (norm) {
           TORCH_CHECK(x[i].scalar_type() == type && x[i].sizes() == at::IntArrayRef(sizes[i]) && x[i].device() == some.device() && (x[i].size(3) == 1 || x[i].stride(3) == 1),
-                      "a saved tensor has come back with another shape, type or device");
+                      kGivenBack);
           (i == 0 ? p.q : p.k) = by_strides(x[i], r.bshd);
         }
       }
-      p.table = p.rotary_dim > 0 ? (const float*)table.const_data_ptr() : nullptr;
-      p.positions = positions.defined() ? positions.const_data_ptr() : nullptr;
       const size_t bytes = fa_rotary_bwd_workspace_bytes(&p);
       at::Tensor ws;
       if (bytes > 0) ws = empty({(int64_t)bytes}, at::kByte, some.device());
