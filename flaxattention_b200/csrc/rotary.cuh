@@ -615,7 +615,8 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_bwd_kernel(const __g
         }
         float sum[2] = {both(ss), both(gx)};
         rot_sums(sum, P.lane_shift);
-        const float r = rsqrtf(sum[0] * per_value + P.eps), m = -(sum[1] * r * per_value);
+        // (beyond the last token: 0, since an eps of 0 would leave no number in dw)
+        const float r = live ? rsqrtf(sum[0] * per_value + P.eps) : 0.f, m = -(sum[1] * r * per_value);
         const F2 rr = f2(r, r), mm = f2(m, m);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
