@@ -111,7 +111,7 @@ std::string cache_dir() {
 }
 
 const char* const kTemplateFiles[] = {"fa_params.h", "fa_common.cuh", "fa_fwd.cuh", "fa_bwd.cuh",
-                                      "fa_decode.cuh", "fa_blockmask.cuh", "fa_sm100.cuh", "fa_fwd_tc.cuh", "fa_bwd_items.cuh", "fa_bwd_tc.cuh", "fa_bwd_tc128.cuh", "fa_bwd_f32.cuh", "fa_selftest.cuh", "fa_paged.cuh", "fa_tanh.cuh"};
+                                      "fa_decode.cuh", "fa_blockmask.cuh", "fa_sm100.cuh", "fa_fwd_tc.cuh", "fa_bwd_items.cuh", "fa_bwd_tc.cuh", "fa_bwd_tc128.cuh", "fa_bwd_f32.cuh", "fa_selftest.cuh", "fa_paged.cuh", "fa_score_math.cuh"};
 std::string g_templates_hash;
 int templates_hash(std::string& out) {
   if (g_templates_hash.empty()) {
@@ -202,7 +202,7 @@ uint64_t kernel_key(KernelId id, std::initializer_list<std::pair<int, int>> fiel
 // Returns the compiled kernel `entry` of `tmpl` with the defines `make_defines` writes (compiling if needed).
 template <class MakeDefines>
 int get_kernel(fa_module* m, uint64_t key, const char* tmpl, MakeDefines make_defines, const char* entry, int smem,
-               Kernel** out, const char* option = nullptr) {
+               Kernel** out) {
   std::lock_guard<std::mutex> lk(g_mu);
   auto it = m->kernels.find(key);
   if (it != m->kernels.end()) {
@@ -215,10 +215,9 @@ int get_kernel(fa_module* m, uint64_t key, const char* tmpl, MakeDefines make_de
   std::string src = defines + "\n" + m->mod_source + "\n#include \"" + std::string(tmpl) + "\"\n";
   std::vector<std::string> opts = {"--gpu-architecture=sm_100a", "-std=c++17", "-lineinfo",
                                    "-I" + kernel_dir()};
-  if (option != nullptr) opts.push_back(option);
   int major = 0, minor = 0;
   nvrtcVersion(&major, &minor);
-  std::string h = hash_hex(src + "|" + th + "|" + std::to_string(major) + "." + std::to_string(minor) + (option != nullptr ? option : ""));
+  std::string h = hash_hex(src + "|" + th + "|" + std::to_string(major) + "." + std::to_string(minor));
   std::string cubin;
   const std::string cdir = cache_dir();
   const std::string cpath = cdir + "/" + h + ".cubin";

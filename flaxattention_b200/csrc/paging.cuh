@@ -348,14 +348,13 @@ int paged_row_tiles(const fa_paged_params* p, const PagedCfg& c) {
 }
 int paged_workers(const PagedCfg& c) { return c.per_sm * device_sm_count(); }
 
-// 16-bit types: a score_mod's divisions to two units in the last place of fp32, without the branches of exact ones (a score of 30 is then off by 4e-6,
-// its probability by as much in proportion, where the rounding of results to fp16 takes 5e-4).
+// (16-bit types: quotients and tanh of scores without branches, fa_score_math.cuh)
 int get_paged_kernel(fa_module* m, const fa_paged_params* p, const PagedCfg& c, Kernel** k) {
   return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.slots, 4}, {c.tma ? 1 : 0, 1}, {c.few, 2}, {c.fr, 5}, {c.CG, 4}, {c.one_each ? 1 : 0, 1}, {c.per_sm, 3}}), "fa_paged.cuh",
-                    [&] { return std::string(p->dtype == FA_F32 ? "" : "#include \"fa_tanh.cuh\"\n") +
+                    [&] { return std::string(p->dtype == FA_F32 ? "" : "#include \"fa_score_math.cuh\"\n") +
                                 defs({{"FA_DTYPE", p->dtype}, {"FA_D", p->D}, {"FA_DV", p->Dv}, {"FA_RG", c.RG}, {"FA_WN", c.WN},
                                        {"FA_SLOTS", c.slots}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_CG", c.CG}, {"FA_SHORT", c.one_each ? 1 : 0}, {"FA_CTAS", c.per_sm}}); },
-                    "fa_paged_kernel", c.smem, k, p->dtype == FA_F32 ? nullptr : "--prec-div=false");
+                    "fa_paged_kernel", c.smem, k);
 }
 
 int paged_check(fa_module* m, const fa_paged_params* p, PagedCfg& c) {

@@ -1278,10 +1278,28 @@ _CUDA_UN_F = {
 }
 
 
+# What passes a small relative error of an argument on as a small error of the value.  (Of a select: its two values.)
+_SMOOTH = {"add", "sub", "mul", "div", "neg", "abs", "min", "max", "exp", "exp2", "log", "log2", "sqrt", "tanh", "sigmoid", "sin", "cos", "erf", "select"}
+
+
+def _score_quotients(root: Expr) -> set:
+    """ids of the fp32 quotients and tanh in ``root`` whose argument depends on the score, which is off by some roundings itself, and
+    which reach the result through smooth functions only: they need not be exact to the last bit.  Any other may decide something (a
+    comparison, a rounding, an index)."""
+    decides = set() if root.dtype == F32 else {id(root)}
+    for e in reversed(_topo(root)):  # (a value comes behind everything that uses it)
+        for i, a in enumerate(e.args):
+            if id(e) in decides or e.op not in _SMOOTH or a.dtype != F32 or (e.op == "select" and i == 0):
+                decides.add(id(a))
+    dep: Dict[int, bool] = {}
+    return {id(e) for e in _topo(root) if e.op in ("div", "tanh") and id(e) not in decides and _depends_on_score(e.args[0], dep)}
+
+
 def to_cuda(mod: TracedMod, name: str) -> str:
     """Device function text.  Signature:
     ``float name(float score, int b, int h, int q, int kv)`` for a score mod (and its
     derivative), ``bool name(int b, int h, int q, int kv)`` for a mask mod."""
+    of_scores = _score_quotients(mod.root)
     lines: List[str] = []
     names: Dict[int, str] = {}
     ranges: Dict[int, Optional[Tuple[int, int]]] = {}
@@ -1308,6 +1326,12 @@ def to_cuda(mod: TracedMod, name: str) -> str:
                 rhs = f"(int)((unsigned){a[0]} {sym} (unsigned){a[1]})"
             else:
                 rhs = _CUDA_BIN[op].format(*a)
+        elif op == "div" and id(e) in of_scores:
+            c = e.args[1]
+            by = c.op == "const" and 2.0 ** -100 <= abs(c.value) <= 2.0 ** 100
+            rhs = f"FA_QUOTIENT{'_BY' if by else ''}({a[0]}, {a[1]})"
+        elif op == "tanh" and id(e) in of_scores:
+            rhs = f"FA_TANH({a[0]})"
         elif op == "div":
             rhs = f"({a[0]} / {a[1]})"
         elif op == "floordiv":
@@ -1691,6 +1715,16 @@ __device__ __forceinline__ float fa_pymod_f32(float a, float b) {
 """
 
 
+# (kernels that have quicker forms define them in front: fa_score_math.cuh)
+_QUOTIENT_PRELUDE = r"""
+#ifndef FA_QUOTIENT
+#define FA_QUOTIENT(a, b) ((a) / (b))
+#define FA_QUOTIENT_BY(a, c) ((a) / (c))
+#define FA_TANH(x) tanhf(x)
+#endif
+"""
+
+
 _BUFFER_PRELUDE = r"""
 // Captured buffers: every kernel fills this table from its parameters (FA_MOD_BUFS_INIT).
 __shared__ const void* fa_mod_buf[FA_NUM_MOD_BUFS];
@@ -1777,6 +1811,8 @@ class ModSet:
                 parts.append("#define FA_HAS_MASK_RANGE 1\n" + over_range)
         else:
             parts.append("__device__ __forceinline__ bool fa_mask_mod(int, int, int, int) { return true; }\n")
+        if any("FA_QUOTIENT" in t or "FA_TANH" in t for t in parts):
+            parts.insert(1, _QUOTIENT_PRELUDE)
         self.source = "".join(parts)
         self.key = hashlib.sha256(self.source.encode()).hexdigest()
 
