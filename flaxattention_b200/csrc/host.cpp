@@ -617,20 +617,38 @@ PyObject* build_block_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---- rotary positions, pages ------------------------------------------------------------------
 // These calls have no Python layer behind them: what is wrong with their arguments is said here.
+
+// Whether a tensor of a class of its own wants to see what is done with it
+bool looks_on(PyObject* o) {
+  if (THPVariable_Unpack(o).unsafeGetTensorImpl()->is_python_dispatch()) return true;
+  const auto function = [](PyObject* type) {  // what its __torch_function__ runs
+    PyObject* f = PyObject_GetAttrString(type, "__torch_function__");
+    if (f == nullptr) throw python_error();
+    if (PyMethod_Check(f)) {
+      PyObject* inner = PyMethod_GET_FUNCTION(f);
+      Py_INCREF(inner);
+      Py_DECREF(f);
+      f = inner;
+    }
+    return f;
+  };
+  Ref own(function((PyObject*)Py_TYPE(o))), plain(function(THPVariableClass)), c(PyImport_ImportModule("torch._C"));
+  if (c.p == nullptr) throw python_error();
+  Ref none(PyObject_GetAttrString(c.p, "_disabled_torch_function_impl"));
+  if (none.p == nullptr) throw python_error();
+  return own.p != plain.p && own.p != none.p;
+}
 const at::Tensor& cuda_tensor(PyObject* o, const char* name) {
   TORCH_CHECK_TYPE(THPVariable_Check(o), name, ": a tensor is expected, got ", Py_TYPE(o)->tp_name);
+  TORCH_CHECK_NOT_IMPLEMENTED(THPVariable_CheckExact(o) || !looks_on(o), name, ": a tensor of class ", Py_TYPE(o)->tp_name, " would not see what is done with it; pass a plain one");
   const at::Tensor& t = THPVariable_Unpack(o);
   TORCH_CHECK(t.is_cuda() && t.layout() == at::kStrided && t.has_storage(),
               name, ": flaxattention_b200 runs on CUDA tensors only; there is no CPU path");
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, ": there is no forward-mode derivative");
   return t;
 }
-// nothing that would look on is on (see watched): a trace or a transform would not see what these calls do
-void check_unwatched() {
-  TORCH_CHECK_NOT_IMPLEMENTED(!at::tracer::impl::is_dispatch_enabled() &&
-                                  !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode),
-                              "not under a tracer or a functorch transform");
-}
+// nothing that would look on is on (see watched): it would not see what these calls do
+void check_unwatched() { TORCH_CHECK_NOT_IMPLEMENTED(!watched(), "not under a tracer, a dispatch mode or a functorch transform"); }
 int dtype_code(const at::Tensor& t, const char* name) {
   const auto dt = t.scalar_type();
   TORCH_CHECK_VALUE(dt == at::kHalf || dt == at::kBFloat16 || dt == at::kFloat, "unsupported dtype ", dt, " of ", name, "; use float16, bfloat16 or float32");

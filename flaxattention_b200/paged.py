@@ -6,6 +6,8 @@ A cache is two tensors ``[pages, kv heads, page_size, D]`` (any strides with a c
 
 A decoding step is ``page_step`` once, and then, for every layer, ``rotary_append`` and ``paged_attention``.  None of
 them waits for the GPU or depends on a length that only the GPU knows, so that a step can be captured in a CUDA graph.
+What would look on (a tracer, a dispatch mode, a functorch transform, a tensor class with a ``__torch_function__`` of its own) is
+refused with ``NotImplementedError``.
 (No counterpart in the reference, whose keys and values are contiguous.)
 """
 from __future__ import annotations

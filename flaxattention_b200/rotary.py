@@ -78,6 +78,7 @@ def rotary_embedding(query, key, table, positions=None, *, query_weight=None, ke
     ``FlaxAttnError`` (``check_status``).  ``interleaved``: neighbouring values make a pair, instead of ``i`` and ``i + rotary_dim / 2``.
     ``query_weight`` / ``key_weight`` ``[D]`` (the tensors' dtype or float32): an RMS norm over the head dimension in front.
 
-    Gradients of the weights are sums over all rows in a fixed order.
+    Gradients of the weights are sums over all rows in a fixed order.  What would look on (a tracer, a dispatch mode, a functorch transform, a
+    tensor class with a ``__torch_function__`` of its own) is refused with ``NotImplementedError``.
     """
     return native().rotary(query, key, table, positions, query_weight, key_weight, eps, interleaved, not bhln)
