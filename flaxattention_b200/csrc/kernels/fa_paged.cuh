@@ -393,7 +393,8 @@ struct Rows {
     }
   }
   // Up to 8 rows the probabilities go in as two parts, rounded and what the rounding left: with one, bf16 results were 2.3e-3 off in place of the
-  // 1.7e-3 that rounding the output takes (D 128, 16384 keys).  With more rows the products would cost time.
+  // 1.7e-3 that rounding the output takes (D 128, 16384 keys).  With 17 to 24 rows the products would cost time: 8 % at D 64, 10 % at D 128 over calls of 100 to
+  // 131072 keys (20 rows, 32 x 8 segments of 8192, D 128: 179 us, 203 in two parts), for an error of 2.1e-4 in place of 2.9e-4 (fp16).
   __device__ __forceinline__ void values(const unsigned char*, fa_u32 tile, int) {
     constexpr bool TWO = NQ == 1;
 #pragma unroll
@@ -475,15 +476,23 @@ struct Rows {
       }
     }
   }
+  // Probabilities in two parts up to 16 rows (9 to 16: 3 % of the time; 32 x 8 segments of 8192 keys, D 128, 16 rows 177 / 180 us, one request of 131072, D 64, 52.5 / 53.2), as the decode kernel
+  // has them; not with more, where they would cost 4 to 9 % (28 rows, 32 x 8 segments of 8192, D 128: 217 / 242) and one part is what the forward kernel has.
   __device__ __forceinline__ void values(const unsigned char*, fa_u32 tile, int rows) {
+    constexpr bool TWO = RG == 1;
     if (RG > 1 && first_row >= rows) return;
 #pragma unroll
     for (int kj = 0; kj < WN / 16; ++kj) {
-      fa_u32 a[4];
+      fa_u32 a[4], rest[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float(&v)[4] = s[2 * kj + (i >> 1)];
         a[i] = fa_pack2<DT>(v[(i & 1) * 2], v[(i & 1) * 2 + 1]);
+        if (TWO) {
+          float x, y;
+          fa_rest2<DT>(v[(i & 1) * 2], v[(i & 1) * 2 + 1], x, y);
+          rest[i] = fa_pack2<DT>(x, y);
+        }
       }
 #pragma unroll
       for (int dj = 0; dj < DV / 16; ++dj) {
@@ -491,6 +500,10 @@ struct Rows {
         fa_ldsm_x4_t(chunk_at<PV>(tile, kj * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), dj * 2 + (lane >> 4)), r0, r1, r2, r3);
         fa_mma16816<DT>(o[2 * dj], a, r0, r1);
         fa_mma16816<DT>(o[2 * dj + 1], a, r2, r3);
+        if (TWO) {
+          fa_mma16816<DT>(o[2 * dj], rest, r0, r1);
+          fa_mma16816<DT>(o[2 * dj + 1], rest, r2, r3);
+        }
       }
     }
   }

@@ -76,8 +76,8 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, score_m
     first token) is 0, with a logsumexp of ``-inf``.  Returns the output in the shape of ``query`` and, with ``return_lse``, the natural-log
     logsumexp ``[B, Hq, Sq]`` in float32.
 
-    Scores, softmax and sums are in fp32; 16-bit probabilities are rounded to the dtype for the product with the values, and
-    a ``score_mod`` over 16-bit inputs divides scores and takes their ``tanh`` to some 2^-22; where a quotient decides something (a mask, a comparison, a
+    Scores, softmax and sums are in fp32; 16-bit probabilities are rounded to the dtype for the product with the values (up to
+    16 query rows per kv head in two parts, which leaves nothing of it), and a ``score_mod`` over 16-bit inputs divides scores and takes their ``tanh`` to some 2^-22; where a quotient decides something (a mask, a comparison, a
     rounding, an index) it is exact, as in ``flax_attention``.  Cached values of keys
     that ``mask_mod`` takes out must be finite; what lies behind a request's length or out of the window is not looked at, so that pages which the window
     has left may be given back.  A table entry that is no page, or a length beyond the table, leaves the keys out, and the next call raises
