@@ -711,8 +711,8 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid
         float c, sn;
         unit(k, i, j, c, sn);
         const float a = rot_get<DT>(x, i), d = j >= 0 ? rot_get<DT>(x, j) : 0.f;
-        m += (Real)(a * c - d * sn) * weight(i) * rot_get<DT>(in, i);
-        if (j >= 0) m += (Real)(d * c + a * sn) * weight(j) * rot_get<DT>(in, j);
+        m += ((Real)a * c - (Real)d * sn) * weight(i) * rot_get<DT>(in, i);
+        if (j >= 0) m += ((Real)d * c + (Real)a * sn) * weight(j) * rot_get<DT>(in, j);
       }
       m = rot_sum(m) * r / D;
     }
@@ -730,16 +730,16 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid
         a *= r * weight(i);
         if (j >= 0) d *= r * weight(j);
       }
-      float p = a * c - d * sn, q = d * c + a * sn;
+      Real p = (Real)a * c - (Real)d * sn, q = (Real)d * c + (Real)a * sn;
       if (BACK && norm) {
         const Real u = rot_get<DT>(in, i) * r, v = j >= 0 ? rot_get<DT>(in, j) * r : 0;
-        sums[warp][i] += p * (float)u;
-        if (j >= 0) sums[warp][j] += q * (float)v;
-        p = (float)(r * ((Real)p * weight(i) - u * m));
-        if (j >= 0) q = (float)(r * ((Real)q * weight(j) - v * m));
+        sums[warp][i] += (float)(p * u);
+        if (j >= 0) sums[warp][j] += (float)(q * v);
+        p = r * (p * weight(i) - u * m);
+        if (j >= 0) q = r * (q * weight(j) - v * m);
       }
-      rot_put<DT>(y, i, p);
-      if (j >= 0) rot_put<DT>(y, j, q);
+      rot_put<DT>(y, i, (float)p);
+      if (j >= 0) rot_put<DT>(y, j, (float)q);
     }
   }
   if (!BACK || P.dw[kind < 2 ? kind : 0] == nullptr) return;

@@ -6,6 +6,7 @@ import torch
 import flaxattention_b200 as fa
 from _pages import ROUNDOFF, normal
 from _util import DTYPES
+from test_rotary_gpu import run
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,10 @@ def test_norm_without_eps(dtype, S, D):
         for g, r, bound in ((got[i], want[0], 2.0 ** -20 * (8 + D ** 0.5) * want[0].abs().amax(-1, keepdim=True)),
                             (got[2 + i], want[1], 2.0 ** -20 * (8 + 4 * (x.numel() // D) ** 0.5))):
             assert ((g.cpu().double() - r).abs() <= ROUNDOFF[dt] * r.abs() + bound + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("seed", [66, 67, 68])
+def test_gradients_that_nearly_cancel(seed):
+    """Two values in a row under a norm: their gradient is what two terms leave, of some rows next to nothing."""
+    run(4, 33, 3, 64, 2, 2, "f32", norm=True, interleaved=True, bhln=False, seed=seed, which=(0,))
+    run(4, 33, 3, 64, 2, 2, "f32", norm=True, seed=seed)
