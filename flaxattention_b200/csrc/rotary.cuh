@@ -890,10 +890,6 @@ int rot_launch(FaRotParams& k, int dtype, void* stream) {
   });
 }
 
-#ifndef ROT_BH
-#define ROT_BH 8
-#endif
-constexpr int kRotBwdHeads = ROT_BH;  // heads of a group there
 // Blocks along the tokens of the backward with norm weights: about four per SM in all, two of which it holds at once.
 unsigned rot_bwd_blocks(const FaRotParams& k, long long token_blocks) {
   return (unsigned)std::min<long long>(token_blocks, std::max(1, 4 * device_sm_count() / (k.groups[0] + k.groups[1])));
