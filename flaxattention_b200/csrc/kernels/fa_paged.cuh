@@ -7,7 +7,7 @@
 // table[b][j / page_size].  Query i of the Sq is token len - Sq + i, which is also the index the mods see.
 //
 // The G query heads of a kv head share its K and V: their G * Sq rows (query-major, row r is head r % G of query r / G) are
-// cut into row tiles of 16, 32 or 64.  A segment is the keys that a row tile of a kv head of a request has to see, in tiles of FA_WN
+// cut into row tiles of 8, 16, 24, 32 or 64.  A segment is the keys that a row tile of a kv head of a request has to see, in tiles of FA_WN
 // keys.  Memory sets the pace: K and V are read once per segment.
 //
 // Who takes which tiles:
@@ -21,7 +21,7 @@
 //
 // Measured (us on the GPU, bf16, up to 8 rows; of the bytes of K and V): 32 requests of 1640 to 16384 keys in pages of 64, 32 / 8 heads, D 128, 1.21 GB,
 // 182, 6.7 TB/s; one of 131072, 0.54 GB, 84 and 4 for the merge, 6.1 TB/s: DRAM, and 5.5 in front of the first product (the launch, the lengths,
-// the table, the first tiles) and behind the last.  64 requests of 16 keys 6.3: that chain alone.  20 rows and a score_mod 40: the chains of products
+// the table, the first tiles) and behind the last.  64 requests of 16 keys 6.3: that chain alone.  20 rows under a capped score, 16 x 4 segments of 4097 keys (floor 20.6), 43: the chains of products
 // and exponentials of 8 warps per SM, more than which 255 registers a thread do not allow.
 //
 // CTA = FA_CG key groups of FA_RG warps with 16 query rows each.  The warps of a key group share its tiles of K and V, which come by TMA

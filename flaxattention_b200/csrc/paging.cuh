@@ -284,7 +284,10 @@ FaDiv divide_by(int d) {
 
 // Tiles, buffers and CTAs per SM (the map of fa_paged.cuh).
 //   * Rows: a warp takes 16; of 16-bit types up to 8, and 17 to 24 where the registers allow it, in the way made for few (`few` groups of 8);
-//     fp32 rounds up to a power of two.
+//     fp32 rounds up to a power of two.  17 to 24 rows, three groups in a warp against two warps of 16 (us, 20 rows, D 64 and D 128): 32 x 8 segments of
+//     8192 keys 103 / 166 and 182 / 211, one request of 131072 61 / 88 and 99 / 111, 64 x 8 segments of 400 26 / 35 and 34 / 44, 8 x 8 of 100 6.1 / 9.0 and 8.0 / 10.2.  Two warps
+//     are faster where a table has room for far more than there is, so that segments are cut, and a worker's run is a few tiles (8 x 8 segments of 500 in tables of 16384
+//     17.5 / 11.0 and 16.4 / 14.6, 64 x 8 of 400 38 / 35 and 48 / 44); lengths are not known here.  All of 17 to 24 rows, lengths and mods timed: 12 % faster on average.
 //   * Keys of a tile: 32; fewer for wide heads, so that a tile of K or V stays at 8 KB and an SM has room for as many of them.
 //   * CTAs of four warps, as many per SM as hold two slots (a tile of K and one of V) for each key group, up to four: that many warps hide each
 //     other's waits, and more slots for fewer do not (us, two CTAs with three or more slots / three or four with two: 32 requests of up to 16384 keys D 128

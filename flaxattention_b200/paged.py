@@ -42,7 +42,8 @@ def page_step(lengths, new_tokens, block_table, free_pages, page_size: int, num_
 
     Where the free list or the row of a table is too short, tokens get the slot -1 (``rotary_append`` leaves them out) and table
     entries -1; ``taken`` then is beyond the list's length.  If ``num_tokens`` is larger than the sum, the rest is padding: position 0,
-    slot and request -1.  Nothing else is changed, so that a call may be repeated, with the same results.
+    slot and request -1.  Nothing else is changed, so that a call may be repeated, with the same results.  The list is only gone through
+    forwards: pages that are given back go into a new one, with ``taken`` beginning at 0 again.
     """
     return PageStep._make(native().page_step(lengths, new_tokens, block_table, free_pages, page_size, num_tokens, taken))
 
@@ -76,13 +77,14 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, score_m
     first token) is 0, with a logsumexp of ``-inf``.  Returns the output in the shape of ``query`` and, with ``return_lse``, the natural-log
     logsumexp ``[B, Hq, Sq]`` in float32.
 
-    Scores, softmax and sums are in fp32; 16-bit probabilities are rounded to the dtype for the product with the values (up to
-    16 query rows per kv head in two parts, which leaves nothing of it), and a ``score_mod`` over 16-bit inputs divides scores and takes their ``tanh`` to some 2^-22; where a quotient decides something (a mask, a comparison, a
-    rounding, an index) it is exact, as in ``flax_attention``.  Cached values of keys
-    that ``mask_mod`` takes out must be finite; what lies behind a request's length or out of the window is not looked at, so that pages which the window
-    has left may be given back.  A table entry that is no page, or a length beyond the table, leaves the keys out, and the next call raises
-    ``FlaxAttnError`` (``check_status``).  Meant for a few tokens per request; there is no
-    gradient.  ``kernel_options``: ``{"kernels": "general"}`` takes keys and values in 16-byte pieces where TMA would do.
+    Scores, softmax and sums are in fp32; 16-bit probabilities are rounded to the dtype for the product with the values (up to 16 query rows per
+    kv head in two parts, which leaves nothing of it), and a ``score_mod`` over 16-bit inputs divides scores and takes their ``tanh`` to some 2^-22; where a
+    quotient decides something (a mask, a comparison, a rounding, an index) it is exact, as in ``flax_attention``.  As there, a ``score_mod`` takes a key out with
+    any score below -2.3e38 (the lowest of float32, ``-inf``), and a row with no other is 0.  Cached values of keys that ``mask_mod`` takes out must be
+    finite; what lies behind a request's length or out of the window is not looked at, so that pages which the window has left may be given back.  A
+    table entry that is no page, or a length beyond the table, leaves the keys out, and the next call raises ``FlaxAttnError``
+    (``check_status``).  Meant for a few tokens per request; there is no gradient.  ``kernel_options``: ``{"kernels": "general"}`` takes keys and values in
+    16-byte pieces where TMA would do.
     """
     general = kernel_options is not None and kernel_options.get("kernels") == "general"
     call = native().paged_attention

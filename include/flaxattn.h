@@ -263,7 +263,7 @@ int fa_mask_bits(fa_module* m, int B, int H, int Q_LEN, int KV_LEN, int b_offset
  *   (a, b) -> (a cos - b sin, b cos + a sin)         for the pairs of the first rotary_dim values of y
  *
  * in one pass, in fp32, rounded once.  Pairs are i and i + rotary_dim / 2, or neighbours (interleaved).  Any strides with a
- * contiguous head dimension are taken; 16-byte aligned ones whose head and rotary dims are multiples of 32 bytes are fast. */
+ * contiguous head dimension are taken; 16-byte aligned ones whose head dims are multiples of 16 bytes are fast, most of all with a rotary_dim of whole 32 bytes. */
 typedef struct fa_rotary_params {
   int32_t dtype;        /* of all tensors */
   int32_t weight_dtype; /* of the norm weights and their gradients: dtype or FA_F32 */
