@@ -83,7 +83,7 @@ def main(steps=8, prompts=(5, 33, 1, 70), check=False):
         q, k, v = layer.split(x)
         q2 = fa.rotary_append(q, k, v, layer.keys, layer.values, step.slots, table, step.positions[None], query_weight=layer.wq, key_weight=layer.wk, bhln=False)
         # (the keys as attention needs them here are the ones in the cache)
-        k2 = layer.keys.transpose(1, 2).reshape(-1, KV_HEADS, DIM)[step.slots][None]
+        k2 = layer.keys[step.slots // PAGE, :, step.slots % PAGE][None]
         o = fa.flax_attention_pallas(q2, k2, v, score_mod=softcap, mask_mod=same_request, bhln=False, enable_gqa=True)
         x = x + o.reshape(len(x), -1) @ layer.out
     outputs = [x]
