@@ -476,8 +476,9 @@ struct Rows {
       }
     }
   }
-  // Probabilities in two parts up to 16 rows (9 to 16: 3 % of the time; 32 x 8 segments of 8192 keys, D 128, 16 rows 177 / 180 us, one request of 131072, D 64, 52.5 / 53.2), as the decode kernel
-  // has them; not with more, where they would cost 4 to 9 % (28 rows, 32 x 8 segments of 8192, D 128: 217 / 242) and one part is what the forward kernel has.
+  // Probabilities in two parts up to 16 rows, as the decode kernel has them (9 to 16: 3 % of the time at D 64 to 256 on average, 6 at D 32, 11 at most; 16 rows,
+  // 32 x 8 segments of 8192 keys, D 128 177 / 180 us, one request of 131072, D 64 52.5 / 53.2); not with more, where they would cost 4 to 9 % (28 rows,
+  // 32 x 8 segments of 8192, D 128: 217 / 242) and one part is what the forward kernel has.
   __device__ __forceinline__ void values(const unsigned char*, fa_u32 tile, int rows) {
     constexpr bool TWO = RG == 1;
     if (RG > 1 && first_row >= rows) return;
