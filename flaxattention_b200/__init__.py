@@ -4,7 +4,7 @@ Export list follows flaxattention/__init__.py:11-22 (without the matplotlib visu
 """
 from .attention import check_status, flax_attention, flax_attention_pallas, math_attention
 from .blockmask import BlockMask, and_masks, create_block_mask, noop_mask, or_masks
-from .paged import PageStep, page_step, paged_attention, rotary_append
+from .paged import PageStep, page_step, paged_attention, read_pages, rotary_append
 from .pipeline import HostPipeline
 from .rotary import rotary_embedding, rotary_table
 from . import fnp, masks, mods  # noqa: F401
@@ -31,6 +31,7 @@ __all__ = [
     "rotary_append",
     "PageStep",
     "page_step",
+    "read_pages",
     "paged_attention",
     "fnp",
     "masks",

@@ -69,7 +69,7 @@ class FaRotaryParams(C.Structure):
         ("v", FaTensor), ("k_pages", FaTensor), ("v_pages", FaTensor),
         ("num_pages", C.c_int64), ("page_size", C.c_int32),
         ("slots", C.c_void_p), ("slot_stride_b", C.c_int64), ("slot_stride_s", C.c_int64),
-        ("status", C.c_void_p),
+        ("status", C.c_void_p), ("k_scales", FaTensor), ("v_scales", FaTensor),
     ]
 
 
@@ -82,6 +82,17 @@ class FaPagedParams(C.Structure):
         ("num_pages", C.c_int64), ("page_size", C.c_int32),
         ("block_table", C.c_void_p), ("block_table_stride", C.c_int64), ("table_width", C.c_int32),
         ("lengths", C.c_void_p), ("window", C.c_int32), ("lse", C.c_void_p), ("flags", C.c_int32), ("status", C.c_void_p),
+        ("k_scales", FaTensor), ("v_scales", FaTensor),
+    ]
+
+
+class FaReadParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("Dv", C.c_int32), ("num_tokens", C.c_int64),
+        ("k_pages", FaTensor), ("v_pages", FaTensor), ("k_scales", FaTensor), ("v_scales", FaTensor),
+        ("num_pages", C.c_int64), ("page_size", C.c_int32),
+        ("block_table", C.c_void_p), ("block_table_stride", C.c_int64), ("table_width", C.c_int32), ("starts", C.c_void_p),
+        ("k", FaTensor), ("v", FaTensor), ("status", C.c_void_p),
     ]
 
 
@@ -104,7 +115,7 @@ EXPORTS = [
     "fa_snapshot_bytes", "fa_snapshot", "fa_snapshot_holds",
     "fa_fwd_workspace_bytes", "fa_fwd_ws",
     "fa_rotary", "fa_rotary_bwd_workspace_bytes", "fa_rotary_bwd", "fa_rotary_append",
-    "fa_page_step", "fa_paged_workspace_bytes", "fa_paged", "fa_paged_prepare",
+    "fa_page_step", "fa_read_pages", "fa_paged_workspace_bytes", "fa_paged", "fa_paged_prepare",
 ]
 
 
@@ -169,6 +180,7 @@ def lib() -> C.CDLL:
     L.fa_rotary_append.argtypes = [C.POINTER(FaRotaryParams), C.c_void_p]
     L.fa_page_step.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
                                C.c_int, C.c_int64] + [C.c_void_p] * 7
+    L.fa_read_pages.argtypes = [C.POINTER(FaReadParams), C.c_void_p]
     L.fa_paged_workspace_bytes.restype = C.c_size_t
     L.fa_paged_workspace_bytes.argtypes = [C.POINTER(FaPagedParams)]
     L.fa_paged.argtypes = [C.c_void_p, C.POINTER(FaPagedParams), C.c_void_p, C.c_size_t, C.c_void_p]

@@ -1207,20 +1207,22 @@ int encode_fn(EncodeTiledFn* out) {
   return FA_OK;
 }
 
-// 4-d map (D, S, H, B) over a [.., S, D]-strided tensor; box = 128 bytes x box_rows rows, 128-byte swizzle
-int make_map(FaTensorMapHost* out, int dtype, const fa_tensor& t, int D, int S, int H, int B, int box_rows = 128) {
+// 4-d map (D, S, H, B) over a [.., S, D]-strided tensor; box = 128 bytes (or 64) x box_rows rows, swizzled over as many
+constexpr int kMapInt8 = 3;  // (a type beside FA_F16, FA_BF16 and FA_F32)
+int make_map(FaTensorMapHost* out, int dtype, const fa_tensor& t, int D, int S, int H, int B, int box_rows = 128, int box_bytes = 128) {
   EncodeTiledFn enc = nullptr;
   if (int rc = encode_fn(&enc)) return rc;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
-  const cuuint64_t es = (cuuint64_t)esize(dtype);
+  const cuuint64_t es = dtype == kMapInt8 ? 1 : (cuuint64_t)esize(dtype);
   const cuuint64_t strides[3] = {(cuuint64_t)t.stride_s * es, (cuuint64_t)t.stride_h * es, (cuuint64_t)t.stride_b * es};
-  const cuuint32_t box[4] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows, 1, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)(box_bytes / es), (cuuint32_t)box_rows, 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType type = dtype == FA_F16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+  const CUtensorMapDataType type = dtype == kMapInt8  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : dtype == FA_F16  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                    : dtype == FA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   CUresult r = enc((CUtensorMap*)out, type, 4,
-                   t.ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   t.ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FA_ECUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
   return FA_OK;

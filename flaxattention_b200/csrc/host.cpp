@@ -19,6 +19,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -923,12 +924,17 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// pages as fa_rotary_params and fa_paged_params have them: [pages, heads, tokens of a page, D] by strides
-void read_pages(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& as, int64_t heads, int64_t D, fa_tensor& k, fa_tensor& v, int64_t& n, int32_t& size) {
+// pages as fa_rotary_params and fa_paged_params have them: [pages, heads, tokens of a page, D] by strides; eight: of int8
+void pages_of(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& as, int64_t heads, int64_t D, fa_tensor& k, fa_tensor& v, int64_t& n, int32_t& size, bool eight = false) {
   rows_of(kp, "key_pages");
   rows_of(vp, "value_pages");
-  same_kind(kp, as, "key_pages");
-  same_kind(vp, as, "value_pages");
+  if (eight) {
+    int_kind(kp, at::kChar, as.device(), "key_pages (with scales)");
+    int_kind(vp, at::kChar, as.device(), "value_pages (with scales)");
+  } else {
+    same_kind(kp, as, "key_pages");
+    same_kind(vp, as, "value_pages");
+  }
   TORCH_CHECK_VALUE(kp.size(1) == heads && kp.size(3) == D, "key_pages must be [pages, ", heads, ", page_size, ", D, "], got ", kp.sizes());
   TORCH_CHECK_VALUE(vp.size(0) == kp.size(0) && vp.size(1) == kp.size(1) && vp.size(2) == kp.size(2), "value_pages must be the same pages as key_pages, got ", vp.sizes(), " and ", kp.sizes());
   TORCH_CHECK_VALUE(kp.size(2) > 0, "the pages hold no tokens");
@@ -938,10 +944,41 @@ void read_pages(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& as
   size = (int32_t)kp.size(2);
 }
 
-// rotary_append(q or None, k, v, key_pages, value_pages, slots, table, positions, query_weight, key_weight, eps, interleaved, bshd) -> q' or None
+// The scales of pages in 8 bits: [pages, heads, tokens of a page] of float32 by strides, both or none
+struct Scales {
+  at::Tensor k, v;
+  bool given = false;
+  Scales(PyObject* ko, PyObject* vo) {
+    TORCH_CHECK_VALUE((ko == Py_None) == (vo == Py_None), "key_scales and value_scales: both or none");
+    if (ko == Py_None) return;
+    given = true;
+    k = cuda_tensor(ko, "key_scales");
+    v = cuda_tensor(vo, "value_scales");
+  }
+  static fa_tensor one(const at::Tensor& t, const at::Tensor& pages, const char* name) {
+    int_kind(t, at::kFloat, pages.device(), name);
+    TORCH_CHECK_VALUE(t.dim() == 3 && t.size(0) == pages.size(0) && t.size(1) == pages.size(1) && t.size(2) == pages.size(2), name, " must be [pages, kv heads, page_size] = ",
+                      pages.sizes().slice(0, 3), ", got ", t.sizes());
+    return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+  }
+  // (pages that hold nothing: the address says whether there are scales)
+  static fa_tensor there(fa_tensor t) {
+    static float nothing;
+    if (t.ptr == nullptr) t.ptr = &nothing;
+    return t;
+  }
+  void fill(const at::Tensor& kp, const at::Tensor& vp, fa_tensor& ks, fa_tensor& vs) const {
+    if (!given) return;
+    ks = there(one(k, kp, "key_scales"));
+    vs = there(one(v, vp, "value_scales"));
+  }
+};
+
+// rotary_append(q or None, k, v, key_pages, value_pages, slots, table, positions, query_weight, key_weight, eps, interleaved, bshd, key_scales, value_scales)
+// -> q' or None
 PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK(n == 13, "rotary_append takes 13 arguments");
+  TORCH_CHECK(n == 15, "rotary_append takes 15 arguments");
   check_unwatched();
   const bool has_q = a[0] != Py_None;
   const at::Tensor k = cuda_tensor(a[1], "key"), v = cuda_tensor(a[2], "value"), q = has_q ? cuda_tensor(a[0], "query") : at::Tensor();
@@ -968,7 +1005,16 @@ PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.Hkv = (int)k.size(ih);
   p.Dv = (int)v.size(3);
   int64_t pages = 0;
-  read_pages(kp, vp, k, p.Hkv, p.D, p.k_pages, p.v_pages, pages, p.page_size);
+  const Scales scales(a[13], a[14]);
+  TORCH_CHECK_NOT_IMPLEMENTED(!scales.given || p.dtype != FA_F32, "pages in 8 bits take float16 and bfloat16 tensors");
+  pages_of(kp, vp, k, p.Hkv, p.D, p.k_pages, p.v_pages, pages, p.page_size, scales.given);
+  scales.fill(kp, vp, p.k_scales, p.v_scales);
+  if (scales.given) {
+    writable(scales.k, "key_scales");
+    writable(scales.v, "value_scales");
+    no_gradient(scales.k, "key_scales", "rotary_append");
+    no_gradient(scales.v, "value_scales", "rotary_append");
+  }
   TORCH_CHECK_VALUE(vp.size(3) == p.Dv, "value_pages must have the embedding dimension of value, got ", vp.size(3), " and ", p.Dv);
   p.num_pages = pages;
   writable(kp, "key_pages");
@@ -1000,6 +1046,10 @@ PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (rc != FA_OK) raise(rc);
     written(kp);
     written(vp);
+    if (scales.given) {
+      written(scales.k);
+      written(scales.v);
+    }
   }
   if (!has_q) Py_RETURN_NONE;
   return THPVariable_Wrap(qo);
@@ -1071,11 +1121,84 @@ PyObject* page_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// a block table of B requests
+void table_of(const at::Tensor& table, int64_t B, c10::Device dev) {
+  int_kind(table, at::kInt, dev, "block_table");
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) == B && (table.size(1) <= 1 || table.stride(1) == 1) && table.size(1) <= INT32_MAX,
+                    "block_table must be [", B, ", pages of a request] with contiguous rows, got ", table.sizes());
+}
+
+// read_pages(key_pages, value_pages, block_table, starts, num_tokens, key_scales, value_scales, dtype or None, bshd) -> key, value
+PyObject* read_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 9, "read_pages takes 9 arguments");
+  check_unwatched();
+  const at::Tensor kp = cuda_tensor(a[0], "key_pages"), vp = cuda_tensor(a[1], "value_pages"), table = cuda_tensor(a[2], "block_table"), starts = cuda_tensor(a[3], "starts");
+  const Scales scales(a[5], a[6]);
+  const bool bshd = truth(a[8]);
+  fa_read_params p;
+  memset(&p, 0, sizeof p);
+  p.num_tokens = integer(a[4]);
+  TORCH_CHECK_VALUE(p.num_tokens >= 0 && p.num_tokens <= INT32_MAX - 256, "num_tokens must be from 0 to 2^31 - 257, got ", p.num_tokens);
+  TORCH_CHECK_VALUE(kp.dim() == 4 && vp.dim() == 4, "key_pages and value_pages must be [pages, kv heads, page_size, embedding dimension]");
+  at::ScalarType out = kp.scalar_type();
+  if (a[7] != Py_None) {
+    TORCH_CHECK_TYPE(THPDtype_Check(a[7]), "dtype: a torch.dtype is expected, got ", Py_TYPE(a[7])->tp_name);
+    out = ((THPDtype*)a[7])->scalar_type;
+  }
+  TORCH_CHECK_VALUE(!scales.given || a[7] != Py_None, "pages in 8 bits need the dtype to read them as");
+  TORCH_CHECK_VALUE(scales.given || out == kp.scalar_type(), "pages without scales are read as they are, in ", kp.scalar_type(), ", not as ", out);
+  TORCH_CHECK_VALUE(out == at::kHalf || out == at::kBFloat16 || out == at::kFloat, "unsupported dtype ", out, "; use float16, bfloat16 or float32");
+  p.dtype = out == at::kHalf ? FA_F16 : out == at::kBFloat16 ? FA_BF16 : FA_F32;
+  p.Hkv = (int)kp.size(1);
+  p.D = (int)kp.size(3);
+  p.Dv = (int)vp.size(3);
+  pages_of(kp, vp, kp, p.Hkv, p.D, p.k_pages, p.v_pages, p.num_pages, p.page_size, scales.given);
+  scales.fill(kp, vp, p.k_scales, p.v_scales);
+  int_kind(starts, at::kInt, kp.device(), "starts");
+  TORCH_CHECK_VALUE(starts.dim() == 1 && starts.size(0) >= 1 && starts.size(0) <= INT32_MAX && starts.is_contiguous(), "starts must be a contiguous [requests + 1] tensor, got ", starts.sizes());
+  p.B = (int)(starts.size(0) - 1);
+  table_of(table, p.B, kp.device());
+  no_gradient(kp, "key_pages", "read_pages");
+  no_gradient(vp, "value_pages", "read_pages");
+  if (scales.given) {
+    no_gradient(scales.k, "key_scales", "read_pages");
+    no_gradient(scales.v, "value_scales", "read_pages");
+  }
+  p.block_table = (const int32_t*)table.const_data_ptr();
+  p.block_table_stride = table.stride(0);
+  p.table_width = (int)table.size(1);
+  p.starts = (const int32_t*)starts.const_data_ptr();
+  p.status = (int32_t*)g_status;
+  check_status();
+  at::Tensor k, v;
+  {
+    pybind11::gil_scoped_release no_gil;
+    c10::cuda::OptionalCUDAGuard guard(kp.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto rows = [&](int64_t D) {
+      return bshd ? empty({1, p.num_tokens, p.Hkv, D}, out, kp.device()) : empty({1, p.Hkv, p.num_tokens, D}, out, kp.device());
+    };
+    k = rows(p.D);
+    v = rows(p.Dv);
+    p.k = by_strides(k, bshd);
+    p.v = by_strides(v, bshd);
+    if (k.numel() > 0 || v.numel() > 0) {
+      const int rc = fa_read_pages(&p, (void*)c10::cuda::getCurrentCUDAStream(kp.device().index()).stream());
+      if (rc != FA_OK) raise(rc);
+    }
+  }
+  Ref x(THPVariable_Wrap(k)), y(THPVariable_Wrap(v));
+  if (x.p == nullptr || y.p == nullptr) return nullptr;
+  return PyTuple_Pack(2, x.p, y.p);
+  END_HANDLE_TH_ERRORS
+}
+
 // paged_attention(q, key_pages, value_pages, block_table, lengths, score_mod, mask_mod, window or None, scale or None, bshd, return_lse, b_offset,
-//                 h_offset, general, module: None or (handle, buffers)) -> out or (out, lse); None: the mods are not known here
+//                 h_offset, general, key_scales, value_scales, module: None or (handle, buffers)) -> out or (out, lse); None: the mods are not known here
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK(n == 15, "paged_attention takes 15 arguments");
+  TORCH_CHECK(n == 17, "paged_attention takes 17 arguments");
   check_unwatched();
   const at::Tensor q = cuda_tensor(a[0], "query"), kp = cuda_tensor(a[1], "key_pages"), vp = cuda_tensor(a[2], "value_pages"),
                    table = cuda_tensor(a[3], "block_table"), lengths = cuda_tensor(a[4], "lengths");
@@ -1089,17 +1212,22 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_VALUE(kp.dim() == 4 && vp.dim() == 4, "key_pages and value_pages must be [pages, kv heads, page_size, embedding dimension]");
   p.Hkv = (int)kp.size(1);
   p.Dv = (int)vp.size(3);
-  read_pages(kp, vp, q, p.Hkv, p.D, p.k_pages, p.v_pages, p.num_pages, p.page_size);
+  const Scales scales(a[14], a[15]);
+  TORCH_CHECK_NOT_IMPLEMENTED(!scales.given || p.dtype != FA_F32, "pages in 8 bits take float16 and bfloat16 queries");
+  pages_of(kp, vp, q, p.Hkv, p.D, p.k_pages, p.v_pages, p.num_pages, p.page_size, scales.given);
+  scales.fill(kp, vp, p.k_scales, p.v_scales);
   TORCH_CHECK_VALUE(p.Hkv > 0 ? p.Hq % p.Hkv == 0 : p.Hq == 0, "Expect number of query heads to be a multiple of kv heads, but got Hq=", p.Hq, " and Hkv=", p.Hkv, ".");
   TORCH_CHECK_VALUE(p.Dv <= p.D, "value embedding dimension must not exceed that of query and key, got Ev=", p.Dv, " and E=", p.D);
-  int_kind(table, at::kInt, q.device(), "block_table");
+  table_of(table, p.B, q.device());
   int_kind(lengths, at::kInt, q.device(), "lengths");
-  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) == p.B && (table.size(1) <= 1 || table.stride(1) == 1) && table.size(1) <= INT32_MAX,
-                    "block_table must be [", p.B, ", pages of a request] with contiguous rows, got ", table.sizes());
   TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.size(0) == p.B && lengths.is_contiguous(), "lengths must be a contiguous [", p.B, "] tensor, got ", lengths.sizes());
   no_gradient(q, "query", "paged_attention");
   no_gradient(kp, "key_pages", "paged_attention");
   no_gradient(vp, "value_pages", "paged_attention");
+  if (scales.given) {
+    no_gradient(scales.k, "key_scales", "paged_attention");
+    no_gradient(scales.v, "value_scales", "paged_attention");
+  }
   p.block_table = (const int32_t*)table.const_data_ptr();
   p.block_table_stride = table.stride(0);
   p.table_width = (int)table.size(1);
@@ -1120,11 +1248,11 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   ModsPtr hold;
   std::vector<at::Tensor> given;
   const std::vector<at::Tensor>* buffers = &given;
-  if (a[14] != Py_None) {
-    TORCH_CHECK(PyTuple_Check(a[14]) && PyTuple_GET_SIZE(a[14]) == 2, "module: a handle and a tuple of buffers");
-    module = (fa_module*)PyLong_AsVoidPtr(PyTuple_GET_ITEM(a[14], 0));
+  if (a[16] != Py_None) {
+    TORCH_CHECK(PyTuple_Check(a[16]) && PyTuple_GET_SIZE(a[16]) == 2, "module: a handle and a tuple of buffers");
+    module = (fa_module*)PyLong_AsVoidPtr(PyTuple_GET_ITEM(a[16], 0));
     if (PyErr_Occurred()) return nullptr;
-    given = tensors(PyTuple_GET_ITEM(a[14], 1));
+    given = tensors(PyTuple_GET_ITEM(a[16], 1));
   } else {
     const auto hit = g_mods->find({a[5] == Py_None || a[5] == g_identity ? nullptr : a[5], a[6] == Py_None || a[6] == g_noop ? nullptr : a[6]});
     if (hit == g_mods->end()) Py_RETURN_NONE;
@@ -1212,6 +1340,7 @@ PyMethodDef kMethods[] = {
     {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, nullptr},
     {"rotary_append", (PyCFunction)(void*)rotary_append, METH_FASTCALL, nullptr},
     {"page_step", (PyCFunction)(void*)page_step, METH_FASTCALL, nullptr},
+    {"read_pages", (PyCFunction)(void*)read_pages, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void*)paged_attention, METH_FASTCALL, nullptr},
     {"register", (PyCFunction)(void*)register_mods, METH_FASTCALL, nullptr},
     {"forget", (PyCFunction)(void*)forget, METH_FASTCALL, nullptr},

@@ -35,15 +35,20 @@
 //   * fp32: on the FMA pipes, in fp32 throughout; a lane has a key, or from 8 rows on four keys of eight rows, and a part of the head dim for the
 //     scores, columns for the values.
 //
+// Pages in 8 bits (FA_KV8): whole numbers w and a scale per key and kv head, k = ks w, v = vs w'.  The scales go where they cost least, on the scores
+// and on the probabilities,  s_ij = scale ks_j (q_i . w_j),  o_i = sum_j (p_ij vs_j) w'_j / sum_j p_ij,  and the whole numbers become 16-bit values, exactly,
+// in the registers that the products take them from: the way for few rows, in which a thread reads 16 bytes of a key, or its columns of
+// four keys, and has the operands of four products.
+//
 // Compile-time parameters (macros): FA_DTYPE, FA_D, FA_DV, FA_RG (1, 2, 4), FA_WN (keys of a tile: 32 or 16; fp32: 32, 16, 8), FA_SLOTS, FA_TMA,
-// FA_FEW (0: the other way), FA_FR (fp32: rows of a warp), FA_CG, FA_SHORT.
+// FA_FEW (0: the other way), FA_FR (fp32: rows of a warp), FA_CG, FA_SHORT, FA_KV8.
 #pragma once
 #include "fa_sm100.cuh"
 
 struct FaPagedLaunch {
   FaPagedParams p;
 #if FA_TMA
-  FaTensorMap tk, tv;  // 4-d maps (D, token in page, head, page), box 128 bytes x p.box x 1 x 1, 128-byte swizzle
+  FaTensorMap tk, tv;  // 4-d maps (D, token in page, head, page), box 128 bytes x p.box x 1 x 1, 128-byte swizzle (FA_KV8 and D <= 64: of 64 bytes)
 #endif
 };
 
@@ -65,9 +70,14 @@ constexpr int BM = FEW ? NQ * 8 : RG * 16;  // rows of a row tile
 constexpr int WN = FA_WN;
 constexpr int SLOTS = FA_SLOTS;
 constexpr int ES = F32 ? 4 : 2;
-constexpr int PK = TMA ? D * ES : FaTile<D, ES>::PITCH;
-constexpr int PV = TMA ? DV * ES : FaTile<DV, ES>::PITCH;
-constexpr int ATOMS_K = D * ES / 128, ATOMS_V = DV * ES / 128;  // 128-byte column groups of a row (TMA)
+constexpr bool KV8 = FA_KV8 != 0;
+constexpr int EK = KV8 ? 1 : ES;  // bytes of a cached value
+// Rows in 8 bits are column groups of 128 bytes, or one of 64, whole ones also where the head dim is not: what lies behind it is some whole number or
+// other and is multiplied with zeros, or in columns that nobody writes out.  Tiles lie as TMA leaves them however they come.
+constexpr int GROUP = KV8 && D <= 64 ? 64 : 128;
+constexpr int PK = KV8 ? (D + GROUP - 1) / GROUP * GROUP : TMA ? D * ES : FaTile<D, ES>::PITCH;
+constexpr int PV = KV8 ? (DV + GROUP - 1) / GROUP * GROUP : TMA ? DV * ES : FaTile<DV, ES>::PITCH;
+constexpr int ATOMS_K = (KV8 ? PK : D * ES) / GROUP, ATOMS_V = (KV8 ? PV : DV * ES) / GROUP;  // column groups of a row (TMA)
 // A key group's buffers are a ring of slots that take a tile of K or of V: K, V, K of the next, ..; what was in a slot has been used up, and the
 // tile half a ring ahead is asked for.  Two slots and as many warps per SM as fit, so that one's products run under the
 // others' softmax: a warp alone takes 1.5 us per tile (D 128, up to 8 rows), and fewer warps with more slots are slower (the host's rule).
@@ -86,9 +96,10 @@ constexpr int BAR_BYTES = TMA ? CG * SLOTS * 8 + 16 : 0;
 constexpr int SMEM_BYTES = CG * PIPE_BYTES + Q_BYTES + MERGE_BYTES + BAR_BYTES + (TMA ? 1024 : 0);
 constexpr float RISE = 8.f;  // (log2 units) what scores may rise before a row's maximum is looked for again
 constexpr fa_u32 ALL = WN == 32 ? 0xffffffffu : (1u << (WN & 31)) - 1u;  // every key of a tile
-static_assert(!TMA || (D * ES % 128 == 0 && DV * ES % 128 == 0), "TMA: whole column groups");
+static_assert(!TMA || KV8 || (D * ES % 128 == 0 && DV * ES % 128 == 0), "TMA: whole column groups");
 static_assert(F32 || WN == 32 || WN == 16, "tiles of 16 or 32 keys");
 static_assert(!FEW || (RG == 1 && !F32), "few rows: one warp, 16-bit types");
+static_assert(!KV8 || (FEW && WN == 32), "8 bits: few rows, a key per lane");
 
 __device__ __forceinline__ int divided(int n, const FaDiv& d) { return d.shift < 0 ? n : (int)(__umulhi((fa_u32)n, d.mul) >> d.shift); }
 
@@ -147,27 +158,32 @@ struct Load {
   int row;      // token in it
   fa_u32 keep;  // keys of the tile that are there, bit by bit
   fa_u32 boxes; // lanes with a page
+#if FA_KV8
+  float ks, vs; // scales of this lane's key; 0: it is not there
+#endif
 };
+
+// The address of 16-byte chunk c of row r in a tile: rows with a pad behind, or as TMA leaves them, 64 columns of all rows one behind
+// the other, chunk c of 8 at c ^ (r & 7).  (Of 64-byte rows chunk c of 4 at c ^ (r / 2 & 3).)
+template <int PITCH>
+__device__ __forceinline__ fa_u32 chunk_at(fa_u32 tile, int r, int c) {
+  if (KV8 && GROUP == 64) return tile + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+  return TMA || KV8 ? tile + (c >> 3) * (WN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) : tile + r * PITCH + c * 16;
+}
 
 // The rows of a tile in 16-byte pieces, those that are not there as zeros
 template <int COLS, int PITCH>
 __device__ __forceinline__ void load_pieces(const FaTensor& t, fa_u32 dst, const Load& n, int tid) {
-  constexpr int CPR = COLS * ES / 16, NL = RG * 32;  // (the threads of a key group)
-  const long long at = n.page >= 0 ? (n.page * t.sb + n.hk * t.sh + n.row * t.ss) * ES : -1;
+  constexpr int CPR = COLS * EK / 16, NL = RG * 32;  // (the threads of a key group)
+  const long long at = n.page >= 0 ? (n.page * t.sb + n.hk * t.sh + n.row * t.ss) * EK : -1;
 #pragma unroll 4
   for (int i = tid; i < (WN * CPR + 31) / 32 * 32; i += NL) {  // (whole warps: the shuffle)
     const int r = i / CPR, c = i - r * CPR;
     const long long row = __shfl_sync(0xffffffffu, at, r & 31);
-    if (i < WN * CPR) fa_cp_async16(dst + r * PITCH + c * 16, (const char*)t.ptr + (row >= 0 ? row + c * 16 : 0), row >= 0 ? 16 : 0);
+    if (i < WN * CPR) fa_cp_async16(KV8 ? chunk_at<PITCH>(dst, r, c) : dst + r * PITCH + c * 16, (const char*)t.ptr + (row >= 0 ? row + c * 16 : 0), row >= 0 ? 16 : 0);
   }
 }
 
-// The address of 16-byte chunk c of row r in a tile: rows with a pad behind, or as TMA leaves them, 64 columns of all rows one behind
-// the other, chunk c of 8 at c ^ (r & 7).
-template <int PITCH>
-__device__ __forceinline__ fa_u32 chunk_at(fa_u32 tile, int r, int c) {
-  return TMA ? tile + (c >> 3) * (WN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) : tile + r * PITCH + c * 16;
-}
 __device__ __forceinline__ fa_u32 transposed(fa_u32 x) {  // an 8 x 8 matrix of 16-bit values, a row over four lanes
   fa_u32 r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -345,6 +361,168 @@ struct Rows {
       if (lane + 32 * i < DV) f(h, lane + 32 * i, o[h][i]);
   }
   __device__ __forceinline__ bool speaks() const { return lane == 0; }  // writes a row's max and sum
+};
+#elif FA_KV8
+constexpr int HR = 2 * NQ, NS = WN / 8;
+constexpr int BLOCKS = (D + 63) / 64;  // of 64 columns of K, four products each
+constexpr int VB = PV / 8;             // columns of V of a thread, beside each other
+// Which of eight keys is row g of a product.  Lanes that are served together then read different banks: 16 bytes of the keys of two rows g beside each other
+// (K), and two threads' columns of the keys of every other row (V).
+__device__ __forceinline__ int key_of(int g) { return GROUP == 128 ? (g & 1 ? (g - 1) ^ 5 : g) : g ^ ((g >> 1) & 1); }
+// Four whole numbers as 16-bit values, two to a register.  fp16: in the low byte of 1024, made positive by 128.  bf16 has 8 bits: 128 plus the low seven of
+// the number, minus 128, or 256 of a negative one, whose sign is the bit that tells the two apart.
+template <int TO>
+__device__ __forceinline__ fa_u32 whole2(fa_u32 w, fa_u32 which) {  // which: 0x4140, bytes 0 and 1; 0x4342, 2 and 3 (fp16: of w ^ 0x80808080)
+  fa_u32 r;
+  if (TO == FA_DT_F16) {
+    asm("{\n\t.reg .b32 x;\n\tprmt.b32 x, %1, 0x64646464, %2;\n\tsub.rn.f16x2 %0, x, %3;\n\t}" : "=r"(r) : "r"(w), "r"(which), "r"(0x64806480u));
+  } else {
+    asm("{\n\t.reg .b32 x, y;\n\tprmt.b32 x, %1, 0x43434343, %2;\n\tand.b32 y, x, 0xff80ff80;\n\tand.b32 x, x, 0xff7fff7f;\n\tsub.rn.bf16x2 %0, x, y;\n\t}"
+        : "=r"(r) : "r"(w), "r"(which));
+  }
+  return r;
+}
+template <int TO>
+__device__ __forceinline__ fa_u32 biased(fa_u32 w) { return TO == FA_DT_F16 ? w ^ 0x80808080u : w; }
+__device__ __forceinline__ fa_u32 bytes_of(fa_u32 a, fa_u32 b, fa_u32 which) {
+  fa_u32 r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(which));
+  return r;
+}
+__device__ __forceinline__ uint4 lds16(fa_u32 at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(fa_u32 at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+struct Rows {
+  float s[WN / 16][NQ][4], o[VB / 2][NQ][4], m[HR], l[HR];
+  fa_u32 qf[BLOCKS * 4][NQ][2];
+  float ks, vs;  // scales of this lane's key of the tile
+  int lane;
+  __device__ __forceinline__ float& score(int h, int j) { return s[j >> 1][h >> 1][(j & 1) * 2 + (h & 1)]; }
+  __device__ __forceinline__ int key(int j) const { return key_of(lane >> 2) + j * 8; }
+  __device__ __forceinline__ int row(int h) const { return (h >> 1) * 8 + (lane & 3) * 2 + (h & 1); }
+  __device__ __forceinline__ bool idle(int h, int rows) const { return (h >> 1) * 8 + (h & 1) >= rows; }
+  template <class F>
+  static __device__ __forceinline__ void over_keys(float (&v)[HR], F f) {
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+      for (int h = 0; h < HR; ++h) v[h] = f(v[h], __shfl_xor_sync(0xffffffffu, v[h], off));
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < VB / 2; ++i)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o[i][q][0] = o[i][q][1] = o[i][q][2] = o[i][q][3] = 0.f;
+  }
+  __device__ __forceinline__ void rescale(int h, float c) {
+#pragma unroll
+    for (int i = 0; i < VB / 2; ++i) {
+      o[i][h >> 1][h & 1] *= c;
+      o[i][h >> 1][2 + (h & 1)] *= c;
+    }
+  }
+  // S' = K Q'.  A product's 16 columns are bytes 4 i .. 4 i + 3 of the 16 that each of four threads has of a key (of 64 columns in all); the queries lie
+  // in their registers in the same order.
+  __device__ __forceinline__ void scores(const unsigned char*, fa_u32 tile, int) {
+#pragma unroll
+    for (int i = 0; i < WN / 16; ++i) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) s[i][q][0] = s[i][q][1] = s[i][q][2] = s[i][q][3] = 0.f;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        const uint4 x = lds16(chunk_at<PK>(tile, i * 16 + key_of(lane >> 2), b * 4 + (lane & 3)));
+        const uint4 y = lds16(chunk_at<PK>(tile, i * 16 + 8 + key_of(lane >> 2), b * 4 + (lane & 3)));
+        const fa_u32 xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const fa_u32 u = biased<DT>(xs[k]), v = biased<DT>(ys[k]);
+          const fa_u32 a[4] = {whole2<DT>(u, 0x4140u), whole2<DT>(v, 0x4140u), whole2<DT>(u, 0x4342u), whole2<DT>(v, 0x4342u)};
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) fa_mma16816<DT>(s[i][q], a, qf[b * 4 + k][q][0], qf[b * 4 + k][q][1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const float f = __shfl_sync(0xffffffffu, ks, key(j));
+#pragma unroll
+      for (int h = 0; h < HR; ++h) score(h, j) *= f;
+    }
+  }
+  // O' = V' P'.  Probabilities times scales may have any size, so they go in as bf16, in two parts, rounded and what the rounding left: 16 bits of them.
+  __device__ __forceinline__ void values(const unsigned char*, fa_u32 tile, int) {
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const float f = __shfl_sync(0xffffffffu, vs, key(j));
+#pragma unroll
+      for (int h = 0; h < HR; ++h) score(h, j) *= f;
+    }
+#pragma unroll
+    for (int kj = 0; kj < WN / 16; ++kj) {
+      fa_u32 b[NQ][2], rest[NQ][2];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p0 = s[kj][q][2 * e], p1 = s[kj][q][2 * e + 1];
+          float r0, r1;
+          b[q][e] = transposed(fa_pack2<FA_DT_BF16>(p0, p1));
+          fa_rest2<FA_DT_BF16>(p0, p1, r0, r1);
+          rest[q][e] = transposed(fa_pack2<FA_DT_BF16>(r0, r1));
+        }
+      // columns VB g .. VB g + VB - 1 of the keys of rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9 (g = lane / 4, t = lane % 4), eight at a time
+      const int g = lane >> 2, t = lane & 3, k0 = kj * 16 + key_of(2 * t), k1 = kj * 16 + key_of(2 * t + 1);
+#pragma unroll
+      for (int c = 0; c < VB; c += VB < 16 ? 8 : 16) {
+        fa_u32 w[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = (k & 1 ? k1 : k0) + (k >> 1) * 8;
+          if (VB < 16) {
+            const uint2 x = lds8(chunk_at<PV>(tile, r, g >> 1) + (g & 1) * 8);
+            w[k][0] = x.x; w[k][1] = x.y; w[k][2] = w[k][3] = 0u;
+          } else {
+            const uint4 x = lds16(chunk_at<PV>(tile, r, g * (VB / 16) + c / 16));
+            w[k][0] = x.x; w[k][1] = x.y; w[k][2] = x.z; w[k][3] = x.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < (VB < 16 ? 2 : 4); ++i) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {  // two columns at a time: rows g and g + 8 of a product
+            const fa_u32 x = bytes_of(w[0][i], w[1][i], hf ? 0x7362u : 0x5140u), y = bytes_of(w[2][i], w[3][i], hf ? 0x7362u : 0x5140u);
+            const fa_u32 a[4] = {whole2<FA_DT_BF16>(x, 0x4140u), whole2<FA_DT_BF16>(x, 0x4342u), whole2<FA_DT_BF16>(y, 0x4140u), whole2<FA_DT_BF16>(y, 0x4342u)};
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+              fa_mma16816<FA_DT_BF16>(o[c / 2 + i * 2 + hf][q], a, b[q][0], b[q][1]);
+              fa_mma16816<FA_DT_BF16>(o[c / 2 + i * 2 + hf][q], a, rest[q][0], rest[q][1]);
+            }
+          }
+        }
+      }
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(int b, F f) {
+    if ((lane >> 2) * VB / 32 != b) return;
+#pragma unroll
+    for (int i = 0; i < VB / 2; ++i)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = (lane >> 2) * VB + 2 * i + (e >> 1);
+          if (PV == DV || c < DV) f(2 * q + (e & 1), c, o[i][q][e]);
+        }
+  }
+  __device__ __forceinline__ bool speaks() const { return lane < 4; }
 };
 #elif FA_FEW
 constexpr int HR = 2 * NQ, NS = WN / 8;
@@ -685,15 +863,21 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
         n.keep &= ~((p.box >= 32 ? 0xffffffffu : (1u << p.box) - 1u) << first);
       }
     }
+#if FA_KV8
+    const int box = divided(lane, p.by_box), page = __shfl_sync(0xffffffffu, n.page, box), row = __shfl_sync(0xffffffffu, n.row, box) + lane - box * p.box;
+    const bool in = page >= 0 && ((n.keep >> lane) & 1u);
+    n.ks = in ? ((const float*)p.k_scales.ptr)[page * p.k_scales.sb + n.hk * p.k_scales.sh + row * p.k_scales.ss] : 0.f;
+    n.vs = in ? ((const float*)p.v_scales.ptr)[page * p.v_scales.sb + n.hk * p.v_scales.sh + row * p.v_scales.ss] : 0.f;
+#endif
   };
 #if FA_TMA
   auto load = [&](const FaTensorMap* map, fa_u32 dst, fa_u32 bar, int atoms, const Load& n) {
     if (rg != 0) return;
-    if (lane == 0) fa_mbar_expect_tx(bar, __popc(n.boxes) * p.box * 128 * atoms);
+    if (lane == 0) fa_mbar_expect_tx(bar, __popc(n.boxes) * p.box * GROUP * atoms);
     __syncwarp();
     if (n.page >= 0) {
       for (int a = 0; a < atoms; ++a)
-        fa_tma_load_4d(dst + a * (WN * 128) + lane * p.box * 128, map, bar, a * (128 / ES), n.row, n.hk, n.page);
+        fa_tma_load_4d(dst + a * (WN * GROUP) + lane * p.box * GROUP, map, bar, a * (GROUP / EK), n.row, n.hk, n.page);
     }
   };
   auto load_k = [&](int slot, const Load& n) { load(&L.tk, ring + slot * SLOT_BYTES, bars + slot * 8, ATOMS_K, n); };
@@ -705,6 +889,18 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #endif
 
   fa_u32 keep[AHEAD];
+#if FA_KV8
+  float scales_k[AHEAD], scales_v[AHEAD];
+  auto push_scales = [&](const Load& n) {
+#pragma unroll
+    for (int i = 0; i + 1 < AHEAD; ++i) {
+      scales_k[i] = scales_k[i + 1];
+      scales_v[i] = scales_v[i + 1];
+    }
+    scales_k[AHEAD - 1] = n.any ? n.ks : 0.f;
+    scales_v[AHEAD - 1] = n.any ? n.vs : 0.f;
+  };
+#endif
   Load pending, next, after;  // the tile whose V is asked for next, the one whose K is, and the one behind that
   pending.any = next.any = after.any = false;
   int asked = 0;  // slots asked for
@@ -720,6 +916,9 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
       keep[AHEAD - 1] = next.keep;
       load_k(2 * st, next);
     }
+#if FA_KV8
+    push_scales(next);
+#endif
     fa_cp_commit();
     if (2 * st + 1 < SLOTS) {
       if (next.any) load_v(2 * st + 1, next);
@@ -772,7 +971,24 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #pragma unroll
     for (int q = 0; q < (FEW ? NQ : 2); ++q) {
       const int row = rt * BM + row0 + q * 8 + (lane >> 2), i = divided(row, p.by_group);
-      const fa_u32* src = (const fa_u32*)(qb + (i * p.q.ss + (long long)(seg.hk * G + row - i * G) * p.q.sh) * ES) + (lane & 3);
+      const fa_u32* src = (const fa_u32*)(qb + (i * p.q.ss + (long long)(seg.hk * G + row - i * G) * p.q.sh) * ES) + (KV8 ? 0 : (lane & 3));
+#if FA_KV8
+      // (columns 16 t .. of each 64, t = lane % 4, as K's)
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        const int c = b * 64 + (lane & 3) * 16;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
+        if (i < p.Sq && (D % 64 == 0 || c < D)) {
+          x = *(const uint4*)(src + c / 2);
+          y = *(const uint4*)(src + c / 2 + 4);
+        }
+        R.qf[b * 4][q][0] = x.x; R.qf[b * 4][q][1] = x.y;
+        R.qf[b * 4 + 1][q][0] = x.z; R.qf[b * 4 + 1][q][1] = x.w;
+        R.qf[b * 4 + 2][q][0] = y.x; R.qf[b * 4 + 2][q][1] = y.y;
+        R.qf[b * 4 + 3][q][0] = y.z; R.qf[b * 4 + 3][q][1] = y.w;
+      }
+      continue;
+#endif
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const fa_u32 lo = i < p.Sq ? src[kk * 8] : 0u, hi = i < p.Sq ? src[kk * 8 + 4] : 0u;
@@ -821,6 +1037,10 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
       // (its pages were looked up a tile ago; here, so that nothing waits for them when a slot is free)
       if (next.any) settle(next);
       int at = arrived();
+#if FA_KV8
+      R.ks = scales_k[0];
+      R.vs = scales_v[0];
+#endif
       R.scores(bufs + at * SLOT_BYTES, ring + at * SLOT_BYTES, rows);
       used();
       if (failed) break;
@@ -911,7 +1131,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #if FA_TMA
       // Rows of keys that are not there hold whatever was in the page or the buffer, perhaps no number: 0, since a weight of 0
       // does not take that out of the product.  (Each warp for itself; all write the same.)
-      if (kept != ALL) {
+      if (!KV8 && kept != ALL) {  // (whole numbers are numbers, and their scale is 0)
         for (int i = lane; i < WN * ATOMS_V * 8; i += 32) {
           const int r = (i >> 3) % WN;
           if (!((kept >> r) & 1u)) *(uint4*)(bufs + at * SLOT_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
@@ -935,6 +1155,9 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #pragma unroll
       for (int i = 0; i + 1 < AHEAD; ++i) keep[i] = keep[i + 1];
       keep[AHEAD - 1] = next.any ? next.keep : 0u;
+#if FA_KV8
+      push_scales(next);
+#endif
       next = after;
     }
 

@@ -104,6 +104,8 @@ struct FaPagedParams {
   int box;                            // keys that one look-up in the table gives (1, or the rows of a TMA box)
   float scale;
   const void* mod_buf[FA_MAX_MOD_BUFS];
+  FaTensor k_scales, v_scales;        // pages in 8 bits: float32, strides of page, head and token in a page
+  FaDiv by_box;
 };
 
 // Status bits that kernels OR into a status word, beside those of the bounded waits (fa_sm100.cuh)

@@ -180,6 +180,121 @@ __global__ void __launch_bounds__(kStepThreads) fa_page_step_kernel(const __grid
   }
 }
 
+// ---- tokens out of their pages ---------------------------------------------------------------
+//   row t of key and value = token t - starts[b] of request b: w scale of pages in 8 bits, rounded once, or a copy.
+//
+// A block takes a run of tokens: it finds their requests and pages (the requests that end in front of the first are counted by all threads, the
+// others are walked through from there), then goes through their rows in pieces of eight values, four of a thread on their way at a time.
+constexpr int kReadThreads = 256, kReadTokens = 16, kReadEight = 3;  // (kReadEight: the type of pages in 8 bits, beside FA_F16, FA_BF16 and FA_F32)
+
+struct FaReadKernelParams {
+  FaRotTensor pages[2], out[2];  // byte strides
+  const float* scales[2];        // element strides of page, head and token in a page
+  long long scale_sp[2], scale_sh[2], scale_ss[2];
+  const int *table, *starts;
+  long long table_stride;
+  int B, Hkv, D[2], width, num_pages, page_size, tokens, per_block;
+  int* status;
+};
+
+// Four values of 8 bits: in the low byte of 2^23, which is subtracted with the 128 that makes them positive.
+__device__ __forceinline__ void read_four(unsigned w, float scale, float* f) {
+  w ^= 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | i)) - 8388736.f) * scale;
+}
+
+template <int IN, int OUT, bool PIECES>
+__global__ void __launch_bounds__(kReadThreads) fa_read_pages_kernel(const __grid_constant__ FaReadKernelParams P) {
+  grid_wait();
+  constexpr bool EIGHT = IN == kReadEight;
+  constexpr int V = PIECES ? 8 : 1, ES = OUT == FA_F32 ? 4 : 2, EI = EIGHT ? 1 : ES;
+  __shared__ long long page_of[kReadTokens];  // -1: the token has none
+  __shared__ int row_of[kReadTokens];
+  const int t0 = blockIdx.x * P.per_block, n = min(P.per_block, P.tokens - t0), tid = threadIdx.x;
+  int before = 0;
+  for (int b0 = 0; b0 < P.B; b0 += kReadThreads) before += __syncthreads_count(b0 + tid < P.B && P.starts[min(b0 + tid, P.B - 1) + 1] <= t0);
+  if (tid < n) {
+    const int t = t0 + tid;
+    int b = before;
+    while (b < P.B && P.starts[b + 1] <= t) ++b;
+    long long page = -1;
+    int row = 0;
+    if (b < P.B && P.starts[b] <= t) {
+      const int j = (int)min((long long)t - P.starts[b], (long long)INT_MAX), slot = j / P.page_size;
+      row = j - slot * P.page_size;
+      if (slot < P.width) page = P.table[b * P.table_stride + slot];
+      if (page < 0 || page >= P.num_pages) {
+        page = -1;
+        if (P.status != nullptr) atomicOr(P.status, FA_STATUS_BAD_PAGE);
+      }
+    }
+    page_of[tid] = page;
+    row_of[tid] = row;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int kind = 0; kind < 2; ++kind) {
+    const FaRotTensor& src = P.pages[kind];
+    const FaRotTensor& dst = P.out[kind];
+    const int C = P.D[kind] / V, all = P.Hkv * n * C;
+    constexpr int U = 4, WORDS = V * EI <= 4 ? 1 : V * EI / 4;
+#pragma unroll 1
+    for (int i0 = tid; i0 < all; i0 += U * kReadThreads) {
+      unsigned raw[U][WORDS];
+      float scale[U];
+      char* to[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // (all of them on their way at once)
+        const int i = i0 + u * kReadThreads, row = i / C, c = i - row * C, h = row / n, t = row - h * n;
+        to[u] = nullptr;
+        scale[u] = 0.f;
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) raw[u][w] = 0u;
+        if (i >= all) continue;
+        to[u] = dst.ptr + h * dst.sh + (t0 + t) * dst.ss + (long long)c * V * ES;
+        const long long page = page_of[t];
+        if (page < 0) continue;
+        const char* from = src.ptr + page * src.sb + h * src.sh + row_of[t] * src.ss + (long long)c * V * EI;
+        if (EIGHT) scale[u] = P.scales[kind][page * P.scale_sp[kind] + h * P.scale_sh[kind] + row_of[t] * P.scale_ss[kind]];
+        if (!PIECES) raw[u][0] = EI == 1 ? (unsigned)*(const unsigned char*)from : EI == 2 ? (unsigned)*(const unsigned short*)from : *(const unsigned*)from;
+        else if (EI == 1) *(uint2*)raw[u] = *(const uint2*)from;
+        else
+#pragma unroll
+          for (int w = 0; w < WORDS; w += 4) *(uint4*)&raw[u][w] = *(const uint4*)(from + w * 4);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (to[u] == nullptr) continue;
+        if constexpr (!EIGHT) {
+          if (!PIECES) {
+            if (ES == 2) *(unsigned short*)to[u] = (unsigned short)raw[u][0];
+            else *(unsigned*)to[u] = raw[u][0];
+          } else {
+#pragma unroll
+            for (int w = 0; w < WORDS; w += 4) *(uint4*)(to[u] + w * 4) = *(const uint4*)&raw[u][w];
+          }
+        } else {
+          float f[8];
+          read_four(raw[u][0], scale[u], f);
+          if (!PIECES) {
+            rot_put<OUT>(to[u], 0, f[0]);
+          } else {
+            read_four(raw[u][WORDS - 1], scale[u], f + 4);
+#pragma unroll
+            for (int w = 0; w < 8 * ES / 16; ++w) {
+              F2 g[kRotPairs<OUT>];
+#pragma unroll
+              for (int k = 0; k < kRotPairs<OUT>; ++k) g[k] = f2(f[w * kRotVec<OUT> + 2 * k], f[w * kRotVec<OUT> + 2 * k + 1]);
+              *(uint4*)(to[u] + w * 16) = rot_pack<OUT>(g);
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
 // ---- attention: the parts of segments that several workers share ---------------------------
 // WARPS warps per query row, which take the row's parts in turn: eight where a row may have many (one request of 131072 keys, 444 workers, 32 rows: 4.4 us,
 // a chain of plan, parts and sums), else one (3.4).
@@ -273,6 +388,7 @@ struct FaPagedLaunchHost {
 struct PagedCfg {
   int RG, CG, BM, WN, slots, smem, per_sm, box, few, fr;
   bool tma, one_each;  // one_each: a CTA per segment (FA_SHORT)
+  bool eight;          // pages in 8 bits (FA_KV8)
 };
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
 FaDiv divide_by(int d) {
@@ -303,17 +419,19 @@ void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   const long long rows = (long long)(p->Hq / p->Hkv) * p->Sq;
   const bool f32 = p->dtype == FA_F32;
   const int es = esize(p->dtype);
-  c.few = f32 ? 0 : rows <= 8 ? 1 : rows > 16 && rows <= 24 && p->D <= 128 ? 3 : 0;
+  c.eight = p->k_scales.ptr != nullptr;
+  c.few = c.eight ? (rows <= 8 || p->D > 128 ? 1 : rows <= 16 ? 2 : 3) : f32 ? 0 : rows <= 8 ? 1 : rows > 16 && rows <= 24 && p->D <= 128 ? 3 : 0;
   c.RG = rows <= 16 || c.few > 0 ? 1 : rows <= 32 ? 2 : 4;
   c.BM = c.few > 0 ? c.few * 8 : c.RG * 16;
-  c.WN = !f32 ? (p->D <= 128 ? 32 : 16) : p->D <= 64 ? 32 : p->D <= 128 ? 16 : 8;
+  c.WN = c.eight ? 32 : !f32 ? (p->D <= 128 ? 32 : 16) : p->D <= 64 ? 32 : p->D <= 128 ? 16 : 8;
   c.fr = 0;
   if (f32)
     for (c.fr = 1; c.fr < std::min<long long>(rows, 16);) c.fr *= 2;
   c.box = gcd(p->page_size, c.WN);
-  c.tma = p->D * es % 128 == 0 && p->Dv * es % 128 == 0 && c.box >= 8 && p->num_pages > 0 && !(p->flags & FA_FLAG_GENERAL_KERNELS);
+  c.tma = (c.eight || (p->D * es % 128 == 0 && p->Dv * es % 128 == 0)) && c.box >= 8 && p->num_pages > 0 && !(p->flags & FA_FLAG_GENERAL_KERNELS);
   if (!c.tma) c.box = 1;
-  const int slot = c.WN * (c.tma ? p->D * es : pitch(p->D, es));  // (K's: the value dim is no larger)
+  const int group = p->D <= 64 ? 64 : 128;  // (8 bits: whole column groups)
+  const int slot = c.WN * (c.eight ? (p->D + group - 1) / group * group : c.tma ? p->D * es : pitch(p->D, es));  // (K's: the value dim is no larger)
   const int mrows = f32 && c.RG == 1 ? c.fr : c.BM;
   const auto smem = [&](int slots) {
     const int q = f32 ? (c.RG == 1 ? c.fr : c.RG * 16) * p->D * 4 + c.CG * c.RG * c.fr * c.WN * 4 : 0;
@@ -353,10 +471,10 @@ int paged_workers(const PagedCfg& c) { return c.per_sm * device_sm_count(); }
 
 // (16-bit types: quotients and tanh of scores without branches, fa_score_math.cuh)
 int get_paged_kernel(fa_module* m, const fa_paged_params* p, const PagedCfg& c, Kernel** k) {
-  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.slots, 4}, {c.tma ? 1 : 0, 1}, {c.few, 2}, {c.fr, 5}, {c.CG, 4}, {c.one_each ? 1 : 0, 1}, {c.per_sm, 3}}), "fa_paged.cuh",
+  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.slots, 4}, {c.tma ? 1 : 0, 1}, {c.few, 2}, {c.fr, 5}, {c.CG, 4}, {c.one_each ? 1 : 0, 1}, {c.per_sm, 3}, {c.eight ? 1 : 0, 1}}), "fa_paged.cuh",
                     [&] { return std::string(p->dtype == FA_F32 ? "" : "#include \"fa_score_math.cuh\"\n") +
                                 defs({{"FA_DTYPE", p->dtype}, {"FA_D", p->D}, {"FA_DV", p->Dv}, {"FA_RG", c.RG}, {"FA_WN", c.WN},
-                                       {"FA_SLOTS", c.slots}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_CG", c.CG}, {"FA_SHORT", c.one_each ? 1 : 0}, {"FA_CTAS", c.per_sm}}); },
+                                       {"FA_SLOTS", c.slots}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_CG", c.CG}, {"FA_SHORT", c.one_each ? 1 : 0}, {"FA_CTAS", c.per_sm}, {"FA_KV8", c.eight ? 1 : 0}}); },
                     "fa_paged_kernel", c.smem, k);
 }
 
@@ -377,8 +495,11 @@ int paged_check(fa_module* m, const fa_paged_params* p, PagedCfg& c) {
   const int es = esize(p->dtype);
   if (int rc = check_tensor(p->q, "q", es)) return rc;
   if (int rc = check_tensor(p->o, "o", es)) return rc;
-  if (int rc = check_tensor(p->k_pages, "k_pages", es, p->num_pages > 0)) return rc;
-  if (int rc = check_tensor(p->v_pages, "v_pages", es, p->num_pages > 0)) return rc;
+  const bool eight = p->k_scales.ptr || p->v_scales.ptr;
+  if (eight && !(p->k_scales.ptr && p->v_scales.ptr)) return fail(FA_EINVAL, "scales of keys and of values, or none");
+  if (eight && p->dtype == FA_F32) return fail(FA_EUNSUPPORTED, "pages in 8 bits take queries of 16 bits");
+  if (int rc = check_tensor(p->k_pages, "k_pages", eight ? 1 : es, p->num_pages > 0)) return rc;
+  if (int rc = check_tensor(p->v_pages, "v_pages", eight ? 1 : es, p->num_pages > 0)) return rc;
   pick_paged(p, c);
   if ((long long)p->B * p->Hq * p->Sq > 0x7fffffffll - 1024) return fail(FA_EUNSUPPORTED, "B * Hq * Sq must stay below 2^31");
   const long long longest = std::min<long long>((long long)p->table_width * p->page_size, 0x7fffffffll);
@@ -420,6 +541,50 @@ int fa_page_step(const int32_t* lengths, const int32_t* new_tokens, int B, int32
   const unsigned blocks = (unsigned)std::max<long long>(1, (num_tokens + k.per_block - 1) / k.per_block);
   k.pages_per_block = (int)((num_tokens / page_size + B) / blocks + 1);  // (n tokens more take ceil(n / page_size) pages more at most)
   return launch_here("fa_page_step_kernel", fa_page_step_kernel, dim3(blocks), dim3(kStepThreads), stream, k);
+}
+
+int fa_read_pages(const fa_read_params* p, void* stream) {
+  if (!p) return fail(FA_EINVAL, "params is null");
+  if (p->dtype < FA_F16 || p->dtype > FA_F32) return fail(FA_EINVAL, "unknown dtype");
+  if (p->B < 0 || p->Hkv < 0 || p->D <= 0 || p->Dv <= 0 || p->num_tokens < 0) return fail(FA_EINVAL, "B, Hkv and num_tokens must not be negative, head dims must be positive");
+  if (p->D > 256 || p->Dv > 256) return fail(FA_EUNSUPPORTED, "head dims from 1 to 256");
+  if (p->Hkv > 65535) return fail(FA_EUNSUPPORTED, "Hkv must not exceed 65535");
+  if (p->num_tokens > 0x7fffffffll - 256 || p->num_pages > 0x7fffffffll) return fail(FA_EUNSUPPORTED, "num_tokens and num_pages must stay below 2^31");
+  if (p->page_size <= 0 || p->num_pages < 0 || p->table_width < 0) return fail(FA_EINVAL, "page_size must be positive, num_pages and table_width not negative");
+  const bool eight = p->k_scales.ptr || p->v_scales.ptr;
+  if (eight && !(p->k_scales.ptr && p->v_scales.ptr)) return fail(FA_EINVAL, "scales of keys and of values, or none");
+  prof_reset();
+  if (p->num_tokens == 0 || p->Hkv == 0) return FA_OK;
+  if (!p->k.ptr || !p->v.ptr || (p->num_pages > 0 && (!p->k_pages.ptr || !p->v_pages.ptr))) return fail(FA_EINVAL, "a tensor is null");
+  if (p->B > 0 && (!p->starts || (p->table_width > 0 && !p->block_table))) return fail(FA_EINVAL, "starts or block_table is null");
+  FaReadKernelParams k;
+  memset(&k, 0, sizeof k);
+  const int es = esize(p->dtype), ei = eight ? 1 : es;
+  const fa_tensor *from[2] = {&p->k_pages, &p->v_pages}, *to[2] = {&p->k, &p->v}, *scales[2] = {&p->k_scales, &p->v_scales};
+  bool pieces = p->D % 8 == 0 && p->Dv % 8 == 0;
+  for (int i = 0; i < 2; ++i) {
+    k.pages[i] = rot_tensor(*from[i], ei);
+    k.out[i] = rot_tensor(*to[i], es);
+    k.out[i].sb = 0;
+    k.scales[i] = (const float*)scales[i]->ptr;
+    k.scale_sp[i] = scales[i]->stride_b; k.scale_sh[i] = scales[i]->stride_h; k.scale_ss[i] = scales[i]->stride_s;
+    pieces = pieces && rot_aligned(k.pages[i], eight ? 8 : 16) && rot_aligned(k.out[i]);
+  }
+  k.D[0] = p->D; k.D[1] = p->Dv;
+  k.table = p->block_table; k.table_stride = p->block_table_stride; k.width = p->table_width;
+  k.starts = p->starts; k.B = p->B; k.Hkv = p->Hkv;
+  k.num_pages = (int)p->num_pages; k.page_size = p->page_size; k.tokens = (int)p->num_tokens;
+  k.status = p->status;
+  // As many tokens of a block as leave four blocks per SM: the search for the requests is paid once for them.
+  k.per_block = kReadTokens;
+  while (k.per_block > 1 && p->num_tokens / k.per_block < 4LL * device_sm_count()) k.per_block /= 2;
+  const dim3 grid((unsigned)((p->num_tokens + k.per_block - 1) / k.per_block));
+  return rot_dispatch(p->dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    void (*const fns[2][2])(FaReadKernelParams) = {{fa_read_pages_kernel<DT, DT, false>, fa_read_pages_kernel<DT, DT, true>},
+                                                   {fa_read_pages_kernel<kReadEight, DT, false>, fa_read_pages_kernel<kReadEight, DT, true>}};
+    return launch_here("fa_read_pages_kernel", fns[eight][pieces], grid, dim3(kReadThreads), stream, k);
+  });
 }
 
 size_t fa_paged_workspace_bytes(const fa_paged_params* p) {
@@ -465,10 +630,12 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
   k.max_len = (int)std::min<long long>((long long)p->table_width * p->page_size, 0x7fffffffll - 64);
   k.window = p->window < 0 ? -1 : std::min(p->window, 1 << 30);
   k.b_off = p->b_offset; k.h_off = p->h_offset; k.scale = p->scale;
+  k.k_scales = cvt(p->k_scales); k.v_scales = cvt(p->v_scales);
   if (c.tma) {
     // (strides that no tensor map takes: 16-byte pieces)
-    if (make_map(&L.tk, p->dtype, p->k_pages, p->D, p->page_size, p->Hkv, (int)p->num_pages, c.box) != FA_OK ||
-        make_map(&L.tv, p->dtype, p->v_pages, p->Dv, p->page_size, p->Hkv, (int)p->num_pages, c.box) != FA_OK) {
+    const int type = c.eight ? kMapInt8 : p->dtype, group = c.eight && p->D <= 64 ? 64 : 128;
+    if (make_map(&L.tk, type, p->k_pages, p->D, p->page_size, p->Hkv, (int)p->num_pages, c.box, group) != FA_OK ||
+        make_map(&L.tv, type, p->v_pages, p->Dv, p->page_size, p->Hkv, (int)p->num_pages, c.box, group) != FA_OK) {
       fa_paged_params q = *p;
       q.flags |= FA_FLAG_GENERAL_KERNELS;
       pick_paged(&q, c);
@@ -484,6 +651,7 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
   k.part_ml = (float*)((char*)workspace + paged_up(rows * p->Dv * 4));
   k.plan = (int*)((char*)k.part_ml + paged_up(rows * 8));
   k.box = c.box;
+  k.by_box = divide_by(c.box);
   Kernel* kernel = nullptr;
   if (int rc = get_paged_kernel(m, p, c, &kernel)) return rc;
   const dim3 block((unsigned)(c.CG * c.RG * 32));

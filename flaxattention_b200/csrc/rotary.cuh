@@ -38,6 +38,8 @@ struct FaRotParams {
   int lane_shift;            // log2 of the lanes that share a row
   float eps, sign;           // sign of sin: -1 turns back
   int* status;
+  float* scales[2];          // of keys and values in 8 bits, element strides of page, head and token in a page
+  long long scale_sp[2], scale_sh[2], scale_ss[2];
 };
 
 template <int DT>
@@ -142,8 +144,8 @@ __device__ __forceinline__ long long rot_position(const FaRotParams& P, int b, i
   return -1;
 }
 // byte offset of token (b, s) in the destination; -1: it has none (keys and values of a slot below 0 or, with the
-// status bit, beyond the pages)
-__device__ __forceinline__ long long rot_destination(const FaRotParams& P, int kind, int b, int s) {
+// status bit, beyond the pages); scale_at: where its scale is
+__device__ __forceinline__ long long rot_destination(const FaRotParams& P, int kind, int b, int s, long long* scale_at = nullptr) {
   const FaRotTensor& y = P.y[kind];
   if (P.slots == nullptr || kind == 0) return b * y.sb + s * y.ss;
   const long long slot = P.slots[b * P.slot_sb + s * P.slot_ss];
@@ -160,6 +162,7 @@ __device__ __forceinline__ long long rot_destination(const FaRotParams& P, int k
     page = slot / P.page_size;
     at = slot % P.page_size;
   }
+  if (scale_at != nullptr) *scale_at = page * P.scale_sp[kind - 1] + at * P.scale_ss[kind - 1];
   return page * y.sb + at * y.ss;
 }
 
@@ -346,6 +349,39 @@ __device__ __forceinline__ void rot_sums(float (&v)[N], int lane_shift) {
   }
 }
 
+// ---- rows in 8 bits ------------------------------------------------------------------------
+//   scale = max|y| / 127,  w = y / scale rounded to the nearest whole number, ties to the even one,
+// both as fp32 divides, so that w is what the two formulas say to the last bit of y.  A row of zeros has the scale 0; of a row with an infinity or
+// no number in it the scale is no number, which its values then are too when they are read.
+__device__ __forceinline__ unsigned rot_size(unsigned most, F2 v) {  // (as bits: no number is the largest)
+  float x, y;
+  f2_get(v, x, y);
+  return max(most, max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu));
+}
+__device__ __forceinline__ float rot_scale(unsigned most) { return most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(most) / 127.f; }
+__device__ __forceinline__ int rot_whole(float y, float scale) { return scale > 0.f ? (int)fminf(fmaxf(rintf(y / scale), -127.f), 127.f) : 0; }
+// Four values.  y times 1 / scale, added to 1.5 * 2^23, has the whole number in its low byte.  It is off by less than 5e-5 (127 times the errors of
+// the reciprocal and of the product, 2^-23 at most each), so only what that brings near a tie is divided; and all where the reciprocal may overflow.
+__device__ __forceinline__ unsigned rot_eight(F2 a, F2 b, float scale, float inverse) {
+  constexpr float kMagic = 12582912.f;
+  const F2 m = f2(kMagic, kMagic), r = f2(inverse, inverse), minus = f2(-1.f, -1.f);
+  const F2 na = fma(a, r, m), nb = fma(b, r, m);
+  const F2 da = fma(a, r, fma(na, minus, m)), db = fma(b, r, fma(nb, minus, m));
+  float v[4], d[4];
+  f2_get(na, v[0], v[1]);
+  f2_get(nb, v[2], v[3]);
+  f2_get(da, d[0], d[1]);
+  f2_get(db, d[2], d[3]);
+  if (scale >= 1e-30f && fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3]))) < 0.4999f)
+    return __byte_perm(__byte_perm(__float_as_uint(v[0]), __float_as_uint(v[1]), 0x0040), __byte_perm(__float_as_uint(v[2]), __float_as_uint(v[3]), 0x0040), 0x5410);
+  f2_get(a, v[0], v[1]);
+  f2_get(b, v[2], v[3]);
+  unsigned w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w |= (unsigned)(rot_whole(v[i], scale) & 0xff) << (8 * i);
+  return w;
+}
+
 // Two 16-byte pieces of a row per lane: the two that hold its pairs.  A thread keeps the angles of its token, times the weights, in
 // registers for all heads of its group, and the lanes of a warp beside each other are tokens beside each other.  Four rows are computed
 // while the next four are on their way.
@@ -355,7 +391,8 @@ __device__ __forceinline__ void rot_sums(float (&v)[N], int lane_shift) {
 // and the weights in the angles.  Two rows at a time 61, more blocks per SM (fewer registers) 85 and more.
 // 16384 tokens appended to pages (H32/8 D128 bf16): 70 us for 411 MB, 5.8 TB/s: the values only change place, and keys and values are written
 // in runs of a row (256 bytes).  One token of 32 requests: 3.9 us, the launch, the slot and the row one behind the other.
-template <int DT, RotMode MODE>
+// Q8: keys and values are written in 8 bits, and their scales.
+template <int DT, RotMode MODE, bool Q8 = false>
 __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_constant__ FaRotParams P) {
   grid_wait();
   constexpr int V = kRotVec<DT>, N = V / 2, U = 4;
@@ -367,7 +404,9 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
   const bool turns = MODE >= kNeighboursAny ? kind < 2 && 2 * at.lane * V < P.R : at.lane < pairs;
   const int ca = MODE == kHalves ? (turns ? at.lane : 2 * pairs + 2 * (at.lane - pairs)) : 2 * at.lane;
   const int cb = MODE == kHalves && turns ? at.lane + pairs : ca + 1;
-  const long long to = live ? rot_destination(P, kind, b, s) : -1;
+  const bool eight = Q8 && kind > 0;
+  [[maybe_unused]] long long scale_at = 0;
+  const long long to = live ? rot_destination(P, kind, b, s, eight ? &scale_at : nullptr) : -1;
   const bool have_a = live && to >= 0 && ca < chunks, have_b = live && to >= 0 && cb < chunks;
   const bool norm = kind < 2 && P.w[kind < 2 ? kind : 0] != nullptr;
   // (the first rows are asked for before the angles, which come over the positions)
@@ -442,7 +481,7 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
           rot_others<DT>(P, mine, 32, lane0, cb, oy);
         }
       }
-      if (norm || turns) {
+      if (norm || turns || eight) {
         F2 x[N], y[N];
         rot_unpack<DT>(ra[u], x);
         rot_unpack<DT>(rb[u], y);
@@ -455,7 +494,8 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
             y[i] = y[i] * rr;
           }
         }
-        if constexpr (MODE == kAny) {
+        if (Q8 && kind == 2) {  // (as they are)
+        } else if constexpr (MODE == kAny) {
           const F2 rr = f2(r, r);
 #pragma unroll
           for (int i = 0; i < N; ++i) {
@@ -470,6 +510,20 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
           rot_turn_any<V>(P, cb, y, f.pb, f.qb);
         } else {
           rot_turn<V, MODE>(x, y, f);
+        }
+        if constexpr (Q8) {
+          if (eight) {
+            unsigned most = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) most = rot_size(rot_size(most, x[i]), y[i]);
+            for (int off = 1 << P.lane_shift >> 1; off > 0; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
+            const float scale = rot_scale(most), inverse = 1.f / scale;
+            char* row = dst + (h + u) * P.y[kind].sh;
+            if (have_a) *(uint2*)(row + ca * 8) = make_uint2(rot_eight(x[0], x[1], scale, inverse), rot_eight(x[N - 2], x[N - 1], scale, inverse));
+            if (have_b) *(uint2*)(row + cb * 8) = make_uint2(rot_eight(y[0], y[1], scale, inverse), rot_eight(y[N - 2], y[N - 1], scale, inverse));
+            if (to >= 0 && at.lane == 0) P.scales[kind - 1][scale_at + (h + u) * P.scale_sh[kind - 1]] = scale;
+            continue;
+          }
         }
         const uint4 pa = rot_pack<DT>(x), pb = rot_pack<DT>(y);
         ra[u] = MODE >= kNeighboursAny && !norm ? rot_keep<DT>(P, ca, pa, ra[u]) : pa;
@@ -661,7 +715,7 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_bwd_kernel(const __g
 }
 
 // What no 16-byte pieces fit (head dims, strides, addresses): a warp per row, value by value.  Backward (BACK): the same with dy, as above.
-template <int DT, bool BACK>
+template <int DT, bool BACK, bool Q8 = false>
 __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid_constant__ FaRotParams P) {
   grid_wait();
   __shared__ float sums[BACK ? kRotThreads / 32 : 1][256];
@@ -676,7 +730,8 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid
   const long long rows = (long long)P.tokens * H;
   for (long long row = (long long)blockIdx.x * (kRotThreads / 32) + warp; row < rows; row += (long long)gridDim.x * (kRotThreads / 32)) {
     const int t = (int)(row / H), h = (int)(row - (long long)t * H), b = t / P.S, s = t - b * P.S;
-    const long long to = rot_destination(P, kind, b, s);
+    [[maybe_unused]] long long scale_at = 0;
+    const long long to = rot_destination(P, kind, b, s, Q8 && kind > 0 ? &scale_at : nullptr);
     if (to < 0) continue;
     const char* x = P.x[kind].ptr + b * P.x[kind].sb + s * P.x[kind].ss + h * P.x[kind].sh;
     char* y = P.y[kind].ptr + to + h * P.y[kind].sh;
@@ -715,6 +770,43 @@ __global__ void __launch_bounds__(kRotThreads) fa_rotary_any_kernel(const __grid
         if (j >= 0) m += ((Real)d * c + (Real)a * sn) * weight(j) * rot_get<DT>(in, j);
       }
       m = rot_sum(m) * r / D;
+    }
+    if constexpr (Q8) {
+      if (kind > 0) {
+        float v[8][2];
+        unsigned most = 0;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const int k = lane + 32 * n;
+          v[n][0] = v[n][1] = 0.f;
+          if (k >= units) continue;
+          int i, j;
+          float c, sn;
+          unit(k, i, j, c, sn);
+          float a = rot_get<DT>(x, i), d = j >= 0 ? rot_get<DT>(x, j) : 0.f;
+          if (norm) {
+            a *= r * weight(i);
+            if (j >= 0) d *= r * weight(j);
+          }
+          v[n][0] = j >= 0 ? a * c - d * sn : a;
+          v[n][1] = j >= 0 ? d * c + a * sn : 0.f;
+          most = rot_size(most, f2(v[n][0], v[n][1]));
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        const float scale = rot_scale(most);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const int k = lane + 32 * n;
+          if (k >= units) continue;
+          int i, j;
+          float c, sn;
+          unit(k, i, j, c, sn);
+          y[i] = (char)rot_whole(v[n][0], scale);
+          if (j >= 0) y[j] = (char)rot_whole(v[n][1], scale);
+        }
+        if (lane == 0) P.scales[kind - 1][scale_at + h * P.scale_sh[kind - 1]] = scale;
+        continue;
+      }
     }
     for (int k = lane; k < units; k += 32) {
       int i, j;
@@ -783,7 +875,7 @@ __global__ void __launch_bounds__(1024) fa_rotary_dw_kernel(const __grid_constan
 
 // ---- host --------------------------------------------------------------------------------
 FaRotTensor rot_tensor(const fa_tensor& t, int es) { return {(char*)t.ptr, t.stride_b * es, t.stride_h * es, t.stride_s * es}; }
-bool rot_aligned(const FaRotTensor& t) { return (((uintptr_t)t.ptr | (uintptr_t)t.sb | (uintptr_t)t.sh | (uintptr_t)t.ss) & 15) == 0; }
+bool rot_aligned(const FaRotTensor& t, int to = 16) { return (((uintptr_t)t.ptr | (uintptr_t)t.sb | (uintptr_t)t.sh | (uintptr_t)t.ss) & (to - 1)) == 0; }
 
 int rot_check(const fa_rotary_params* p) {
   if (!p) return fail(FA_EINVAL, "params is null");
@@ -822,7 +914,7 @@ bool rot_by_pieces(const FaRotParams& k, int dtype, int* lane_shift) {
   const int v = dtype == FA_F32 ? 4 : 8;
   if (k.D % v || k.Dv % v || k.Dv > k.D) return false;
   for (int i = 0; i < 3; ++i)
-    if (k.heads[i] > 0 && !(rot_aligned(k.x[i]) && rot_aligned(k.y[i]) && (i == 2 || k.in[i].ptr == nullptr || rot_aligned(k.in[i])))) return false;
+    if (k.heads[i] > 0 && !(rot_aligned(k.x[i]) && rot_aligned(k.y[i], i > 0 && k.scales[0] != nullptr ? 8 : 16) && (i == 2 || k.in[i].ptr == nullptr || rot_aligned(k.in[i])))) return false;
   int shift = 0;
   while ((1 << shift) < (k.D + 2 * v - 1) / (2 * v)) ++shift;
   *lane_shift = shift;
@@ -879,6 +971,10 @@ int rot_launch(FaRotParams& k, int dtype, void* stream) {
     const dim3 grid((unsigned)token_blocks, (unsigned)(k.groups[0] + k.groups[1] + k.groups[2]));
     return rot_dispatch(dtype, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
+      if constexpr (DT != FA_F32) {
+        void (*const eight[])(FaRotParams) = {fa_rotary_kernel<DT, kHalves, true>, fa_rotary_kernel<DT, kNeighbours, true>, fa_rotary_kernel<DT, kNeighboursAny, true>, fa_rotary_kernel<DT, kAny, true>};
+        if (k.scales[0]) return launch_here("fa_rotary_kernel", eight[rot_mode(k, dtype)], grid, dim3(kRotThreads), stream, k);
+      }
       void (*const of_mode[])(FaRotParams) = {fa_rotary_kernel<DT, kHalves>, fa_rotary_kernel<DT, kNeighbours>, fa_rotary_kernel<DT, kNeighboursAny>, fa_rotary_kernel<DT, kAny>};
       return launch_here("fa_rotary_kernel", of_mode[rot_mode(k, dtype)], grid, dim3(kRotThreads), stream, k);
     });
@@ -886,6 +982,9 @@ int rot_launch(FaRotParams& k, int dtype, void* stream) {
   const long long rows = (long long)k.tokens * std::max(k.heads[0], std::max(k.heads[1], k.heads[2]));
   const dim3 grid((unsigned)std::min<long long>((rows + kRotThreads / 32 - 1) / (kRotThreads / 32), 1 << 20), k.heads[2] > 0 ? 3 : 2);
   return rot_dispatch(dtype, [&](auto dt) {
+    if constexpr (decltype(dt)::value != FA_F32) {
+      if (k.scales[0]) return launch_here("fa_rotary_any_kernel", fa_rotary_any_kernel<decltype(dt)::value, false, true>, grid, dim3(kRotThreads), stream, k);
+    }
     return launch_here("fa_rotary_any_kernel", fa_rotary_any_kernel<decltype(dt)::value, false>, grid, dim3(kRotThreads), stream, k);
   });
 }
@@ -998,11 +1097,18 @@ int fa_rotary_append(const fa_rotary_params* p, void* stream) {
   if (k.heads[1] > 0 && (!p->k.ptr || !p->v.ptr || !p->slots)) return fail(FA_EINVAL, "a tensor is null");
   if (k.heads[1] > 0 && p->num_pages > 0 && (!p->k_pages.ptr || !p->v_pages.ptr)) return fail(FA_EINVAL, "a tensor is null");
   if (k.heads[0] > 0 && !p->q_out.ptr) return fail(FA_EINVAL, "a tensor is null");
+  const bool eight = p->k_scales.ptr || p->v_scales.ptr;
+  if (eight && p->dtype == FA_F32) return fail(FA_EUNSUPPORTED, "pages in 8 bits take 16-bit tensors");
+  if (eight && !(p->k_scales.ptr && p->v_scales.ptr)) return fail(FA_EINVAL, "scales of keys and of values, or none");
   const int es = esize(p->dtype);
-  const fa_tensor *from[3] = {&p->q, &p->k, &p->v}, *to[3] = {&p->q_out, &p->k_pages, &p->v_pages};
+  const fa_tensor *from[3] = {&p->q, &p->k, &p->v}, *to[3] = {&p->q_out, &p->k_pages, &p->v_pages}, *scales[2] = {&p->k_scales, &p->v_scales};
   for (int i = 0; i < 3; ++i) {
     k.x[i] = rot_tensor(*from[i], es);
-    k.y[i] = rot_tensor(*to[i], es);
+    k.y[i] = rot_tensor(*to[i], eight && i > 0 ? 1 : es);
+  }
+  for (int i = 0; i < 2; ++i) {
+    k.scales[i] = (float*)scales[i]->ptr;
+    k.scale_sp[i] = scales[i]->stride_b; k.scale_sh[i] = scales[i]->stride_h; k.scale_ss[i] = scales[i]->stride_s;
   }
   k.slots = (const long long*)p->slots;
   k.slot_sb = p->slot_stride_b; k.slot_ss = p->slot_stride_s;

@@ -4,6 +4,10 @@ A cache is two tensors ``[pages, kv heads, page_size, D]`` (any strides with a c
 ``[pages, page_size, kv heads, D]`` will do).  A request's tokens lie in the pages that its row of the block table lists; token
 ``j`` is token ``j % page_size`` of page ``block_table[b, j // page_size]``, and its slot is ``page * page_size + j % page_size``.
 
+The pages may be in 8 bits: int8, with a float32 scale for each token and kv head (``key_scales`` and ``value_scales``, ``[pages, kv heads, page_size]``,
+any strides).  ``rotary_append`` then stores a row ``y`` as ``round(y / scale)`` with ``scale = max|y| / 127``, which keeps it to 1 / 254 of its largest
+value, in half of the memory and of the time that reading takes.
+
 A decoding step is ``page_step`` once, and then, for every layer, ``rotary_append`` and ``paged_attention``.  None of
 them waits for the GPU or depends on a length that only the GPU knows, so that a step can be captured in a CUDA graph.
 What would look on (a tracer, a dispatch mode, a functorch transform, a tensor class with a ``__torch_function__`` of its own) is
@@ -49,7 +53,8 @@ def page_step(lengths, new_tokens, block_table, free_pages, page_size: int, num_
 
 
 def rotary_append(query, key, value, key_pages, value_pages, slots, table=None, positions=None, *, query_weight=None,
-                  key_weight=None, eps: float = 1e-6, interleaved: bool = False, bhln: bool = True) -> Optional[torch.Tensor]:
+                  key_weight=None, eps: float = 1e-6, interleaved: bool = False, bhln: bool = True, key_scales=None,
+                  value_scales=None) -> Optional[torch.Tensor]:
     """``rotary_embedding`` for new tokens, whose keys and values go straight into the cache: ``key`` (normed and rotated)
     and ``value`` (as it is) are written to ``slots`` of ``key_pages`` and ``value_pages`` **in place**; the normed and rotated
     ``query`` is returned.  One launch.
@@ -58,15 +63,34 @@ def rotary_append(query, key, value, key_pages, value_pages, slots, table=None, 
     for instance ``[1, tokens, H, D]`` for the prompts of a batch laid end to end.  ``slots`` (int64 ``[B, S]`` or ``[B * S]``) as ``page_step`` gives
     them; a slot below 0 is left out, one beyond the pages too, and the next call raises ``FlaxAttnError``.  No two
     tokens may have the same slot.  ``table``, ``positions`` and the weights are those of ``rotary_embedding``.
+
+    With ``key_scales`` and ``value_scales`` the pages are int8 and the scales are written too (float16 and bfloat16 tensors).  What is stored is
+    rounded once, from the fp32 value behind the rotation.  A row of zeros has the scale 0; one with an infinity or no number in it has no number
+    for a scale, and is read as that throughout.
     """
     return native().rotary_append(query, key, value, key_pages, value_pages, slots, table, positions, query_weight, key_weight, eps,
-                                  interleaved, not bhln)
+                                  interleaved, not bhln, key_scales, value_scales)
+
+
+def read_pages(key_pages, value_pages, block_table, starts, num_tokens: int, *, key_scales=None, value_scales=None, dtype: Optional[torch.dtype] = None,
+               bhln: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The cached tokens of a batch laid end to end, ``(key, value)`` of ``[1, kv heads, num_tokens, D]`` (``bhln=False``: ``[1, num_tokens, kv heads, D]``).
+
+    Row ``t`` is token ``t - starts[b]`` of the request ``b`` with ``starts[b] <= t < starts[b + 1]`` (``starts``: int32 ``[B + 1]``, never decreasing; of whole requests
+    the sums of their lengths).  ``num_tokens`` is ``starts[B]``, which the host has to know; rows beyond it, or in front of ``starts[0]``, are 0.
+    Pages in 8 bits (with their scales) are multiplied out and rounded to ``dtype``, others are copied.  A table entry that is no page, or a token that the table has no
+    room for, leaves the row 0, and the next call raises ``FlaxAttnError`` (``check_status``).
+
+    It is what attention over more than a few new tokens takes: the next piece of a prompt (``prompt_attention`` with ``key_starts``), or the
+    tokens that requests have in common (``prefix`` of ``paged_attention``).  One launch, no gradient.
+    """
+    return native().read_pages(key_pages, value_pages, block_table, starts, num_tokens, key_scales, value_scales, dtype, not bhln)
 
 
 def paged_attention(query, key_pages, value_pages, block_table, lengths, score_mod: Optional[Callable] = None,
                     mask_mod: Optional[Callable] = None, *, window: Optional[int] = None, sm_scale: Optional[float] = None,
                     bhln: bool = True, return_lse: bool = False, b_offset: int = 0, h_offset: int = 0,
-                    kernel_options: Optional[dict] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+                    kernel_options: Optional[dict] = None, key_scales=None, value_scales=None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Attention of the newest tokens of each request over its pages.
 
     ``query`` ``[B, Hq, Sq, D]`` (``bhln=False``: ``[B, Sq, Hq, D]``) holds the last ``Sq`` tokens of each request, ``lengths`` (int32 ``[B]``) counts
@@ -89,12 +113,12 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, score_m
     general = kernel_options is not None and kernel_options.get("kernels") == "general"
     call = native().paged_attention
     res = call(query, key_pages, value_pages, block_table, lengths, score_mod, mask_mod, window, sm_scale, not bhln, return_lse, b_offset,
-               h_offset, general, None)
+               h_offset, general, key_scales, value_scales, None)
     if res is None:
         # mods that are not known yet, or tensors that they capture elsewhere than the query
         module = module_for(score_mod, mask_mod)
         lowered = lower_mods(None if score_mod is identity_score else score_mod, None if mask_mod is noop_mask else mask_mod)
         buffers = tuple(device_buffers(lowered, query.device))
         res = call(query, key_pages, value_pages, block_table, lengths, score_mod, mask_mod, window, sm_scale, not bhln, return_lse, b_offset,
-                   h_offset, general, (module.handle.value, buffers))
+                   h_offset, general, key_scales, value_scales, (module.handle.value, buffers))
     return res

@@ -287,6 +287,9 @@ typedef struct fa_rotary_params {
   const int64_t* slots;       /* page * page_size + token of the page, for each token; below 0: k and v go nowhere */
   int64_t slot_stride_b, slot_stride_s;
   int32_t* status; /* optional status word: 8 = a position beyond the table (its pairs become 0), 16 = a slot beyond the pages (not written) */
+  /* fa_rotary_append, pages in 8 bits (int8, strides in bytes; tensors of 16 bits): the scales of keys and values, float32, by the strides of page, head and
+   * token in a page.  A row y is stored as round(y / scale) with scale = max|y| / 127.  ptr NULL: pages of the tensors' type. */
+  fa_tensor k_scales, v_scales;
 } fa_rotary_params;
 
 int fa_rotary(const fa_rotary_params* p, void* stream);
@@ -315,6 +318,26 @@ int fa_page_step(const int32_t* lengths, const int32_t* new_tokens, int B, int32
                  int32_t* out_lengths, int32_t* positions, int64_t* slots, int32_t* requests, int32_t* starts, int32_t* out_taken,
                  void* stream);
 
+/* The tokens of requests out of their pages, laid end to end: row t of key and value is token t - starts[b] of the request b with
+ * starts[b] <= t < starts[b + 1] (starts [B + 1], never decreasing).  Rows of no request, of tokens that the table has no room for and of table entries that are
+ * no page are 0; the last two set 4 in the status word.  Pages in 8 bits (scales given) are multiplied out and rounded once; others are copied.  One launch. */
+typedef struct fa_read_params {
+  int32_t dtype;              /* of key and value, and of pages that are not in 8 bits */
+  int32_t B, Hkv, D, Dv;
+  int64_t num_tokens;
+  fa_tensor k_pages, v_pages; /* as in fa_rotary_params */
+  fa_tensor k_scales, v_scales;
+  int64_t num_pages;
+  int32_t page_size;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  int32_t table_width;
+  const int32_t* starts;
+  fa_tensor k, v;             /* stride_h of a head, stride_s of a token */
+  int32_t* status;
+} fa_read_params;
+int fa_read_pages(const fa_read_params* p, void* stream);
+
 /* Attention of the Sq newest tokens of each request over its pages.  Query i is token lengths[b] - Sq + i, sees the keys up to
  * itself, at most `window` behind it, and those that mask_mod keeps; that token's number is the q index of the mods.  A row that sees
  * nothing is 0 with an lse of -inf.  The work is split over the requests' lengths on the device: the launches depend on none of them. */
@@ -336,6 +359,9 @@ typedef struct fa_paged_params {
   int32_t flags;              /* FA_FLAG_GENERAL_KERNELS: K and V in 16-byte pieces instead of by TMA */
   int32_t* status;            /* optional status word: 4 = a block table entry that is no page, or a length that is
                                  negative or beyond the table (such keys are left out) */
+  /* pages in 8 bits (int8, strides in bytes; queries of 16 bits), as fa_rotary_append writes them: the scales, float32, by the strides of page, head
+   * and token in a page.  ptr NULL: pages of the queries' type. */
+  fa_tensor k_scales, v_scales;
 } fa_paged_params;
 size_t fa_paged_workspace_bytes(const fa_paged_params* p);
 int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t workspace_bytes, void* stream);

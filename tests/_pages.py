@@ -92,3 +92,37 @@ def check_attention(out, lse, want, dtype):
         assert torch.equal(torch.isneginf(lse), empty)
         assert ((lse - ref_lse)[~empty].abs() <= 2.0 ** -20 * (4 + top) + 2.0 ** -22 * ref_lse[~empty].abs()).all()
         assert (got[empty] == 0).all()
+
+
+def eight_bits(x):
+    """The whole numbers and scales that rows of x (last dimension) have in a cache of 8 bits: the definition, in fp32 divisions."""
+    x = x.float()
+    scale = torch.where(torch.isfinite(x).all(-1), x.abs().amax(-1) / 127, math.nan)
+    whole = torch.where(scale[..., None] > 0, (x / scale[..., None]).round().clamp(-127, 127), torch.zeros(()))
+    return whole.nan_to_num(0.0).to(torch.int8), scale
+
+
+class Cache8(Cache):
+    """The same in 8 bits: `keys` and `values` are what the pages stand for, in 64 bits.  Scales of what holds no token are NaN."""
+
+    def __init__(self, seed, lengths, Hkv, D, page, dtype, *args, token_major=False, **kw):
+        super().__init__(seed, lengths, Hkv, D, page, dtype, *args, token_major=token_major, **kw)
+        device = self.k_pages.device
+        for n in ("k", "v"):
+            whole, scale = eight_bits(getattr(self, n + "_pages").cpu())
+            empty = torch.isnan(scale)
+            whole[empty] = torch.randint(-128, 128, whole[empty].shape, generator=torch.Generator().manual_seed(seed)).to(torch.int8)
+            if token_major:
+                whole, scale = (t.transpose(1, 2).contiguous().to(device).transpose(1, 2) for t in (whole, scale))
+            setattr(self, n + "_pages", whole.to(device))
+            setattr(self, n + "_scales", scale.to(device))
+        for n in ("keys", "values"):
+            got = []
+            for x in getattr(self, n):
+                whole, scale = eight_bits(x)
+                got.append(whole.double() * scale.double()[..., None])
+            setattr(self, n, got)
+
+    @property
+    def scales(self):
+        return dict(key_scales=self.k_scales, value_scales=self.v_scales)
