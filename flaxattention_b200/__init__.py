@@ -6,6 +6,7 @@ from .attention import check_status, flax_attention, flax_attention_pallas, math
 from .blockmask import BlockMask, and_masks, create_block_mask, noop_mask, or_masks
 from .paged import PageStep, page_step, paged_attention, read_pages, rotary_append
 from .pipeline import HostPipeline
+from .prompts import prompt_attention
 from .rotary import rotary_embedding, rotary_table
 from . import fnp, masks, mods  # noqa: F401
 from typing import Callable
@@ -33,6 +34,7 @@ __all__ = [
     "page_step",
     "read_pages",
     "paged_attention",
+    "prompt_attention",
     "fnp",
     "masks",
     "mods",

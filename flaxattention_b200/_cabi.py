@@ -82,7 +82,16 @@ class FaPagedParams(C.Structure):
         ("num_pages", C.c_int64), ("page_size", C.c_int32),
         ("block_table", C.c_void_p), ("block_table_stride", C.c_int64), ("table_width", C.c_int32),
         ("lengths", C.c_void_p), ("window", C.c_int32), ("lse", C.c_void_p), ("flags", C.c_int32), ("status", C.c_void_p),
-        ("k_scales", FaTensor), ("v_scales", FaTensor),
+        ("k_scales", FaTensor), ("v_scales", FaTensor), ("prefix_length", C.c_int32), ("k_prefix", FaTensor), ("v_prefix", FaTensor),
+    ]
+
+
+class FaPromptParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("Dv", C.c_int32),
+        ("tokens", C.c_int64), ("keys", C.c_int64), ("scale", C.c_float), ("b_offset", C.c_int32), ("h_offset", C.c_int32),
+        ("q", FaTensor), ("k", FaTensor), ("v", FaTensor), ("o", FaTensor), ("starts", C.c_void_p), ("key_starts", C.c_void_p),
+        ("window", C.c_int32), ("lse", C.c_void_p), ("flags", C.c_int32), ("status", C.c_void_p),
     ]
 
 
@@ -116,6 +125,7 @@ EXPORTS = [
     "fa_fwd_workspace_bytes", "fa_fwd_ws",
     "fa_rotary", "fa_rotary_bwd_workspace_bytes", "fa_rotary_bwd", "fa_rotary_append",
     "fa_page_step", "fa_read_pages", "fa_paged_workspace_bytes", "fa_paged", "fa_paged_prepare",
+    "fa_prompt", "fa_prompt_prepare",
 ]
 
 
@@ -185,6 +195,8 @@ def lib() -> C.CDLL:
     L.fa_paged_workspace_bytes.argtypes = [C.POINTER(FaPagedParams)]
     L.fa_paged.argtypes = [C.c_void_p, C.POINTER(FaPagedParams), C.c_void_p, C.c_size_t, C.c_void_p]
     L.fa_paged_prepare.argtypes = [C.c_void_p, C.POINTER(FaPagedParams)]
+    L.fa_prompt.argtypes = [C.c_void_p, C.POINTER(FaPromptParams), C.c_void_p]
+    L.fa_prompt_prepare.argtypes = [C.c_void_p, C.POINTER(FaPromptParams)]
     L.fa_mask_bits_row_words.restype = C.c_int64
     L.fa_mask_bits_row_words.argtypes = [C.c_int]
     L.fa_mask_bits.argtypes = [C.c_void_p] + [C.c_int] * 6 + [C.c_void_p, C.c_void_p]

@@ -99,7 +99,7 @@ def check_status() -> None:
         raise _cabi.FlaxAttnError(-3, f"a kernel reported status bits {bits:#x} (bit 0: a bounded barrier wait ran out; "
                                       "bit 1: a launch configuration the kernel refused; bit 2: a block table entry that is "
                                       "no page, or a length beyond the table; bit 3: a position beyond the rotary table; "
-                                      "bit 4: a slot beyond the pages); the results of that launch are incomplete")
+                                      "bit 4: a slot beyond the pages; bit 5: starts of requests that decrease or lie beyond the tokens); the results of that launch are incomplete")
 
 
 def _tensor(t: torch.Tensor, layout: str) -> _cabi.FaTensor:

@@ -40,7 +40,7 @@ def is_current() -> bool:
 
 
 def host_sources():
-    srcs = [os.path.join(HERE, "flaxattn.cu"), os.path.join(HERE, "rotary.cuh"), os.path.join(HERE, "paging.cuh"),
+    srcs = [os.path.join(HERE, "flaxattn.cu"), os.path.join(HERE, "rotary.cuh"), os.path.join(HERE, "prompts.cuh"), os.path.join(HERE, "paging.cuh"),
             os.path.join(PKG, "..", "include", "flaxattn.h")]
     kdir = os.path.join(HERE, "kernels")
     # the templates count too: the library's launch code mirrors their shared-memory maps

@@ -111,7 +111,7 @@ std::string cache_dir() {
 }
 
 const char* const kTemplateFiles[] = {"fa_params.h", "fa_common.cuh", "fa_fwd.cuh", "fa_bwd.cuh",
-                                      "fa_decode.cuh", "fa_blockmask.cuh", "fa_sm100.cuh", "fa_fwd_tc.cuh", "fa_bwd_items.cuh", "fa_bwd_tc.cuh", "fa_bwd_tc128.cuh", "fa_bwd_f32.cuh", "fa_selftest.cuh", "fa_paged.cuh", "fa_score_math.cuh"};
+                                      "fa_decode.cuh", "fa_blockmask.cuh", "fa_sm100.cuh", "fa_fwd_tc.cuh", "fa_bwd_items.cuh", "fa_bwd_tc.cuh", "fa_bwd_tc128.cuh", "fa_bwd_f32.cuh", "fa_selftest.cuh", "fa_paged.cuh", "fa_score_math.cuh", "fa_packed_rows.cuh", "fa_packed.cuh"};
 std::string g_templates_hash;
 int templates_hash(std::string& out) {
   if (g_templates_hash.empty()) {
@@ -192,7 +192,7 @@ const char* const kDefaultMods =
 
 // A kernel variant of a module as a number: every launch looks its kernel up by it, and the define text
 // is only put together when the variant has to be compiled or fetched from the cache on disk.
-enum KernelId : int { kIdFwd, kIdFwdRerun, kIdBwdRerun, kIdFwdTc, kIdBwdDq, kIdBwdDkdv, kIdBwdTc, kIdBwdF32, kIdDecode, kIdMaskScan, kIdMaskClassify, kIdSelftest, kIdPaged };
+enum KernelId : int { kIdFwd, kIdFwdRerun, kIdBwdRerun, kIdFwdTc, kIdBwdDq, kIdBwdDkdv, kIdBwdTc, kIdBwdF32, kIdDecode, kIdMaskScan, kIdMaskClassify, kIdSelftest, kIdPaged, kIdPacked };
 uint64_t kernel_key(KernelId id, std::initializer_list<std::pair<int, int>> fields) {  // (value, bits)
   uint64_t k = 0;
   for (auto& f : fields) k = (k << f.second) | (uint64_t)f.first;
@@ -2179,4 +2179,5 @@ int fa_decode_static(fa_module* m, const fa_attn_params* p, int num_splits, void
 // Around the attention of a language model: rotary positions, and pages of a key / value cache
 // ======================================================================================
 #include "rotary.cuh"
+#include "prompts.cuh"
 #include "paging.cuh"

@@ -1128,6 +1128,37 @@ void table_of(const at::Tensor& table, int64_t B, c10::Device dev) {
                     "block_table must be [", B, ", pages of a request] with contiguous rows, got ", table.sizes());
 }
 
+// The module of a call's mods, and the tensors that they capture: as the Python layer gives them, or those known for the pair
+struct Launched {
+  fa_module* module = nullptr;
+  ModsPtr hold;
+  std::vector<at::Tensor> given;
+  const std::vector<at::Tensor>* buffers = &given;
+  bool known = true;
+  Launched(PyObject* score_mod, PyObject* mask_mod, PyObject* as_given, c10::Device dev) {
+    if (as_given != Py_None) {
+      TORCH_CHECK(PyTuple_Check(as_given) && PyTuple_GET_SIZE(as_given) == 2, "module: a handle and a tuple of buffers");
+      module = (fa_module*)PyLong_AsVoidPtr(PyTuple_GET_ITEM(as_given, 0));
+      if (PyErr_Occurred()) throw python_error();
+      given = tensors(PyTuple_GET_ITEM(as_given, 1));
+      return;
+    }
+    const auto hit = g_mods->find({score_mod == Py_None || score_mod == g_identity ? nullptr : score_mod, mask_mod == Py_None || mask_mod == g_noop ? nullptr : mask_mod});
+    known = hit != g_mods->end();
+    if (!known) return;
+    hold = hit->second;
+    for (const auto& t : hold->buffers) known = known && t.device() == dev;
+    module = hold->module;
+    buffers = &hold->buffers;
+  }
+};
+int window_of(PyObject* o) {
+  if (o == Py_None) return -1;
+  const int64_t w = integer(o);
+  TORCH_CHECK_VALUE(w >= 0, "window must not be negative, got ", w);
+  return (int)std::min<int64_t>(w, INT32_MAX);
+}
+
 // read_pages(key_pages, value_pages, block_table, starts, num_tokens, key_scales, value_scales, dtype or None, bshd) -> key, value
 PyObject* read_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1195,10 +1226,11 @@ PyObject* read_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // paged_attention(q, key_pages, value_pages, block_table, lengths, score_mod, mask_mod, window or None, scale or None, bshd, return_lse, b_offset,
-//                 h_offset, general, key_scales, value_scales, module: None or (handle, buffers)) -> out or (out, lse); None: the mods are not known here
+//                 h_offset, general, key_scales, value_scales, prefix: None or (key, value), module: None or (handle, buffers))
+// -> out or (out, lse); None: the mods are not known here
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK(n == 17, "paged_attention takes 17 arguments");
+  TORCH_CHECK(n == 18, "paged_attention takes 18 arguments");
   check_unwatched();
   const at::Tensor q = cuda_tensor(a[0], "query"), kp = cuda_tensor(a[1], "key_pages"), vp = cuda_tensor(a[2], "value_pages"),
                    table = cuda_tensor(a[3], "block_table"), lengths = cuda_tensor(a[4], "lengths");
@@ -1232,36 +1264,34 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.block_table_stride = table.stride(0);
   p.table_width = (int)table.size(1);
   p.lengths = (const int32_t*)lengths.const_data_ptr();
-  p.window = -1;
-  if (a[7] != Py_None) {
-    const int64_t w = integer(a[7]);
-    TORCH_CHECK_VALUE(w >= 0, "window must not be negative, got ", w);
-    p.window = (int)std::min<int64_t>(w, INT32_MAX);
-  }
+  p.window = window_of(a[7]);
   p.scale = a[8] == Py_None ? (float)(1.0 / std::sqrt((double)std::max(p.D, 1))) : (float)number(a[8]);
   const bool return_lse = truth(a[10]);
   p.b_offset = (int)integer(a[11]);
   p.h_offset = (int)integer(a[12]);
   p.flags = truth(a[13]) ? FA_FLAG_GENERAL_KERNELS : 0;
   p.status = (int32_t*)g_status;
-  fa_module* module = nullptr;
-  ModsPtr hold;
-  std::vector<at::Tensor> given;
-  const std::vector<at::Tensor>* buffers = &given;
+  at::Tensor prefix[2];
   if (a[16] != Py_None) {
-    TORCH_CHECK(PyTuple_Check(a[16]) && PyTuple_GET_SIZE(a[16]) == 2, "module: a handle and a tuple of buffers");
-    module = (fa_module*)PyLong_AsVoidPtr(PyTuple_GET_ITEM(a[16], 0));
-    if (PyErr_Occurred()) return nullptr;
-    given = tensors(PyTuple_GET_ITEM(a[16], 1));
-  } else {
-    const auto hit = g_mods->find({a[5] == Py_None || a[5] == g_identity ? nullptr : a[5], a[6] == Py_None || a[6] == g_noop ? nullptr : a[6]});
-    if (hit == g_mods->end()) Py_RETURN_NONE;
-    hold = hit->second;
-    for (const auto& t : hold->buffers)
-      if (t.device() != q.device()) Py_RETURN_NONE;
-    module = hold->module;
-    buffers = &hold->buffers;
+    TORCH_CHECK_TYPE((PyTuple_Check(a[16]) || PyList_Check(a[16])) && PySequence_Size(a[16]) == 2, "prefix: a pair of tensors, key and value, is expected");
+    Ref items(PySequence_Tuple(a[16]));
+    if (items.p == nullptr) throw python_error();
+    const char* const names[2] = {"the key of prefix", "the value of prefix"};
+    for (int i = 0; i < 2; ++i) {
+      const at::Tensor& t = prefix[i] = cuda_tensor(PyTuple_GET_ITEM(items.p, i), names[i]);
+      rows_of(t, names[i]);
+      same_kind(t, q, names[i]);
+      no_gradient(t, names[i], "paged_attention");
+      TORCH_CHECK_VALUE(t.size(0) == 1 && t.size(ih) == p.Hkv && t.size(3) == (i == 0 ? p.D : p.Dv) && t.size(is) == prefix[0].size(is),
+                        "prefix must be one sequence of ", p.Hkv, " kv heads and the embedding dimensions of the pages, got ", prefix[0].sizes(), i == 0 ? "" : " and ",
+                        i == 0 ? at::IntArrayRef() : t.sizes());
+      (i == 0 ? p.k_prefix : p.v_prefix) = by_strides(t, bshd);
+    }
+    TORCH_CHECK_NOT_IMPLEMENTED(prefix[0].size(is) <= 1 << 23, "a prefix of more than 2^23 tokens");
+    p.prefix_length = (int)prefix[0].size(is);
   }
+  Launched launched(a[5], a[6], a[17], q.device());
+  if (!launched.known) Py_RETURN_NONE;
   check_status();
   at::Tensor out, lse;
   {
@@ -1277,8 +1307,79 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const size_t bytes = fa_paged_workspace_bytes(&p);
       at::Tensor ws;
       if (bytes > 0) ws = empty({(int64_t)bytes}, at::kByte, q.device());
-      BuffersLock lock(module, *buffers);
-      const int rc = lock.rc != FA_OK ? lock.rc : fa_paged(module, &p, bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, (void*)c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+      BuffersLock lock(launched.module, *launched.buffers);
+      const int rc = lock.rc != FA_OK ? lock.rc : fa_paged(launched.module, &p, bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, (void*)c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+      if (rc != FA_OK) raise(rc);
+    }
+  }
+  if (!return_lse) return THPVariable_Wrap(out);
+  Ref o(THPVariable_Wrap(out)), l(THPVariable_Wrap(lse));
+  if (o.p == nullptr || l.p == nullptr) return nullptr;
+  return PyTuple_Pack(2, o.p, l.p);
+  END_HANDLE_TH_ERRORS
+}
+
+// prompt_attention(q, k, v, starts, key_starts or None, score_mod, mask_mod, window or None, scale or None, bshd, return_lse, b_offset, h_offset, general,
+//                  module: None or (handle, buffers)) -> out or (out, lse); None: the mods are not known here
+PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 15, "prompt_attention takes 15 arguments");
+  check_unwatched();
+  const at::Tensor q = cuda_tensor(a[0], "query"), k = cuda_tensor(a[1], "key"), v = cuda_tensor(a[2], "value"), starts = cuda_tensor(a[3], "starts");
+  const at::Tensor key_starts = a[4] != Py_None ? cuda_tensor(a[4], "key_starts") : starts;
+  rows_of(q, "query");
+  rows_of(k, "key");
+  rows_of(v, "value");
+  same_kind(k, q, "key");
+  same_kind(v, q, "value");
+  fa_prompt_params p;
+  memset(&p, 0, sizeof p);
+  const bool bshd = truth(a[9]);
+  const int ih = bshd ? 2 : 1, is = bshd ? 1 : 2;
+  p.dtype = dtype_code(q, "query");
+  TORCH_CHECK_VALUE(q.size(0) == 1 && k.size(0) == 1 && v.size(0) == 1, "prompts lie end to end in one sequence, so that the batch dimension is 1, got ", q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+  p.Hq = (int)q.size(ih); p.Hkv = (int)k.size(ih); p.D = (int)q.size(3); p.Dv = (int)v.size(3);
+  p.tokens = q.size(is); p.keys = k.size(is);
+  TORCH_CHECK_VALUE(v.size(ih) == p.Hkv && v.size(is) == p.keys, "key and value must have the same heads and sequence, but got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_VALUE(k.size(3) == p.D, "query and key must have the same embedding dimension, but got ", q.sizes(), " and ", k.sizes());
+  TORCH_CHECK_VALUE(p.Dv <= p.D, "value embedding dimension must not exceed that of query and key, got Ev=", p.Dv, " and E=", p.D);
+  TORCH_CHECK_VALUE(p.Hkv > 0 ? p.Hq % p.Hkv == 0 : p.Hq == 0, "Expect number of query heads to be a multiple of kv heads, but got Hq=", p.Hq, " and Hkv=", p.Hkv, ".");
+  for (const auto& [t, name] : {std::pair<const at::Tensor&, const char*>{starts, "starts"}, {key_starts, "key_starts"}}) {
+    int_kind(t, at::kInt, q.device(), name);
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) >= 1 && t.size(0) == starts.size(0) && t.size(0) < INT32_MAX && t.is_contiguous(), name, " must be a contiguous [requests + 1] tensor, got ", t.sizes());
+  }
+  TORCH_CHECK_VALUE(a[4] != Py_None || p.tokens == p.keys, "without key_starts, queries and keys are the same tokens, but got ", p.tokens, " and ", p.keys);
+  no_gradient(q, "query", "prompt_attention");
+  no_gradient(k, "key", "prompt_attention");
+  no_gradient(v, "value", "prompt_attention");
+  p.B = (int)(starts.size(0) - 1);
+  p.starts = (const int32_t*)starts.const_data_ptr();
+  p.key_starts = (const int32_t*)key_starts.const_data_ptr();
+  p.window = window_of(a[7]);
+  p.scale = a[8] == Py_None ? (float)(1.0 / std::sqrt((double)std::max(p.D, 1))) : (float)number(a[8]);
+  const bool return_lse = truth(a[10]);
+  p.b_offset = (int)integer(a[11]);
+  p.h_offset = (int)integer(a[12]);
+  p.flags = truth(a[13]) ? FA_FLAG_GENERAL_KERNELS : 0;
+  p.status = (int32_t*)g_status;
+  Launched launched(a[5], a[6], a[14], q.device());
+  if (!launched.known) Py_RETURN_NONE;
+  check_status();
+  at::Tensor out, lse;
+  {
+    pybind11::gil_scoped_release no_gil;
+    c10::cuda::OptionalCUDAGuard guard(q.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = bshd ? empty({1, p.tokens, p.Hq, p.Dv}, q.scalar_type(), q.device()) : empty({1, p.Hq, p.tokens, p.Dv}, q.scalar_type(), q.device());
+    if (return_lse) lse = empty({1, p.Hq, p.tokens}, at::kFloat, q.device());
+    if (p.Hq > 0 && p.tokens > 0) {
+      p.q = by_strides(q, bshd);
+      p.k = by_strides(k, bshd);
+      p.v = by_strides(v, bshd);
+      p.o = by_strides(out, bshd);
+      p.lse = return_lse ? lse.mutable_data_ptr<float>() : nullptr;
+      BuffersLock lock(launched.module, *launched.buffers);
+      const int rc = lock.rc != FA_OK ? lock.rc : fa_prompt(launched.module, &p, (void*)c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
       if (rc != FA_OK) raise(rc);
     }
   }
@@ -1342,6 +1443,7 @@ PyMethodDef kMethods[] = {
     {"page_step", (PyCFunction)(void*)page_step, METH_FASTCALL, nullptr},
     {"read_pages", (PyCFunction)(void*)read_pages, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void*)paged_attention, METH_FASTCALL, nullptr},
+    {"prompt_attention", (PyCFunction)(void*)prompt_attention, METH_FASTCALL, nullptr},
     {"register", (PyCFunction)(void*)register_mods, METH_FASTCALL, nullptr},
     {"forget", (PyCFunction)(void*)forget, METH_FASTCALL, nullptr},
     {"setup", (PyCFunction)(void*)setup, METH_FASTCALL, nullptr},

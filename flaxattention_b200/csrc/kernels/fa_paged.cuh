@@ -41,7 +41,8 @@
 // four keys, and has the operands of four products.
 //
 // Compile-time parameters (macros): FA_DTYPE, FA_D, FA_DV, FA_RG (1, 2, 4), FA_WN (keys of a tile: 32 or 16; fp32: 32, 16, 8), FA_SLOTS, FA_TMA,
-// FA_FEW (0: the other way), FA_FR (fp32: rows of a warp), FA_CG, FA_SHORT, FA_KV8.
+// FA_FEW (0: the other way), FA_FR (fp32: rows of a warp), FA_CG, FA_SHORT, FA_KV8, FA_AFTER (the keys lie behind a prefix, over which
+// another kernel goes: results in float32 with their sums, for fa_prefix_merge_kernel).
 #pragma once
 #include "fa_sm100.cuh"
 
@@ -71,6 +72,8 @@ constexpr int WN = FA_WN;
 constexpr int SLOTS = FA_SLOTS;
 constexpr int ES = F32 ? 4 : 2;
 constexpr bool KV8 = FA_KV8 != 0;
+constexpr bool AFTER = FA_AFTER != 0;
+constexpr int EO = F32 || AFTER ? 4 : 2;  // bytes of a result
 constexpr int EK = KV8 ? 1 : ES;  // bytes of a cached value
 // Rows in 8 bits are column groups of 128 bytes, or one of 64, whole ones also where the head dim is not: what lies behind it is some whole number or
 // other and is multiplied with zeros, or in columns that nobody writes out.  Tiles lie as TMA leaves them however they come.
@@ -706,17 +709,22 @@ struct Sum {
 
 // a value of an output row
 __device__ __forceinline__ void put1(char* row, int c, float x) {
-  if (F32) *(float*)(row + c * 4) = x;
+  if (EO == 4) *(float*)(row + c * 4) = x;
   else *(fa_u16*)(row + c * 2) = (fa_u16)fa_pack2<DT>(x, 0.f);
 }
 // two beside each other
 __device__ __forceinline__ void put2(char* row, int c, float x, float y) {
-  if (F32) *(float2*)(row + c * 4) = make_float2(x, y);
+  if (EO == 4) *(float2*)(row + c * 4) = make_float2(x, y);
   else *(fa_u32*)(row + c * 2) = fa_pack2<DT>(x, y);
 }
 // 1 / sum; 0 of a row that has seen nothing, no number of a sum that is none
 __device__ __forceinline__ float inverse(float l) { return l > 0.f ? 1.f / l : l; }
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? FA_NEG_INF : (m + log2f(l)) * FA_LN2; }
+// what is left of a whole row's maximum and sum
+__device__ __forceinline__ void put_sums(const FaPagedParams& p, long long row, float m, float l) {
+  if (AFTER) *(float2*)(p.out_ml + row * 2) = make_float2(m, l);
+  else if (p.lse != nullptr) p.lse[row] = log_sum(m, l);
+}
 
 // The warps of a key group wait for one another; true where any of their threads says so.
 __device__ __forceinline__ bool group_sync(int cg, bool v) {
@@ -1069,10 +1077,10 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
       for (int h = 0; h < HR; ++h) {
         top[h] = FA_NEG_INF;
         if (R.idle(h, rows)) continue;  // (the rows of all lanes)
-        [[maybe_unused]] const int qp = max(qpos[h], 0), gh = head[h] + p.h_off;
+        [[maybe_unused]] const int qp = max(qpos[h], 0) + (AFTER ? p.after : 0), gh = head[h] + p.h_off;
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-          [[maybe_unused]] const int kv = n0 + R.key(j);
+          [[maybe_unused]] const int kv = n0 + R.key(j) + (AFTER ? p.after : 0);
           float x = R.score(h, j);
 #if FA_HAS_SCORE_MOD && defined(FA_SCORE_AFFINE)
           x = fmaf(x, fa_score_mul(0.f, gb, gh, qp, kv) * sc2, fa_score_add2(0.f, gb, gh, qp, kv));
@@ -1089,7 +1097,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
             const int kv = n0 + R.key(j);
             bool see = kv <= qpos[h] && (p.window < 0 || qpos[h] - kv <= p.window) && ((kept >> R.key(j)) & 1u);
 #if FA_HAS_MASK_MOD
-            see = see && fa_mask_mod(gb, gh, qp, kv);
+            see = see && fa_mask_mod(gb, gh, qp, kv + (AFTER ? p.after : 0));
 #endif
             if (!see) R.score(h, j) = FA_NEG_INF;
           }
@@ -1202,9 +1210,9 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
             if (!in) continue;
             if (whole) {
               f *= inverse(l);
-              if (i % CG == 0 && p.lse != nullptr) {
+              if (i % CG == 0) {
                 const int qi = divided(rt * BM + r, p.by_group), hd = hk * G + rt * BM + r - qi * G;
-                p.lse[((long long)b * p.Hq + hd) * p.Sq + qi] = log_sum(m_use, l);
+                put_sums(p, ((long long)b * p.Hq + hd) * p.Sq + qi, m_use, l);
               }
             } else if (i % CG == 0) {
               *(float2*)(part_ml + r * 2) = make_float2(m, l);
@@ -1228,7 +1236,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
           }
           if (whole) {
             const int qi = divided(rt * BM + r, p.by_group), hd = hk * G + rt * BM + r - qi * G;
-            put2((char*)p.o.ptr + (b * p.o.sb + hd * p.o.sh + qi * p.o.ss) * ES, blk * 32 + c, x, y);
+            put2((char*)p.o.ptr + (b * p.o.sb + hd * p.o.sh + qi * p.o.ss) * EO, blk * 32 + c, x, y);
           } else {
             *(float2*)(part_o + r * DV + blk * 32 + c) = make_float2(x, y);
           }
@@ -1241,11 +1249,11 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #pragma unroll
       for (int h = 0; h < HR; ++h) {
         const int i = divided(rt * BM + R.row(h), p.by_group);
-        out[h] = (char*)p.o.ptr + (b * p.o.sb + head[h] * p.o.sh + i * p.o.ss) * ES;
+        out[h] = (char*)p.o.ptr + (b * p.o.sb + head[h] * p.o.sh + i * p.o.ss) * EO;
         inv[h] = inverse(R.l[h]);
         if (R.row(h) >= rows || !R.speaks()) continue;
         if (!whole) *(float2*)(part_ml + R.row(h) * 2) = make_float2(R.m[h], R.l[h]);
-        else if (p.lse != nullptr) p.lse[((long long)b * p.Hq + head[h]) * p.Sq + i] = log_sum(R.m[h], R.l[h]);
+        else put_sums(p, ((long long)b * p.Hq + head[h]) * p.Sq + i, R.m[h] == FA_NEG_INF ? 0.f : R.m[h], R.l[h]);
       }
 #pragma unroll
       for (int blk = 0; blk < (DV + 31) / 32; ++blk)

@@ -106,12 +106,36 @@ struct FaPagedParams {
   const void* mod_buf[FA_MAX_MOD_BUFS];
   FaTensor k_scales, v_scales;        // pages in 8 bits: float32, strides of page, head and token in a page
   FaDiv by_box;
+  // Behind a prefix (FA_AFTER): o is float32, the rows' maxima (log2 units) and sums go to out_ml [B, Hq, Sq, 2], and token 0 of a request is
+  // token `after` to the mods
+  float* out_ml;
+  int after;
+};
+
+// Attention of prompts laid end to end, and of the newest tokens of requests over a prefix that they share (fa_packed.cuh, fa_fwd_tc.cuh)
+struct FaPackedParams {
+  FaTensor q, k, v, o;     // prompts: ss is the stride of a token, sb is not used
+  float* lse;              // prompts: [Hq, tokens] or null
+  float* part_o;           // prefix: [splits, Hkv, tokens * G, Dv] not divided, G = Hq / Hkv
+  float* part_ml;          // prefix: [splits, Hkv, tokens * G, 2] maximum (log2 units) and sum
+  const int* starts;       // prompts: [B + 1] where the queries of each request begin
+  const int* key_starts;   // prompts: [B + 1] where its keys begin
+  const int* lengths;      // prefix: [B] tokens that each request has behind the prefix, the Sq newest included
+  int* status;
+  int B, Hq, Hkv, Sq, D, Dv;
+  int tokens, keys;        // rows of q (prefix: B * Sq) and of k
+  int window;              // keys more than this far behind a query are not seen (-1: all are)
+  int b_off, h_off, splits;
+  FaDiv by_group, by_sq;   // by Hq / Hkv, Sq
+  float scale;
+  const void* mod_buf[FA_MAX_MOD_BUFS];
 };
 
 // Status bits that kernels OR into a status word, beside those of the bounded waits (fa_sm100.cuh)
 #define FA_STATUS_BAD_PAGE 4      // a block table entry that is no page, or a length beyond the table
 #define FA_STATUS_BAD_POSITION 8  // a position beyond the rotary table
 #define FA_STATUS_BAD_SLOT 16     // a slot beyond the pages
+#define FA_STATUS_BAD_START 32    // starts of requests that decrease or lie beyond the tokens
 
 // Evaluation of mask_mod over a block grid: the class of every block and, optionally, the mask itself as
 // bit matrices.  `B`, `H`: entries evaluated (1 where the mask does not read the batch / head index).

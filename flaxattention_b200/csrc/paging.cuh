@@ -368,6 +368,13 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) fa_paged_combin
   }
   const float m_use = m == -INFINITY ? 0.f : m;
   const float inv = l > 0.f ? 1.f / l : l;  // (0 and no number stay)
+  if (p.out_ml != nullptr) {  // (behind a prefix: fa_prefix_merge_kernel goes on from here)
+    float* const to = (float*)p.o.ptr + (long long)b * p.o.sb + (long long)h * p.o.sh + (long long)q * p.o.ss;
+    if (active) *(float4*)(to + lane * 4) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (second) *(float4*)(to + lane * 4 + 128) = make_float4(acc2.x * inv, acc2.y * inv, acc2.z * inv, acc2.w * inv);
+    if (lane == 0) *(float2*)(p.out_ml + (((long long)b * p.Hq + h) * p.Sq + q) * 2) = make_float2(m_use, l);
+    return;
+  }
   char* og = (char*)p.o.ptr + ((long long)b * p.o.sb + (long long)h * p.o.sh + (long long)q * p.o.ss) * (DT == FA_F32 ? 4 : 2);
   const auto put = [&](int col, const float4& v) {
     const float f[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
@@ -388,15 +395,9 @@ struct FaPagedLaunchHost {
 struct PagedCfg {
   int RG, CG, BM, WN, slots, smem, per_sm, box, few, fr;
   bool tma, one_each;  // one_each: a CTA per segment (FA_SHORT)
-  bool eight;          // pages in 8 bits (FA_KV8)
+  bool eight, after;   // pages in 8 bits (FA_KV8), keys behind a prefix (FA_AFTER)
 };
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
-FaDiv divide_by(int d) {
-  FaDiv r{0, -1};
-  while (d > 1 && (d - 1) >> (r.shift + 1) != 0) ++r.shift;  // 2^shift < d <= 2^(shift + 1)
-  if (d > 1) r.mul = (unsigned)((1ull << (32 + r.shift)) / (unsigned)d + 1);
-  return r;
-}
 
 // Tiles, buffers and CTAs per SM (the map of fa_paged.cuh).
 //   * Rows: a warp takes 16; of 16-bit types up to 8, and 17 to 24 where the registers allow it, in the way made for few (`few` groups of 8);
@@ -420,6 +421,7 @@ void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   const bool f32 = p->dtype == FA_F32;
   const int es = esize(p->dtype);
   c.eight = p->k_scales.ptr != nullptr;
+  c.after = p->prefix_length > 0;
   c.few = c.eight ? (rows <= 8 || p->D > 128 ? 1 : rows <= 16 ? 2 : 3) : f32 ? 0 : rows <= 8 ? 1 : rows > 16 && rows <= 24 && p->D <= 128 ? 3 : 0;
   c.RG = rows <= 16 || c.few > 0 ? 1 : rows <= 32 ? 2 : 4;
   c.BM = c.few > 0 ? c.few * 8 : c.RG * 16;
@@ -471,10 +473,10 @@ int paged_workers(const PagedCfg& c) { return c.per_sm * device_sm_count(); }
 
 // (16-bit types: quotients and tanh of scores without branches, fa_score_math.cuh)
 int get_paged_kernel(fa_module* m, const fa_paged_params* p, const PagedCfg& c, Kernel** k) {
-  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.slots, 4}, {c.tma ? 1 : 0, 1}, {c.few, 2}, {c.fr, 5}, {c.CG, 4}, {c.one_each ? 1 : 0, 1}, {c.per_sm, 3}, {c.eight ? 1 : 0, 1}}), "fa_paged.cuh",
+  return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.slots, 4}, {c.tma ? 1 : 0, 1}, {c.few, 2}, {c.fr, 5}, {c.CG, 4}, {c.one_each ? 1 : 0, 1}, {c.per_sm, 3}, {c.eight ? 1 : 0, 1}, {c.after ? 1 : 0, 1}}), "fa_paged.cuh",
                     [&] { return std::string(p->dtype == FA_F32 ? "" : "#include \"fa_score_math.cuh\"\n") +
                                 defs({{"FA_DTYPE", p->dtype}, {"FA_D", p->D}, {"FA_DV", p->Dv}, {"FA_RG", c.RG}, {"FA_WN", c.WN},
-                                       {"FA_SLOTS", c.slots}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_CG", c.CG}, {"FA_SHORT", c.one_each ? 1 : 0}, {"FA_CTAS", c.per_sm}, {"FA_KV8", c.eight ? 1 : 0}}); },
+                                       {"FA_SLOTS", c.slots}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_CG", c.CG}, {"FA_SHORT", c.one_each ? 1 : 0}, {"FA_CTAS", c.per_sm}, {"FA_KV8", c.eight ? 1 : 0}, {"FA_AFTER", c.after ? 1 : 0}}); },
                     "fa_paged_kernel", c.smem, k);
 }
 
@@ -498,6 +500,12 @@ int paged_check(fa_module* m, const fa_paged_params* p, PagedCfg& c) {
   const bool eight = p->k_scales.ptr || p->v_scales.ptr;
   if (eight && !(p->k_scales.ptr && p->v_scales.ptr)) return fail(FA_EINVAL, "scales of keys and of values, or none");
   if (eight && p->dtype == FA_F32) return fail(FA_EUNSUPPORTED, "pages in 8 bits take queries of 16 bits");
+  if (p->prefix_length < 0) return fail(FA_EINVAL, "prefix_length must not be negative");
+  if (p->prefix_length > 0) {
+    if (int rc = check_tensor(p->k_prefix, "k_prefix", es)) return rc;
+    if (int rc = check_tensor(p->v_prefix, "v_prefix", es)) return rc;
+    if (p->prefix_length > 1 << 23) return fail(FA_EUNSUPPORTED, "a prefix of more than 2^23 tokens");
+  }
   if (int rc = check_tensor(p->k_pages, "k_pages", eight ? 1 : es, p->num_pages > 0)) return rc;
   if (int rc = check_tensor(p->v_pages, "v_pages", eight ? 1 : es, p->num_pages > 0)) return rc;
   pick_paged(p, c);
@@ -508,10 +516,41 @@ int paged_check(fa_module* m, const fa_paged_params* p, PagedCfg& c) {
 }
 
 size_t paged_up(size_t n) { return (n + 255) / 256 * 256; }
-size_t paged_bytes(const fa_paged_params* p, const PagedCfg& c) {
+// what the pages' part of a call needs
+size_t paged_own_bytes(const fa_paged_params* p, const PagedCfg& c) {
   if (c.one_each) return 0;
   const size_t rows = 2 * (size_t)paged_workers(c) * c.BM;
   return paged_up(rows * p->Dv * 4) + paged_up(rows * 8) + paged_up(((size_t)p->B * paged_row_tiles(p, c) + 1) * 4);
+}
+// Behind a prefix: the sums of its parts and of the pages, too
+size_t paged_bytes(const fa_paged_params* p, const PagedCfg& c) {
+  if (!c.after) return paged_own_bytes(p, c);
+  const size_t rows = (size_t)p->B * p->Hq * p->Sq;
+  return paged_own_bytes(p, c) + (size_t)(prefix_parts(p) + 1) * (paged_up(rows * p->Dv * 4) + paged_up(rows * 8));
+}
+
+// the kernels over the pages; `rows`: of the parts in the workspace
+int launch_paged(fa_module* m, const fa_paged_params* p, const PagedCfg& c, FaPagedLaunchHost& L, void* workspace, size_t rows, void* stream) {
+  FaPagedParams& k = L.p;
+  k.part_o = (float*)workspace;
+  k.part_ml = (float*)((char*)workspace + paged_up(rows * p->Dv * 4));
+  k.plan = (int*)((char*)k.part_ml + paged_up(rows * 8));
+  k.box = c.box;
+  k.by_box = divide_by(c.box);
+  Kernel* kernel = nullptr;
+  if (int rc = get_paged_kernel(m, p, c, &kernel)) return rc;
+  const dim3 block((unsigned)(c.CG * c.RG * 32));
+  if (c.one_each) return launch(kernel, dim3((unsigned)((long long)p->B * k.row_tiles * p->Hkv)), block, &L, stream);
+  if (int rc = launch(kernel, dim3((unsigned)k.workers), block, &L, stream)) return rc;
+  // Few segments for the workers: many parts each, and eight warps add up a row's.
+  const long long segments = (long long)p->B * k.row_tiles * p->Hkv;
+  const int n_rows = p->B * p->Hq * p->Sq;
+  const bool wide = k.workers / segments >= 16;
+  return rot_dispatch(p->dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    return wide ? launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 8>, dim3((unsigned)n_rows), dim3(256), stream, k, c.BM, p->Dv, n_rows)
+                : launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 1>, dim3((unsigned)((n_rows + 3) / 4)), dim3(128), stream, k, c.BM, p->Dv, n_rows);
+  });
 }
 
 }  // namespace
@@ -647,25 +686,25 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
   k.by_tiles = divide_by(k.row_tiles);
   k.workers = paged_workers(c);
   const size_t rows = 2 * (size_t)k.workers * c.BM;
-  k.part_o = (float*)workspace;
-  k.part_ml = (float*)((char*)workspace + paged_up(rows * p->Dv * 4));
-  k.plan = (int*)((char*)k.part_ml + paged_up(rows * 8));
-  k.box = c.box;
-  k.by_box = divide_by(c.box);
-  Kernel* kernel = nullptr;
-  if (int rc = get_paged_kernel(m, p, c, &kernel)) return rc;
-  const dim3 block((unsigned)(c.CG * c.RG * 32));
-  if (c.one_each) return launch(kernel, dim3((unsigned)((long long)p->B * k.row_tiles * p->Hkv)), block, &L, stream);
-  if (int rc = launch(kernel, dim3((unsigned)k.workers), block, &L, stream)) return rc;
-  // Few segments for the workers: many parts each, and eight warps add up a row's.
-  const long long segments = (long long)p->B * k.row_tiles * p->Hkv;
-  const int n_rows = p->B * p->Hq * p->Sq;
-  const bool wide = k.workers / segments >= 16;
-  return rot_dispatch(p->dtype, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    return wide ? launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 8>, dim3((unsigned)n_rows), dim3(256), stream, k, c.BM, p->Dv, n_rows)
-                : launch_here("fa_paged_combine_kernel", fa_paged_combine_kernel<DT, 1>, dim3((unsigned)((n_rows + 3) / 4)), dim3(128), stream, k, c.BM, p->Dv, n_rows);
-  });
+  if (c.after) {
+    // the prefix first: its kernel has the most to do, and the pages' begins while it ends
+    char* at = (char*)workspace;
+    const size_t all = (size_t)p->B * p->Hq * p->Sq, parts = (size_t)prefix_parts(p);
+    const auto take = [&](size_t n) {
+      char* r = at;
+      at += paged_up(n);
+      return (float*)r;
+    };
+    float *const po = take(parts * all * p->Dv * 4), *const pml = take(parts * all * 8), *const own = take(all * p->Dv * 4);
+    k.out_ml = take(all * 8);
+    k.after = p->prefix_length;
+    k.o = FaTensor{own, (long long)p->Hq * p->Sq * p->Dv, (long long)p->Sq * p->Dv, p->Dv};
+    workspace = at;
+    if (int rc = launch_prefix(m, p, po, pml, stream)) return rc;
+    if (int rc = launch_paged(m, p, c, L, workspace, rows, stream)) return rc;
+    return launch_prefix_merge(p, po, pml, own, k.out_ml, (int)parts, stream);
+  }
+  return launch_paged(m, p, c, L, workspace, rows, stream);
 }
 
 }  // extern "C"

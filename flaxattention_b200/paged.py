@@ -87,10 +87,18 @@ def read_pages(key_pages, value_pages, block_table, starts, num_tokens: int, *, 
     return native().read_pages(key_pages, value_pages, block_table, starts, num_tokens, key_scales, value_scales, dtype, not bhln)
 
 
+def known_mods(score_mod, mask_mod, device):
+    """(handle, buffers) of mods that the native path does not know yet, or that capture tensors elsewhere than on `device`."""
+    module = module_for(score_mod, mask_mod)
+    lowered = lower_mods(None if score_mod is identity_score else score_mod, None if mask_mod is noop_mask else mask_mod)
+    return module.handle.value, tuple(device_buffers(lowered, device))
+
+
 def paged_attention(query, key_pages, value_pages, block_table, lengths, score_mod: Optional[Callable] = None,
                     mask_mod: Optional[Callable] = None, *, window: Optional[int] = None, sm_scale: Optional[float] = None,
                     bhln: bool = True, return_lse: bool = False, b_offset: int = 0, h_offset: int = 0,
-                    kernel_options: Optional[dict] = None, key_scales=None, value_scales=None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+                    kernel_options: Optional[dict] = None, key_scales=None, value_scales=None,
+                    prefix: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Attention of the newest tokens of each request over its pages.
 
     ``query`` ``[B, Hq, Sq, D]`` (``bhln=False``: ``[B, Sq, Hq, D]``) holds the last ``Sq`` tokens of each request, ``lengths`` (int32 ``[B]``) counts
@@ -109,16 +117,19 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, score_m
     table entry that is no page, or a length beyond the table, leaves the keys out, and the next call raises ``FlaxAttnError``
     (``check_status``).  Meant for a few tokens per request; there is no gradient.  ``kernel_options``: ``{"kernels": "general"}`` takes keys and values in
     16-byte pieces where TMA would do.
+
+    With ``key_scales`` and ``value_scales`` (float32 ``[pages, kv heads, page_size]``) the pages are in 8 bits, as ``rotary_append`` writes them, and queries float16 or
+    bfloat16.  A scale that is no number makes the rows that see its token that.
+
+    ``prefix``: keys and values ``[1, kv heads, tokens, D]`` (``bhln=False``: ``[1, tokens, kv heads, D]``) that all requests begin with, in front of those in
+    their pages, of the queries' dtype also where the pages are in 8 bits (``read_pages`` takes them out of pages).  They are read once for all requests, not
+    once for each.  ``lengths`` still counts what lies in the pages; a query's token is ``p = tokens + lengths[b] - Sq + i``, for the mods and the window too.
     """
     general = kernel_options is not None and kernel_options.get("kernels") == "general"
     call = native().paged_attention
     res = call(query, key_pages, value_pages, block_table, lengths, score_mod, mask_mod, window, sm_scale, not bhln, return_lse, b_offset,
-               h_offset, general, key_scales, value_scales, None)
+               h_offset, general, key_scales, value_scales, prefix, None)
     if res is None:
-        # mods that are not known yet, or tensors that they capture elsewhere than the query
-        module = module_for(score_mod, mask_mod)
-        lowered = lower_mods(None if score_mod is identity_score else score_mod, None if mask_mod is noop_mask else mask_mod)
-        buffers = tuple(device_buffers(lowered, query.device))
         res = call(query, key_pages, value_pages, block_table, lengths, score_mod, mask_mod, window, sm_scale, not bhln, return_lse, b_offset,
-                   h_offset, general, key_scales, value_scales, (module.handle.value, buffers))
+                   h_offset, general, key_scales, value_scales, prefix, known_mods(score_mod, mask_mod, query.device))
     return res

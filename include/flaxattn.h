@@ -362,11 +362,37 @@ typedef struct fa_paged_params {
   /* pages in 8 bits (int8, strides in bytes; queries of 16 bits), as fa_rotary_append writes them: the scales, float32, by the strides of page, head
    * and token in a page.  ptr NULL: pages of the queries' type. */
   fa_tensor k_scales, v_scales;
+  /* Tokens that all requests begin with, in front of those in their pages: keys and values [Hkv, prefix_length] by the strides of head and token, of the
+   * queries' type.  lengths, as before, counts what lies in the pages; the mods and the window see the prefix in front of it.  0: none. */
+  int32_t prefix_length;
+  fa_tensor k_prefix, v_prefix;
 } fa_paged_params;
 size_t fa_paged_workspace_bytes(const fa_paged_params* p);
 int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t workspace_bytes, void* stream);
 /* Compiles (or fetches from the cache) the kernel that a call of these sizes, type, page_size and flags runs.  Needs no GPU. */
 int fa_paged_prepare(fa_module* m, const fa_paged_params* p);
+
+/* Causal attention of prompts laid end to end, or of pieces of them.  Queries starts[b] .. starts[b + 1] - 1 of `tokens` are those of request b, keys
+ * key_starts[b] .. of `keys` its keys (starts [B + 1], never decreasing; NULL key_starts: as starts); its last query is its last key's token.  A query sees the
+ * keys of its request up to itself, at most `window` behind it, and those that mask_mod keeps; the mods see the places in the request.  Rows that see nothing, and those of no
+ * request, are 0 with an lse of -inf.  Nothing depends on a length on the host. */
+typedef struct fa_prompt_params {
+  int32_t dtype;
+  int32_t B, Hq, Hkv, D, Dv;
+  int64_t tokens, keys;
+  float scale;
+  int32_t b_offset, h_offset;
+  fa_tensor q, k, v, o;       /* stride_h of a head, stride_s of a token */
+  const int32_t* starts;
+  const int32_t* key_starts;
+  int32_t window;             /* below 0: no window */
+  float* lse;                 /* [Hq, tokens] natural-log logsumexp or NULL */
+  int32_t flags;              /* FA_FLAG_GENERAL_KERNELS: not the tcgen05 kernel */
+  int32_t* status;            /* optional status word: 32 = starts that decrease or lie beyond the tokens (what lies beyond is left out) */
+} fa_prompt_params;
+int fa_prompt(fa_module* m, const fa_prompt_params* p, void* stream);
+/* Compiles (or fetches from the cache) the kernel that a call of these sizes, type and flags runs.  Needs no GPU. */
+int fa_prompt_prepare(fa_module* m, const fa_prompt_params* p);
 
 #ifdef __cplusplus
 }

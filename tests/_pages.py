@@ -126,3 +126,44 @@ class Cache8(Cache):
     @property
     def scales(self):
         return dict(key_scales=self.k_scales, value_scales=self.v_scales)
+
+
+class Prompts:
+    """Requests of `lengths` new tokens behind `past` others, laid end to end; rows of no request (`pad` in front and behind) are NaN."""
+
+    def __init__(self, seed, lengths, Hq, Hkv, D, dtype, Dv=None, past=None, pad=(0, 0), bhln=True, device="cuda"):
+        rng = np.random.default_rng(seed)
+        Dv = D if Dv is None else Dv
+        self.lengths, self.dtype, self.pad, self.bhln = lengths, dtype, pad, bhln
+        total = [n + p for n, p in zip(lengths, past or [0] * len(lengths))]
+        self.queries = [normal(rng, Hq, n, D, dtype=dtype) for n in lengths]
+        self.keys = [normal(rng, Hkv, n, D, dtype=dtype) for n in total]
+        self.values = [normal(rng, Hkv, n, Dv, dtype=dtype) for n in total]
+        self.starts, self.key_starts = (torch.tensor([pad[0]] + [int(x) for x in pad[0] + np.cumsum(n)], dtype=torch.int32, device=device) for n in (lengths, total))
+        self.q, self.k, self.v = (self.laid(x, device) for x in (self.queries, self.keys, self.values))
+        self.past = past is not None
+
+    def laid(self, parts, device):
+        front, back = (torch.full((parts[0].shape[0], n, parts[0].shape[2]), math.nan, dtype=self.dtype) for n in self.pad)
+        x = torch.cat([front, *parts, back], 1)[None]
+        return (x if self.bhln else x.transpose(1, 2).contiguous()).to(device)
+
+    def want(self, score=None, mask=None, window=None, scale=None):
+        """The definition in 64 bits: (out, lse, spread, top) of all requests' rows."""
+        outs, top = [], 1.0
+        for b, (q, k, v) in enumerate(zip(self.queries, self.keys, self.values)):
+            f = None if score is None else lambda x, _, h, i, j: score(x, torch.tensor(b), h, i, j)  # noqa: B023
+            g = None if mask is None else lambda _, h, i, j: mask(torch.tensor(b), h, i, j)  # noqa: B023
+            *r, t = attend(q[None], [k], [v], f, g, window, scale)
+            outs.append([x[0] for x in r])
+            top = max(top, t)
+        return (*(torch.cat([o[i] for o in outs], 1)[None] for i in range(3)), top)
+
+    def check(self, out, lse, want):
+        front, back = self.pad
+        if not self.bhln:
+            out = out.transpose(1, 2)
+        n = sum(self.lengths)
+        for t, nothing in ((out, 0.0), (lse[..., None], -math.inf)):
+            assert (t[:, :, :front] == nothing).all() and (t[:, :, front + n:] == nothing).all()
+        check_attention(out[:, :, front: front + n], lse[:, :, front: front + n], want, self.dtype)

@@ -1,0 +1,226 @@
+"""prompt_attention against its definition in 64 bits: types, head layouts, lengths around tiles, pieces of prompts, windows and mods, rows of no request."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import flaxattention_b200 as fa
+from _pages import Prompts
+from _util import DTYPES
+
+pytestmark = pytest.mark.gpu
+
+
+def run(seed, lengths, Hq, Hkv, D, dtype, score=None, mask=None, window=None, scale=None, kernels=None, **kw):
+    p = Prompts(seed, lengths, Hq, Hkv, D, DTYPES[dtype], **kw)
+    out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, score, mask, key_starts=p.key_starts if p.past else None, window=window, sm_scale=scale, bhln=p.bhln,
+                                   return_lse=True, kernel_options={"kernels": kernels} if kernels else None)
+    assert out.dtype == p.dtype and lse.dtype == torch.float32
+    p.check(out, lse, p.want(score, mask, window, scale))
+    torch.cuda.synchronize()
+    fa.check_status()
+    return out
+
+
+LENGTHS = [5, 0, 1, 63, 64, 65, 0, 127, 128, 129, 255, 256, 257, 300]
+
+
+@pytest.mark.parametrize("kernels", [None, "general"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,Hkv", [(2, 2), (4, 1), (6, 2)])
+def test_lengths_and_heads(kernels, dtype, D, Hq, Hkv):
+    run(1, LENGTHS, Hq, Hkv, D, dtype, kernels=kernels, pad=(3, 7))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("D,Dv", [(16, 16), (32, 16), (48, 48), (80, 80), (96, 96), (96, 32), (112, 64), (128, 64), (192, 128), (256, 256), (256, 16)])
+def test_head_dims(dtype, D, Dv):
+    run(2, [1, 40, 333], 4, 2, D, dtype, Dv=Dv)
+
+
+@pytest.mark.parametrize("G", [1, 3, 5, 7, 8, 12, 32, 130])
+def test_groups(G):
+    run(3, [1, 33, 140], G, 1, 64, "bf16")
+
+
+@pytest.mark.parametrize("kernels", [None, "general"])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("bhln", [True, False])
+def test_pieces(kernels, D, bhln):
+    """Queries behind keys that were there before; also fewer keys than queries, whose first then see nothing."""
+    run(4, [1, 2, 130, 64, 7], 4, 2, D, "bf16", past=[500, 0, 126, 64, 3], bhln=bhln, kernels=kernels)
+    p = Prompts(5, [40, 9], 4, 2, D, torch.float16, bhln=bhln)
+    short = torch.tensor([0, 15, 20], dtype=torch.int32, device="cuda")
+    out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, key_starts=short, bhln=bhln, return_lse=True)
+    full_k, full_v = (torch.cat(x, 1) for x in (p.keys, p.values))
+    p.keys, p.values = ([x[:, :15], x[:, 15:20]] for x in (full_k, full_v))
+    p.check(out, lse, p.want())
+    assert torch.isneginf(lse[0, :, :25]).all() and torch.isfinite(lse[0, :, 25:40]).all()
+
+
+def softcap(score, b, h, q_idx, kv_idx):
+    return 5.0 * torch.tanh(score / 5.0)
+
+
+def distance(score, b, h, q_idx, kv_idx):
+    return score - (q_idx - kv_idx) * torch.exp2((h + 1) * -0.5)
+
+
+def of_request(score, b, h, q_idx, kv_idx):
+    return score * (b + 1) * 0.5
+
+
+def parity(b, h, q_idx, kv_idx):
+    return (q_idx + kv_idx + h + b) % 2 == 0
+
+
+def nothing(b, h, q_idx, kv_idx):
+    return (kv_idx < 0) & (q_idx < 0)
+
+
+def no_odd_head(b, h, q_idx, kv_idx):
+    return (h % 2 == 0) & (kv_idx >= 0)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("score", [None, softcap, distance, of_request])
+@pytest.mark.parametrize("mask", [None, parity, nothing, no_odd_head])
+def test_mods(dtype, score, mask):
+    run(6, [1, 70, 400, 200], 4, 2, 64, dtype, score=score, mask=mask)
+    run(6, [1, 70, 400], 4, 2, 128, dtype, score=score, mask=mask, past=[3, 200, 0])
+
+
+@pytest.mark.parametrize("kernels", [None, "general"])
+@pytest.mark.parametrize("window", [0, 1, 63, 64, 127, 128, 129, 300, 5000, 2 ** 31])
+@pytest.mark.parametrize("D", [64, 128])
+def test_windows(kernels, window, D):
+    run(7, [1, 3, 129, 700], 4, 1, D, "bf16", window=window, kernels=kernels)
+    run(8, [40, 200], 2, 2, D, "f16", window=window, kernels=kernels, past=[300, 100], score=distance)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+def test_scales(D, scale):
+    run(9, [100, 30], 2, 1, D, "f16", scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_other_requests_may_hold_anything(dtype, D):
+    p = Prompts(10, [130, 100, 50], 2, 2, D, DTYPES[dtype])
+    a, b = 130, 230
+    p.k[:, :, a:b], p.v[:, :, a:b], p.q[:, :, a:b] = math.nan, math.inf, -math.inf
+    out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, return_lse=True)
+    want = p.want()
+    keep = torch.cat([torch.arange(a), torch.arange(b, 280)])
+    from _pages import check_attention
+    check_attention(out.cpu()[:, :, keep], lse.cpu()[:, :, keep], (*(x[:, :, keep] for x in want[:3]), want[3]), p.dtype)
+
+
+def test_many_requests():
+    """More requests than a warp keeps, most of them of no tokens."""
+    rng = np.random.default_rng(11)
+    lengths = [int(rng.integers(0, 40)) if b % 3 == 0 else 0 for b in range(700)]
+    lengths[500] = 600
+    run(12, lengths, 2, 1, 64, "bf16")
+    run(12, lengths, 2, 1, 128, "f32")
+
+
+def test_nothing_there():
+    q = torch.zeros(1, 2, 0, 64, device="cuda", dtype=torch.float16)
+    starts = torch.zeros(4, dtype=torch.int32, device="cuda")
+    assert fa.prompt_attention(q, q, q, starts).shape == (1, 2, 0, 64)
+    # tokens, but no requests, or none with tokens; queries without keys
+    q = torch.full((1, 2, 300, 64), math.nan, device="cuda", dtype=torch.float16)
+    for s in (torch.zeros(1, dtype=torch.int32, device="cuda"), starts, starts + 7):
+        out, lse = fa.prompt_attention(q, q, q, s, return_lse=True)
+        assert (out == 0).all() and torch.isneginf(lse).all()
+    out, lse = fa.prompt_attention(q, q[:, :, :0], q[:, :, :0], torch.tensor([0, 300], dtype=torch.int32, device="cuda"), key_starts=starts[:2], return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    torch.cuda.synchronize()
+    fa.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("starts", [[0, 50, 20, 100], [0, 30, 500, 100], [-5, 30, 60, 100], [70, 10, 2 ** 31 - 1, -2 ** 31]])
+def test_broken_starts(dtype, starts):
+    """Cut to what is there, and reported."""
+    p = Prompts(13, [100], 2, 1, 64, DTYPES[dtype])
+    fa.prompt_attention(p.q, p.k, p.v, torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    with pytest.raises(fa._cabi.FlaxAttnError, match="starts"):
+        fa.check_status()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_strides(D):
+    """Parts of one projection, read by their strides; rows of 16 bytes beside each other and not."""
+    lengths = [100, 30, 61]
+    p = Prompts(14, lengths, 4, 2, D, torch.bfloat16, bhln=False)
+    qkv = torch.cat([p.q, p.k, p.v], 2)
+    q, k, v = qkv.split([4, 2, 2], 2)
+    out, lse = fa.prompt_attention(q, k, v, p.starts, bhln=False, return_lse=True)
+    p.check(out, lse, p.want())
+    wide = torch.zeros(1, 191, 2, 2 * D + 8, dtype=torch.bfloat16, device="cuda")
+    wide[..., 8: D + 8], wide[..., D + 8:] = p.k, p.v
+    out2, _ = fa.prompt_attention(q, wide[..., 8: D + 8], wide[..., D + 8:], p.starts, bhln=False, return_lse=True)
+    assert torch.equal(out, out2)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_long_prompt(D):
+    run(15, [3000], 2, 1, D, "bf16")
+
+
+def test_offsets_and_captured_tensors():
+    """b and h as the mods see them, and a mod over a tensor."""
+    bias = torch.randn(8, 4, generator=torch.Generator().manual_seed(0))
+    on_gpu = bias.cuda()
+
+    def by_table(score, b, h, q_idx, kv_idx):
+        return score + on_gpu[b, h]
+
+    p = Prompts(16, [70, 150], 2, 1, 64, torch.float16)
+    out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, by_table, return_lse=True, b_offset=5, h_offset=2)
+    p.check(out, lse, p.want(lambda x, b, h, i, j: x + bias[b + 5, h + 2]))
+
+
+def test_graph_and_stream():
+    """Captured once, replayed over other lengths; on another stream than the current one's."""
+    p = Prompts(17, [200, 90, 40], 4, 2, 128, torch.bfloat16)
+    fa.prompt_attention(p.q, p.k, p.v, p.starts)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, return_lse=True)
+        graph.replay()
+    side.synchronize()
+    p.check(out, lse, p.want())
+    p.lengths = [10, 300, 20]
+    cut = torch.tensor(p.lengths).cumsum(0)[:-1]
+    p.queries, p.keys, p.values = ([x.contiguous() for x in torch.cat(t, 1).tensor_split(cut, 1)] for t in (p.queries, p.keys, p.values))
+    p.starts.copy_(torch.tensor([0, 10, 310, 330], dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    p.check(out, lse, p.want())
+
+
+def test_refusals():
+    p = Prompts(18, [20, 30], 4, 2, 64, torch.float16)
+    call = lambda **kw: fa.prompt_attention(*({"query": p.q, "key": p.k, "value": p.v, "starts": p.starts} | kw).values()) if "key_starts" not in kw else None  # noqa: E731
+    call()
+    for kw, match in ((dict(query=torch.cat([p.q, p.q])), "batch dimension"), (dict(query=p.q[..., :48]), "embedding"), (dict(key=p.k[:, :, :40], value=p.v[:, :, :40]), "key_starts"),
+                      (dict(value=p.v[:, :, :40]), "same heads and sequence"), (dict(starts=p.starts.long()), "starts"), (dict(starts=p.starts[::2]), "starts"),
+                      (dict(starts=p.starts[:0]), "starts"), (dict(query=p.q[:, :3]), "multiple"), (dict(key=p.k.float()), "dtype"), (dict(query=p.q.clone().requires_grad_()), "no gradient")):
+        with pytest.raises(ValueError, match=match):
+            call(**kw)
+    with pytest.raises(ValueError, match="window"):
+        fa.prompt_attention(p.q, p.k, p.v, p.starts, window=-1)
+    with pytest.raises(ValueError, match="key_starts"):
+        fa.prompt_attention(p.q, p.k, p.v, p.starts, key_starts=p.key_starts[:2])
+    with pytest.raises(fa._cabi.FlaxAttnError, match="16"):
+        fa.prompt_attention(p.q[..., :60], p.k[..., :60], p.v[..., :60], p.starts)
