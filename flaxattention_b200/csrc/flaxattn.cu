@@ -192,7 +192,7 @@ const char* const kDefaultMods =
 
 // A kernel variant of a module as a number: every launch looks its kernel up by it, and the define text
 // is only put together when the variant has to be compiled or fetched from the cache on disk.
-enum KernelId : int { kIdFwd, kIdFwdRerun, kIdBwdRerun, kIdFwdTc, kIdBwdDq, kIdBwdDkdv, kIdBwdTc, kIdBwdF32, kIdDecode, kIdMaskScan, kIdMaskClassify, kIdSelftest, kIdPaged, kIdPacked };
+enum KernelId : int { kIdFwd, kIdFwdRerun, kIdBwdRerun, kIdFwdTc, kIdBwdDq, kIdBwdDkdv, kIdBwdTc, kIdBwdF32, kIdDecode, kIdMaskScan, kIdMaskClassify, kIdSelftest, kIdPaged, kIdPacked, kIdPackedTc };
 uint64_t kernel_key(KernelId id, std::initializer_list<std::pair<int, int>> fields) {  // (value, bits)
   uint64_t k = 0;
   for (auto& f : fields) k = (k << f.second) | (uint64_t)f.first;

@@ -46,18 +46,39 @@
 // Every mbarrier wait is bounded; on expiry the CTA raises FA_STATUS_WAIT_TIMEOUT in the
 // status word, all roles leave their loops, TMEM is freed and the kernel returns.
 //
+// Requests of different lengths (FA_TC_PACKED, fa_packed_rows.cuh): 1, prompts laid end to end; 2, the newest tokens of many requests over a prefix that they
+// share, a part of it per CTA (kv heads, row tiles, parts).  A row is a (token, head of the group): its query is loaded and its result
+// stored by the threads of its warp, and the steps are those of the keys that any row sees, with no tables: a tile that all rows see whole is a
+// plain step, another one applies each row's range of keys.  K and V are read as [tokens, heads] by one map each; what the last tile of a
+// request has behind its keys is the next request's, perhaps no number, so the idle warp writes zeros over those rows of V.  Head dims below FA_D are
+// filled up with zeros by the loads.
+//
 // Compile-time parameters (macros): FA_DTYPE (0 fp16, 1 bf16, 2 fp32), FA_D (64 or 128), FA_TC_DECODE
-// (split-KV variant, see below), FA_TC_NQ (query tiles of a CTA, see below).
+// (split-KV variant, see below), FA_TC_NQ (query tiles of a CTA, see below), FA_TC_PACKED.
 #pragma once
 #include "fa_sm100.cuh"
-
+#ifndef FA_TC_PACKED
+#define FA_TC_PACKED 0
+#endif
+#if FA_TC_PACKED
+#include "fa_packed_rows.cuh"
+struct FaTcParams {
+  FaPackedParams p;
+  FaTensorMap tk, tv;  // 4-d maps (D, token, H, 1), box 64 x 128 x 1 x 1, 128-byte swizzle
+};
+typedef FaPackedParams FaTcProblem;
+#else
 struct FaTcParams {
   FaParams p;
   FaTensorMap tq, tk, tv;  // 4-d maps (D, S, H, B), box 64 x 128 x 1 x 1, 128-byte swizzle
   FaTensorMap to;          // the output, like tq (unused by the decode variant, which writes partial results)
 };
+typedef FaParams FaTcProblem;
+#endif
 
 namespace fa_tc {
+
+constexpr bool PACKED = FA_TC_PACKED != 0, PREFIX = FA_TC_PACKED == 2;
 
 constexpr bool F32 = FA_DTYPE == FA_DT_F32;
 constexpr int DT = F32 ? FA_DT_BF16 : FA_DTYPE;  // type of the tensor-core operands
@@ -96,7 +117,7 @@ constexpr int NSTAGE = DECODE ? 5 : (F32 ? 1 : (D == 64 ? NQ + 1 : NQ));
 constexpr int Q_BYTES = NQ * ATOMS * ATOM_BYTES;
 constexpr int KV_STAGE = ATOMS * ATOM_BYTES;
 constexpr int MAXT = 256;                // kv tiles per row of the block grid (Skv <= 32768)
-constexpr int NBARS = 1 + 4 * NSTAGE + 13;
+constexpr int NBARS = 1 + 4 * NSTAGE + 13 + (PACKED ? 1 : 0);
 constexpr int OFF_K = Q_BYTES;
 constexpr int OFF_V = OFF_K + NSTAGE * KV_STAGE;
 constexpr int OFF_BAR = OFF_V + NSTAGE * KV_STAGE;
@@ -158,6 +179,7 @@ constexpr int BAR_S = 1 + 4 * NSTAGE, BAR_P = BAR_S + 2, BAR_O = BAR_S + 6;
 // the softmax warps hold the scores in registers, and S of the next step is produced during the softmax.
 constexpr int BAR_SFREE2 = BAR_S + 10;
 constexpr int BAR_LAG = BAR_S + 12;  // (ROT) the first PV product of the second tile is complete; used once
+constexpr int BAR_TAIL = BAR_S + 13;  // (PACKED) the last tile of V has come, and waits for zeros behind its keys; used once
 constexpr bool EARLY_S = ROT || DECODE;
 // Head dim 128: P is handed over in two parts, keys 0-95 (BAR_P) and 96-127 (BAR_P2), so that most of the PV product
 // runs under the last exponentials.  It is the first link of the chain PV(j), S(j+1) that the tile then waits for.
@@ -256,6 +278,66 @@ __device__ __forceinline__ void mask_bits(fa_u32 (&w)[NW], bool use_mask, int kv
   }
 #endif
 }
+#if FA_TC_PACKED
+// the same for a row that sees the keys from `from` to `to` - 1
+template <int NW>
+__device__ __forceinline__ void range_bits(fa_u32 (&w)[NW], int kv0, int from, int to, int qi, int gb, int gh) {
+  const auto upto = [](int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : ((1u << n) - 1u)); };
+#pragma unroll
+  for (int c = 0; c < NW; ++c) w[c] = upto(to - (kv0 + 32 * c)) & ~upto(from - (kv0 + 32 * c));
+#if FA_HAS_MASK_MOD
+  fa_u32 m[NW];
+#pragma unroll
+  for (int c = 0; c < NW; ++c) m[c] = 0u;
+#pragma unroll 2
+  for (int e = 0; e < 32; ++e) {
+#pragma unroll
+    for (int c = 0; c < NW; ++c) m[c] |= (fa_mask_mod(gb, gh, qi, kv0 + 32 * c + e) ? 1u : 0u) << e;
+  }
+#pragma unroll
+  for (int c = 0; c < NW; ++c) w[c] &= m[c];
+#endif
+}
+// What a CTA works on, in shared memory: its rows, and the kv tiles of its steps, from `first` on.  Of a query tile those that a row of it sees (x to y - 1), and
+// of these the ones that all rows see whole (z to w - 1).
+struct Plan {
+  int4 tile[NQ];
+  int first, nsteps, beyond;  // beyond: rows of the last tile of V that are the next request's
+  FaPlace place;
+  __device__ __forceinline__ static fa_u32 mode(const int4& b, int t) { return t < b.x || t >= b.y ? 0u : t >= b.z && t < b.w ? 2u : 1u; }
+  __device__ __forceinline__ fa_u32 word(int j) const {  // as in the schedule
+    const int t = first + j;
+    fa_u32 w = (fa_u32)t;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) w |= mode(tile[i], t) << (16 + 8 * i);
+    return w;
+  }
+  __device__ __forceinline__ void set(int i, const FaPackedParams& p, int from, int to, int all_from, int all_to) {
+    tile[i] = make_int4(to > 0 ? from / BN : 0, (to + BN - 1) / BN, (all_from + BN - 1) / BN, FA_HAS_MASK_MOD ? 0 : min(all_to, p.keys) / BN);
+  }
+  __device__ __forceinline__ void finish(const FaPackedParams& p) {
+    int last = 0;
+    first = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      if (tile[i].x < tile[i].y) first = min(first, tile[i].x);
+      last = max(last, tile[i].y);
+    }
+    if (last == 0) first = 0;
+    if (PREFIX) {  // this CTA's part
+      const int per = (last - first + p.splits - 1) / p.splits;
+      first = min(first + (int)blockIdx.z * per, last);
+      last = min(first + per, last);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) tile[i].y = min(tile[i].y, last);
+    }
+    nsteps = last - first;
+    beyond = PREFIX || nsteps == 0 ? 0 : max(last * BN - place.nk, 0);
+  }
+};
+constexpr int OFF_PLAN = (OFF_SCHED + 15) / 16 * 16;
+static_assert(OFF_PLAN + (int)sizeof(Plan) <= OFF_CLS, "the plan takes the place of the schedule");
+#endif
 // the words of a row of the bit matrix for the NW * 32 keys from kv0 on
 template <int NW>
 __device__ __forceinline__ uint4 mask_words(const unsigned* rowbits, int kv0) {
@@ -281,7 +363,7 @@ __device__ __forceinline__ void pass2_part(const float (&v)[32], fa_u32 (&pk)[16
     // and SM) is what bounds this loop
     float p0, p1;
     if (FA_TC_POLY_EVERY > 0 && (e % (FA_TC_POLY_EVERY > 0 ? FA_TC_POLY_EVERY : 1)) == (FA_TC_POLY_EVERY - 1)) {
-      fa_ex2_poly2(a0, a1, p0, p1);
+      fa_ex2_poly2<PACKED>(a0, a1, p0, p1);
     } else {
       p0 = fa_ex2(a0);
       p1 = fa_ex2(a1);
@@ -301,7 +383,7 @@ __device__ __forceinline__ void pass2_chunk(const float (&v)[32], fa_u32 (&pk)[1
 
 // State of one softmax warpgroup thread that a kv step reads and updates.
 struct SoftmaxCtx {
-  const FaParams& p;
+  const FaTcProblem& p;
   fa_u32 sb, t_s, t_o, t_p;
   int i, warp, qi, gb, gh;
   int half;  // decode variant: which 64 kv columns of a tile this thread owns (0 in the forward)
@@ -311,6 +393,7 @@ struct SoftmaxCtx {
   fa_u32 cnt;
   const unsigned* rowbits;  // this query row of the mask bit matrix, or null
   ModLinear lin;            // a score_mod that is linear over kv
+  int from, to;             // (PACKED) keys that the row sees
 };
 
 // One kv step of this warpgroup's tile.  The few tiles that need mask_mod or end beyond the
@@ -322,7 +405,7 @@ struct SoftmaxCtx {
 template <int VARIANT>
 __device__ __forceinline__ bool softmax_step(SoftmaxCtx& c, const int tile, const int mode, const bool masked_rt) {
   const bool masked = VARIANT == 2 ? masked_rt : VARIANT == 1;
-  const FaParams& p = c.p;
+  const FaTcProblem& p = c.p;
   const fa_u32 sb = c.sb, t_o = c.t_o;
   const int i = c.i, qi = c.qi, gb = c.gb, gh = c.gh;
   const float sc2 = c.sc2;
@@ -352,7 +435,7 @@ __device__ __forceinline__ bool softmax_step(SoftmaxCtx& c, const int tile, cons
   const float m_base = m_ref >= REL_FLOOR ? m_ref : 0.f;
 #endif
   const bool use_mask = FA_HAS_MASK_MOD && mode == 1;
-  const bool have_words = masked && use_mask && c.rowbits != nullptr;
+  const bool have_words = !PACKED && masked && use_mask && c.rowbits != nullptr;
   uint4 words = make_uint4(0u, 0u, 0u, 0u);
   // The mask words are on their way during the wait for the scores; not where few of many steps are partial (two tiles at head dim 64), where
   // they cost registers in every step
@@ -398,7 +481,11 @@ __device__ __forceinline__ bool softmax_step(SoftmaxCtx& c, const int tile, cons
     // (the row maximum taken on the way is of the unmasked scores: it is taken again)
     fa_u32 keep[DECODE ? 2 : 4];
     if (LATE_WORDS && have_words) words = mask_words<DECODE ? 2 : 4>(c.rowbits, n0);
+#if FA_TC_PACKED
+    range_bits(keep, n0, c.from, c.to, qi, gb, gh);
+#else
     mask_bits(keep, use_mask, n0, qi, gb, gh, p.Skv, have_words, words);
+#endif
     mask_apply(s0, keep[0]);
     mask_apply(s1, keep[1]);
     rm = {FA_NEG_INF, FA_NEG_INF, FA_NEG_INF, FA_NEG_INF};
@@ -624,9 +711,14 @@ __device__ __forceinline__ bool softmax_step_f32(SoftmaxCtx& c, float (&acc)[D],
 
 }  // namespace fa_tc
 
-extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) fa_fwd_tc_kernel(const __grid_constant__ FaTcParams P) {
+#if FA_TC_PACKED
+#define FA_TC_KERNEL fa_packed_tc_kernel
+#else
+#define FA_TC_KERNEL fa_fwd_tc_kernel
+#endif
+extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) FA_TC_KERNEL(const __grid_constant__ FaTcParams P) {
   using namespace fa_tc;
-  const FaParams& p = P.p;
+  const FaTcProblem& p = P.p;
   extern __shared__ unsigned char smem_raw[];
   // a launch that does not fit the shared-memory map below (a host library built for another
   // version of this file) is refused before anything is written
@@ -641,6 +733,89 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
   unsigned char* sm = smem_raw + (sb - raw);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* misc = (volatile int*)(sm + OFF_MISC);  // [0] tmem base, [1] abort, [2] nsteps
+#if FA_TC_PACKED
+  // ---- set-up: this CTA's rows, barriers, TMEM, the steps ------------------------------------
+  const int hk = blockIdx.x, G = p.Hq / p.Hkv;
+  Plan* const plan = (Plan*)(sm + OFF_PLAN);
+  int* const bounds = (int*)(sm + OFF_CLS);  // (prefix) of each query tile: first key that a row sees, one behind the last, the same of what all see
+  if (warp == 0) {
+    if (PREFIX) {
+      if (lane < 4 * NQ) bounds[lane] = (lane & 3) == 0 || (lane & 3) == 3 ? 0x7fffffff : 0;
+      if (lane == 0) plan->place = {0, p.tokens, 0, p.keys, 0, (int)blockIdx.y * NQ * BM, 1};
+    } else {
+      const FaPlace at = fa_find_item<NQ * BM>(p, (long long)blockIdx.z * gridDim.y + blockIdx.y);
+      if (lane == 0) {
+        plan->place = at;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          // rows are in the order of their tokens: the first and the last of the tile have the bounds
+          const int r0 = at.first + i * BM, r1 = min(r0 + BM, at.n * G) - 1;
+          const FaRow a = fa_row<PREFIX>(p, at, r0), z = fa_row<PREFIX>(p, at, max(r1, r0));
+          plan->set(i, p, a.from, r1 >= r0 ? z.to : 0, z.from, a.to);
+        }
+        plan->finish(p);
+      }
+    }
+  }
+  if (!PREFIX && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && warp >= 4) fa_check_starts(p, tid - 128, NT - 128);
+  if (tid == 32) {
+    fa_mbar_init(bar_addr(sb, BAR_Q), NSOFT);
+    for (int s = 0; s < NSTAGE; ++s) {
+      fa_mbar_init(bar_addr(sb, BAR_KFULL + s), 1);
+      fa_mbar_init(bar_addr(sb, BAR_KEMPTY + s), ROT ? NQ : 1);
+      fa_mbar_init(bar_addr(sb, BAR_VFULL + s), 1);
+      fa_mbar_init(bar_addr(sb, BAR_VEMPTY + s), ROT ? NQ : 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      fa_mbar_init(bar_addr(sb, BAR_S + i), 1);
+      fa_mbar_init(bar_addr(sb, BAR_P + i), 128);
+      fa_mbar_init(bar_addr(sb, BAR_P + 2 + i), 128);
+      fa_mbar_init(bar_addr(sb, BAR_O + i), 1);
+      fa_mbar_init(bar_addr(sb, BAR_O + 2 + i), 1);
+      fa_mbar_init(bar_addr(sb, BAR_SFREE2 + i), 128);
+    }
+    fa_mbar_init(bar_addr(sb, BAR_LAG), 1);
+    fa_mbar_init(bar_addr(sb, BAR_TAIL), 1);
+    fa_mbar_init_fence();
+    misc[1] = 0;
+  }
+  if (warp == WARP_MMA) fa_tmem_alloc(sb + OFF_MISC, TMEM_COLS);
+  fa_tc_fence_before();
+  __syncthreads();
+  fa_tc_fence_after();
+  const fa_u32 tmem = (fa_u32)misc[0];
+  volatile int* abort_flag = misc + 1;
+  if (!plan->place.any) {  // (all threads)
+    if (warp == WARP_MMA) fa_tmem_dealloc(tmem, TMEM_COLS);
+    return;
+  }
+  if (PREFIX) {
+    if (warp < NSOFT) {
+      const FaRow row = fa_row<PREFIX>(p, plan->place, plan->place.first + tid);
+      const bool sees = row.from < row.to, in = row.at >= 0;
+      const int b0 = (int)__reduce_min_sync(0xffffffffu, (fa_u32)(sees ? row.from : 0x7fffffff)), b1 = __reduce_max_sync(0xffffffffu, sees ? row.to : 0);
+      const int b2 = __reduce_max_sync(0xffffffffu, in ? row.from : 0), b3 = __reduce_min_sync(0xffffffffu, in ? row.to : 0x7fffffff);
+      int* const b = bounds + (warp >> 2) * 4;
+      if (lane == 0) {
+        atomicMin(b, b0);
+        atomicMax(b + 1, b1);
+        atomicMax(b + 2, b2);
+        atomicMin(b + 3, b3);
+      }
+    }
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) plan->set(i, p, bounds[4 * i], bounds[4 * i + 1], bounds[4 * i + 2], bounds[4 * i + 3]);
+      plan->finish(p);
+    }
+    __syncthreads();
+  }
+  const int nsteps = plan->nsteps, nloads = nsteps;
+  const auto step_word = [&](int j) { return plan->word(j); };
+  constexpr int m0 = 0;
+#else
 #if FA_TC_DECODE
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;  // grid: (kv shares, heads, batch)
   const int m0 = 0;
@@ -652,7 +827,6 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
   const int hk = h / (p.Hq / p.Hkv);
   const int gb = b + p.b_off, gh = h + p.h_off;
 
-  volatile int* misc = (volatile int*)(sm + OFF_MISC);  // [0] tmem base, [1] abort, [2] nsteps
   volatile fa_u32* sched = (volatile fa_u32*)(sm + OFF_SCHED);
   unsigned char* cls = sm + OFF_CLS;
 
@@ -801,6 +975,8 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
   const int nsteps = misc[2];   // steps of the softmax / MMA loops
   const int nloads = misc[3];   // kv tiles the producer brings in (two per step in the decode variant)
   volatile int* abort_flag = misc + 1;
+  const auto step_word = [&](int j) { return sched[j]; };
+#endif
 
   if (warp >= NSOFT) fa_setmaxnreg_dec<REGS_OTHER>();
   if (warp == WARP_PRODUCER) {
@@ -813,7 +989,13 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
       for (int j = 0; j < nloads && ok; ++j) {
         const int s = j % NSTAGE;
         const fa_u32 ph = (fa_u32)((j / NSTAGE) & 1);
+#if FA_TC_PACKED
+        const int n0 = plan->place.k0 + (plan->first + j) * BN, b = 0;
+        const int v_bar = plan->beyond > 0 && j == nloads - 1 ? BAR_TAIL : BAR_VFULL + s;
+#else
         const int n0 = (int)(sched[j] & 0xffffu) * BN;
+        const int v_bar = BAR_VFULL + s;
+#endif
         if (j >= NSTAGE) ok = fa_mbar_wait(bar_addr(sb, BAR_KEMPTY + s), ph ^ 1u, abort_flag);
         if (!ok) break;
         fa_mbar_expect_tx(bar_addr(sb, BAR_KFULL + s), KV_STAGE);
@@ -821,11 +1003,28 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
           fa_tma_load_4d(sb + OFF_K + s * KV_STAGE + a * ATOM_BYTES, &P.tk, bar_addr(sb, BAR_KFULL + s), a * 64, n0, hk, b);
         if (j >= NSTAGE) ok = fa_mbar_wait(bar_addr(sb, BAR_VEMPTY + s), ph ^ 1u, abort_flag);
         if (!ok) break;
-        fa_mbar_expect_tx(bar_addr(sb, BAR_VFULL + s), KV_STAGE);
+        fa_mbar_expect_tx(bar_addr(sb, v_bar), KV_STAGE);
         for (int a = 0; a < ATOMS; ++a)
-          fa_tma_load_4d(sb + OFF_V + s * KV_STAGE + a * ATOM_BYTES, &P.tv, bar_addr(sb, BAR_VFULL + s), a * 64, n0, hk, b);
+          fa_tma_load_4d(sb + OFF_V + s * KV_STAGE + a * ATOM_BYTES, &P.tv, bar_addr(sb, v_bar), a * 64, n0, hk, b);
       }
     }
+#if FA_TC_PACKED
+  } else if (warp == NSOFT + 3) {
+    // ================================ zeros behind the last keys ==========================
+    const int beyond = plan->beyond;
+    if (beyond > 0 && fa_mbar_wait_warp(bar_addr(sb, BAR_TAIL), 0, abort_flag)) {
+      const int s = (nloads - 1) % NSTAGE;
+      unsigned char* const v = sm + OFF_V + s * KV_STAGE;
+      for (int i = lane; i < beyond * 8 * ATOMS; i += 32) {
+        const int a = i / (beyond * 8), c = i - a * (beyond * 8);
+        *(uint4*)(v + a * ATOM_BYTES + (BN - beyond) * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) fa_mbar_arrive(bar_addr(sb, BAR_VFULL + s));
+    }
+#endif
+#if FA_TC_DECODE
   } else if (DECODE && (warp == WARP_MMA || warp == WARP_MMA_B)) {
     // ============ decode variant: warp A issues the S products, warp B the PV products ======
     // With P in its own TMEM columns the two streams only meet through the softmax warps, so each
@@ -884,6 +1083,7 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
         }
       }
     }
+#endif
   } else if (ROT && warp >= WARP_MMA && warp < WARP_MMA + NQ) {
     // ============ head dim 64: an issuing warp per query tile ==============================
     // S(j+1) lies over the P columns of step j-1, whose product this warp has issued before it.  The whole warp runs the loop and one elected lane issues: in uniform control flow the
@@ -898,7 +1098,7 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
     constexpr fa_u32 HI = fa_desc_hi_sw128();
     bool ok = nsteps_u == 0 || fa_mbar_wait_all(bar_addr(sb, BAR_Q), 0, abort_flag);
     fa_u32 ns = 0, cnt = 0;  // S and PV products issued so far
-    auto word = [&](int j) { return __shfl_sync(0xffffffffu, sched[j], 0); };
+    auto word = [&](int j) { return __shfl_sync(0xffffffffu, step_word(j), 0); };
     auto active = [&](fa_u32 w) { return ((w >> (16 + 8 * i)) & 0xffu) != 0u; };
     auto wait_k = [&](int j) { return fa_mbar_wait_all(bar_addr(sb, BAR_KFULL + j % NSTAGE), (fa_u32)((j / NSTAGE) & 1), abort_flag); };
     const fa_u32 loQ = fa_desc_lo(sb + i * ATOMS * ATOM_BYTES, 16);
@@ -975,7 +1175,7 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
     // Descriptors: constant high word; the low word (start address and MN-chunk distance in
     // 16-byte units) is stepped with one add per k-step.
     constexpr fa_u32 HI = fa_desc_hi_sw128();
-    auto word = [&](int j) { return __shfl_sync(0xffffffffu, sched[j], 0); };
+    auto word = [&](int j) { return __shfl_sync(0xffffffffu, step_word(j), 0); };
     auto active = [&](fa_u32 w, int i) { return ((w >> (16 + 8 * i)) & 0xffu) != 0u; };
     auto wait_k = [&](int j) { return fa_mbar_wait_all(bar_addr(sb, BAR_KFULL + j % NSTAGE), (fa_u32)((j / NSTAGE) & 1), abort_flag); };
     auto have_k = [&](int j) { return __all_sync(0xffffffffu, fa_mbar_try(bar_addr(sb, BAR_KFULL + j % NSTAGE), (fa_u32)((j / NSTAGE) & 1))) != 0; };
@@ -1081,20 +1281,56 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
     const int i = warp >> 2;                       // query tile of this warpgroup
     const int lane_base = (warp & 3) * 32;         // TMEM lanes this warp may touch
     const int r = lane_base + lane;                // row inside the tile
+#if FA_TC_PACKED
+    FaRow mine = fa_row<PREFIX>(p, plan->place, plan->place.first + tid);
+    const int qi = mine.pos, gb = mine.b + p.b_off, gh = hk * G + mine.head + p.h_off;
+#else
     const int qi = DECODE ? (r & 63) : m0 + i * BM + r;  // query index
+#endif
     const int half = DECODE ? (r >> 6) : 0;               // decode variant: kv columns 64 * half .. + 63 of every tile
     // decode variant: warps whose 32 rows are all padding (fewer than 33 queries) only keep the barrier protocol going
+#if FA_TC_PACKED
+    const bool warp_active = true;
+#else
     const bool warp_active = !DECODE || (lane_base & 63) < p.Sq;
+#endif
     fa_u32 idle_cnt = 0;
     const fa_u32 t_s = tmem + ((fa_u32)lane_base << 16) + COL_S + i * S_STRIDE;
     const fa_u32 t_o = tmem + ((fa_u32)lane_base << 16) + COL_O + i * D;
     const fa_u32 t_p = DECODE ? tmem + ((fa_u32)lane_base << 16) + COL_P + i * 64 : t_s;
     bool ok = true;
+#if FA_TC_PACKED
+    // this warp's rows of the query tile, in 16-byte pieces; those that are not there, and columns beyond the head dim, as zeros
+    {
+      constexpr int CPR = D / 8, STEP = 32 / CPR;
+      const char* const qg = (const char*)p.q.ptr + (long long)hk * G * p.q.sh * 2;
+      const int c = lane % CPR;
+#pragma unroll
+      for (int it = 0; it < CPR; ++it) {
+        const int rr = it * STEP + lane / CPR;
+        const long long at = __shfl_sync(0xffffffffu, mine.at, rr);
+        const bool there = at >= 0 && c * 8 < p.D;
+        const int row = lane_base + rr;
+        fa_cp_async16(sb + (i * ATOMS + (c >> 3)) * ATOM_BYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4), qg + (there ? at * 2 + c * 16 : 0), there ? 16 : 0);
+      }
+      fa_cp_commit();
+      fa_cp_wait<0>();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) fa_mbar_arrive(bar_addr(sb, BAR_Q));
+    }
+    const unsigned* const rowbits = nullptr;
+#else
     // (rows beyond Sq have no row in the bit matrix: their scores are never stored, the mask is evaluated)
     const unsigned* rowbits = (p.t.mask_bits != nullptr && qi < p.Sq && (p.t.mask_hold == nullptr || *p.t.mask_hold != 0))
         ? p.t.mask_bits + (((long long)(p.t.mask_B == 1 ? 0 : b) * p.t.mask_H + (p.t.mask_H == 1 ? 0 : h)) * p.t.mask_rows + qi) * p.t.mask_stride
         : nullptr;
-    SoftmaxCtx c = {p, sb, t_s, t_o, t_p, i, warp, qi, gb, gh, half, p.scale * FA_LOG2E, abort_flag, FA_NEG_INF, 0.f, 0u, rowbits, {}};
+#endif
+    SoftmaxCtx c = {p, sb, t_s, t_o, t_p, i, warp, qi, gb, gh, half, p.scale * FA_LOG2E, abort_flag, FA_NEG_INF, 0.f, 0u, rowbits, {}, 0, 0};
+#if FA_TC_PACKED
+    c.from = mine.from;
+    c.to = mine.to;
+#endif
 #if FA_HAS_SCORE_MOD && defined(FA_SCORE_AFFINE) && defined(FA_SCORE_LINEAR_KV)
     {
       const float mul = fa_score_mul(0.f, gb, gh, qi, 0) * c.sc2, slope = fa_score_add2_dkv(0.f, gb, gh, qi, 0);
@@ -1118,10 +1354,10 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
     for (int e = 0; e < D; ++e) acc[e] = 0.f;
 #endif
     // (the schedule entry of a step is read during the one before)
-    fa_u32 w_next = sched[DECODE ? i : 0];
+    fa_u32 w_next = step_word(DECODE ? i : 0);
     for (int j = 0; j < nsteps && ok; ++j) {
       const fa_u32 w = w_next;
-      w_next = sched[DECODE ? min(2 * j + 2 + i, MAXT) : j + 1];
+      w_next = step_word(DECODE ? min(2 * j + 2 + i, MAXT) : j + 1);
       const int mode = DECODE ? (int)(w >> 16) : (int)((w >> (16 + 8 * i)) & 0xffu);
       const int tile = (int)(w & 0xffffu);
       if (mode == 0) continue;
@@ -1140,7 +1376,11 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
         ++idle_cnt;
         continue;
       }
+#if FA_TC_PACKED
+      const bool masked = mode == 1;
+#else
       const bool masked = (FA_HAS_MASK_MOD && mode == 1) || tile * BN + BN > p.Skv;
+#endif
 #if FA_DTYPE == FA_DT_F32
       ok = softmax_step_f32(c, acc, tile, mode, masked);
       continue;
@@ -1215,6 +1455,70 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
           for (int e = 0; e < 16; e += 4)
             *(float4*)(p.part_o + prow * D + c0 + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
           if ((mt & 3) == 0) *(float2*)(p.part_ml + prow * 2) = make_float2(mstar, lsum);
+        }
+      }
+    }
+#elif FA_TC_PACKED
+    {
+      if (ok && cnt == 0) ok = fa_mbar_wait_warp(bar_addr(sb, BAR_Q), 0, abort_flag);
+      if (ok && *abort_flag == 0) {
+        fa_tc_fence_after();
+        // (a row that has seen no key may hold the tiny values that the polynomial gives for -inf; a sum that is no number stays so)
+        const bool none = m_ref == FA_NEG_INF && l == l;
+        const float inv = none ? 0.f : l > 0.f ? 1.f / l : l;
+        const FaPlace place = plan->place;
+        mine = fa_row<PREFIX>(p, place, place.first + tid);  // (again: it has not been kept through the steps)
+        const bool there = mine.at >= 0;
+        if (PREFIX) {
+          const long long part = ((long long)blockIdx.z * p.Hkv + hk) * p.tokens * G + place.first + tid;
+          if (there) *(float2*)(p.part_ml + part * 2) = make_float2(m_ref, none ? 0.f : l);
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            if (cnt > 0) {
+              fa_tmem_ld32(t_o + c * 32, o);
+              fa_tmem_wait_ld();
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (there && c * 32 + e < p.Dv) *(float4*)(p.part_o + part * p.Dv + c * 32 + e) = cnt > 0 && !none ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        } else {
+          // The rows leave through this warp's rows of the query tile, which nothing reads any more (every S product of the tile is complete), in whole lines.
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            if (cnt > 0) {
+              fa_tmem_ld32(t_o + c * 32, o);
+              fa_tmem_wait_ld();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = 0.f;
+            }
+            unsigned char* strow = sm + (i * ATOMS + (c >> 1)) * ATOM_BYTES + r * 128;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 w;
+              w.x = fa_pack2<DT>(o[e] * inv, o[e + 1] * inv);
+              w.y = fa_pack2<DT>(o[e + 2] * inv, o[e + 3] * inv);
+              w.z = fa_pack2<DT>(o[e + 4] * inv, o[e + 5] * inv);
+              w.w = fa_pack2<DT>(o[e + 6] * inv, o[e + 7] * inv);
+              *(uint4*)(strow + ((((c & 1) * 4 + (e >> 3)) ^ (r & 7)) * 16)) = none ? make_uint4(0u, 0u, 0u, 0u) : w;
+            }
+          }
+          if (p.lse != nullptr && there)
+            p.lse[(long long)(hk * G + mine.head) * p.tokens + place.q0 + mine.token] = none ? FA_NEG_INF : (m_ref + fa_lg2(l)) * FA_LN2;
+          __syncwarp();
+          constexpr int CPR = D / 8, STEP = 32 / CPR;
+          const long long to = there ? fa_row_out(p, place, mine, hk) : -1;
+          const int c = lane % CPR;
+#pragma unroll
+          for (int it = 0; it < CPR; ++it) {
+            const int rr = it * STEP + lane / CPR, row = lane_base + rr;
+            const long long at = __shfl_sync(0xffffffffu, to, rr);
+            if (at >= 0 && c * 8 < p.Dv)
+              *(uint4*)((char*)p.o.ptr + at * 2 + c * 16) = *(const uint4*)(sm + (i * ATOMS + (c >> 3)) * ATOM_BYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+          }
         }
       }
     }

@@ -392,16 +392,6 @@ __device__ __forceinline__ fa_u32 bytes_of(fa_u32 a, fa_u32 b, fa_u32 which) {
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(which));
   return r;
 }
-__device__ __forceinline__ uint4 lds16(fa_u32 at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds8(fa_u32 at) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
-  return v;
-}
 struct Rows {
   float s[WN / 16][NQ][4], o[VB / 2][NQ][4], m[HR], l[HR];
   fa_u32 qf[BLOCKS * 4][NQ][2];
@@ -433,15 +423,15 @@ struct Rows {
   }
   // S' = K Q'.  A product's 16 columns are bytes 4 i .. 4 i + 3 of the 16 that each of four threads has of a key (of 64 columns in all); the queries lie
   // in their registers in the same order.
-  __device__ __forceinline__ void scores(const unsigned char*, fa_u32 tile, int) {
+  __device__ __forceinline__ void scores(const unsigned char* bytes, fa_u32, int) {
 #pragma unroll
     for (int i = 0; i < WN / 16; ++i) {
 #pragma unroll
       for (int q = 0; q < NQ; ++q) s[i][q][0] = s[i][q][1] = s[i][q][2] = s[i][q][3] = 0.f;
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
-        const uint4 x = lds16(chunk_at<PK>(tile, i * 16 + key_of(lane >> 2), b * 4 + (lane & 3)));
-        const uint4 y = lds16(chunk_at<PK>(tile, i * 16 + 8 + key_of(lane >> 2), b * 4 + (lane & 3)));
+        const uint4 x = *(const uint4*)(bytes + chunk_at<PK>(0, i * 16 + key_of(lane >> 2), b * 4 + (lane & 3)));
+        const uint4 y = *(const uint4*)(bytes + chunk_at<PK>(0, i * 16 + 8 + key_of(lane >> 2), b * 4 + (lane & 3)));
         const fa_u32 xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -460,7 +450,7 @@ struct Rows {
     }
   }
   // O' = V' P'.  Probabilities times scales may have any size, so they go in as bf16, in two parts, rounded and what the rounding left: 16 bits of them.
-  __device__ __forceinline__ void values(const unsigned char*, fa_u32 tile, int) {
+  __device__ __forceinline__ void values(const unsigned char* bytes, fa_u32, int) {
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
       const float f = __shfl_sync(0xffffffffu, vs, key(j));
@@ -489,10 +479,10 @@ struct Rows {
         for (int k = 0; k < 4; ++k) {
           const int r = (k & 1 ? k1 : k0) + (k >> 1) * 8;
           if (VB < 16) {
-            const uint2 x = lds8(chunk_at<PV>(tile, r, g >> 1) + (g & 1) * 8);
+            const uint2 x = *(const uint2*)(bytes + chunk_at<PV>(0, r, g >> 1) + (g & 1) * 8);
             w[k][0] = x.x; w[k][1] = x.y; w[k][2] = w[k][3] = 0u;
           } else {
-            const uint4 x = lds16(chunk_at<PV>(tile, r, g * (VB / 16) + c / 16));
+            const uint4 x = *(const uint4*)(bytes + chunk_at<PV>(0, r, g * (VB / 16) + c / 16));
             w[k][0] = x.x; w[k][1] = x.y; w[k][2] = x.z; w[k][3] = x.w;
           }
         }

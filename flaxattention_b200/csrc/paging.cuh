@@ -410,6 +410,9 @@ int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
 //     other's waits, and more slots for fewer do not (us, two CTAs with three or more slots / three or four with two: 32 requests of up to 16384 keys D 128
 //     191 / 182, one of 131072 88 / 84, 300 of up to 700 D 64 78 / 58, D 96 105 / 87, fp32 D 64 103 / 99).  Two where registers are short: more than 8
 //     rows of wide heads (D 128, 12 rows 37 / 41), two and four row groups.
+//   * 8 bits: three CTAs, and two for more than 8 rows, with two slots: the whole numbers' way to 16 bits takes registers, and with four CTAs (128 registers a
+//     thread) they spill.  (us, four / three / two CTAs: 32 requests of up to 16384 keys D 128 171 / 147 / 168, 20 rows over 16 x 4 segments of 4097 140 / 95 / 57;
+//     with more slots 257 / 150 / 171 and 140 / 99 / 60.)
 //   * A CTA per segment, one launch and no parts, instead of cut segments:
 //     - no more segments than SMs, and tables with room for four tiles per key group: as many groups as fit, four slots each.  (us on the GPU, cut / a
 //       CTA each: 64 segments of 32 tiles, D 64, eight groups 12.1 / 8.7; D 128, four groups, 8 tiles 9.3 / 7.0, 16 10.2 / 9.8, 32 14.6 / 15.5.)
@@ -442,7 +445,7 @@ void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   long long keys = (long long)p->table_width * p->page_size;
   if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + p->Sq + c.WN);
   const long long segments = (long long)p->B * p->Hkv, sms = device_sm_count();
-  const int most = c.RG > 1 || (f32 ? c.fr > 8 : c.few != 1 && p->D > 64) ? 2 : c.few == 1 || f32 ? 4 : 3;  // CTAs of an SM
+  const int most = c.eight ? (c.few == 1 ? 3 : 2) : c.RG > 1 || (f32 ? c.fr > 8 : c.few != 1 && p->D > 64) ? 2 : c.few == 1 || f32 ? 4 : 3;  // CTAs of an SM
   // as many as there is room for with `slots`
   const auto fit = [&](int slots) {
     for (c.per_sm = most; c.per_sm > 1 && smem(slots) > 227 * 1024 / c.per_sm - 1024;) --c.per_sm;
@@ -463,7 +466,7 @@ void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   if (c.RG == 1 && segments > sms && keys <= (2 * segments > 3 * sms ? 64LL : 32LL) * c.WN) return;
   c.one_each = false;
   const int room = std::min(227 * 1024 / c.per_sm - 1024, kMaxSmem);
-  while (c.slots < 8 && smem(c.slots + 1) <= room) ++c.slots;
+  while (c.slots < (c.eight ? 2 : 8) && smem(c.slots + 1) <= room) ++c.slots;
   c.smem = smem(c.slots);
 }
 int paged_row_tiles(const fa_paged_params* p, const PagedCfg& c) {

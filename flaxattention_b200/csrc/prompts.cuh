@@ -15,6 +15,9 @@ struct PackedShape {
   float scale;
 };
 
+// (16-bit types: quotients and tanh of scores without branches, as over pages)
+std::string packed_math(const PackedShape& s) { return s.dtype == FA_F32 ? "" : "#include \"fa_score_math.cuh\"\n"; }
+
 // ---- general kernel: tiles of fa_packed.cuh ---------------------------------------------------
 // Keys of a tile: as many as leave room for two CTAs on an SM.
 int packed_bn(int dtype, int D) { return dtype == FA_F32 ? (D <= 64 ? 64 : D <= 128 ? 32 : 16) : D <= 128 ? 64 : 32; }
@@ -23,8 +26,29 @@ int get_packed_kernel(fa_module* m, const PackedShape& s, bool prefix, Kernel** 
   // (the map of fa_packed.cuh)
   const int smem = 64 * pitch(s.D, es) + 2 * BN * (pitch(s.D, es) + pitch(s.Dv, es)) + (s.dtype == FA_F32 ? 64 * pitch(BN, 4) : 0);
   return get_kernel(m, kernel_key(kIdPacked, {{s.dtype, 2}, {s.D, 9}, {s.Dv, 9}, {BN, 9}, {prefix ? 1 : 0, 1}}), "fa_packed.cuh",
-                    [&] { return defs({{"FA_DTYPE", s.dtype}, {"FA_D", s.D}, {"FA_DV", s.Dv}, {"FA_BN", BN}, {"FA_PREFIX", prefix ? 1 : 0}}); },
+                    [&] { return packed_math(s) + defs({{"FA_DTYPE", s.dtype}, {"FA_D", s.D}, {"FA_DV", s.Dv}, {"FA_BN", BN}, {"FA_PREFIX", prefix ? 1 : 0}}); },
                     "fa_packed_kernel", smem, k);
+}
+
+// ---- tcgen05 kernel: fa_fwd_tc.cuh with FA_TC_PACKED --------------------------------------------
+struct FaTcPackedHost {
+  FaPackedParams p;
+  FaTensorMapHost tk, tv;
+};
+bool packed_tc_takes(const PackedShape& s, long long keys) {
+  return s.dtype != FA_F32 && s.D <= 128 && s.scale > 0.f && keys > 0 && keys <= 1 << 23 && !(s.flags & FA_FLAG_GENERAL_KERNELS);
+}
+int get_packed_tc_kernel(fa_module* m, const PackedShape& s, bool prefix, int nq, Kernel** k) {
+  // (must match the shared-memory map of fa_fwd_tc.cuh)
+  const int D = s.D <= 64 ? 64 : 128, atoms = D / 64, nstage = D == 64 ? nq + 1 : nq;
+  const int smem = nq * atoms * 16384 + 2 * nstage * atoms * 16384 + (1 + 4 * nstage + 14) * 8 + 16 + (256 + 4) * 4 + 2 * 256 + (256 / 32) * 4 + 1024;
+  return get_kernel(m, kernel_key(kIdPackedTc, {{s.dtype, 2}, {D, 9}, {nq, 2}, {prefix ? 1 : 0, 1}}), "fa_fwd_tc.cuh",
+                    [&] { return packed_math(s) + defs({{"FA_DTYPE", s.dtype}, {"FA_D", D}, {"FA_ROUND_SCORES", 0}, {"FA_TC_DECODE", 0}, {"FA_TC_NQ", nq}, {"FA_TC_PACKED", prefix ? 2 : 1}}); },
+                    "fa_packed_tc_kernel", smem, k);
+}
+// keys and values as [tokens, heads]; false: strides that no tensor map takes
+bool packed_maps(const PackedShape& s, const fa_tensor& k, const fa_tensor& v, int keys, FaTcPackedHost& L) {
+  return make_map(&L.tk, s.dtype, k, s.D, keys, s.Hkv, 1) == FA_OK && make_map(&L.tv, s.dtype, v, s.Dv, keys, s.Hkv, 1) == FA_OK;
 }
 
 // items of `rows` rows for `n` rows of B requests, dealt over the y and z dimension of a grid (and those of rows of no request, in front and behind)
@@ -105,13 +129,19 @@ __global__ void __launch_bounds__(128) fa_prefix_merge_kernel(const __grid_const
 }
 
 PackedShape shape_of(const fa_paged_params* p) { return {p->dtype, p->Hq, p->Hkv, p->D, p->Dv, p->flags, p->scale}; }
-// Parts that the prefix is cut into: as many as fill the SMs with CTAs of the heads' rows, but a tile each at least.
-int prefix_parts(const fa_paged_params* p) {
-  const long long rows = (long long)p->B * p->Sq * (p->Hq / p->Hkv), ctas = p->Hkv * ((rows + 63) / 64);
-  const int tiles = (p->prefix_length + packed_bn(p->dtype, p->D) - 1) / packed_bn(p->dtype, p->D);
-  return (int)std::max<long long>(1, std::min<long long>(std::min(tiles, 64), 2LL * device_sm_count() / ctas));
+// rows of an item: two query tiles where there are more than fill one
+int prefix_rows(const fa_paged_params* p) {
+  if (!packed_tc_takes(shape_of(p), p->prefix_length)) return 64;
+  return (long long)p->B * p->Sq * (p->Hq / p->Hkv) > 128 ? 256 : 128;
 }
-int prefix_fill(fa_module* m, const fa_paged_params* p, float* part_o, float* part_ml, FaPackedParams& k) {
+// Parts that the prefix is cut into: as many as fill the SMs with CTAs of the heads' rows (two on an SM but for those of 256 rows), but a tile each at least.
+int prefix_parts(const fa_paged_params* p) {
+  const int R = prefix_rows(p), BN = R == 64 ? packed_bn(p->dtype, p->D) : 128;
+  const long long rows = (long long)p->B * p->Sq * (p->Hq / p->Hkv), ctas = p->Hkv * ((rows + R - 1) / R);
+  const int tiles = (p->prefix_length + BN - 1) / BN;
+  return (int)std::max<long long>(1, std::min<long long>(std::min(tiles, 64), (R == 256 ? 1LL : 2LL) * device_sm_count() / ctas));
+}
+void prefix_fill(fa_module* m, const fa_paged_params* p, float* part_o, float* part_ml, FaPackedParams& k) {
   memset(&k, 0, sizeof k);
   fill_buffers(m, k.mod_buf);
   k.q = cvt(p->q); k.k = cvt(p->k_prefix); k.v = cvt(p->v_prefix);
@@ -122,16 +152,17 @@ int prefix_fill(fa_module* m, const fa_paged_params* p, float* part_o, float* pa
   k.b_off = p->b_offset; k.h_off = p->h_offset; k.splits = prefix_parts(p);
   k.by_group = divide_by(p->Hq / p->Hkv); k.by_sq = divide_by(p->Sq);
   k.scale = p->scale;
-  return FA_OK;
 }
 int launch_prefix(fa_module* m, const fa_paged_params* p, float* part_o, float* part_ml, void* stream) {
-  FaPackedParams k;
-  if (int rc = prefix_fill(m, p, part_o, part_ml, k)) return rc;
+  FaTcPackedHost L;
+  prefix_fill(m, p, part_o, part_ml, L.p);
   Kernel* kernel = nullptr;
-  if (int rc = get_packed_kernel(m, shape_of(p), true, &kernel)) return rc;
-  const long long items = ((long long)k.tokens * (p->Hq / p->Hkv) + 63) / 64;
+  int R = prefix_rows(p);
+  if (R != 64 && !packed_maps(shape_of(p), p->k_prefix, p->v_prefix, p->prefix_length, L)) R = 64;
+  if (int rc = R == 64 ? get_packed_kernel(m, shape_of(p), true, &kernel) : get_packed_tc_kernel(m, shape_of(p), true, R / 128, &kernel)) return rc;
+  const long long items = ((long long)p->B * p->Sq * (p->Hq / p->Hkv) + R - 1) / R;
   if (items > 65535) return fail(FA_EUNSUPPORTED, "too many rows for a prefix");
-  return launch(kernel, dim3((unsigned)p->Hkv, (unsigned)items, (unsigned)k.splits), dim3(128), &k, stream);
+  return launch(kernel, dim3((unsigned)p->Hkv, (unsigned)items, (unsigned)L.p.splits), dim3(R == 64 ? 128 : R == 128 ? 256 : 384), &L, stream);
 }
 int launch_prefix_merge(const fa_paged_params* p, const float* part_o, const float* part_ml, const float* own_o, const float* own_ml, int parts, void* stream) {
   FaMergeParams k{part_o, part_ml, own_o, own_ml, cvt(p->o), p->lse, p->B, p->Hq, p->Hkv, p->Sq, p->Dv, parts};
@@ -141,6 +172,21 @@ int launch_prefix_merge(const fa_paged_params* p, const float* part_o, const flo
 
 // ---- prompts -----------------------------------------------------------------------------------
 PackedShape shape_of(const fa_prompt_params* p) { return {p->dtype, p->Hq, p->Hkv, p->D, p->Dv, p->flags, p->scale}; }
+// Query tiles of a CTA of the tcgen05 kernel; 0: the general kernel.  The host knows the rows and the requests, not their lengths.
+//   * A few short prompts, whose rows fill no tile of 128 or whose CTAs of 64 rows the SMs hold at once: the general kernel, whose CTAs begin sooner.  (us, general /
+//     one tile, eight prompts of 30 and 64 tokens: D 64 6.7 / 7.5 and 6.8 / 7.9, 32 / 8 heads 6.8 / 8.3 and 7.6 / 8.6, D 128 8.4 / 8.9 and 8.5 / 9.3; of 128 tokens 8.9 / 8.1.)
+//     No more than 1024 keys in all, since they may be one prompt's (37.8 / 15.4).
+//   * Else one tile, two CTAs on an SM, at head dims up to 64 (one / two: one prompt of 4096 tokens, 8 heads, 47.8 / 60.9, eight, 32 / 8 heads, 931 / 948), and above
+//     where there are few tiles or short prompts (one of 4096, 8 heads, 62.4 / 66.1; 64 of 256, 32 / 8 heads, 155 / 165; eight of 1024 118.5 / 119.6).
+//   * Two tiles, which share the loads of K and V, for long ones at head dims above 64 (32 / 8 heads: one of 2048 51.5 / 45.4, eight of 4096 1466 / 1297, eight pieces of 200 behind
+//     4000 149 / 134).
+int prompt_query_tiles(const fa_prompt_params* p) {
+  const long long G = p->Hq / p->Hkv, B = std::max(p->B, 1), rows = p->tokens * G, sms = device_sm_count();
+  if (p->keys <= std::min<long long>(64 * B, 1024) && (rows <= 64 * B || p->Hkv * (rows / 64 + B) <= 2 * sms)) return 0;
+  long long keys = p->keys / B;
+  if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + 128);
+  return p->D > 64 && keys >= 1536 && p->Hkv * ((rows + 127) / 128) >= 2 * sms ? 2 : 1;
+}
 int prompt_sizes(fa_module* m, const fa_prompt_params* p) {
   if (!m) return fail(FA_EINVAL, "module is null");
   if (!p) return fail(FA_EINVAL, "params is null");
@@ -173,6 +219,11 @@ extern "C" {
 int fa_prompt_prepare(fa_module* m, const fa_prompt_params* p) {
   if (int rc = prompt_sizes(m, p)) return rc;
   Kernel* kernel = nullptr;
+  if (packed_tc_takes(shape_of(p), p->keys)) {
+    for (int nq = 1; nq <= 2; ++nq)
+      if (int rc = get_packed_tc_kernel(m, shape_of(p), false, nq, &kernel)) return rc;
+    return FA_OK;
+  }
   return get_packed_kernel(m, shape_of(p), false, &kernel);
 }
 
@@ -186,11 +237,17 @@ int fa_prompt(fa_module* m, const fa_prompt_params* p, void* stream) {
   if (int rc = check_tensor(p->o, "o", es)) return rc;
   if (int rc = check_tensor(p->k, "k", es, p->keys > 0)) return rc;
   if (int rc = check_tensor(p->v, "v", es, p->keys > 0)) return rc;
-  FaPackedParams k;
-  prompt_fill(m, p, k);
+  FaTcPackedHost L;
+  prompt_fill(m, p, L.p);
   Kernel* kernel = nullptr;
+  const long long rows = p->tokens * (p->Hq / p->Hkv);
+  const int nq = packed_tc_takes(shape_of(p), p->keys) ? prompt_query_tiles(p) : 0;
+  if (nq > 0 && packed_maps(shape_of(p), p->k, p->v, (int)p->keys, L)) {
+    if (int rc = get_packed_tc_kernel(m, shape_of(p), false, nq, &kernel)) return rc;
+    return launch(kernel, packed_grid(p->Hkv, rows, 128 * nq, p->B), dim3(nq == 1 ? 256 : 384), &L, stream);
+  }
   if (int rc = get_packed_kernel(m, shape_of(p), false, &kernel)) return rc;
-  return launch(kernel, packed_grid(p->Hkv, p->tokens * (p->Hq / p->Hkv), 64, p->B), dim3(128), &k, stream);
+  return launch(kernel, packed_grid(p->Hkv, rows, 64, p->B), dim3(128), &L.p, stream);
 }
 
 }  // extern "C"

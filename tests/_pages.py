@@ -128,6 +128,12 @@ class Cache8(Cache):
         return dict(key_scales=self.k_scales, value_scales=self.v_scales)
 
 
+def with_slope(want, slope):
+    """The tcgen05 kernels take a bias that is linear over the keys from that of the first key of a tile of 128, which the sums of up to 128 slopes are added to:
+    three roundings of 128 slopes at most, 3 * 2^-24 * 128 |slope|, written as 2^-20 of a larger `top`."""
+    return (*want[:3], want[3] + 3 * 2.0 ** -24 * 128 * slope / 2.0 ** -20)
+
+
 class Prompts:
     """Requests of `lengths` new tokens behind `past` others, laid end to end; rows of no request (`pad` in front and behind) are NaN."""
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import flaxattention_b200 as fa
-from _pages import Cache, Cache8, attend, check_attention, normal
+from _pages import Cache, Cache8, attend, check_attention, normal, with_slope
 from _util import DTYPES
 
 pytestmark = pytest.mark.gpu
@@ -28,7 +28,8 @@ def run(seed, P, lengths, Hq, Hkv, Sq, D, page, dtype, Dv=None, score=None, mask
         return see if mask is None else see & mask(b, h, i, j)
 
     join = lambda x, y: [torch.cat([x[0].double(), t.double()], 1) for t in y]  # noqa: E731
-    check_attention(out if bhln else out.transpose(1, 2), lse, attend(q, join(pk, c.keys), join(pv, c.values), score, behind, window, scale), dt)
+    want = attend(q, join(pk, c.keys), join(pv, c.values), score, behind, window, scale)
+    check_attention(out if bhln else out.transpose(1, 2), lse, with_slope(want, 2.0 ** -0.5 if score is distance else 0.0), dt)
     torch.cuda.synchronize()
     fa.check_status()
 

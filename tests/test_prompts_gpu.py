@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import flaxattention_b200 as fa
-from _pages import Prompts
+from _pages import Prompts, check_attention, with_slope
 from _util import DTYPES
 
 pytestmark = pytest.mark.gpu
@@ -17,7 +17,7 @@ def run(seed, lengths, Hq, Hkv, D, dtype, score=None, mask=None, window=None, sc
     out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, score, mask, key_starts=p.key_starts if p.past else None, window=window, sm_scale=scale, bhln=p.bhln,
                                    return_lse=True, kernel_options={"kernels": kernels} if kernels else None)
     assert out.dtype == p.dtype and lse.dtype == torch.float32
-    p.check(out, lse, p.want(score, mask, window, scale))
+    p.check(out, lse, with_slope(p.want(score, mask, window, scale), 2.0 ** -0.5 if score is distance else 0.0))
     torch.cuda.synchronize()
     fa.check_status()
     return out
@@ -115,7 +115,6 @@ def test_other_requests_may_hold_anything(dtype, D):
     out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, return_lse=True)
     want = p.want()
     keep = torch.cat([torch.arange(a), torch.arange(b, 280)])
-    from _pages import check_attention
     check_attention(out.cpu()[:, :, keep], lse.cpu()[:, :, keep], (*(x[:, :, keep] for x in want[:3]), want[3]), p.dtype)
 
 
@@ -224,3 +223,10 @@ def test_refusals():
         fa.prompt_attention(p.q, p.k, p.v, p.starts, key_starts=p.key_starts[:2])
     with pytest.raises(fa._cabi.FlaxAttnError, match="16"):
         fa.prompt_attention(p.q[..., :60], p.k[..., :60], p.v[..., :60], p.starts)
+
+
+@pytest.mark.parametrize("D", [96, 128])
+def test_two_query_tiles(D):
+    """Long prompts at wide heads take two tiles per CTA: rows of one end in the first, between, in the second."""
+    run(19, [2300, 1900, 2101], 64, 8, D, "bf16")
+    run(20, [300, 260, 200], 32, 8, D, "f16", past=[1700, 2000, 1500], score=distance, window=1900)
