@@ -29,6 +29,7 @@ extern "C" __global__ void __launch_bounds__(fa_pk::NT) fa_packed_kernel(const _
   __shared__ FaPlace found;
   FA_MOD_BUFS_INIT(p);
   fa_grid_wait();
+  if (PREFIX) fa_grid_release();  // (the pages' kernel runs beside this one)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hk = blockIdx.x, G = p.Hq / p.Hkv;
   if (PREFIX) {
     if (tid == 0) found = {0, p.tokens, 0, p.keys, 0, (int)blockIdx.y * BM, 1};  // (grid: kv heads, items, parts of the prefix)

@@ -78,42 +78,33 @@ __global__ void __launch_bounds__(128) fa_prefix_merge_kernel(const __grid_const
   const long long at = (long long)hk * p.B * p.Sq * G + ((long long)b * p.Sq + q) * G + (h - hk * G);
   const bool active = lane * 4 < p.Dv, second = lane * 4 + 128 < p.Dv;
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-  const auto weight = [](float m, float l, float top) { return l == 0.f ? 0.f : exp2f(m - (top == -INFINITY ? 0.f : top)); };
-  // the pages' first, as sums: times l
+  // Weights first: lane k has those of parts k and k + 32 (there are 64 at most), so that all rows of values can be on their way at once.
   const float2 own = *(const float2*)(p.own_ml + row * 2);
-  float m = own.y == 0.f ? -INFINITY : own.x, l = own.y;
+  float2 ml[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) ml[i] = lane + 32 * i < p.parts ? *(const float2*)(p.part_ml + ((lane + 32 * i) * n_rows + at) * 2) : make_float2(-INFINITY, 0.f);
   float4 x = active ? *(const float4*)(p.own_o + row * p.Dv + lane * 4) : zero, y = second ? *(const float4*)(p.own_o + row * p.Dv + lane * 4 + 128) : zero;
+  // (a part that has seen nothing counts for nothing; one whose sum is no number stays so)
+  float m = fmaxf(own.y == 0.f ? -INFINITY : own.x, fmaxf(ml[0].x, ml[1].x));
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  const float top = m == -INFINITY ? 0.f : m;
+  const auto weight = [&](const float2& v) { return v.y == 0.f ? 0.f : exp2f(v.x - top); };
+  const float w_own = weight(own) * own.y, w[2] = {weight(ml[0]), weight(ml[1])};  // (the pages' rows are divided already)
+  const float l = w_own + rot_sum(w[0] * ml[0].y + w[1] * ml[1].y);
   const auto scale = [&](float f) {
     x.x *= f; x.y *= f; x.z *= f; x.w *= f;
     y.x *= f; y.y *= f; y.z *= f; y.w *= f;
   };
-  scale(l);
-  constexpr int U = 4;
-  for (int k = 0; k < p.parts; k += U) {
-    float2 ml[U];
-    float4 u[U], v[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {  // (all of them on their way at once)
-      const bool in = k + i < p.parts;
-      const long long a = in ? (k + i) * n_rows + at : 0;
-      ml[i] = in ? *(const float2*)(p.part_ml + a * 2) : make_float2(-INFINITY, 0.f);
-      u[i] = in && active ? *(const float4*)(p.part_o + a * p.Dv + lane * 4) : zero;
-      v[i] = in && second ? *(const float4*)(p.part_o + a * p.Dv + lane * 4 + 128) : zero;
-    }
-    float top = m;
-#pragma unroll
-    for (int i = 0; i < U; ++i) top = fmaxf(top, ml[i].x);
-    const float f = weight(m, l, top);
-    l *= f;
-    scale(f);
-    m = top;
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const float g = weight(ml[i].x, ml[i].y, top);
-      l += g * ml[i].y;
-      x.x += g * u[i].x; x.y += g * u[i].y; x.z += g * u[i].z; x.w += g * u[i].w;
-      y.x += g * v[i].x; y.y += g * v[i].y; y.z += g * v[i].z; y.w += g * v[i].w;
-    }
+  scale(w_own);
+  const float* from = p.part_o + at * p.Dv + lane * 4;
+  const long long step = n_rows * p.Dv;
+#pragma unroll 8
+  for (int k = 0; k < p.parts; ++k, from += step) {
+    const float f = __shfl_sync(0xffffffffu, k < 32 ? w[0] : w[1], k & 31);
+    const float4 u = active ? *(const float4*)from : zero, v = second ? *(const float4*)(from + 128) : zero;
+    x.x += f * u.x; x.y += f * u.y; x.z += f * u.z; x.w += f * u.w;
+    y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
   }
   scale(l > 0.f ? 1.f / l : l);  // (0 and no number stay)
   char* to = (char*)p.o.ptr + ((long long)b * p.o.sb + (long long)h * p.o.sh + (long long)q * p.o.ss) * (DT == FA_F32 ? 4 : 2);
@@ -125,21 +116,24 @@ __global__ void __launch_bounds__(128) fa_prefix_merge_kernel(const __grid_const
   };
   if (active) put(lane * 4, x);
   if (second) put(lane * 4 + 128, y);
-  if (lane == 0 && p.lse != nullptr) p.lse[row] = l == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m) + log2f(l)) * 0.6931471805599453f;
+  if (lane == 0 && p.lse != nullptr) p.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
 }
 
 PackedShape shape_of(const fa_paged_params* p) { return {p->dtype, p->Hq, p->Hkv, p->D, p->Dv, p->flags, p->scale}; }
-// rows of an item: two query tiles where there are more than fill one
+// Rows of an item: 128, one query tile of the tcgen05 kernel; 64, the general kernel, also for short prefixes of few rows, since its CTAs begin sooner (us of the whole
+// call, general / tcgen05, one to eight requests behind 500 tokens, D 64 8.7 / 9.8, D 128 10.3 / 11.2; behind 4000 20.0 / 18.1 and 24.5 / 21.6).
 int prefix_rows(const fa_paged_params* p) {
-  if (!packed_tc_takes(shape_of(p), p->prefix_length)) return 64;
-  return (long long)p->B * p->Sq * (p->Hq / p->Hkv) > 128 ? 256 : 128;
+  const bool few = p->prefix_length <= 1024 && (long long)p->B * p->Sq * (p->Hq / p->Hkv) <= 64;
+  return few || !packed_tc_takes(shape_of(p), p->prefix_length) ? 64 : 128;
 }
-// Parts that the prefix is cut into: as many as fill the SMs with CTAs of the heads' rows (two on an SM but for those of 256 rows), but a tile each at least.
+// Parts that the prefix is cut into, at least a tile each.  As many as make a CTA for each SM: the pages' kernel runs beside them, and every part has to be written
+// and read again (us, 64 requests with 500 tokens of their own behind 8192, 32 / 8 heads, D 128, pages alone 28: half a CTA per SM 61, one 49, two 58).  Two where the rows alone make half a
+// CTA per SM or more, whose tiles then are what takes the time (500 requests: one part 189, two 155).
 int prefix_parts(const fa_paged_params* p) {
   const int R = prefix_rows(p), BN = R == 64 ? packed_bn(p->dtype, p->D) : 128;
-  const long long rows = (long long)p->B * p->Sq * (p->Hq / p->Hkv), ctas = p->Hkv * ((rows + R - 1) / R);
+  const long long rows = (long long)p->B * p->Sq * (p->Hq / p->Hkv), ctas = p->Hkv * ((rows + R - 1) / R), sms = device_sm_count();
   const int tiles = (p->prefix_length + BN - 1) / BN;
-  return (int)std::max<long long>(1, std::min<long long>(std::min(tiles, 64), (R == 256 ? 1LL : 2LL) * device_sm_count() / ctas));
+  return (int)std::max<long long>(1, std::min<long long>(std::min(tiles, 64), (2 * ctas > sms ? 2 : 1) * sms / ctas));
 }
 void prefix_fill(fa_module* m, const fa_paged_params* p, float* part_o, float* part_ml, FaPackedParams& k) {
   memset(&k, 0, sizeof k);
@@ -159,10 +153,10 @@ int launch_prefix(fa_module* m, const fa_paged_params* p, float* part_o, float* 
   Kernel* kernel = nullptr;
   int R = prefix_rows(p);
   if (R != 64 && !packed_maps(shape_of(p), p->k_prefix, p->v_prefix, p->prefix_length, L)) R = 64;
-  if (int rc = R == 64 ? get_packed_kernel(m, shape_of(p), true, &kernel) : get_packed_tc_kernel(m, shape_of(p), true, R / 128, &kernel)) return rc;
+  if (int rc = R == 64 ? get_packed_kernel(m, shape_of(p), true, &kernel) : get_packed_tc_kernel(m, shape_of(p), true, 1, &kernel)) return rc;
   const long long items = ((long long)p->B * p->Sq * (p->Hq / p->Hkv) + R - 1) / R;
   if (items > 65535) return fail(FA_EUNSUPPORTED, "too many rows for a prefix");
-  return launch(kernel, dim3((unsigned)p->Hkv, (unsigned)items, (unsigned)L.p.splits), dim3(R == 64 ? 128 : R == 128 ? 256 : 384), &L, stream);
+  return launch(kernel, dim3((unsigned)p->Hkv, (unsigned)items, (unsigned)L.p.splits), dim3(R == 64 ? 128 : 256), &L, stream);
 }
 int launch_prefix_merge(const fa_paged_params* p, const float* part_o, const float* part_ml, const float* own_o, const float* own_ml, int parts, void* stream) {
   FaMergeParams k{part_o, part_ml, own_o, own_ml, cvt(p->o), p->lse, p->B, p->Hq, p->Hkv, p->Sq, p->Dv, parts};
