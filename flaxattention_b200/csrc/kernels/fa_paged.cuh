@@ -193,6 +193,13 @@ __device__ __forceinline__ fa_u32 transposed(fa_u32 x) {  // an 8 x 8 matrix of 
   return r;
 }
 
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Sum {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+
 // ---- the rows of a warp: scores, softmax and values of a tile --------------------------------
 // HR rows per thread with NS scores each: row(h) is row h's number in the row tile, key(j) the j-th key's in the tile.
 #if FA_DTYPE == FA_DT_F32
@@ -372,6 +379,219 @@ constexpr int VB = PV / 8;             // columns of V of a thread, beside each 
 // Which of eight keys is row g of a product.  Lanes that are served together then read different banks: 16 bytes of the keys of two rows g beside each other
 // (K), and two threads' columns of the keys of every other row (V).
 __device__ __forceinline__ int key_of(int g) { return GROUP == 128 ? (g & 1 ? (g - 1) ^ 5 : g) : g ^ ((g >> 1) & 1); }
+#if FA_FEW == 1
+// Whole numbers with whole numbers: products of 8 bits, summed in 32 (m16n8k32), which take K as it lies in the tile and V with its bytes exchanged
+// (12 instructions for 16 values of K and of V together, where their way to 16 bits takes 68).
+//   Scores: a row of queries is 2^(e - 22) times whole numbers of 23 bits (2^(e - 1) <= max|q| < 2^e), which are three digits of 8 bits, -128 to 127, so a score is
+//   three sums, exact, and one rounding to fp32.  What 16-bit queries lose is below 2^-23 of the row's largest.
+//   Values: of a tile, probabilities times scales are whole numbers of 16 bits, in two digits, of 1 / 32639 of the largest of the row's 32: 2^-16 of that is what one is off by
+//   at most.  (A single rounding to fp16 is off by more than the three-fold of that, by the rms of a tile, and to bf16 by the 25-fold; with a third digit a tile
+//   would take 9 % more instructions.)
+__device__ __forceinline__ fa_u32 bytes_of(fa_u32 a, fa_u32 b, fa_u32 which) {
+  fa_u32 r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(which));
+  return r;
+}
+__device__ __forceinline__ void imma(int (&c)[4], const fa_u32 (&a)[4], fa_u32 b0, fa_u32 b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+constexpr int MAGIC = 0x4b400000;  // the bits of 1.5 * 2^23: with n added, below 2^22 in size, those of that number plus n
+__device__ __forceinline__ float from_magic(int c) { return __int_as_float(c) - 12582912.f; }
+// the three digits of four whole numbers, a register each
+__device__ __forceinline__ void digits(const int (&x)[4], fa_u32 (&d)[3]) {
+  int y[4], z[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    y[i] = (x[i] + 128) >> 8;  // (what is left above the low digit)
+    z[i] = (y[i] + 128) >> 8;
+  }
+  d[0] = bytes_of(bytes_of(x[0], x[1], 0x0040u), bytes_of(x[2], x[3], 0x0040u), 0x5410u);
+  d[1] = bytes_of(bytes_of(y[0], y[1], 0x0040u), bytes_of(y[2], y[3], 0x0040u), 0x5410u);
+  d[2] = bytes_of(bytes_of(z[0], z[1], 0x0040u), bytes_of(z[2], z[3], 0x0040u), 0x5410u);
+}
+struct Rows {
+  float s[WN / 16][1][4], o[VB / 2][1][4], m[HR], l[HR];
+  fa_u32 qf[BLOCKS * 2][3][2]; // digits of 16 values of each 64 of query g = lane / 4
+  float qs[HR];                // 2^(e - 22) of this lane's rows
+  float ks, vs;                // scales of this lane's key of the tile
+  int lane;
+  __device__ __forceinline__ float& score(int h, int j) { return s[j >> 1][0][(j & 1) * 2 + h]; }
+  __device__ __forceinline__ int key(int j) const { return key_of(lane >> 2) + j * 8; }
+  __device__ __forceinline__ int row(int h) const { return (lane & 3) * 2 + h; }
+  __device__ __forceinline__ bool idle(int h, int rows) const { return h >= rows; }
+  template <class F>
+  static __device__ __forceinline__ void over_keys(float (&v)[HR], F f) {
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+      for (int h = 0; h < HR; ++h) v[h] = f(v[h], __shfl_xor_sync(0xffffffffu, v[h], off));
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < VB / 2; ++i) o[i][0][0] = o[i][0][1] = o[i][0][2] = o[i][0][3] = 0.f;
+  }
+  __device__ __forceinline__ void rescale(int h, float c) {
+#pragma unroll
+    for (int i = 0; i < VB / 2; ++i) {
+      o[i][0][h] *= c;
+      o[i][0][2 + h] *= c;
+    }
+  }
+  __device__ __forceinline__ void take_queries(const fa_u32 (&raw)[BLOCKS * 8]) {  // 16 values of each 64, as they were loaded
+    fa_u32 most = 0;  // (sizes as bits: infinities and no numbers are the largest)
+#pragma unroll
+    for (int i = 0; i < BLOCKS * 8; ++i) most = max(most, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    most = __float_as_uint(fa_to_float<DT>((fa_u16)most));
+    // (below 2^-100 a row has fewer bits, and no score that shows)
+    const int e = max((int)(most >> 23) - 126, -100);
+    const float up = __uint_as_float((fa_u32)(22 - e + 127) << 23);
+    const float down = most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float((fa_u32)(e - 22 + 127) << 23);
+#pragma unroll
+    for (int h = 0; h < HR; ++h) qs[h] = __shfl_sync(0xffffffffu, down, ((lane & 3) * 2 + h) * 4);
+#pragma unroll
+    for (int i = 0; i < BLOCKS * 4; ++i) {
+      int n[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n[k] = __float2int_rn(fa_to_float<DT>((fa_u16)(raw[2 * i + (k >> 1)] >> (16 * (k & 1)))) * up);
+      fa_u32 d[3];
+      digits(n, d);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) qf[i >> 1][k][i & 1] = d[k];
+    }
+  }
+  // S' = K Q'.  A product's 32 columns are bytes 8 i .. 8 i + 7 of the 16 that each of four threads has of a key (of 64 columns in all); the queries'
+  // digits lie in their registers in the same order.
+  __device__ __forceinline__ void scores(const unsigned char* bytes, fa_u32, int) {
+#pragma unroll
+    for (int i = 0; i < WN / 16; ++i) {
+      int c[3][4];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) c[k][0] = c[k][1] = c[k][2] = c[k][3] = MAGIC;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        const uint4 x = *(const uint4*)(bytes + chunk_at<PK>(0, i * 16 + key_of(lane >> 2), b * 4 + (lane & 3)));
+        const uint4 y = *(const uint4*)(bytes + chunk_at<PK>(0, i * 16 + 8 + key_of(lane >> 2), b * 4 + (lane & 3)));
+        const fa_u32 a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          imma(c[k], a0, qf[b * 2][k][0], qf[b * 2][k][1]);
+          imma(c[k], a1, qf[b * 2 + 1][k][0], qf[b * 2 + 1][k][1]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][0][e] = fmaf(fmaf(from_magic(c[2][e]), 256.f, from_magic(c[1][e])), 256.f, from_magic(c[0][e]));
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const float f = __shfl_sync(0xffffffffu, ks, key(j));
+#pragma unroll
+      for (int h = 0; h < HR; ++h) score(h, j) *= f * qs[h];
+    }
+  }
+  // O' = V' P'
+  __device__ __forceinline__ void values(const unsigned char* bytes, fa_u32, int) {
+    float top[HR] = {0.f, 0.f};
+    fa_u32 nan = 0;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const float f = __shfl_sync(0xffffffffu, vs, key(j));
+#pragma unroll
+      for (int h = 0; h < HR; ++h) {
+        score(h, j) *= f;
+        top[h] = fmaxf(top[h], fabsf(score(h, j)));
+        nan |= !(fabsf(score(h, j)) <= 3.4e38f) ? 1u << h : 0u;
+      }
+    }
+    over_keys(top, Max());
+    float step[HR];
+#pragma unroll
+    for (int h = 0; h < HR; ++h) {
+      // (a largest value below 2^-100 counts as 2^-100, whose reciprocal is a number)
+      const float t = fmaxf(top[h], 7.9e-31f), up = 32639.f / t;
+      step[h] = t * (1.f / 32639.f);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) score(h, j) = fmaf(score(h, j), up, 12582912.f);  // (the whole number in the low 16 bits)
+    }
+    if (__any_sync(0xffffffffu, nan != 0)) {  // of a row with no number in it, nothing is one
+#pragma unroll
+      for (int h = 0; h < HR; ++h) {
+        fa_u32 any = nan >> h & 1u;
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) any |= __shfl_xor_sync(0xffffffffu, any, off);
+        if (any) step[h] = __uint_as_float(0x7fffffffu);
+      }
+    }
+    // Of every 8 keys the numbers of two rows in a register become those of two keys of row g = lane / 4; the low digit is taken out of the high one
+    // (which is one more where the low one is negative) before.
+    fa_u32 r[NS], b[2][2];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const fa_u32 x = bytes_of(__float_as_uint(score(0, j)), __float_as_uint(score(1, j)), 0x5410u);
+      fa_u32 y;
+      asm("add.u16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"((x & 0x00800080u) << 1));
+      r[j] = transposed(y);
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {  // digit d of the keys of rows 16 hf + 2 t, 2 t + 1, 2 t + 8 and 2 t + 9
+      b[0][hf] = bytes_of(r[2 * hf], r[2 * hf + 1], 0x6420u);
+      b[1][hf] = bytes_of(r[2 * hf], r[2 * hf + 1], 0x7531u);
+    }
+    // columns VB g .. VB g + VB - 1 of those keys
+    const int g = lane >> 2, t = lane & 3, k0 = key_of(2 * t), k1 = key_of(2 * t + 1);
+#pragma unroll
+    for (int c = 0; c < VB; c += 8) {
+      fa_u32 w[8][2];  // (16 bytes at once would take registers that the tiles on their way need)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint2 x = *(const uint2*)(bytes + chunk_at<PV>(0, (k & 1 ? k1 : k0) + (k >> 1) * 8, (g * VB + c) >> 4) + ((VB < 16 ? g : c >> 3) & 1) * 8);
+        w[k][0] = x.x;
+        w[k][1] = x.y;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // four columns of four keys: columns and keys change places
+        fa_u32 col[2][4];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const fa_u32 lo0 = bytes_of(w[4 * hf][i], w[4 * hf + 1][i], 0x5140u), hi0 = bytes_of(w[4 * hf][i], w[4 * hf + 1][i], 0x7362u);
+          const fa_u32 lo1 = bytes_of(w[4 * hf + 2][i], w[4 * hf + 3][i], 0x5140u), hi1 = bytes_of(w[4 * hf + 2][i], w[4 * hf + 3][i], 0x7362u);
+          col[hf][0] = bytes_of(lo0, lo1, 0x5410u);
+          col[hf][1] = bytes_of(lo0, lo1, 0x7632u);
+          col[hf][2] = bytes_of(hi0, hi1, 0x5410u);
+          col[hf][3] = bytes_of(hi0, hi1, 0x7632u);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const fa_u32 a[4] = {col[0][2 * u], col[0][2 * u + 1], col[1][2 * u], col[1][2 * u + 1]};
+          int acc[4] = {0, 0, 0, 0};
+          imma(acc, a, b[1][0], b[1][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] *= 256;
+          imma(acc, a, b[0][0], b[0][1]);
+          float(&out)[4] = o[c / 2 + i * 2 + u][0];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[e] = fmaf((float)acc[e], step[e & 1], out[e]);
+        }
+      }
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(int b, F f) {
+    if ((lane >> 2) * VB / 32 != b) return;
+#pragma unroll
+    for (int i = 0; i < VB / 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = (lane >> 2) * VB + 2 * i + (e >> 1);
+        if (PV == DV || c < DV) f(e & 1, c, o[i][0][e]);
+      }
+  }
+  __device__ __forceinline__ bool speaks() const { return lane < 4; }
+};
+#else
 // Four whole numbers as 16-bit values, two to a register.  fp16: in the low byte of 1024, made positive by 128.  bf16 has 8 bits: 128 plus the low seven of
 // the number, minus 128, or 256 of a negative one, whose sign is the bit that tells the two apart.
 template <int TO>
@@ -517,6 +737,7 @@ struct Rows {
   }
   __device__ __forceinline__ bool speaks() const { return lane < 4; }
 };
+#endif
 #elif FA_FEW
 constexpr int HR = 2 * NQ, NS = WN / 8;
 struct Rows {
@@ -689,13 +910,6 @@ struct Rows {
   __device__ __forceinline__ bool speaks() const { return (lane & 3) == 0; }
 };
 #endif
-
-struct Max {
-  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
-};
-struct Sum {
-  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
-};
 
 // a value of an output row
 __device__ __forceinline__ void put1(char* row, int c, float x) {
@@ -977,6 +1191,9 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
       const fa_u32* src = (const fa_u32*)(qb + (i * p.q.ss + (long long)(seg.hk * G + row - i * G) * p.q.sh) * ES) + (KV8 ? 0 : (lane & 3));
 #if FA_KV8
       // (columns 16 t .. of each 64, t = lane % 4, as K's)
+#if FA_FEW == 1
+      fa_u32 raw[BLOCKS * 8];
+#endif
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
         const int c = b * 64 + (lane & 3) * 16;
@@ -985,11 +1202,19 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
           x = *(const uint4*)(src + c / 2);
           y = *(const uint4*)(src + c / 2 + 4);
         }
+#if FA_FEW == 1
+        raw[b * 8] = x.x; raw[b * 8 + 1] = x.y; raw[b * 8 + 2] = x.z; raw[b * 8 + 3] = x.w;
+        raw[b * 8 + 4] = y.x; raw[b * 8 + 5] = y.y; raw[b * 8 + 6] = y.z; raw[b * 8 + 7] = y.w;
+#else
         R.qf[b * 4][q][0] = x.x; R.qf[b * 4][q][1] = x.y;
         R.qf[b * 4 + 1][q][0] = x.z; R.qf[b * 4 + 1][q][1] = x.w;
         R.qf[b * 4 + 2][q][0] = y.x; R.qf[b * 4 + 2][q][1] = y.y;
         R.qf[b * 4 + 3][q][0] = y.z; R.qf[b * 4 + 3][q][1] = y.w;
+#endif
       }
+#if FA_FEW == 1
+      R.take_queries(raw);
+#endif
       continue;
 #endif
 #pragma unroll
