@@ -184,8 +184,9 @@ __global__ void __launch_bounds__(kStepThreads) fa_page_step_kernel(const __grid
 //   row t of key and value = token t - starts[b] of request b: w scale of pages in 8 bits, rounded once, or a copy.
 //
 // A block takes a run of tokens: it finds their requests and pages (the requests that end in front of the first are counted by all threads, the
-// others are walked through from there), then goes through their rows in pieces of eight values, four of a thread on their way at a time.
-constexpr int kReadThreads = 256, kReadTokens = 16, kReadEight = 3;  // (kReadEight: the type of pages in 8 bits, beside FA_F16, FA_BF16 and FA_F32)
+// others are walked through from there), then goes through their rows, a group of lanes to a row and 16 bytes of it to a lane, four rows of a lane on their way at a
+// time.  Rows of tokens beside each other, which lie one behind the other in a page, are in groups beside each other.
+constexpr int kReadThreads = 256, kReadTokens = 64, kReadEight = 3;  // (kReadEight: the type of pages in 8 bits, beside FA_F16, FA_BF16 and FA_F32)
 
 struct FaReadKernelParams {
   FaRotTensor pages[2], out[2];  // byte strides
@@ -193,25 +194,29 @@ struct FaReadKernelParams {
   long long scale_sp[2], scale_sh[2], scale_ss[2];
   const int *table, *starts;
   long long table_stride;
-  int B, Hkv, D[2], width, num_pages, page_size, tokens, per_block;
+  int B, Hkv, D[2], width, num_pages, page_size, tokens;
+  int token_shift, lane_shift;   // log2 of a block's tokens, of the lanes that share a row
   int* status;
 };
 
 // Four values of 8 bits: in the low byte of 2^23, which is subtracted with the 128 that makes them positive.
-__device__ __forceinline__ void read_four(unsigned w, float scale, float* f) {
+__device__ __forceinline__ void read_four(unsigned w, F2 scale, F2* f) {
   w ^= 0x80808080u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | i)) - 8388736.f) * scale;
+  const auto at = [&](int i) { return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | i)); };
+  const F2 one = f2(1.f, 1.f), bias = f2(-8388736.f, -8388736.f);
+  f[0] = fma(f2(at(0), at(1)), one, bias) * scale;
+  f[1] = fma(f2(at(2), at(3)), one, bias) * scale;
 }
 
+// PIECES: 16 bytes of the pages at a time; else value by value
 template <int IN, int OUT, bool PIECES>
 __global__ void __launch_bounds__(kReadThreads) fa_read_pages_kernel(const __grid_constant__ FaReadKernelParams P) {
   grid_wait();
   constexpr bool EIGHT = IN == kReadEight;
-  constexpr int V = PIECES ? 8 : 1, ES = OUT == FA_F32 ? 4 : 2, EI = EIGHT ? 1 : ES;
-  __shared__ long long page_of[kReadTokens];  // -1: the token has none
-  __shared__ int row_of[kReadTokens];
-  const int t0 = blockIdx.x * P.per_block, n = min(P.per_block, P.tokens - t0), tid = threadIdx.x;
+  constexpr int ES = OUT == FA_F32 ? 4 : 2, EI = EIGHT ? 1 : ES, V = PIECES ? 16 / EI : 1, U = 4;
+  __shared__ long long from_of[kReadTokens], scale_of[kReadTokens];  // where a token's row of head 0 is; below 0: it has none
+  const int kind = blockIdx.y;  // keys or values
+  const int t0 = blockIdx.x << P.token_shift, n = min(1 << P.token_shift, P.tokens - t0), tid = threadIdx.x;
   int before = 0;
   for (int b0 = 0; b0 < P.B; b0 += kReadThreads) before += __syncthreads_count(b0 + tid < P.B && P.starts[min(b0 + tid, P.B - 1) + 1] <= t0);
   if (tid < n) {
@@ -229,63 +234,61 @@ __global__ void __launch_bounds__(kReadThreads) fa_read_pages_kernel(const __gri
         if (P.status != nullptr) atomicOr(P.status, FA_STATUS_BAD_PAGE);
       }
     }
-    page_of[tid] = page;
-    row_of[tid] = row;
+    from_of[tid] = page < 0 ? -1 : page * P.pages[kind].sb + row * P.pages[kind].ss;
+    if (EIGHT) scale_of[tid] = page < 0 ? 0 : page * P.scale_sp[kind] + row * P.scale_ss[kind];
   }
   __syncthreads();
+  const int groups = kReadThreads >> P.lane_shift, lane = tid & ((1 << P.lane_shift) - 1), rows = P.Hkv << P.token_shift, D = P.D[kind];
+  const FaRotTensor src = P.pages[kind], dst = P.out[kind];
+  const float* const scales = P.scales[kind];
+  const long long scale_sh = P.scale_sh[kind];
 #pragma unroll 1
-  for (int kind = 0; kind < 2; ++kind) {
-    const FaRotTensor& src = P.pages[kind];
-    const FaRotTensor& dst = P.out[kind];
-    const int C = P.D[kind] / V, all = P.Hkv * n * C;
-    constexpr int U = 4, WORDS = V * EI <= 4 ? 1 : V * EI / 4;
+  for (int r0 = tid >> P.lane_shift; r0 < rows; r0 += U * groups) {
 #pragma unroll 1
-    for (int i0 = tid; i0 < all; i0 += U * kReadThreads) {
-      unsigned raw[U][WORDS];
+    for (int c = lane;; c += 1 << P.lane_shift) {
+      if (c * V >= D) break;
+      uint4 raw[U];
       float scale[U];
       char* to[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {  // (all of them on their way at once)
-        const int i = i0 + u * kReadThreads, row = i / C, c = i - row * C, h = row / n, t = row - h * n;
+        const int r = r0 + u * groups, t = r & ((1 << P.token_shift) - 1), h = r >> P.token_shift;
         to[u] = nullptr;
+        raw[u] = make_uint4(0, 0, 0, 0);
         scale[u] = 0.f;
-#pragma unroll
-        for (int w = 0; w < WORDS; ++w) raw[u][w] = 0u;
-        if (i >= all) continue;
-        to[u] = dst.ptr + h * dst.sh + (t0 + t) * dst.ss + (long long)c * V * ES;
-        const long long page = page_of[t];
-        if (page < 0) continue;
-        const char* from = src.ptr + page * src.sb + h * src.sh + row_of[t] * src.ss + (long long)c * V * EI;
-        if (EIGHT) scale[u] = P.scales[kind][page * P.scale_sp[kind] + h * P.scale_sh[kind] + row_of[t] * P.scale_ss[kind]];
-        if (!PIECES) raw[u][0] = EI == 1 ? (unsigned)*(const unsigned char*)from : EI == 2 ? (unsigned)*(const unsigned short*)from : *(const unsigned*)from;
-        else if (EI == 1) *(uint2*)raw[u] = *(const uint2*)from;
-        else
-#pragma unroll
-          for (int w = 0; w < WORDS; w += 4) *(uint4*)&raw[u][w] = *(const uint4*)(from + w * 4);
+        if (r >= rows || t >= n) continue;
+        to[u] = dst.ptr + h * dst.sh + (t0 + t) * dst.ss + c * V * ES;
+        const long long at = from_of[t];
+        if (at < 0) continue;
+        const char* from = src.ptr + at + h * src.sh + c * V * EI;
+        if (EIGHT) scale[u] = scales[scale_of[t] + h * scale_sh];
+        if (PIECES) raw[u] = *(const uint4*)from;
+        else raw[u].x = EI == 1 ? (unsigned)*(const unsigned char*)from : EI == 2 ? (unsigned)*(const unsigned short*)from : *(const unsigned*)from;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (to[u] == nullptr) continue;
         if constexpr (!EIGHT) {
-          if (!PIECES) {
-            if (ES == 2) *(unsigned short*)to[u] = (unsigned short)raw[u][0];
-            else *(unsigned*)to[u] = raw[u][0];
-          } else {
-#pragma unroll
-            for (int w = 0; w < WORDS; w += 4) *(uint4*)(to[u] + w * 4) = *(const uint4*)&raw[u][w];
-          }
+          if (PIECES) *(uint4*)to[u] = raw[u];
+          else if (ES == 2) *(unsigned short*)to[u] = (unsigned short)raw[u].x;
+          else *(unsigned*)to[u] = raw[u].x;
         } else {
-          float f[8];
-          read_four(raw[u][0], scale[u], f);
+          const F2 s = f2(scale[u], scale[u]);
+          F2 f[8];
+          read_four(raw[u].x, s, f);
           if (!PIECES) {
-            rot_put<OUT>(to[u], 0, f[0]);
+            float x, y;
+            f2_get(f[0], x, y);
+            rot_put<OUT>(to[u], 0, x);
           } else {
-            read_four(raw[u][WORDS - 1], scale[u], f + 4);
+            read_four(raw[u].y, s, f + 2);
+            read_four(raw[u].z, s, f + 4);
+            read_four(raw[u].w, s, f + 6);
 #pragma unroll
-            for (int w = 0; w < 8 * ES / 16; ++w) {
+            for (int w = 0; w < ES; ++w) {
               F2 g[kRotPairs<OUT>];
 #pragma unroll
-              for (int k = 0; k < kRotPairs<OUT>; ++k) g[k] = f2(f[w * kRotVec<OUT> + 2 * k], f[w * kRotVec<OUT> + 2 * k + 1]);
+              for (int k = 0; k < kRotPairs<OUT>; ++k) g[k] = f[w * kRotPairs<OUT> + k];
               *(uint4*)(to[u] + w * 16) = rot_pack<OUT>(g);
             }
           }
@@ -445,7 +448,7 @@ void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   long long keys = (long long)p->table_width * p->page_size;
   if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + p->Sq + c.WN);
   const long long segments = (long long)p->B * p->Hkv, sms = device_sm_count();
-  const int most = c.eight ? (c.few == 1 ? 3 : 2) : c.RG > 1 || (f32 ? c.fr > 8 : c.few != 1 && p->D > 64) ? 2 : c.few == 1 || f32 ? 4 : 3;  // CTAs of an SM
+  const int most = c.eight ? (c.few > 1 || p->D > 128 ? 2 : p->D > 64 ? 3 : 4) : c.RG > 1 || (f32 ? c.fr > 8 : c.few != 1 && p->D > 64) ? 2 : c.few == 1 || f32 ? 4 : 3;  // CTAs of an SM
   // as many as there is room for with `slots`
   const auto fit = [&](int slots) {
     for (c.per_sm = most; c.per_sm > 1 && smem(slots) > 227 * 1024 / c.per_sm - 1024;) --c.per_sm;
@@ -603,14 +606,15 @@ int fa_read_pages(const fa_read_params* p, void* stream) {
   memset(&k, 0, sizeof k);
   const int es = esize(p->dtype), ei = eight ? 1 : es;
   const fa_tensor *from[2] = {&p->k_pages, &p->v_pages}, *to[2] = {&p->k, &p->v}, *scales[2] = {&p->k_scales, &p->v_scales};
-  bool pieces = p->D % 8 == 0 && p->Dv % 8 == 0;
+  const int v = 16 / ei;
+  bool pieces = p->D % v == 0 && p->Dv % v == 0;
   for (int i = 0; i < 2; ++i) {
     k.pages[i] = rot_tensor(*from[i], ei);
     k.out[i] = rot_tensor(*to[i], es);
     k.out[i].sb = 0;
     k.scales[i] = (const float*)scales[i]->ptr;
     k.scale_sp[i] = scales[i]->stride_b; k.scale_sh[i] = scales[i]->stride_h; k.scale_ss[i] = scales[i]->stride_s;
-    pieces = pieces && rot_aligned(k.pages[i], eight ? 8 : 16) && rot_aligned(k.out[i]);
+    pieces = pieces && rot_aligned(k.pages[i]) && rot_aligned(k.out[i]);
   }
   k.D[0] = p->D; k.D[1] = p->Dv;
   k.table = p->block_table; k.table_stride = p->block_table_stride; k.width = p->table_width;
@@ -618,9 +622,9 @@ int fa_read_pages(const fa_read_params* p, void* stream) {
   k.num_pages = (int)p->num_pages; k.page_size = p->page_size; k.tokens = (int)p->num_tokens;
   k.status = p->status;
   // As many tokens of a block as leave four blocks per SM: the search for the requests is paid once for them.
-  k.per_block = kReadTokens;
-  while (k.per_block > 1 && p->num_tokens / k.per_block < 4LL * device_sm_count()) k.per_block /= 2;
-  const dim3 grid((unsigned)((p->num_tokens + k.per_block - 1) / k.per_block));
+  while (1 << k.token_shift < kReadTokens && (p->num_tokens >> (k.token_shift + 1)) >= 3LL * device_sm_count()) ++k.token_shift;
+  while (1 << k.lane_shift < 32 && (pieces ? v : 1) << k.lane_shift < std::max(p->D, p->Dv)) ++k.lane_shift;
+  const dim3 grid((unsigned)((p->num_tokens + (1ll << k.token_shift) - 1) >> k.token_shift), 2);
   return rot_dispatch(p->dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     void (*const fns[2][2])(FaReadKernelParams) = {{fa_read_pages_kernel<DT, DT, false>, fa_read_pages_kernel<DT, DT, true>},

@@ -358,30 +358,51 @@ __device__ __forceinline__ unsigned rot_size(unsigned most, F2 v) {  // (as bits
   f2_get(v, x, y);
   return max(most, max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu));
 }
-__device__ __forceinline__ float rot_scale(unsigned most) { return most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(most) / 127.f; }
-__device__ __forceinline__ int rot_whole(float y, float scale) { return scale > 0.f ? (int)fminf(fmaxf(rintf(y / scale), -127.f), 127.f) : 0; }
-// Four values.  y times 1 / scale, added to 1.5 * 2^23, has the whole number in its low byte.  It is off by less than 5e-5 (127 times the errors of
-// the reciprocal and of the product, 2^-23 at most each), so only what that brings near a tie is divided; and all where the reciprocal may overflow.
-__device__ __forceinline__ unsigned rot_eight(F2 a, F2 b, float scale, float inverse) {
-  constexpr float kMagic = 12582912.f;
-  const F2 m = f2(kMagic, kMagic), r = f2(inverse, inverse), minus = f2(-1.f, -1.f);
-  const F2 na = fma(a, r, m), nb = fma(b, r, m);
-  const F2 da = fma(a, r, fma(na, minus, m)), db = fma(b, r, fma(nb, minus, m));
-  float v[4], d[4];
-  f2_get(na, v[0], v[1]);
-  f2_get(nb, v[2], v[3]);
-  f2_get(da, d[0], d[1]);
-  f2_get(db, d[2], d[3]);
-  if (scale >= 1e-30f && fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3]))) < 0.4999f)
-    return __byte_perm(__byte_perm(__float_as_uint(v[0]), __float_as_uint(v[1]), 0x0040), __byte_perm(__float_as_uint(v[2]), __float_as_uint(v[3]), 0x0040), 0x5410);
-  f2_get(a, v[0], v[1]);
-  f2_get(b, v[2], v[3]);
-  unsigned w = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w |= (unsigned)(rot_whole(v[i], scale) & 0xff) << (8 * i);
-  return w;
+// Quotients as an fp32 division rounds them: the product with the reciprocal, itself rounded to nearest, and once more with what that left (Markstein's theorem on the
+// last step of a quotient), three instructions for two values.  Where nothing underflows: below 2^-100 by a division.
+constexpr float kRotTiny = 7.9e-31f;
+__device__ __forceinline__ float rot_scale(unsigned most) {
+  if (most >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
+  const float a = __uint_as_float(most);
+  if (a < kRotTiny) return a / 127.f;
+  const float q = a * (1.f / 127.f);
+  return fmaf(fmaf(-127.f, q, a), 1.f / 127.f, q);
 }
-
+__device__ __forceinline__ int rot_whole(float y, float scale) { return scale > 0.f ? (int)fminf(fmaxf(rintf(y / scale), -127.f), 127.f) : 0; }
+// A lane's two pieces.  A quotient added to 1.5 * 2^23 has the whole number in its low byte.  (By divisions of what is near a tie only, which a warp has in every
+// tenth row, 8000 tokens took 64 us, 40 without any; an IEEE division is some 30 instructions.)
+template <int N>
+__device__ __forceinline__ void rot_eight(F2 (&x)[N], F2 (&y)[N], float scale, uint2& to_x, uint2& to_y) {
+  static_assert(N == 4, "eight values of each piece");
+  if (scale < kRotTiny && scale > 0.f) {  // the same quotients 2^100 higher up; one of subnormals may be beyond 127
+    constexpr float kUp = 1.2676506e30f;
+    scale *= kUp;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float a, b;
+      f2_get(x[i], a, b);
+      x[i] = f2(fminf(fmaxf(a * kUp, -127.f * scale), 127.f * scale), fminf(fmaxf(b * kUp, -127.f * scale), 127.f * scale));
+      f2_get(y[i], a, b);
+      y[i] = f2(fminf(fmaxf(a * kUp, -127.f * scale), 127.f * scale), fminf(fmaxf(b * kUp, -127.f * scale), 127.f * scale));
+    }
+  }
+  const float inverse = __frcp_rn(scale);
+  const F2 r = f2(inverse, inverse), minus = f2(-scale, -scale), one = f2(1.f, 1.f), magic = f2(12582912.f, 12582912.f);
+  unsigned w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const F2 a = i < 2 ? x[2 * i + k] : y[2 * i - 4 + k], q = a * r;
+      f2_get(fma(fma(fma(q, minus, a), r, q), one, magic), v[2 * k], v[2 * k + 1]);
+    }
+    w[i] = __byte_perm(__byte_perm(__float_as_uint(v[0]), __float_as_uint(v[1]), 0x0040), __byte_perm(__float_as_uint(v[2]), __float_as_uint(v[3]), 0x0040), 0x5410);
+    if (!(scale > 0.f)) w[i] = 0u;
+  }
+  to_x = make_uint2(w[0], w[1]);
+  to_y = make_uint2(w[2], w[3]);
+}
 // Two 16-byte pieces of a row per lane: the two that hold its pairs.  A thread keeps the angles of its token, times the weights, in
 // registers for all heads of its group, and the lanes of a warp beside each other are tokens beside each other.  Four rows are computed
 // while the next four are on their way.
@@ -440,6 +461,101 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
   }
   char* dst = P.y[kind].ptr + to;
   const float per_value = 1.f / P.D;
+  if constexpr (Q8) {
+    if (eight) {
+      // Two rows at a time, side by side, with nothing that branches between them: the shuffles of one are waited for under the other's.
+      for (int h = at.h0; h < at.h1; h += 2) {
+        uint4 ra[2], rb[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          ra[u] = na[u];
+          rb[u] = nb[u];
+          na[u] = na[u + 2];
+          nb[u] = nb[u + 2];
+        }
+        if (((h - at.h0) & 2) && h + 2 < at.h1) load(h + 2);
+        F2 x[2][N], y[2][N];
+        float ss[2] = {0.f, 0.f};
+        unsigned most[2] = {0u, 0u};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          rot_unpack<DT>(ra[u], x[u]);
+          rot_unpack<DT>(rb[u], y[u]);
+          if (norm) {
+            F2 sum = x[u][0] * x[u][0];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              if (i > 0) sum = fma(x[u][i], x[u][i], sum);
+              sum = fma(y[u][i], y[u][i], sum);
+            }
+            ss[u] = both(sum);
+          }
+        }
+        if (norm) rot_sums(ss, P.lane_shift);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float r = norm ? rsqrtf(ss[u] * per_value + P.eps) : 1.f;
+          const F2 rr = f2(r, r);
+          if (norm) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              x[u][i] = x[u][i] * rr;
+              y[u][i] = y[u][i] * rr;
+            }
+          }
+          if (kind == 2) {  // (as they are)
+          } else if constexpr (MODE == kAny) {
+            F2 ox[N], oy[N];
+            uint4* const mine = planes[threadIdx.x >> 5];
+            __syncwarp();  // (the row before has been read)
+            mine[threadIdx.x & 31] = ra[u];
+            mine[32 + (threadIdx.x & 31)] = rb[u];
+            __syncwarp();
+            if (turns) {
+              const int lane0 = (threadIdx.x & 31) - at.lane;
+              rot_others<DT>(P, mine, 32, lane0, ca, ox);
+              rot_others<DT>(P, mine, 32, lane0, cb, oy);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              x[u][i] = x[u][i] * f.pa[i];
+              y[u][i] = y[u][i] * f.pb[i];
+              if (!turns) continue;
+              x[u][i] = fma(ox[i] * rr, f.qa[i], x[u][i]);
+              y[u][i] = fma(oy[i] * rr, f.qb[i], y[u][i]);
+            }
+          } else if constexpr (MODE == kNeighboursAny) {
+            rot_turn_any<V>(P, ca, x[u], f.pa, f.qa);
+            rot_turn_any<V>(P, cb, y[u], f.pb, f.qb);
+          } else {
+            rot_turn<V, MODE>(x[u], y[u], f);
+          }
+#pragma unroll
+          for (int i = 0; i < N; ++i) most[u] = rot_size(rot_size(most[u], x[u][i]), y[u][i]);
+        }
+        for (int off = 1 << P.lane_shift >> 1; off > 0; off >>= 1) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) most[u] = max(most[u], __shfl_xor_sync(0xffffffffu, most[u], off));
+        }
+        float scale[2];
+        uint2 wa[2], wb[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          scale[u] = rot_scale(most[u]);
+          rot_eight(x[u], y[u], scale[u], wa[u], wb[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (h + u >= at.h1) break;
+          char* row = dst + (h + u) * P.y[kind].sh;
+          if (have_a) *(uint2*)(row + ca * 8) = wa[u];
+          if (have_b) *(uint2*)(row + cb * 8) = wb[u];
+          if (to >= 0 && at.lane == 0) P.scales[kind - 1][scale_at + (h + u) * P.scale_sh[kind - 1]] = scale[u];
+        }
+      }
+      return;
+    }
+  }
   for (int h = at.h0; h < at.h1; h += U) {
     uint4 ra[U], rb[U];
 #pragma unroll
@@ -481,7 +597,7 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
           rot_others<DT>(P, mine, 32, lane0, cb, oy);
         }
       }
-      if (norm || turns || eight) {
+      if (norm || turns) {
         F2 x[N], y[N];
         rot_unpack<DT>(ra[u], x);
         rot_unpack<DT>(rb[u], y);
@@ -494,8 +610,7 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
             y[i] = y[i] * rr;
           }
         }
-        if (Q8 && kind == 2) {  // (as they are)
-        } else if constexpr (MODE == kAny) {
+        if constexpr (MODE == kAny) {
           const F2 rr = f2(r, r);
 #pragma unroll
           for (int i = 0; i < N; ++i) {
@@ -510,20 +625,6 @@ __global__ void __launch_bounds__(kRotThreads, 2) fa_rotary_kernel(const __grid_
           rot_turn_any<V>(P, cb, y, f.pb, f.qb);
         } else {
           rot_turn<V, MODE>(x, y, f);
-        }
-        if constexpr (Q8) {
-          if (eight) {
-            unsigned most = 0;
-#pragma unroll
-            for (int i = 0; i < N; ++i) most = rot_size(rot_size(most, x[i]), y[i]);
-            for (int off = 1 << P.lane_shift >> 1; off > 0; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
-            const float scale = rot_scale(most), inverse = 1.f / scale;
-            char* row = dst + (h + u) * P.y[kind].sh;
-            if (have_a) *(uint2*)(row + ca * 8) = make_uint2(rot_eight(x[0], x[1], scale, inverse), rot_eight(x[N - 2], x[N - 1], scale, inverse));
-            if (have_b) *(uint2*)(row + cb * 8) = make_uint2(rot_eight(y[0], y[1], scale, inverse), rot_eight(y[N - 2], y[N - 1], scale, inverse));
-            if (to >= 0 && at.lane == 0) P.scales[kind - 1][scale_at + (h + u) * P.scale_sh[kind - 1]] = scale;
-            continue;
-          }
         }
         const uint4 pa = rot_pack<DT>(x), pb = rot_pack<DT>(y);
         ra[u] = MODE >= kNeighboursAny && !norm ? rot_keep<DT>(P, ca, pa, ra[u]) : pa;
