@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kReadThreads) fa_read_pages_kernel(const __gri
         if (at < 0) continue;
         const char* from = src.ptr + at + h * src.sh + c * V * EI;
         if (EIGHT) scale[u] = scales[scale_of[t] + h * scale_sh];
-        if (PIECES) raw[u] = *(const uint4*)from;
+        if (PIECES) raw[u] = __ldcs((const uint4*)from);
         else raw[u].x = EI == 1 ? (unsigned)*(const unsigned char*)from : EI == 2 ? (unsigned)*(const unsigned short*)from : *(const unsigned*)from;
       }
 #pragma unroll
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kReadThreads) fa_read_pages_kernel(const __gri
               F2 g[kRotPairs<OUT>];
 #pragma unroll
               for (int k = 0; k < kRotPairs<OUT>; ++k) g[k] = f[w * kRotPairs<OUT> + k];
-              *(uint4*)(to[u] + w * 16) = rot_pack<OUT>(g);
+              __stcs((uint4*)(to[u] + w * 16), rot_pack<OUT>(g));
             }
           }
         }

@@ -61,9 +61,8 @@ def test_lengths_and_pages(dtype, D, page):
     run(1, LENGTHS, 4, 2, 1, D, page, dtype)
 
 
-@pytest.mark.parametrize("page", [16, 6])
-@pytest.mark.parametrize("D,Dv", [(16, 16), (32, 16), (48, 48), (80, 80), (96, 96), (112, 64), (128, 64), (192, 128), (256, 256), (256, 16)])
-def test_head_dims(D, Dv, page):
+@pytest.mark.parametrize("page,D,Dv", [(16, 16, 16), (6, 32, 16), (16, 48, 48), (6, 80, 80), (16, 96, 96), (6, 112, 64), (16, 128, 64), (16, 192, 128), (6, 256, 256), (16, 256, 16)])
+def test_head_dims(page, D, Dv):
     run(2, [1, 40, 333], 4, 4, 2, D, page, "f16", Dv=Dv)
 
 
@@ -105,8 +104,7 @@ def parity(b, h, q_idx, kv_idx):
     return (q_idx + kv_idx + h) % 2 == 0
 
 
-@pytest.mark.parametrize("score", [None, softcap, distance])
-@pytest.mark.parametrize("mask,window", [(None, None), (parity, None), (nothing, None), (None, 0), (None, 33), (None, 100)])
+@pytest.mark.parametrize("score,mask,window", [(None, parity, None), (None, nothing, None), (None, None, 0), (softcap, None, 33), (distance, None, 100), (distance, None, 33)])
 def test_mods_and_windows(score, mask, window):
     run(6, [0, 1, 70, 400], 4, 2, 3, 64, 16, "f16", score=score, mask=mask, window=window)
     run(6, [0, 1, 70, 400], 4, 2, 3, 96, 10, "bf16", score=score, mask=mask, window=window)

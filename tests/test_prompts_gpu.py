@@ -34,8 +34,8 @@ def test_lengths_and_heads(kernels, dtype, D, Hq, Hkv):
     run(1, LENGTHS, Hq, Hkv, D, dtype, kernels=kernels, pad=(3, 7))
 
 
-@pytest.mark.parametrize("dtype", ["f16", "f32"])
-@pytest.mark.parametrize("D,Dv", [(16, 16), (32, 16), (48, 48), (80, 80), (96, 96), (96, 32), (112, 64), (128, 64), (192, 128), (256, 256), (256, 16)])
+@pytest.mark.parametrize("dtype,D,Dv", [*(("f16", *x) for x in ((16, 16), (48, 48), (80, 80), (96, 32), (112, 64), (128, 64), (192, 128), (256, 256))),
+                                        *(("f32", *x) for x in ((16, 16), (96, 96), (256, 256), (256, 16)))])
 def test_head_dims(dtype, D, Dv):
     run(2, [1, 40, 333], 4, 2, D, dtype, Dv=Dv)
 
@@ -84,9 +84,8 @@ def no_odd_head(b, h, q_idx, kv_idx):
     return (h % 2 == 0) & (kv_idx >= 0)
 
 
-@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("score", [None, softcap, distance, of_request])
-@pytest.mark.parametrize("mask", [None, parity, nothing, no_odd_head])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("score,mask", [(softcap, None), (of_request, parity), (None, nothing), (distance, no_odd_head)])
 def test_mods(dtype, score, mask):
     run(6, [1, 70, 400, 200], 4, 2, 64, dtype, score=score, mask=mask)
     run(6, [1, 70, 400], 4, 2, 128, dtype, score=score, mask=mask, past=[3, 200, 0])
@@ -228,5 +227,5 @@ def test_refusals():
 @pytest.mark.parametrize("D", [96, 128])
 def test_two_query_tiles(D):
     """Long prompts at wide heads take two tiles per CTA: rows of one end in the first, between, in the second."""
-    run(19, [2300, 1900, 2101], 64, 8, D, "bf16")
-    run(20, [300, 260, 200], 32, 8, D, "f16", past=[1700, 2000, 1500], score=distance, window=1900)
+    run(19, [2300, 1900, 2101], 8, 1, D, "bf16")
+    run(20, [700, 660, 600], 24, 1, D, "f16", past=[1700, 2000, 1500], score=distance, window=1900)
