@@ -125,7 +125,7 @@ EXPORTS = [
     "fa_fwd_workspace_bytes", "fa_fwd_ws",
     "fa_rotary", "fa_rotary_bwd_workspace_bytes", "fa_rotary_bwd", "fa_rotary_append",
     "fa_page_step", "fa_read_pages", "fa_paged_workspace_bytes", "fa_paged", "fa_paged_prepare",
-    "fa_prompt", "fa_prompt_prepare",
+    "fa_prompt", "fa_prompt_prepare", "fa_prompt_workspace_bytes",
 ]
 
 
@@ -195,7 +195,9 @@ def lib() -> C.CDLL:
     L.fa_paged_workspace_bytes.argtypes = [C.POINTER(FaPagedParams)]
     L.fa_paged.argtypes = [C.c_void_p, C.POINTER(FaPagedParams), C.c_void_p, C.c_size_t, C.c_void_p]
     L.fa_paged_prepare.argtypes = [C.c_void_p, C.POINTER(FaPagedParams)]
-    L.fa_prompt.argtypes = [C.c_void_p, C.POINTER(FaPromptParams), C.c_void_p]
+    L.fa_prompt_workspace_bytes.restype = C.c_size_t
+    L.fa_prompt_workspace_bytes.argtypes = [C.POINTER(FaPromptParams)]
+    L.fa_prompt.argtypes = [C.c_void_p, C.POINTER(FaPromptParams), C.c_void_p, C.c_size_t, C.c_void_p]
     L.fa_prompt_prepare.argtypes = [C.c_void_p, C.POINTER(FaPromptParams)]
     L.fa_mask_bits_row_words.restype = C.c_int64
     L.fa_mask_bits_row_words.argtypes = [C.c_int]

@@ -1378,8 +1378,11 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.v = by_strides(v, bshd);
       p.o = by_strides(out, bshd);
       p.lse = return_lse ? lse.mutable_data_ptr<float>() : nullptr;
+      const size_t bytes = fa_prompt_workspace_bytes(&p);
+      at::Tensor ws;
+      if (bytes > 0) ws = empty({(int64_t)bytes}, at::kByte, q.device());
       BuffersLock lock(launched.module, *launched.buffers);
-      const int rc = lock.rc != FA_OK ? lock.rc : fa_prompt(launched.module, &p, (void*)c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+      const int rc = lock.rc != FA_OK ? lock.rc : fa_prompt(launched.module, &p, bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, (void*)c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
       if (rc != FA_OK) raise(rc);
     }
   }

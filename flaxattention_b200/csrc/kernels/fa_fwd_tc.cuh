@@ -47,7 +47,7 @@
 // status word, all roles leave their loops, TMEM is freed and the kernel returns.
 //
 // Requests of different lengths (FA_TC_PACKED, fa_packed_rows.cuh): 1, prompts laid end to end; 2, the newest tokens of many requests over a prefix that they
-// share, a part of it per CTA (kv heads, row tiles, parts).  A row is a (token, head of the group): its query is loaded and its result
+// share, in parts; 3, prompts in parts.  (Parts: a CTA goes through a share of its rows' keys, and what it has is joined with the others' by fa_merge_kernel.)  A row is a (token, head of the group): its query is loaded and its result
 // stored by the threads of its warp, and the steps are those of the keys that any row sees, with no tables: a tile that all rows see whole is a
 // plain step, another one applies each row's range of keys.  K and V are read as [tokens, heads] by one map each; what the last tile of a
 // request has behind its keys is the next request's, perhaps no number, so the idle warp writes zeros over those rows of V.  Head dims below FA_D are
@@ -78,7 +78,7 @@ typedef FaParams FaTcProblem;
 
 namespace fa_tc {
 
-constexpr bool PACKED = FA_TC_PACKED != 0, PREFIX = FA_TC_PACKED == 2;
+constexpr bool PACKED = FA_TC_PACKED != 0, PREFIX = FA_TC_PACKED == 2, PARTS = FA_TC_PACKED >= 2;
 
 constexpr bool F32 = FA_DTYPE == FA_DT_F32;
 constexpr int DT = F32 ? FA_DT_BF16 : FA_DTYPE;  // type of the tensor-core operands
@@ -324,9 +324,9 @@ struct Plan {
       last = max(last, tile[i].y);
     }
     if (last == 0) first = 0;
-    if (PREFIX) {  // this CTA's part
+    if (PARTS) {  // this CTA's part
       const int per = (last - first + p.splits - 1) / p.splits;
-      first = min(first + (int)blockIdx.z * per, last);
+      first = min(first + (int)(blockIdx.x / p.Hkv) * per, last);
       last = min(first + per, last);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) tile[i].y = min(tile[i].y, last);
@@ -737,7 +737,7 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
   volatile int* misc = (volatile int*)(sm + OFF_MISC);  // [0] tmem base, [1] abort, [2] nsteps
 #if FA_TC_PACKED
   // ---- set-up: this CTA's rows, barriers, TMEM, the steps ------------------------------------
-  const int hk = blockIdx.x, G = p.Hq / p.Hkv;
+  const int hk = PARTS ? blockIdx.x % p.Hkv : blockIdx.x, G = p.Hq / p.Hkv;
   Plan* const plan = (Plan*)(sm + OFF_PLAN);
   int* const bounds = (int*)(sm + OFF_CLS);  // (prefix) of each query tile: first key that a row sees, one behind the last, the same of what all see
   if (warp == 0) {
@@ -1470,9 +1470,13 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
         const FaPlace place = plan->place;
         mine = fa_row<PREFIX>(p, place, place.first + tid);  // (again: it has not been kept through the steps)
         const bool there = mine.at >= 0;
-        if (PREFIX) {
-          const long long part = ((long long)blockIdx.z * p.Hkv + hk) * p.tokens * G + place.first + tid;
-          if (there) *(float2*)(p.part_ml + part * 2) = make_float2(m_ref, none ? 0.f : l);
+        if (PARTS) {
+          // The sums leave through this warp's quarter of the K and V buffers, which nothing reads any more, a row at a time.  (Each thread storing its own row: 9 MB of parts
+          // took 5 us more.)
+          static_assert(!PARTS || NQ == 1, "the buffers are one query tile's");
+          const long long part = (long long)blockIdx.x * p.tokens * G + (long long)place.q0 * G + place.first;  // (blockIdx.x: parts, kv heads)
+          if (there) *(float2*)(p.part_ml + (part + tid) * 2) = make_float2(m_ref, none ? 0.f : l);
+          unsigned char* const mine_at = sm + OFF_K + warp * 32 * D * 4;
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             float o[32];
@@ -1482,8 +1486,15 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
             }
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              if (there && c * 32 + e < p.Dv) *(float4*)(p.part_o + part * p.Dv + c * 32 + e) = cnt > 0 && !none ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+              *(float4*)(mine_at + lane * D * 4 + (((c * 8 + e / 4) ^ (lane & 7)) << 4)) = cnt > 0 && !none ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
+          __syncwarp();
+          constexpr int CPR = D / 4, STEP = 32 / CPR;  // 16-byte pieces of a row, rows at a time
+          const int rows = place.n * G - place.first - warp * 32, k = lane % CPR;
+          float* const to = p.part_o + (part + warp * 32) * p.Dv + k * 4;
+#pragma unroll 8
+          for (int row = lane / CPR; row < 32; row += STEP)
+            if (row < rows && k * 4 < p.Dv) *(float4*)(to + (long long)row * p.Dv) = *(const float4*)(mine_at + row * D * 4 + ((k ^ (row & 7)) << 4));
         } else {
           // The rows leave through this warp's rows of the query tile, which nothing reads any more (every S product of the tile is complete), in whole lines.
 #pragma unroll

@@ -2,7 +2,7 @@
 // that is a multiple of 16, fp16 / bf16 / fp32, any strides of 16 bytes.  (fa_fwd_tc.cuh has the one for 16-bit types and head dims up to 128.)
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(score_mod(scale q_i.k_j) - max) over the keys j of query i's request that are not behind it, not
-//   further back than the window and kept by mask_mod;  lse_i = log sum_j p_ij + max.  Over a prefix: the sums and the maximum, for fa_prefix_merge_kernel.
+//   further back than the window and kept by mask_mod;  lse_i = log sum_j p_ij + max.  Over a prefix: the sums and the maximum, for fa_merge_kernel.
 //
 // A CTA takes 64 rows (fa_packed_rows.cuh) in four warps of 16, and their keys in tiles of FA_BN, the next one on its way while one is computed.  16-bit types
 // multiply with mma.sync and fp32 sums, fp32 with FMAs.
@@ -30,9 +30,9 @@ extern "C" __global__ void __launch_bounds__(fa_pk::NT) fa_packed_kernel(const _
   FA_MOD_BUFS_INIT(p);
   fa_grid_wait();
   if (PREFIX) fa_grid_release();  // (the pages' kernel runs beside this one)
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hk = blockIdx.x, G = p.Hq / p.Hkv;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hk = PREFIX ? blockIdx.x % p.Hkv : blockIdx.x, G = p.Hq / p.Hkv;
   if (PREFIX) {
-    if (tid == 0) found = {0, p.tokens, 0, p.keys, 0, (int)blockIdx.y * BM, 1};  // (grid: kv heads, items, parts of the prefix)
+    if (tid == 0) found = {0, p.tokens, 0, p.keys, 0, (int)blockIdx.y * BM, 1};  // (grid: parts of the prefix and kv heads, items)
   } else {
     const long long item = (long long)blockIdx.z * gridDim.y + blockIdx.y;
     if (warp == 0) {
@@ -92,7 +92,7 @@ extern "C" __global__ void __launch_bounds__(fa_pk::NT) fa_packed_kernel(const _
   int t0 = to > 0 ? from / BN : 0, t1 = (to + BN - 1) / BN;
   if (PREFIX) {  // this CTA's part of the tiles
     const int per = (t1 - t0 + p.splits - 1) / p.splits;
-    t0 = min(t0 + (int)blockIdx.z * per, t1);
+    t0 = min(t0 + (int)(blockIdx.x / p.Hkv) * per, t1);
     t1 = min(t0 + per, t1);
   }
   auto load_kv = [&](int stage, int n0) {
@@ -255,7 +255,7 @@ extern "C" __global__ void __launch_bounds__(fa_pk::NT) fa_packed_kernel(const _
     const int rl = warp * 16 + h * 8 + (lane >> 2);
     if (PREFIX) {
       if (row[h].at < 0) continue;
-      const long long part = ((long long)blockIdx.z * p.Hkv + hk) * p.tokens * G + place.first + rl;
+      const long long part = (long long)blockIdx.x * p.tokens * G + place.first + rl;
       if ((lane & 3) == 0) *(float2*)(p.part_ml + part * 2) = make_float2(m[h], l[h]);
 #pragma unroll
       for (int dj = 0; dj < DV / 8; ++dj) *(float2*)(p.part_o + part * DV + dj * 8 + (lane & 3) * 2) = make_float2(o[dj][h * 2], o[dj][h * 2 + 1]);

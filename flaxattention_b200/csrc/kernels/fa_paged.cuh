@@ -42,7 +42,7 @@
 //
 // Compile-time parameters (macros): FA_DTYPE, FA_D, FA_DV, FA_RG (1, 2, 4), FA_WN (keys of a tile: 32 or 16; fp32: 32, 16, 8), FA_SLOTS, FA_TMA,
 // FA_FEW (0: the other way), FA_FR (fp32: rows of a warp), FA_CG, FA_SHORT, FA_KV8, FA_AFTER (the keys lie behind a prefix, over which
-// another kernel goes: results in float32 with their sums, for fa_prefix_merge_kernel).
+// another kernel goes: results in float32 with their sums, for fa_merge_kernel).
 #pragma once
 #include "fa_sm100.cuh"
 

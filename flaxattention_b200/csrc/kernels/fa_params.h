@@ -116,8 +116,8 @@ struct FaPagedParams {
 struct FaPackedParams {
   FaTensor q, k, v, o;     // prompts: ss is the stride of a token, sb is not used
   float* lse;              // prompts: [Hq, tokens] or null
-  float* part_o;           // prefix: [splits, Hkv, tokens * G, Dv] not divided, G = Hq / Hkv
-  float* part_ml;          // prefix: [splits, Hkv, tokens * G, 2] maximum (log2 units) and sum
+  float* part_o;           // parts: [splits, Hkv, tokens * G, Dv] not divided, G = Hq / Hkv
+  float* part_ml;          // parts: [splits, Hkv, tokens * G, 2] maximum (log2 units) and sum
   const int* starts;       // prompts: [B + 1] where the queries of each request begin
   const int* key_starts;   // prompts: [B + 1] where its keys begin
   const int* lengths;      // prefix: [B] tokens that each request has behind the prefix, the Sq newest included

@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) fa_paged_combin
   }
   const float m_use = m == -INFINITY ? 0.f : m;
   const float inv = l > 0.f ? 1.f / l : l;  // (0 and no number stay)
-  if (p.out_ml != nullptr) {  // (behind a prefix: fa_prefix_merge_kernel goes on from here)
+  if (p.out_ml != nullptr) {  // (behind a prefix: fa_merge_kernel goes on from here)
     float* const to = (float*)p.o.ptr + (long long)b * p.o.sb + (long long)h * p.o.sh + (long long)q * p.o.ss;
     if (active) *(float4*)(to + lane * 4) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     if (second) *(float4*)(to + lane * 4 + 128) = make_float4(acc2.x * inv, acc2.y * inv, acc2.z * inv, acc2.w * inv);
@@ -709,7 +709,7 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
     workspace = at;
     if (int rc = launch_prefix(m, p, po, pml, stream)) return rc;
     if (int rc = launch_paged(m, p, c, L, workspace, rows, stream)) return rc;
-    return launch_prefix_merge(p, po, pml, own, k.out_ml, (int)parts, stream);
+    return launch_merge(p->dtype, FaMergeParams{po, pml, own, k.out_ml, cvt(p->o), p->lse, p->B, p->Hq, p->Hkv, p->Sq, p->Dv, (int)parts}, stream);
   }
   return launch_paged(m, p, c, L, workspace, rows, stream);
 }

@@ -1,5 +1,5 @@
 // Attention of prompts laid end to end (fa_prompt) and over a prefix that requests share (the first of the two parts of fa_paged with one; the other is the
-// pages', and fa_prefix_merge_kernel joins them).  Kernels: kernels/fa_packed.cuh.  Part of flaxattn.cu.
+// pages', and fa_merge_kernel joins them).  Kernels: kernels/fa_packed.cuh.  Part of flaxattn.cu.
 namespace {
 
 FaDiv divide_by(int d) {
@@ -38,12 +38,13 @@ struct FaTcPackedHost {
 bool packed_tc_takes(const PackedShape& s, long long keys) {
   return s.dtype != FA_F32 && s.D <= 128 && s.scale > 0.f && keys > 0 && keys <= 1 << 23 && !(s.flags & FA_FLAG_GENERAL_KERNELS);
 }
-int get_packed_tc_kernel(fa_module* m, const PackedShape& s, bool prefix, int nq, Kernel** k) {
+// variant: 1 prompts, 2 over a prefix, 3 prompts in parts
+int get_packed_tc_kernel(fa_module* m, const PackedShape& s, int variant, int nq, Kernel** k) {
   // (must match the shared-memory map of fa_fwd_tc.cuh)
   const int D = s.D <= 64 ? 64 : 128, atoms = D / 64, nstage = D == 64 ? nq + 1 : nq;
   const int smem = nq * atoms * 16384 + 2 * nstage * atoms * 16384 + (1 + 4 * nstage + 14) * 8 + 16 + (256 + 4) * 4 + 2 * 256 + (256 / 32) * 4 + 1024;
-  return get_kernel(m, kernel_key(kIdPackedTc, {{s.dtype, 2}, {D, 9}, {nq, 2}, {prefix ? 1 : 0, 1}}), "fa_fwd_tc.cuh",
-                    [&] { return packed_math(s) + defs({{"FA_DTYPE", s.dtype}, {"FA_D", D}, {"FA_ROUND_SCORES", 0}, {"FA_TC_DECODE", 0}, {"FA_TC_NQ", nq}, {"FA_TC_PACKED", prefix ? 2 : 1}}); },
+  return get_kernel(m, kernel_key(kIdPackedTc, {{s.dtype, 2}, {D, 9}, {nq, 2}, {variant, 2}}), "fa_fwd_tc.cuh",
+                    [&] { return packed_math(s) + defs({{"FA_DTYPE", s.dtype}, {"FA_D", D}, {"FA_ROUND_SCORES", 0}, {"FA_TC_DECODE", 0}, {"FA_TC_NQ", nq}, {"FA_TC_PACKED", variant}}); },
                     "fa_packed_tc_kernel", smem, k);
 }
 // keys and values as [tokens, heads]; false: strides that no tensor map takes
@@ -57,18 +58,19 @@ dim3 packed_grid(int heads, long long n, int rows, int B) {
   return dim3((unsigned)heads, (unsigned)y, (unsigned)((items + y - 1) / y));
 }
 
-// ---- over a prefix -----------------------------------------------------------------------------
-// The parts of a row (from the tiles of the prefix, not divided, with their maximum in log2 units and sum) and what the pages of its request gave (divided,
+// ---- parts -------------------------------------------------------------------------------------
+// The parts of a row (not divided, with their maximum in log2 units and sum) and, behind a prefix, what the pages of its request gave (divided,
 // with the same), joined:  o = sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k.  A warp per row.
+size_t merge_up(size_t n) { return (n + 255) / 256 * 256; }
 struct FaMergeParams {
   const float *part_o, *part_ml;  // [parts, Hkv, tokens * G, ..]
-  const float *own_o, *own_ml;    // [B, Hq, Sq, ..]
+  const float *own_o, *own_ml;    // [B, Hq, Sq, ..] or null
   FaTensor o;
   float* lse;
   int B, Hq, Hkv, Sq, Dv, parts;
 };
 template <int DT>
-__global__ void __launch_bounds__(128) fa_prefix_merge_kernel(const __grid_constant__ FaMergeParams p) {
+__global__ void __launch_bounds__(128) fa_merge_kernel(const __grid_constant__ FaMergeParams p) {
   grid_wait();
   const int lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), n_rows = (long long)p.B * p.Hq * p.Sq;
@@ -79,11 +81,12 @@ __global__ void __launch_bounds__(128) fa_prefix_merge_kernel(const __grid_const
   const bool active = lane * 4 < p.Dv, second = lane * 4 + 128 < p.Dv;
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
   // Weights first: lane k has those of parts k and k + 32 (there are 64 at most), so that all rows of values can be on their way at once.
-  const float2 own = *(const float2*)(p.own_ml + row * 2);
+  const float2 own = p.own_ml != nullptr ? *(const float2*)(p.own_ml + row * 2) : make_float2(-INFINITY, 0.f);
   float2 ml[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) ml[i] = lane + 32 * i < p.parts ? *(const float2*)(p.part_ml + ((lane + 32 * i) * n_rows + at) * 2) : make_float2(-INFINITY, 0.f);
-  float4 x = active ? *(const float4*)(p.own_o + row * p.Dv + lane * 4) : zero, y = second ? *(const float4*)(p.own_o + row * p.Dv + lane * 4 + 128) : zero;
+  const bool has = p.own_o != nullptr;
+  float4 x = has && active ? *(const float4*)(p.own_o + row * p.Dv + lane * 4) : zero, y = has && second ? *(const float4*)(p.own_o + row * p.Dv + lane * 4 + 128) : zero;
   // (a part that has seen nothing counts for nothing; one whose sum is no number stays so)
   float m = fmaxf(own.y == 0.f ? -INFINITY : own.x, fmaxf(ml[0].x, ml[1].x));
 #pragma unroll
@@ -126,14 +129,14 @@ int prefix_rows(const fa_paged_params* p) {
   const bool few = p->prefix_length <= 1024 && (long long)p->B * p->Sq * (p->Hq / p->Hkv) <= 64;
   return few || !packed_tc_takes(shape_of(p), p->prefix_length) ? 64 : 128;
 }
-// Parts that the prefix is cut into, at least a tile each.  As many as make a CTA for each SM: the pages' kernel runs beside them, and every part has to be written
+// Parts that the prefix is cut into, of four tiles at least (one / four, 24 x 3 queries with 400 tokens of their own behind 2000, 16 / 4 heads, D 128: 26 / 19).  As many as make a CTA for each SM: the pages' kernel runs beside them, and every part has to be written
 // and read again (us, 64 requests with 500 tokens of their own behind 8192, 32 / 8 heads, D 128, pages alone 28: half a CTA per SM 61, one 49, two 58).  Two where the rows alone make half a
 // CTA per SM or more, whose tiles then are what takes the time (500 requests: one part 189, two 155).
 int prefix_parts(const fa_paged_params* p) {
   const int R = prefix_rows(p), BN = R == 64 ? packed_bn(p->dtype, p->D) : 128;
   const long long rows = (long long)p->B * p->Sq * (p->Hq / p->Hkv), ctas = p->Hkv * ((rows + R - 1) / R), sms = device_sm_count();
-  const int tiles = (p->prefix_length + BN - 1) / BN;
-  return (int)std::max<long long>(1, std::min<long long>(std::min(tiles, 64), (2 * ctas > sms ? 2 : 1) * sms / ctas));
+  const int shares = (p->prefix_length + 4 * BN - 1) / (4 * BN);
+  return (int)std::max<long long>(1, std::min<long long>(std::min(shares, 64), (2 * ctas > sms ? 2 : 1) * sms / ctas));
 }
 void prefix_fill(fa_module* m, const fa_paged_params* p, float* part_o, float* part_ml, FaPackedParams& k) {
   memset(&k, 0, sizeof k);
@@ -153,15 +156,14 @@ int launch_prefix(fa_module* m, const fa_paged_params* p, float* part_o, float* 
   Kernel* kernel = nullptr;
   int R = prefix_rows(p);
   if (R != 64 && !packed_maps(shape_of(p), p->k_prefix, p->v_prefix, p->prefix_length, L)) R = 64;
-  if (int rc = R == 64 ? get_packed_kernel(m, shape_of(p), true, &kernel) : get_packed_tc_kernel(m, shape_of(p), true, 1, &kernel)) return rc;
+  if (int rc = R == 64 ? get_packed_kernel(m, shape_of(p), true, &kernel) : get_packed_tc_kernel(m, shape_of(p), 2, 1, &kernel)) return rc;
   const long long items = ((long long)p->B * p->Sq * (p->Hq / p->Hkv) + R - 1) / R;
   if (items > 65535) return fail(FA_EUNSUPPORTED, "too many rows for a prefix");
-  return launch(kernel, dim3((unsigned)p->Hkv, (unsigned)items, (unsigned)L.p.splits), dim3(R == 64 ? 128 : 256), &L, stream);
+  return launch(kernel, dim3((unsigned)p->Hkv * L.p.splits, (unsigned)items), dim3(R == 64 ? 128 : 256), &L, stream);
 }
-int launch_prefix_merge(const fa_paged_params* p, const float* part_o, const float* part_ml, const float* own_o, const float* own_ml, int parts, void* stream) {
-  FaMergeParams k{part_o, part_ml, own_o, own_ml, cvt(p->o), p->lse, p->B, p->Hq, p->Hkv, p->Sq, p->Dv, parts};
-  const unsigned blocks = (unsigned)(((long long)p->B * p->Hq * p->Sq + 3) / 4);
-  return rot_dispatch(p->dtype, [&](auto dt) { return launch_here("fa_prefix_merge_kernel", fa_prefix_merge_kernel<decltype(dt)::value>, dim3(blocks), dim3(128), stream, k); });
+int launch_merge(int dtype, const FaMergeParams& k, void* stream) {
+  const unsigned blocks = (unsigned)(((long long)k.B * k.Hq * k.Sq + 3) / 4);
+  return rot_dispatch(dtype, [&](auto dt) { return launch_here("fa_merge_kernel", fa_merge_kernel<decltype(dt)::value>, dim3(blocks), dim3(128), stream, k); });
 }
 
 // ---- prompts -----------------------------------------------------------------------------------
@@ -180,6 +182,20 @@ int prompt_query_tiles(const fa_prompt_params* p) {
   long long keys = p->keys / B;
   if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + 128);
   return p->D > 64 && keys >= 1536 && p->Hkv * ((rows + 127) / 128) >= 2 * sms ? 2 : 1;
+}
+// Parts of the rows' keys, each a CTA's, where the rows alone make a CTA for every other SM at most: as many as make two per SM, of 512 keys at least (what a row sees in the mean).
+// (us, one part / this: 32 / 8 heads, D 128, pieces of 16 tokens behind 4000 57 / 18, eight behind 2000 33 / 22, one of 200 behind 32000 403 / 150; with more CTAs what the
+// parts are written and read for costs more, eight of 64 behind 2000 36.9 / 36.9, 32 of 33 behind 500 38 / 72.)
+int prompt_parts(const fa_prompt_params* p, int nq) {
+  const long long B = std::max(p->B, 1), tiles = (p->tokens * (p->Hq / p->Hkv) + 127) / 128, ctas = p->Hkv * std::max<long long>(B, tiles), sms = device_sm_count();
+  if (nq != 1 || 2 * ctas > sms) return 1;
+  long long keys = (p->keys - std::min(p->tokens, p->keys) / 2) / B;
+  if (p->window >= 0) keys = std::min<long long>(keys, (long long)p->window + 128);
+  return (int)std::max<long long>(1, std::min<long long>({keys / 512, 2 * sms / ctas, 64}));
+}
+size_t prompt_bytes(const fa_prompt_params* p, int parts) {
+  const size_t rows = (size_t)p->tokens * p->Hq;
+  return parts > 1 ? (size_t)parts * (merge_up(rows * p->Dv * 4) + merge_up(rows * 8)) : 0;
 }
 int prompt_sizes(fa_module* m, const fa_prompt_params* p) {
   if (!m) return fail(FA_EINVAL, "module is null");
@@ -215,14 +231,20 @@ int fa_prompt_prepare(fa_module* m, const fa_prompt_params* p) {
   Kernel* kernel = nullptr;
   if (packed_tc_takes(shape_of(p), p->keys)) {
     for (int nq = 1; nq <= 2; ++nq)
-      if (int rc = get_packed_tc_kernel(m, shape_of(p), false, nq, &kernel)) return rc;
-    return FA_OK;
+      if (int rc = get_packed_tc_kernel(m, shape_of(p), 1, nq, &kernel)) return rc;
+    return get_packed_tc_kernel(m, shape_of(p), 3, 1, &kernel);
   }
   return get_packed_kernel(m, shape_of(p), false, &kernel);
 }
 
-int fa_prompt(fa_module* m, const fa_prompt_params* p, void* stream) {
+size_t fa_prompt_workspace_bytes(const fa_prompt_params* p) {
+  if (!p || p->Hkv <= 0 || p->Hq <= 0 || p->Hq % p->Hkv || p->tokens <= 0 || p->Dv <= 0) return 0;
+  return packed_tc_takes(shape_of(p), p->keys) ? prompt_bytes(p, prompt_parts(p, prompt_query_tiles(p))) : 0;
+}
+
+int fa_prompt(fa_module* m, const fa_prompt_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = prompt_sizes(m, p)) return rc;
+  if ((uintptr_t)workspace & 15) return fail(FA_EINVAL, "workspace must be 16-byte aligned");
   prof_reset();
   if (p->tokens == 0) return FA_OK;
   if (p->B > 0 && !p->starts) return fail(FA_EINVAL, "starts is null");
@@ -237,8 +259,16 @@ int fa_prompt(fa_module* m, const fa_prompt_params* p, void* stream) {
   const long long rows = p->tokens * (p->Hq / p->Hkv);
   const int nq = packed_tc_takes(shape_of(p), p->keys) ? prompt_query_tiles(p) : 0;
   if (nq > 0 && packed_maps(shape_of(p), p->k, p->v, (int)p->keys, L)) {
-    if (int rc = get_packed_tc_kernel(m, shape_of(p), false, nq, &kernel)) return rc;
-    return launch(kernel, packed_grid(p->Hkv, rows, 128 * nq, p->B), dim3(nq == 1 ? 256 : 384), &L, stream);
+    const int parts = prompt_parts(p, nq);
+    if (int rc = get_packed_tc_kernel(m, shape_of(p), parts > 1 ? 3 : 1, nq, &kernel)) return rc;
+    const dim3 grid = packed_grid(p->Hkv * parts, rows, 128 * nq, p->B), block(nq == 1 ? 256 : 384);
+    if (parts == 1) return launch(kernel, grid, block, &L, stream);
+    if (!workspace || workspace_bytes < prompt_bytes(p, parts)) return fail(FA_EWORKSPACE, "prompt attention workspace too small");
+    L.p.splits = parts;
+    L.p.part_o = (float*)workspace;
+    L.p.part_ml = (float*)((char*)workspace + parts * merge_up((size_t)p->tokens * p->Hq * p->Dv * 4));
+    if (int rc = launch(kernel, grid, block, &L, stream)) return rc;
+    return launch_merge(p->dtype, FaMergeParams{L.p.part_o, L.p.part_ml, nullptr, nullptr, L.p.o, p->lse, 1, p->Hq, p->Hkv, (int)p->tokens, p->Dv, parts}, stream);
   }
   if (int rc = get_packed_kernel(m, shape_of(p), false, &kernel)) return rc;
   return launch(kernel, packed_grid(p->Hkv, rows, 64, p->B), dim3(128), &L.p, stream);

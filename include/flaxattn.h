@@ -390,7 +390,8 @@ typedef struct fa_prompt_params {
   int32_t flags;              /* FA_FLAG_GENERAL_KERNELS: not the tcgen05 kernel */
   int32_t* status;            /* optional status word: 32 = starts that decrease or lie beyond the tokens (what lies beyond is left out) */
 } fa_prompt_params;
-int fa_prompt(fa_module* m, const fa_prompt_params* p, void* stream);
+size_t fa_prompt_workspace_bytes(const fa_prompt_params* p); /* 0, but for few rows over many keys, which are split */
+int fa_prompt(fa_module* m, const fa_prompt_params* p, void* workspace, size_t workspace_bytes, void* stream);
 /* Compiles (or fetches from the cache) the kernel that a call of these sizes, type and flags runs.  Needs no GPU. */
 int fa_prompt_prepare(fa_module* m, const fa_prompt_params* p);
 

@@ -229,3 +229,19 @@ def test_two_query_tiles(D):
     """Long prompts at wide heads take two tiles per CTA: rows of one end in the first, between, in the second."""
     run(19, [2300, 1900, 2101], 8, 1, D, "bf16")
     run(20, [700, 660, 600], 24, 1, D, "f16", past=[1700, 2000, 1500], score=distance, window=1900)
+
+
+@pytest.mark.parametrize("D,Dv", [(64, 64), (96, 48), (128, 128)])
+@pytest.mark.parametrize("score,window", [(None, None), (distance, 1500), (None, 600)])
+def test_few_rows_over_many_keys(D, Dv, score, window):
+    """Keys in parts: requests that have some of the parts only, no keys, no tokens; rows of no request; what lies behind a request is no number."""
+    p = Prompts(21, [16, 1, 0, 30], 4, 1, D, torch.bfloat16, Dv=Dv, past=[3000, 4100, 100, 0], pad=(2, 3))
+    out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, score, key_starts=p.key_starts, window=window, return_lse=True)
+    p.check(out, lse, with_slope(p.want(score, None, window), 2.0 ** -0.5 if score else 0.0))
+    again, _ = fa.prompt_attention(p.q, p.k, p.v, p.starts, score, key_starts=p.key_starts, window=window, return_lse=True)
+    assert torch.equal(out, again)
+
+
+def test_one_row_over_many_keys():
+    run(22, [1], 1, 1, 64, "f16", past=[20000])
+    run(23, [5], 8, 2, 128, "bf16", past=[9000], mask=parity, score=softcap)
