@@ -655,6 +655,9 @@ int fa_paged_prepare(fa_module* m, const fa_paged_params* p) {
   PagedCfg c;
   pick_paged(p, c);
   Kernel* kernel = nullptr;
+  if (c.eight && p->dtype == FA_F32) return fail(FA_EUNSUPPORTED, "pages in 8 bits take queries of 16 bits");
+  if (p->prefix_length > 0)
+    if (int rc = get_prefix_kernel(m, p, prefix_rows(p), &kernel)) return rc;
   return get_paged_kernel(m, p, c, &kernel);
 }
 

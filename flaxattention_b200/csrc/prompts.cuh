@@ -150,13 +150,16 @@ void prefix_fill(fa_module* m, const fa_paged_params* p, float* part_o, float* p
   k.by_group = divide_by(p->Hq / p->Hkv); k.by_sq = divide_by(p->Sq);
   k.scale = p->scale;
 }
+int get_prefix_kernel(fa_module* m, const fa_paged_params* p, int rows, Kernel** k) {
+  return rows == 64 ? get_packed_kernel(m, shape_of(p), true, k) : get_packed_tc_kernel(m, shape_of(p), 2, 1, k);
+}
 int launch_prefix(fa_module* m, const fa_paged_params* p, float* part_o, float* part_ml, void* stream) {
   FaTcPackedHost L;
   prefix_fill(m, p, part_o, part_ml, L.p);
   Kernel* kernel = nullptr;
   int R = prefix_rows(p);
   if (R != 64 && !packed_maps(shape_of(p), p->k_prefix, p->v_prefix, p->prefix_length, L)) R = 64;
-  if (int rc = R == 64 ? get_packed_kernel(m, shape_of(p), true, &kernel) : get_packed_tc_kernel(m, shape_of(p), 2, 1, &kernel)) return rc;
+  if (int rc = get_prefix_kernel(m, p, R, &kernel)) return rc;
   const long long items = ((long long)p->B * p->Sq * (p->Hq / p->Hkv) + R - 1) / R;
   if (items > 65535) return fail(FA_EUNSUPPORTED, "too many rows for a prefix");
   return launch(kernel, dim3((unsigned)p->Hkv * L.p.splits, (unsigned)items), dim3(R == 64 ? 128 : 256), &L, stream);
