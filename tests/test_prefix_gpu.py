@@ -158,3 +158,19 @@ def test_refusals():
     for bad in ((p[:, :1], p), (p, p[:, :, :40]), (torch.cat([p, p]), torch.cat([p, p])), (p[..., :48], p), (p.float(), p), (p, p.clone().requires_grad_())):
         with pytest.raises(ValueError):
             call(bad)
+
+
+@pytest.mark.parametrize("D,P", [(64, 300), (128, 1400)])
+def test_scores_that_take_keys_out(D, P):
+    """The lowest value as a score, for the whole prefix and for the requests' own keys in turn."""
+    for cut in (lambda j: j < P, lambda j: j >= P, lambda j: j >= 0):
+        def lowest(score, b, h, q_idx, kv_idx):
+            return torch.where(cut(kv_idx), -3.4028234663852886e38, score)
+
+        lengths = [4] * 40 + [50, 1]
+        c = Cache(16, lengths, 2, D, 16, torch.bfloat16)
+        rng = np.random.default_rng(17)
+        q, pk, pv = normal(rng, 42, 4, 1, D, dtype=torch.bfloat16), *(normal(rng, 1, 2, P, D, dtype=torch.bfloat16) for _ in range(2))
+        out, lse = fa.paged_attention(q.cuda(), c.k_pages, c.v_pages, c.table, c.lengths, lowest, return_lse=True, prefix=(pk.cuda(), pv.cuda()))
+        keys, values = ([torch.cat([x[0], t], 1) for t in y] for x, y in ((pk, c.keys), (pv, c.values)))
+        check_attention(out, lse, attend(q, keys, values, None, lambda b, h, i, j: ~cut(j) & (j >= 0)), torch.bfloat16)

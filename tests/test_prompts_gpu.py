@@ -245,3 +245,32 @@ def test_few_rows_over_many_keys(D, Dv, score, window):
 def test_one_row_over_many_keys():
     run(22, [1], 1, 1, 64, "f16", past=[20000])
     run(23, [5], 8, 2, 128, "bf16", past=[9000], mask=parity, score=softcap)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("low", [-3.4028234663852886e38, -math.inf])
+def test_scores_that_take_keys_out(D, dtype, low):
+    """The lowest value and minus infinity as scores: what they leave of a row, or nothing."""
+    def lowest(score, b, h, q_idx, kv_idx):
+        return torch.where((kv_idx < 130) | (kv_idx % 3 == 1), low, score)
+
+    p = Prompts(24, [140, 300], 2, 1, D, DTYPES[dtype])
+    out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, lowest, return_lse=True)
+    p.check(out, lse, p.want(None, lambda b, h, i, j: (j >= 130) & (j % 3 != 1)))
+    assert torch.isneginf(lse[0, :, :131]).all()  # (130 % 3 == 1)
+
+
+def test_scores_far_below_zero_are_no_mask():
+    """A penalty of 1e4 for all keys of the first tiles: the rows that have no others are softmaxes of those, the others do not see them."""
+    def far(score, b, h, q_idx, kv_idx):
+        return torch.where(kv_idx < 200, score - 1e4, score)
+
+    p = Prompts(25, [330], 2, 2, 64, torch.float16)
+    out, lse = fa.prompt_attention(p.q, p.k, p.v, p.starts, far, return_lse=True)
+    out, lse = out.cpu().double(), lse.cpu().double()
+    ref, ref_lse, spread, _ = p.want(far)
+    # (fp32 scores near 1e4 have steps of 2^-10, in log2 units: probabilities are off by as much in proportion)
+    off = torch.where(torch.arange(330) < 200, 2.0 ** -9, 2.0 ** -16)
+    assert ((out - ref).abs() <= 2.0 ** -11 * ref.abs() + (2.0 ** -11 + off)[:, None] * spread + 2.0 ** -24).all()
+    assert ((lse - ref_lse).abs() <= off + 2.0 ** -22 * ref_lse.abs()).all()
