@@ -2,9 +2,11 @@
 // they share.  The G query heads of a kv head share its keys, so rows are (token, head of the group), row r is head r % G of token r / G, and a
 // kernel takes them in items of R rows.
 //
-//   prompts  An item's rows are of one request.  Lengths are known on the device only; every CTA looks its item up.  Items with the most keys
-//            in front: in the order of their place in the request, the last first, over all requests.  Behind the requests' items come those of
-//            the rows that belong to none, in front of the first request and behind the last, which see nothing.
+//   prompts  An item's rows are of one request.  Lengths are known on the device only; every CTA looks its item up.  Up to 256 requests, items
+//            with the most keys in front: in the order of their place in the request, the last first, over all requests.  Of more, request by
+//            request, a third of the items nobody's: a look at all requests for each item takes longer (16 tokens each, 32 / 8 heads, D 128, bf16:
+//            by level 256 requests 67 us, 512 193, 1024 614; by request 81, 161, 329).  Rows that belong to no request, in front of the first and
+//            behind the last, have items too, and see nothing.
 //   prefix   The rows of all requests, one behind the other.
 #pragma once
 #include "fa_common.cuh"
@@ -26,53 +28,61 @@ __device__ __forceinline__ void fa_range(const int* starts, int s, int most, int
   end = min(max(starts[s + 1], begin), most);
 }
 
-// Item `item` of items of R rows, by the 32 lanes of a warp together.  The items of level l are those with l others of their request in front of
-// them; total(l) of all have level l or more, so the level of an item is found by halving, and its request by counting those that
-// reach it.  (The counts of the first 256 requests stay in registers.)
+// the rows of no request in front of the first and behind the last, from their item `item` on
 template <int R>
-__device__ __forceinline__ FaPlace fa_find_item(const FaPackedParams& p, long long item) {
+__device__ __forceinline__ FaPlace fa_no_request(const FaPackedParams& p, bool behind, int front, int back, long long item) {
+  FaPlace r = {0, 0, 0, 0, 0, 0, 0};
+  r.q0 = behind ? back : 0;
+  r.n = behind ? p.tokens - back : front;
+  const long long first = item * R;
+  r.first = (int)min(max(first, 0ll), (long long)0x7fffffff);
+  r.any = first >= 0 && first < (long long)r.n * (p.Hq / p.Hkv);  // (below 0: of broken starts)
+  return r;
+}
+__device__ __forceinline__ FaPlace fa_request(const FaPackedParams& p, int b, int first) {
+  FaPlace r = {0, 0, 0, 0, b, first, 1};
+  int end;
+  fa_range(p.starts, b, p.tokens, r.q0, end);
+  r.n = end - r.q0;
+  fa_range(p.key_starts, b, p.keys, r.k0, end);
+  r.nk = end - r.k0;
+  return r;
+}
+
+// Up to 256 requests, by the 32 lanes of a warp together.  The items of level l are those with l others of their request in front of
+// them; total(l) of all have level l or more, so the level of an item is found by halving, and its request by counting those that
+// reach it.
+template <int R>
+__device__ __forceinline__ FaPlace fa_find_by_level(const FaPackedParams& p, long long item) {
   constexpr int KEEP = 8;
   const int lane = threadIdx.x & 31, G = p.Hq / p.Hkv;
-  const auto items_of = [&](int s) {
-    if (s >= p.B) return 0;
-    int begin, end;
-    fa_range(p.starts, s, p.tokens, begin, end);
-    return (int)(((long long)(end - begin) * G + R - 1) / R);
-  };
   int kept[KEEP], most = 0;
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) {
-    kept[i] = i * 32 < p.B ? items_of(i * 32 + lane) : 0;
+    kept[i] = 0;
+    if (i * 32 + lane < p.B) {
+      int begin, end;
+      fa_range(p.starts, i * 32 + lane, p.tokens, begin, end);
+      kept[i] = (int)(((long long)(end - begin) * G + R - 1) / R);
+    }
     most = max(most, kept[i]);
   }
-#pragma unroll 1
-  for (int s = KEEP * 32; s < p.B; s += 32) most = max(most, items_of(s + lane));
   most = __reduce_max_sync(0xffffffffu, most);
   const auto total = [&](int level) {
     long long sum = 0;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
       if (i * 32 < p.B) sum += max(kept[i] - level, 0);
-#pragma unroll 1
-    for (int s = KEEP * 32; s < p.B; s += 32) sum += max(items_of(s + lane) - level, 0);
     // (of broken starts the sum may need more than 32 bits)
     const fa_u32 lo = __reduce_add_sync(0xffffffffu, (fa_u32)sum & 0xffffffu), hi = __reduce_add_sync(0xffffffffu, (fa_u32)(sum >> 24));
     return (long long)lo + ((long long)hi << 24);
   };
-  FaPlace r = {0, 0, 0, 0, 0, 0, 0};
   const long long all = total(0);
   if (item >= all) {
-    // rows of no request
-    long long left = item - all;
     const int front = p.B > 0 ? min(max(p.starts[0], 0), p.tokens) : 0, back = p.B > 0 ? min(max(p.starts[p.B], 0), p.tokens) : 0;
-    const long long items_front = ((long long)front * G + R - 1) / R;
+    const long long items_front = ((long long)front * G + R - 1) / R, left = item - all;
     const bool behind = left >= items_front;
-    if (behind) left -= items_front;
-    r.q0 = behind ? back : 0;
-    r.n = behind ? p.tokens - back : front;
-    r.first = (int)min(left * R, (long long)0x7fffffff);
-    r.any = left * R < (long long)r.n * G;
-    return r;
+    return fa_no_request<R>(p, behind, front, back, behind ? left - items_front : left);
   }
   int lo = 0, hi = most - 1;  // the last level l with total(l) > item
   while (lo < hi) {
@@ -80,32 +90,45 @@ __device__ __forceinline__ FaPlace fa_find_item(const FaPackedParams& p, long lo
     if (total(mid) > item) lo = mid;
     else hi = mid - 1;
   }
-  int rank = (int)(item - total(lo + 1));
-  r.any = 1;
-  r.first = lo * R;
-  const auto find = [&](int s0, int count) {  // whether the request is among the 32 from s0 on
-    const fa_u32 reach = __ballot_sync(0xffffffffu, count > lo);
-    const int n = __popc(reach);
-    if (rank >= n) {
-      rank -= n;
-      return false;
-    }
-    const fa_u32 below = reach & ((1u << lane) - 1u);
-    r.b = s0 + __ffs(__ballot_sync(0xffffffffu, ((reach >> lane) & 1u) && __popc(below) == rank)) - 1;
-    return true;
-  };
+  int rank = (int)(item - total(lo + 1)), b = 0;
   bool found = false;
 #pragma unroll
-  for (int i = 0; i < KEEP; ++i)
-    if (!found && i * 32 < p.B) found = find(i * 32, kept[i]);
-#pragma unroll 1
-  for (int s = KEEP * 32; s < p.B && !found; s += 32) found = find(s, items_of(s + lane));
-  int end;
-  fa_range(p.starts, r.b, p.tokens, r.q0, end);
-  r.n = end - r.q0;
-  fa_range(p.key_starts, r.b, p.keys, r.k0, end);
-  r.nk = end - r.k0;
+  for (int i = 0; i < KEEP; ++i) {
+    const fa_u32 reach = __ballot_sync(0xffffffffu, kept[i] > lo);
+    const int n = __popc(reach);
+    const fa_u32 mine = __ballot_sync(0xffffffffu, ((reach >> lane) & 1u) && __popc(reach & ((1u << lane) - 1u)) == rank);
+    if (!found && rank < n) {
+      b = i * 32 + __ffs(mine) - 1;
+      found = true;
+    }
+    if (!found) rank -= n;
+  }
+  return fa_request(p, b, lo * R);
+}
+
+// More requests.  Request s, which begins at row x of all, has the item numbers from x / R + s + 1 on up to the next request's: as many as it
+// needs, or one more, which is nobody's.  The request whose numbers an item has is found by looking at 32 of them at a time.
+template <int R>
+__device__ __forceinline__ FaPlace fa_find_by_request(const FaPackedParams& p, long long item) {
+  const int lane = threadIdx.x & 31, G = p.Hq / p.Hkv;
+  const auto row = [&](int s) { return min(max(p.starts[s], 0), p.tokens); };
+  const auto number = [&](int s) { return (long long)row(s) * G / R + s + 1; };
+  int lo = -1, hi = p.B + 1;  // number(lo) <= item < number(hi); -1: in front of all requests, B: behind
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+    const int upto = __popc(__ballot_sync(0xffffffffu, at < hi && number(min(at, p.B)) <= item));  // (never decreasing)
+    lo += upto * step;
+    hi = min(hi, lo + step);
+  }
+  if (lo < 0 || lo >= p.B) return fa_no_request<R>(p, lo >= 0, row(0), row(p.B), lo < 0 ? item : item - number(p.B));
+  const long long first = (item - number(lo)) * R;
+  FaPlace r = fa_request(p, lo, (int)min(max(first, 0ll), (long long)0x7fffffff));
+  r.any = first >= 0 && first < (long long)r.n * G;
   return r;
+}
+template <int R>
+__device__ __forceinline__ FaPlace fa_find_item(const FaPackedParams& p, long long item) {
+  return p.B <= 256 ? fa_find_by_level<R>(p, item) : fa_find_by_request<R>(p, item);
 }
 
 // starts that decrease, or lie where there are no tokens: said once, by the threads of one CTA

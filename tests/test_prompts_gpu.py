@@ -274,3 +274,23 @@ def test_scores_far_below_zero_are_no_mask():
     off = torch.where(torch.arange(330) < 200, 2.0 ** -9, 2.0 ** -16)
     assert ((out - ref).abs() <= 2.0 ** -11 * ref.abs() + (2.0 ** -11 + off)[:, None] * spread + 2.0 ** -24).all()
     assert ((lse - ref_lse).abs() <= off + 2.0 ** -22 * ref_lse.abs()).all()
+
+
+@pytest.mark.parametrize("pad", [(0, 0), (50, 700)])
+@pytest.mark.parametrize("D,dtype", [(64, "bf16"), (128, "f16"), (32, "f32")])
+def test_hundreds_of_requests(pad, D, dtype):
+    """257 and more are found in another way: none with tokens, one, several tiles; rows of no request in front and behind, of several items."""
+    rng = np.random.default_rng(26)
+    lengths = [int(rng.integers(0, 30)) for _ in range(300)]
+    lengths[0], lengths[17], lengths[299] = 0, 400, 129
+    run(27, lengths, 6, 2, D, dtype, pad=pad)
+    run(28, [0] * 256 + [1], 2, 1, D, dtype, pad=pad)
+
+
+def test_broken_starts_of_hundreds_of_requests():
+    p = Prompts(29, [300], 2, 1, 64, torch.float16)
+    starts = torch.randint(-2 ** 31, 2 ** 31 - 1, (400,), generator=torch.Generator().manual_seed(0)).int().cuda()
+    fa.prompt_attention(p.q, p.k, p.v, starts)
+    torch.cuda.synchronize()
+    with pytest.raises(fa._cabi.FlaxAttnError, match="starts"):
+        fa.check_status()
