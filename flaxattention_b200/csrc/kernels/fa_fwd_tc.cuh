@@ -206,6 +206,9 @@ __device__ __forceinline__ void max_chunk(const float (&v)[32], RowMax& mx) {
 // m_base): where that does not move, the exponentials are taken of them as they are, without a subtraction of their own.  An affine score_mod
 // (A * score + B) costs one packed FMA per pair: A and B absorb the scale, log2(e) and the maximum.
 // (Without a score_mod the scores stay raw, the exponent's FMA applies the scale.)
+// (A bias that is linear over the keys is taken from the tile's key LINEAR_AT.  A rounding there is an error of all its keys; from the middle it
+// is half as large, which rows of prompts gain that see a few keys only.)
+constexpr int LINEAR_AT = PACKED ? 64 : 0;
 struct ModLinear {
   fa_u64 m2, od[4];  // multiplier; 0 and 1, 2 and 3, 4 and 5, 6 and 7 times the slope over kv
   float d, b;        // slope; bias at the first key of the tile (with the maximum)
@@ -228,7 +231,7 @@ __device__ __forceinline__ void mod_chunk(float (&v)[32], int n0, int qi, int gb
     // (which shares the SFU with the exponentials) and a multiplication per element.  (A packed FMA per pair with the column
     // numbers as constants needs those in registers, two moves per pair: B2 H1 S8192, D64 rounded 103 us against 99, D128 104 against 103,
     // causal D64 88 against 82.)
-    if (e % 8 == 0) at8 = fmaf((float)(C0 + e), lin.d, lin.b);
+    if (e % 8 == 0) at8 = fmaf((float)(C0 + e - LINEAR_AT), lin.d, lin.b);
     fa_f2_unpack(fa_fma2(fa_f2(x0, x1), lin.m2, fa_add2(fa_f2(at8, at8), lin.od[(e % 8) / 2])), x0, x1);
 #elif FA_HAS_SCORE_MOD && defined(FA_SCORE_MUL_ONLY)
     fa_f2_unpack(fa_fma2(fa_f2(x0, x1), fa_f2(fa_score_mul(0.f, gb, gh, qi, kv0) * sc2, fa_score_mul(0.f, gb, gh, qi, kv1) * sc2), fa_f2(negm, negm)), x0, x1);
@@ -428,7 +431,7 @@ __device__ __forceinline__ bool softmax_step(SoftmaxCtx& c, const int tile, cons
   ModLinear lin = {};
 #if FA_HAS_SCORE_MOD && defined(FA_SCORE_AFFINE) && defined(FA_SCORE_LINEAR_KV)
   lin = c.lin;
-  const float bias0 = fa_score_add2(0.f, gb, gh, qi, n0);
+  const float bias0 = fa_score_add2(0.f, gb, gh, qi, n0 + LINEAR_AT);
   const float m_base = bias0 - m_ref <= 16.f ? m_ref : (fabsf(bias0) < -FA_NEG_INF ? bias0 : 0.f);
   lin.b = bias0 - m_base;
 #else
