@@ -238,6 +238,8 @@ __device__ __forceinline__ void mod_chunk(float (&v)[32], int n0, int qi, int gb
 #elif FA_HAS_SCORE_MOD && defined(FA_SCORE_AFFINE)
     fa_f2_unpack(fa_fma2(fa_f2(x0, x1), fa_f2(fa_score_mul(0.f, gb, gh, qi, kv0) * sc2, fa_score_mul(0.f, gb, gh, qi, kv1) * sc2),
                          fa_add2(fa_f2(fa_score_add2(0.f, gb, gh, qi, kv0), fa_score_add2(0.f, gb, gh, qi, kv1)), fa_f2(negm, negm))), x0, x1);
+#elif FA_HAS_SCORE_MOD && FA_SCORE_PAIRS
+    fa_f2_unpack(fa_fma2(fa_score_mod_pair(fa_mul2(fa_f2(x0, x1), fa_f2(scale, scale)), gb, gh, qi, kv0, kv1), fa_f2(FA_LOG2E, FA_LOG2E), fa_f2(negm, negm)), x0, x1);
 #elif FA_HAS_SCORE_MOD
     x0 = fmaf(fa_score_mod(x0 * scale, gb, gh, qi, kv0), FA_LOG2E, negm);
     x1 = fmaf(fa_score_mod(x1 * scale, gb, gh, qi, kv1), FA_LOG2E, negm);

@@ -163,11 +163,21 @@ extern "C" __global__ void __launch_bounds__(fa_pk::NT) fa_packed_kernel(const _
       float mx = FA_NEG_INF;
 #pragma unroll
       for (int nj = 0; nj < BN / 8; ++nj) {
+#if FA_HAS_SCORE_MOD && FA_SCORE_PAIRS
+        {
+          const int kv = n0 + nj * 8 + (lane & 3) * 2;
+          fa_f2_unpack(fa_score_mod_pair(fa_mul2(fa_f2(s[nj][h * 2], s[nj][h * 2 + 1]), fa_both(p.scale)), gb, gh, qi, kv, kv + 1), s[nj][h * 2], s[nj][h * 2 + 1]);
+        }
+#endif
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int kv = n0 + nj * 8 + (lane & 3) * 2 + e;
+#if FA_HAS_SCORE_MOD && FA_SCORE_PAIRS
+          float x = s[nj][h * 2 + e];
+#else
           float x = s[nj][h * 2 + e] * p.scale;
-#if FA_HAS_SCORE_MOD
+#endif
+#if FA_HAS_SCORE_MOD && !FA_SCORE_PAIRS
           x = fa_score_mod(x, gb, gh, qi, kv);
 #endif
           bool keep = !edge || (kv >= row[h].from && kv < row[h].to);

@@ -1302,7 +1302,14 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
         for (int j = 0; j < NS; ++j) {
           [[maybe_unused]] const int kv = n0 + R.key(j) + (AFTER ? p.after : 0);
           float x = R.score(h, j);
-#if FA_HAS_SCORE_MOD && defined(FA_SCORE_AFFINE)
+#if FA_HAS_SCORE_MOD && FA_SCORE_PAIRS
+          static_assert(NS % 2 == 0, "keys of a thread come in pairs");
+          if (j % 2 == 0) {
+            float y = R.score(h, j + 1);
+            fa_f2_unpack(fa_mul2(fa_score_mod_pair(fa_mul2(fa_f2(x, y), fa_both(p.scale)), gb, gh, qp, kv, n0 + R.key(j + 1) + (AFTER ? p.after : 0)), fa_both(FA_LOG2E)), x, y);
+            R.score(h, j + 1) = y;
+          }
+#elif FA_HAS_SCORE_MOD && defined(FA_SCORE_AFFINE)
           x = fmaf(x, fa_score_mul(0.f, gb, gh, qp, kv) * sc2, fa_score_add2(0.f, gb, gh, qp, kv));
 #elif FA_HAS_SCORE_MOD
           x = fa_score_mod(x * p.scale, gb, gh, qp, kv) * FA_LOG2E;

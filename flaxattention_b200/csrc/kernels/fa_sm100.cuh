@@ -3,6 +3,7 @@
 // Self-contained (no CUDA headers), like fa_common.cuh.
 #pragma once
 #include "fa_common.cuh"
+#include "fa_f2.cuh"
 
 // 128-byte opaque tensor map (same size and alignment as the driver's CUtensorMap)
 struct __align__(64) FaTensorMap {
@@ -265,30 +266,7 @@ __device__ __forceinline__ void fa_mma_commit(fa_u32 bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// ---- packed fp32 pairs and other sm_100 ALU forms -----------------------------------------
-__device__ __forceinline__ fa_u64 fa_f2(float lo, float hi) {
-  fa_u64 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void fa_f2_unpack(fa_u64 v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ fa_u64 fa_mul2(fa_u64 a, fa_u64 b) {
-  fa_u64 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ fa_u64 fa_add2(fa_u64 a, fa_u64 b) {
-  fa_u64 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ fa_u64 fa_fma2(fa_u64 a, fa_u64 b, fa_u64 c) {
-  fa_u64 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
+// ---- forms of packed fp32 pairs (fa_f2.cuh) and others of sm_100's ALU ----------------------
 // A pair of fp32 values as three pairs of bf16 values whose sum is exact: hi is the value rounded to bf16,
 // mid the remainder rounded, lo what is left of it (at most 8 bits, so the last rounding is exact).
 __device__ __forceinline__ void fa_split3(fa_u64 x, fa_u32& hi, fa_u32& mid, fa_u32& lo) {

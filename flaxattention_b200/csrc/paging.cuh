@@ -480,7 +480,7 @@ int paged_workers(const PagedCfg& c) { return c.per_sm * device_sm_count(); }
 // (16-bit types: quotients and tanh of scores without branches, fa_score_math.cuh)
 int get_paged_kernel(fa_module* m, const fa_paged_params* p, const PagedCfg& c, Kernel** k) {
   return get_kernel(m, kernel_key(kIdPaged, {{p->dtype, 2}, {p->D, 9}, {p->Dv, 9}, {c.RG, 3}, {c.WN, 6}, {c.slots, 4}, {c.tma ? 1 : 0, 1}, {c.few, 2}, {c.fr, 5}, {c.CG, 4}, {c.one_each ? 1 : 0, 1}, {c.per_sm, 3}, {c.eight ? 1 : 0, 1}, {c.after ? 1 : 0, 1}}), "fa_paged.cuh",
-                    [&] { return std::string(p->dtype == FA_F32 ? "" : "#include \"fa_score_math.cuh\"\n") +
+                    [&] { return std::string(p->dtype == FA_F32 ? "" : c.eight ? "#define FA_PAIRS 1\n#include \"fa_score_math.cuh\"\n" : "#include \"fa_score_math.cuh\"\n") +
                                 defs({{"FA_DTYPE", p->dtype}, {"FA_D", p->D}, {"FA_DV", p->Dv}, {"FA_RG", c.RG}, {"FA_WN", c.WN},
                                        {"FA_SLOTS", c.slots}, {"FA_TMA", c.tma ? 1 : 0}, {"FA_FEW", c.few}, {"FA_FR", c.fr}, {"FA_CG", c.CG}, {"FA_SHORT", c.one_each ? 1 : 0}, {"FA_CTAS", c.per_sm}, {"FA_KV8", c.eight ? 1 : 0}, {"FA_AFTER", c.after ? 1 : 0}}); },
                     "fa_paged_kernel", c.smem, k);

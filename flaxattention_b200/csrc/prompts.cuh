@@ -15,8 +15,8 @@ struct PackedShape {
   float scale;
 };
 
-// (16-bit types: quotients and tanh of scores without branches, as over pages)
-std::string packed_math(const PackedShape& s) { return s.dtype == FA_F32 ? "" : "#include \"fa_score_math.cuh\"\n"; }
+// (16-bit types: quotients and tanh of scores without branches, two at a time)
+std::string packed_math(const PackedShape& s) { return s.dtype == FA_F32 ? "" : "#define FA_PAIRS 1\n#include \"fa_score_math.cuh\"\n"; }
 
 // ---- general kernel: tiles of fa_packed.cuh ---------------------------------------------------
 // Keys of a tile: as many as leave room for two CTAs on an SM.

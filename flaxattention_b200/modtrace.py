@@ -1410,6 +1410,54 @@ def to_cuda(mod: TracedMod, name: str) -> str:
     return "\n".join([head] + lines + [f"  return {ret};", "}"]) + "\n"
 
 
+_PAIR_OPS = {"add": "fa_add2({0}, {1})", "sub": "fa_fma2({1}, fa_both(-1.0f), {0})", "mul": "fa_mul2({0}, {1})", "neg": "fa_mul2({0}, fa_both(-1.0f))"}
+
+
+def to_cuda_pair(mod: TracedMod, name: str) -> Optional[str]:
+    """The score mod for two keys at once, as packed fp32: ``fa_u64 name(fa_u64 scores, int b, int h, int q, int kv0, int kv1)``, for kernels that define
+    FA_PAIRS.  None unless it has a tanh of the score and what it does with the score are sums, products, quotients by constants and tanh; what does not
+    depend on the score is evaluated for either key."""
+    of_scores, dep = _score_quotients(mod.root), {}
+    lines: List[str] = []
+    parts: List[str] = []
+    names: Dict[int, str] = {}
+    some = False
+
+    def operand(e: Expr) -> str:
+        if id(e) in names:
+            return names[id(e)]
+        if e.op == "const":
+            return f"fa_both({_f32_literal(e.value)})"
+        part = f"{name}_{len(parts)}"
+        parts.append(to_cuda(TracedMod("score", e, mod.buffers), part))
+        lines.append(f"  const fa_u64 {part}_v = fa_f2({part}(0.0f, b, h, q, kv0), {part}(0.0f, b, h, q, kv1));")
+        names[id(e)] = f"{part}_v"
+        return names[id(e)]
+
+    for e in _topo(mod.root):
+        if not _depends_on_score(e, dep):
+            continue
+        if e.op == "score":
+            names[id(e)] = "score"
+            continue
+        if e.dtype != F32:
+            return None
+        if e.op in _PAIR_OPS:
+            rhs = _PAIR_OPS[e.op].format(*(operand(a) for a in e.args))
+        elif e.op == "div" and id(e) in of_scores and e.args[1].op == "const" and 2.0 ** -100 <= builtins.abs(e.args[1].value) <= 2.0 ** 100:
+            rhs = f"fa_mul2({operand(e.args[0])}, fa_both(1.0f / {_f32_literal(e.args[1].value)}))"
+        elif e.op == "tanh" and id(e) in of_scores:
+            rhs, some = f"fa_tanh2({operand(e.args[0])})", True
+        else:
+            return None
+        names[id(e)] = f"t{len(lines)}"
+        lines.append(f"  const fa_u64 {names[id(e)]} = {rhs};")
+    if not some:
+        return None
+    head = f"__device__ __forceinline__ fa_u64 {name}(fa_u64 score, int b, int h, int q, int kv0, int kv1) {{"
+    return "".join(parts) + "\n".join([head] + lines + [f"  return {names[id(mod.root)]};", "}"]) + "\n"
+
+
 class _RangeText:
     """What ``_range_walk`` builds from: C++ text, a line for each pair of bounds."""
 
@@ -1726,6 +1774,9 @@ _QUOTIENT_PRELUDE = r"""
 
 
 _BUFFER_PRELUDE = r"""
+#ifdef FA_MOD_BUFS_INIT
+#error "fa_params.h has to come behind the mods: it asks whether they read tensors"
+#endif
 // Captured buffers: every kernel fills this table from its parameters (FA_MOD_BUFS_INIT).
 __shared__ const void* fa_mod_buf[FA_NUM_MOD_BUFS];
 __device__ __forceinline__ int fa_ld_i32(int k, int i) { return __ldg((const int*)fa_mod_buf[k] + i); }
@@ -1762,6 +1813,9 @@ class ModSet:
             parts.append(to_cuda(self.score, "fa_score_mod"))
             parts.append(to_cuda(self.grad, "fa_score_mod_grad"))
             self.affine = affine_parts(self.score)
+            pair = to_cuda_pair(self.score, "fa_score_mod_pair") if self.affine is None else None
+            if pair is not None:
+                parts.append(f"#if FA_PAIRS\n#define FA_SCORE_PAIRS 1\n{pair}#endif\n")
             if always_finite([self.affine[0].root if self.affine is not None else self.grad.root], False):
                 parts.append("#define FA_SCORE_GRAD_FINITE 1\n")  # (0 times it is 0)
             whole = [t.root for t in self.affine] if self.affine is not None else [self.score.root, self.grad.root]

@@ -294,3 +294,30 @@ def test_broken_starts_of_hundreds_of_requests():
     torch.cuda.synchronize()
     with pytest.raises(fa._cabi.FlaxAttnError, match="starts"):
         fa.check_status()
+
+
+@pytest.mark.parametrize("D,dtype", [(64, "f16"), (128, "bf16"), (32, "f16"), (256, "bf16")])
+@pytest.mark.parametrize("general", [False, True])
+def test_capped_scores_over_the_whole_range(D, dtype, general):
+    """Rows that see one key each (a window of 0): the logsumexp is the capped score itself.
+
+    A score here is one product, exact in fp32, and a scale of 1.  Roundings, in proportion: tanh 4e-7 (3.3e-7 of its form and roundings, a reciprocal off
+    by 2^-23), its argument's two (2^-24 each), the cap's, the way to log2 units and back (4 more): 4e-7 + 7 * 2^-24 < 1e-6.  And the exponential of 0,
+    which is the sum: 1 to within 2.7e-6."""
+    torch_type = {"f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    q = torch.zeros(1, 2048, 1, D, dtype=torch_type, device="cuda")
+    k, v = torch.zeros_like(q), torch.ones_like(q)
+    values = torch.cat([torch.linspace(-300, 300, 1024), torch.logspace(-12, 15.9, 512, base=2), -torch.logspace(-12, 15.9, 512, base=2)]).to(torch_type)
+    q[0, :, 0, 3] = values.cuda()
+    k[0, :, 0, 3] = 1.0
+    starts = torch.tensor([0, 2048], dtype=torch.int32, device="cuda")
+    options = {"kernels": "general"} if general else None
+    for score, want in ((lambda s, b, h, qi, ki: 30.0 * torch.tanh(s / 30.0), 30 * torch.tanh(values.double() / 30)),
+                        (lambda s, b, h, qi, ki: 5.0 - torch.tanh(s * 0.5) * (-2.0) + (qi - ki) * 0.25, 5 + 2 * torch.tanh(values.double() * 0.5))):
+        out, lse = fa.prompt_attention(q, k, v, starts, score, window=0, sm_scale=1.0, bhln=False, return_lse=True, kernel_options=options)
+        size = want.abs() + (0 if want[0] < 0 else 10)  # (of the second, the sum's parts)
+        assert ((lse.reshape(-1).double().cpu() - want).abs() <= 1e-6 * size + 2.7e-6).all()
+        assert (out == 1).all()
+    q[0, 5, 0, 3] = float("nan")
+    out, lse = fa.prompt_attention(q, k, v, starts, lambda s, b, h, qi, ki: 30.0 * torch.tanh(s / 30.0), window=0, sm_scale=1.0, bhln=False, return_lse=True, kernel_options=options)
+    assert lse.reshape(-1)[5].isnan() and out[0, 5].isnan().all() and not lse.reshape(-1)[6:].isnan().any()

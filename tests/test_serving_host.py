@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import flaxattention_b200 as fa
-from flaxattention_b200 import _cabi
+from flaxattention_b200 import _cabi, modtrace
 
 
 def tensor(ptr=0x1000, b=1 << 20, h=1 << 12, s=64):
@@ -120,6 +120,30 @@ def test_eight_bit_kernels_compile(D, Sq, page, prefix):
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="says what happens without a GPU")
+@pytest.mark.parametrize("dtype,D", [(0, 64), (1, 128), (1, 256), (2, 64)])
+def test_capped_scores_with_a_tensor_compile(dtype, D):
+    """What stands in front of the mods must not keep the kernels from seeing that these read a tensor (the mods' text says so to the compiler)."""
+    bias = torch.zeros(8, 4)
+    mods = modtrace.lower_mods(lambda s, b, h, qi, ki: 30.0 * torch.tanh(s / 30.0) + bias[b, h], None)
+    assert "FA_SCORE_PAIRS" in mods.source
+    m = _cabi.Module(mods.source)
+    _cabi.check(_cabi.lib().fa_prompt_prepare(m.handle, C.byref(prompt(dtype=dtype, D=D, Dv=D))))
+
+
+def test_scores_of_two_keys_at_once():
+    """Only where a tanh of the score is between sums and products; nothing that decides."""
+    def pairs(f):
+        return "FA_SCORE_PAIRS" in modtrace.lower_mods(f, None).source
+
+    assert pairs(lambda s, b, h, q, k: 30.0 * torch.tanh(s / 30.0))
+    assert pairs(lambda s, b, h, q, k: -torch.tanh(s) * 3.0 + (q - k) * 0.5)
+    assert not pairs(lambda s, b, h, q, k: s * 2.0)
+    assert not pairs(lambda s, b, h, q, k: s + (q - k) * 0.5)
+    assert not pairs(lambda s, b, h, q, k: torch.where(q > k, 30.0 * torch.tanh(s / 30.0), s))
+    assert not pairs(lambda s, b, h, q, k: torch.exp(torch.tanh(s)))
+    assert not pairs(lambda s, b, h, q, k: torch.tanh(s / (h + 1)))
+
+
 def test_there_is_no_cpu_path():
     q = torch.zeros(1, 2, 4, 64, dtype=torch.float16)
     starts = torch.tensor([0, 4], dtype=torch.int32)
