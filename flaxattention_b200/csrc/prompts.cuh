@@ -80,13 +80,23 @@ __global__ void __launch_bounds__(128) fa_merge_kernel(const __grid_constant__ F
   const long long at = (long long)hk * p.B * p.Sq * G + ((long long)b * p.Sq + q) * G + (h - hk * G);
   const bool active = lane * 4 < p.Dv, second = lane * 4 + 128 < p.Dv;
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-  // Weights first: lane k has those of parts k and k + 32 (there are 64 at most), so that all rows of values can be on their way at once.
+  // Lane k has the weights of parts k and k + 32 (there are 64 at most), so that all rows of values can be on their way at once; the first eight are before the
+  // weights are known.
   const float2 own = p.own_ml != nullptr ? *(const float2*)(p.own_ml + row * 2) : make_float2(-INFINITY, 0.f);
   float2 ml[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) ml[i] = lane + 32 * i < p.parts ? *(const float2*)(p.part_ml + ((lane + 32 * i) * n_rows + at) * 2) : make_float2(-INFINITY, 0.f);
   const bool has = p.own_o != nullptr;
   float4 x = has && active ? *(const float4*)(p.own_o + row * p.Dv + lane * 4) : zero, y = has && second ? *(const float4*)(p.own_o + row * p.Dv + lane * 4 + 128) : zero;
+  constexpr int AHEAD = 8;
+  const float* from = p.part_o + at * p.Dv + lane * 4;
+  const long long step = n_rows * p.Dv;
+  float4 u[AHEAD], v[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    u[k] = active && k < p.parts ? *(const float4*)(from + k * step) : zero;
+    v[k] = second && k < p.parts ? *(const float4*)(from + k * step + 128) : zero;
+  }
   // (a part that has seen nothing counts for nothing; one whose sum is no number stays so)
   float m = fmaxf(own.y == 0.f ? -INFINITY : own.x, fmaxf(ml[0].x, ml[1].x));
 #pragma unroll
@@ -100,14 +110,16 @@ __global__ void __launch_bounds__(128) fa_merge_kernel(const __grid_constant__ F
     y.x *= f; y.y *= f; y.z *= f; y.w *= f;
   };
   scale(w_own);
-  const float* from = p.part_o + at * p.Dv + lane * 4;
-  const long long step = n_rows * p.Dv;
-#pragma unroll 8
-  for (int k = 0; k < p.parts; ++k, from += step) {
-    const float f = __shfl_sync(0xffffffffu, k < 32 ? w[0] : w[1], k & 31);
-    const float4 u = active ? *(const float4*)from : zero, v = second ? *(const float4*)(from + 128) : zero;
+  const auto add = [&](float f, const float4& u, const float4& v) {
     x.x += f * u.x; x.y += f * u.y; x.z += f * u.z; x.w += f * u.w;
     y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) add(__shfl_sync(0xffffffffu, w[0], k), u[k], v[k]);  // (where there is no part, 0 times 0)
+#pragma unroll 8
+  for (int k = AHEAD; k < p.parts; ++k) {
+    const float f = __shfl_sync(0xffffffffu, k < 32 ? w[0] : w[1], k & 31);
+    add(f, active ? *(const float4*)(from + k * step) : zero, second ? *(const float4*)(from + k * step + 128) : zero);
   }
   scale(l > 0.f ? 1.f / l : l);  // (0 and no number stay)
   char* to = (char*)p.o.ptr + ((long long)b * p.o.sb + (long long)h * p.o.sh + (long long)q * p.o.ss) * (DT == FA_F32 ? 4 : 2);
@@ -129,13 +141,19 @@ int prefix_rows(const fa_paged_params* p) {
   const bool few = p->prefix_length <= 1024 && (long long)p->B * p->Sq * (p->Hq / p->Hkv) <= 64;
   return few || !packed_tc_takes(shape_of(p), p->prefix_length) ? 64 : 128;
 }
-// Parts that the prefix is cut into, of four tiles at least (one / four, 24 x 3 queries with 400 tokens of their own behind 2000, 16 / 4 heads, D 128: 26 / 19).  As many as make a CTA for each SM: the pages' kernel runs beside them, and every part has to be written
-// and read again (us, 64 requests with 500 tokens of their own behind 8192, 32 / 8 heads, D 128, pages alone 28: half a CTA per SM 61, one 49, two 58).  Two where the rows alone make half a
-// CTA per SM or more, whose tiles then are what takes the time (500 requests: one part 189, two 155).
+// Parts that the prefix is cut into, of two tiles of 128 keys at least, or one of the general kernel's (us on the GPU, parts of one / two / four tiles:
+// 8 requests with 200 tokens of their own behind 500, 8 heads, D 64, general kernel, 8.9 / 10.2 / 13.6; 16 with 300 behind 2000, 32 / 8 heads, D 128,
+// tcgen05 kernel, 21.8 / 19.9 / 21.3).  As many as make a CTA for each SM: the pages' kernel runs beside them, and every part has to be written and read
+// again (64 requests with 500 tokens of their own behind 8192, 32 / 8 heads, D 128, pages alone 28: half a CTA per SM 61, one 49, two 58).  Two where the rows
+// alone make half a CTA per SM or more, whose tiles then are what takes the time (500 requests: one part 189, two 155).
+long long prefix_tiles(const fa_paged_params* p) {
+  const int R = prefix_rows(p);
+  return p->Hkv * (((long long)p->B * p->Sq * (p->Hq / p->Hkv) + R - 1) / R);
+}
 int prefix_parts(const fa_paged_params* p) {
-  const int R = prefix_rows(p), BN = R == 64 ? packed_bn(p->dtype, p->D) : 128;
-  const long long rows = (long long)p->B * p->Sq * (p->Hq / p->Hkv), ctas = p->Hkv * ((rows + R - 1) / R), sms = device_sm_count();
-  const int shares = (p->prefix_length + 4 * BN - 1) / (4 * BN);
+  const int least = prefix_rows(p) == 64 ? packed_bn(p->dtype, p->D) : 2 * 128;
+  const long long ctas = prefix_tiles(p), sms = device_sm_count();
+  const int shares = (p->prefix_length + least - 1) / least;
   return (int)std::max<long long>(1, std::min<long long>(std::min(shares, 64), (2 * ctas > sms ? 2 : 1) * sms / ctas));
 }
 void prefix_fill(fa_module* m, const fa_paged_params* p, float* part_o, float* part_ml, FaPackedParams& k) {
