@@ -148,7 +148,7 @@ int prefix_rows(const fa_paged_params* p) {
 // alone make half a CTA per SM or more, whose tiles then are what takes the time (500 requests: one part 189, two 155).
 long long prefix_tiles(const fa_paged_params* p) {
   const int R = prefix_rows(p);
-  return p->Hkv * (((long long)p->B * p->Sq * (p->Hq / p->Hkv) + R - 1) / R);
+  return std::max(1ll, p->Hkv * (((long long)p->B * p->Sq * (p->Hq / p->Hkv) + R - 1) / R));
 }
 int prefix_parts(const fa_paged_params* p) {
   const int least = prefix_rows(p) == 64 ? packed_bn(p->dtype, p->D) : 2 * 128;
@@ -227,7 +227,8 @@ int prompt_sizes(fa_module* m, const fa_prompt_params* p) {
   if (p->D <= 0 || p->D % 16 || p->Dv <= 0 || p->Dv % 16) return fail(FA_EUNSUPPORTED, "head dims must be positive multiples of 16");
   if (p->Dv > p->D) return fail(FA_EINVAL, "value head dim must not exceed the query/key head dim");
   if (p->D > 256) return fail(FA_EUNSUPPORTED, "head dim above 256 is not supported");
-  if (p->tokens * (p->Hq / p->Hkv) > 0x7fffffffll - 65536 || p->keys > 0x7fffffffll - 65536 || p->B > 0x7fffffff - 1) return fail(FA_EUNSUPPORTED, "tokens * Hq / Hkv and keys must stay below 2^31");
+  if (p->tokens * (p->Hq / p->Hkv) > 0x7fffffffll - 65536 || p->keys > 0x7fffffffll - 65536) return fail(FA_EUNSUPPORTED, "tokens * Hq / Hkv and keys must stay below 2^31");
+  if (p->B > 1 << 30) return fail(FA_EUNSUPPORTED, "more than 2^30 requests");
   return FA_OK;
 }
 void prompt_fill(fa_module* m, const fa_prompt_params* p, FaPackedParams& k) {

@@ -26,7 +26,7 @@ def prompt(**kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=3), -1), (dict(B=-1), -1), (dict(Hq=0), -1), (dict(Hkv=3), -1), (dict(tokens=-1), -1), (dict(keys=-1), -1), (dict(D=60), -4), (dict(D=272, Dv=16), -4), (dict(Dv=80), -1),
-    (dict(tokens=1 << 31), -4), (dict(tokens=1 << 30, Hq=8), -4), (dict(keys=1 << 31), -4), (dict(starts=None), -1), (dict(q=tensor(0x1008)), -1), (dict(o=tensor(None)), -1),
+    (dict(tokens=1 << 31), -4), (dict(B=(1 << 30) + 1), -4), (dict(tokens=1 << 30, Hq=8), -4), (dict(keys=1 << 31), -4), (dict(starts=None), -1), (dict(q=tensor(0x1008)), -1), (dict(o=tensor(None)), -1),
     (dict(k=tensor(s=63)), -1), (dict(v=tensor(None)), -1)])
 def test_prompt_arguments(kw, code):
     L, m = _cabi.lib(), _cabi.Module(None)
@@ -92,6 +92,22 @@ def test_prefix_workspace():
     own, with_prefix = (L.fa_paged_workspace_bytes(C.byref(paged(prefix_length=n, **kw))) for n in (0, 5000))
     assert with_prefix > own + 2 * 2 * 4 * 64 * 4
     assert L.fa_paged(m.handle, C.byref(paged(prefix_length=5000, **kw)), 0x8000, 100, None) == -5
+
+
+def test_workspace_of_impossible_heads():
+    """Fewer query heads than kv heads: refused by the call, and nothing is divided by their quotient before."""
+    p = paged(Hq=2, Hkv=4, prefix_length=500, k_prefix=tensor(), v_prefix=tensor())
+    assert _cabi.lib().fa_paged_workspace_bytes(C.byref(p)) >= 0
+    m = _cabi.Module(None)
+    assert _cabi.lib().fa_paged(m.handle, C.byref(p), None, 0, None) == -1
+
+
+@pytest.mark.parametrize("D,Sq", [(64, 1), (128, 1), (256, 1), (128, 5), (64, 9), (96, 20), (80, 2)])
+@pytest.mark.parametrize("prefix", [0, 500])
+def test_eight_bit_kernels_with_capped_scores_compile(D, Sq, prefix):
+    m = _cabi.Module(modtrace.lower_mods(lambda s, b, h, q, k: 30.0 * torch.tanh(s / 30.0), None).source)
+    p = paged(D=D, Dv=D, Sq=Sq, page_size=16, k_scales=tensor(), v_scales=tensor(), prefix_length=prefix, k_prefix=tensor(), v_prefix=tensor())
+    _cabi.check(_cabi.lib().fa_paged_prepare(m.handle, C.byref(p)))
 
 
 def test_append_arguments():
