@@ -47,6 +47,13 @@ def test_rows(kernels, Hq, Hkv, Sq, B):
     run(2, 300, [(i * 7) % 50 for i in range(B)], Hq, Hkv, Sq, 64, 8, "bf16", kernels=kernels)
 
 
+@pytest.mark.parametrize("dtype,D,eight", [("bf16", 128, False), ("f16", 64, False), ("f32", 64, False), ("bf16", 128, True), ("f16", 64, True)])
+@pytest.mark.parametrize("G,Sq", [(1, 1), (3, 1), (4, 3)])
+def test_pages_beside_the_prefix(dtype, D, eight, G, Sq):
+    """Requests and parts of the prefix that fill the SMs together: the pages' CTAs are of a form that has room beside the others."""
+    run(20, 2100, [0, 1, 31, 500] + [5 * i for i in range(1, 33)], 4 * G, 4, Sq, D, 16, dtype, eight=eight, score=softcap if G == 3 else None)
+
+
 @pytest.mark.parametrize("dtype,D,Dv", [*(("f16", *x) for x in ((16, 16), (80, 80), (96, 32), (192, 128))), ("f32", 48, 48), ("f32", 256, 256)])
 def test_head_dims(dtype, D, Dv):
     run(3, 200, [3, 70], 4, 2, 2, D, 16, dtype, Dv=Dv)
