@@ -733,7 +733,7 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
   }
   FA_MOD_BUFS_INIT(p);
   fa_grid_wait();
-  if (PREFIX) fa_grid_release();  // (the pages' kernel runs beside this one)
+  if (PREFIX) fa_grid_release();  // (the CTAs of the pages' kernel are there, waiting, when this one ends)
   const fa_u32 raw = fa_smem_u32(smem_raw);
   const fa_u32 sb = (raw + 1023u) & ~1023u;  // shared-window address of the aligned base
   unsigned char* sm = smem_raw + (sb - raw);

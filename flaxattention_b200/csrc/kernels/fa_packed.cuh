@@ -29,7 +29,7 @@ extern "C" __global__ void __launch_bounds__(fa_pk::NT) fa_packed_kernel(const _
   __shared__ FaPlace found;
   FA_MOD_BUFS_INIT(p);
   fa_grid_wait();
-  if (PREFIX) fa_grid_release();  // (the pages' kernel runs beside this one)
+  if (PREFIX) fa_grid_release();  // (the CTAs of the pages' kernel are there, waiting, when this one ends)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hk = PREFIX ? blockIdx.x % p.Hkv : blockIdx.x, G = p.Hq / p.Hkv;
   if (PREFIX) {
     if (tid == 0) found = {0, p.tokens, 0, p.keys, 0, (int)blockIdx.y * BM, 1};  // (grid: parts of the prefix and kv heads, items)

@@ -979,9 +979,9 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
 #endif
   FA_MOD_BUFS_INIT(p);
   __syncthreads();
-  // Behind a prefix this kernel runs beside the one in front of it, the prefix's, whose results it does not need: that one has waited for all that was before
-  // it lets this one go.  The wait is at the end, so that the kernel behind, which waits for this one, has both.
-  if (!AFTER) fa_grid_wait();
+  // (Also behind a prefix, whose kernel is in front and whose results are not needed here: lengths, tables and pages are written by kernels in front of that one, and
+  // only this wait says that they can be seen.)
+  fa_grid_wait();
 
   // ---- this worker's run of tiles --------------------------------------------------------
   const int G = p.Hq / p.Hkv, items = p.B * p.row_tiles;
@@ -1023,10 +1023,7 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
     }
     t0 = (int)min((long long)blockIdx.x * per, (long long)total);
     t1 = min(t0 + per, total);
-    if (t0 >= t1) {
-      if (AFTER) fa_grid_wait();
-      return;
-    }
+    if (t0 >= t1) return;
     const int from = __popc(__ballot_sync(0xffffffffu, (long long)upto * p.Hkv <= t0));  // the lane whose run has tile t0
     int item = __shfl_sync(0xffffffffu, i0, from), before = __shfl_sync(0xffffffffu, upto - own, from);
     seg_open(p, item, seg);
@@ -1493,7 +1490,6 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
   }
   if (!SHORT) fa_grid_release();
   fa_cp_wait<0>();
-  if (AFTER) fa_grid_wait();
 #if FA_TMA
   if (failed) {
     // The copies in flight have to land before the shared memory goes to another CTA (with a limit of its own: the flag is up).

@@ -457,14 +457,6 @@ void pick_paged(const fa_paged_params* p, PagedCfg& c) {
   if (c.RG == 1 && segments <= sms) {
     c.per_sm = 1;
     c.slots = 4;
-    // (beside a prefix whose CTAs leave it no SMs of its own: one that has room on theirs.  us, 16 requests with 300 tokens of their own behind 2000, 32 / 8 heads,
-    //  D 128, 19.9 / 15.4; 24 x 3 queries with 700 in 8 bits behind 5001, 16 / 4 heads, 33.4 / 30.0; on SMs of its own 15.2 / 17.3, 11 with 516 in 8 bits behind 691.)
-    if (c.after && segments + prefix_tiles(p) * prefix_parts(p) > sms && keys <= 4LL * 8 * c.WN) {
-      c.CG = 4;
-      c.slots = 2;
-      c.smem = smem(c.slots);
-      return;
-    }
     for (c.CG = 8; c.CG >= 4; c.CG /= 2) {
       c.smem = smem(c.slots);
       if (c.smem <= kMaxSmem && keys <= 4LL * c.CG * c.WN) return;
@@ -705,7 +697,7 @@ int fa_paged(fa_module* m, const fa_paged_params* p, void* workspace, size_t wor
   k.workers = paged_workers(c);
   const size_t rows = 2 * (size_t)k.workers * c.BM;
   if (c.after) {
-    // the prefix first: its kernel has the most to do, and the pages' begins while it ends
+    // the prefix first: its kernel has the most to do, and the CTAs of the pages' get ready while it ends
     char* at = (char*)workspace;
     const size_t all = (size_t)p->B * p->Hq * p->Sq, parts = (size_t)prefix_parts(p);
     const auto take = [&](size_t n) {

@@ -142,10 +142,10 @@ int prefix_rows(const fa_paged_params* p) {
   return few || !packed_tc_takes(shape_of(p), p->prefix_length) ? 64 : 128;
 }
 // Parts that the prefix is cut into, of two tiles of 128 keys at least, or one of the general kernel's (us on the GPU, parts of one / two / four tiles:
-// 8 requests with 200 tokens of their own behind 500, 8 heads, D 64, general kernel, 8.9 / 10.2 / 13.6; 16 with 300 behind 2000, 32 / 8 heads, D 128,
-// tcgen05 kernel, 21.8 / 19.9 / 21.3).  As many as make a CTA for each SM: the pages' kernel runs beside them, and every part has to be written and read
-// again (64 requests with 500 tokens of their own behind 8192, 32 / 8 heads, D 128, pages alone 28: half a CTA per SM 61, one 49, two 58).  Two where the rows
-// alone make half a CTA per SM or more, whose tiles then are what takes the time (500 requests: one part 189, two 155).
+// 8 requests with 200 tokens of their own behind 500, 8 heads, D 64, general kernel, 11.0 / 12.6; 16 with 300 behind 2000, 32 / 8 heads, D 128,
+// tcgen05 kernel, 21.0 / 20.4 / 23.3).  As many as make a CTA for each SM: every part has to be written and read
+// again (64 requests with 1000 tokens of their own behind 8192, 32 / 8 heads, D 128, pages alone 30: half a CTA per SM 67, one 58, two 61).  Two where the rows
+// alone make half a CTA per SM or more, whose tiles then are what takes the time (500 requests: one part 90, two 83).
 long long prefix_tiles(const fa_paged_params* p) {
   const int R = prefix_rows(p);
   return std::max(1ll, p->Hkv * (((long long)p->B * p->Sq * (p->Hq / p->Hkv) + R - 1) / R));
