@@ -379,6 +379,24 @@ constexpr int VB = PV / 8;             // columns of V of a thread, beside each 
 // Which of eight keys is row g of a product.  Lanes that are served together then read different banks: 16 bytes of the keys of two rows g beside each other
 // (K), and two threads' columns of the keys of every other row (V).
 __device__ __forceinline__ int key_of(int g) { return GROUP == 128 ? (g & 1 ? (g - 1) ^ 5 : g) : g ^ ((g >> 1) & 1); }
+// Probabilities times the scales of their values.  A scale that is no number or infinite is the rows' that see its key: 0 times it, of a row that does not, is 0.  Which
+// those are the scores say in front of the softmax; there is one vote per tile for this and for rows whose maximum rises.
+template <class R>
+__device__ __forceinline__ void find_unseen(R& r) {
+  r.unseen = 0;
+#pragma unroll
+  for (int j = 0; j < NS; ++j)
+#pragma unroll
+    for (int h = 0; h < HR; ++h) r.unseen |= r.score(h, j) == FA_NEG_INF ? 1u << (HR * j + h) : 0u;
+}
+template <class R>
+__device__ __forceinline__ void clear_unseen(R& r) {
+#pragma unroll
+  for (int j = 0; j < NS; ++j)
+#pragma unroll
+    for (int h = 0; h < HR; ++h)
+      if ((r.unseen >> (HR * j + h)) & 1u) r.score(h, j) = 0.f;
+}
 #if FA_FEW == 1
 // Whole numbers with whole numbers: products of 8 bits, summed in 32 (m16n8k32), which take K as it lies in the tile and V with its bytes exchanged
 // (12 instructions for 16 values of K and of V together, where their way to 16 bits takes 68).
@@ -415,6 +433,7 @@ struct Rows {
   fa_u32 qf[BLOCKS * 2][3][2]; // digits of 16 values of each 64 of query g = lane / 4
   float qs[HR];                // 2^(e - 22) of this lane's rows
   float ks, vs;                // scales of this lane's key of the tile
+  fa_u32 unseen;               // scores of the tile that a value's scale must not come to, bit HR j + h
   int lane;
   __device__ __forceinline__ float& score(int h, int j) { return s[j >> 1][0][(j & 1) * 2 + h]; }
   __device__ __forceinline__ int key(int j) const { return key_of(lane >> 2) + j * 8; }
@@ -495,15 +514,29 @@ struct Rows {
   __device__ __forceinline__ void values(const unsigned char* bytes, fa_u32, int) {
     float top[HR] = {0.f, 0.f};
     fa_u32 nan = 0;
+    const auto look = [&]() {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+#pragma unroll
+        for (int h = 0; h < HR; ++h) {
+          top[h] = fmaxf(top[h], fabsf(score(h, j)));
+          nan |= !(fabsf(score(h, j)) <= 3.4e38f) ? 1u << h : 0u;
+        }
+      }
+    };
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
       const float f = __shfl_sync(0xffffffffu, vs, key(j));
 #pragma unroll
-      for (int h = 0; h < HR; ++h) {
-        score(h, j) *= f;
-        top[h] = fmaxf(top[h], fabsf(score(h, j)));
-        nan |= !(fabsf(score(h, j)) <= 3.4e38f) ? 1u << h : 0u;
-      }
+      for (int h = 0; h < HR; ++h) score(h, j) *= f;
+    }
+    look();
+    const bool no_number = __any_sync(0xffffffffu, nan != 0);
+    if (no_number) {
+      clear_unseen(*this);
+      top[0] = top[1] = 0.f;
+      nan = 0;
+      look();
     }
     over_keys(top, Max());
     float step[HR];
@@ -515,7 +548,7 @@ struct Rows {
 #pragma unroll
       for (int j = 0; j < NS; ++j) score(h, j) = fmaf(score(h, j), up, 12582912.f);  // (the whole number in the low 16 bits)
     }
-    if (__any_sync(0xffffffffu, nan != 0)) {  // of a row with no number in it, nothing is one
+    if (no_number) {  // of a row with no number in it, nothing is one
 #pragma unroll
       for (int h = 0; h < HR; ++h) {
         fa_u32 any = nan >> h & 1u;
@@ -616,6 +649,7 @@ struct Rows {
   float s[WN / 16][NQ][4], o[VB / 2][NQ][4], m[HR], l[HR];
   fa_u32 qf[BLOCKS * 4][NQ][2];
   float ks, vs;  // scales of this lane's key of the tile
+  fa_u32 unseen; // scores of the tile that a value's scale must not come to, bit HR j + h
   int lane;
   __device__ __forceinline__ float& score(int h, int j) { return s[j >> 1][h >> 1][(j & 1) * 2 + (h & 1)]; }
   __device__ __forceinline__ int key(int j) const { return key_of(lane >> 2) + j * 8; }
@@ -677,6 +711,7 @@ struct Rows {
 #pragma unroll
       for (int h = 0; h < HR; ++h) score(h, j) *= f;
     }
+    if (unseen != 0) clear_unseen(*this);
 #pragma unroll
     for (int kj = 0; kj < WN / 16; ++kj) {
       fa_u32 b[NQ][2], rest[NQ][2];
@@ -1330,7 +1365,17 @@ extern "C" __global__ void __launch_bounds__(fa_pg::NT, FA_CTAS) fa_paged_kernel
         for (int j = 0; j < NS; ++j) top[h] = fmaxf(top[h], R.score(h, j));
         rises |= top[h] > R.m[h] + RISE;
       }
+#if FA_KV8
+      R.unseen = 0;
+      const bool strange = !(fabsf(R.vs) <= 3.4e38f);
+      if (__any_sync(0xffffffffu, rises || strange)) {
+        if (__any_sync(0xffffffffu, strange)) find_unseen(R);
+        rises = __any_sync(0xffffffffu, rises);
+      }
+      if (rises) {
+#else
       if (__any_sync(0xffffffffu, rises)) {
+#endif
         Rows::over_keys(top, Max());
 #pragma unroll
         for (int h = 0; h < HR; ++h) {

@@ -119,7 +119,7 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, score_m
     16-byte pieces where TMA would do.
 
     With ``key_scales`` and ``value_scales`` (float32 ``[pages, kv heads, page_size]``) the pages are in 8 bits, as ``rotary_append`` writes them, and queries float16 or
-    bfloat16.  A scale that is no number makes the rows that see its token that.
+    bfloat16.  A scale that is no number or infinite makes the rows that see its token no numbers, and no others.
 
     ``prefix``: keys and values ``[1, kv heads, tokens, D]`` (``bhln=False``: ``[1, tokens, kv heads, D]``) that all requests begin with, in front of those in
     their pages, of the queries' dtype also where the pages are in 8 bits (``read_pages`` takes them out of pages).  They are read once for all requests, not
