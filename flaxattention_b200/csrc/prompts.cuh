@@ -251,11 +251,12 @@ extern "C" {
 int fa_prompt_prepare(fa_module* m, const fa_prompt_params* p) {
   if (int rc = prompt_sizes(m, p)) return rc;
   Kernel* kernel = nullptr;
-  if (packed_tc_takes(shape_of(p), p->keys)) {
+  if (packed_tc_takes(shape_of(p), 1)) {
     for (int nq = 1; nq <= 2; ++nq)
       if (int rc = get_packed_tc_kernel(m, shape_of(p), 1, nq, &kernel)) return rc;
-    return get_packed_tc_kernel(m, shape_of(p), 3, 1, &kernel);
+    if (int rc = get_packed_tc_kernel(m, shape_of(p), 3, 1, &kernel)) return rc;
   }
+  // (also where the tcgen05 kernel would do: short prompts take this one, and strides that no tensor map takes)
   return get_packed_kernel(m, shape_of(p), false, &kernel);
 }
 

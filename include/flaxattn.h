@@ -392,7 +392,7 @@ typedef struct fa_prompt_params {
 } fa_prompt_params;
 size_t fa_prompt_workspace_bytes(const fa_prompt_params* p); /* 0, but for few rows over many keys, which are split */
 int fa_prompt(fa_module* m, const fa_prompt_params* p, void* workspace, size_t workspace_bytes, void* stream);
-/* Compiles (or fetches from the cache) the kernel that a call of these sizes, type and flags runs.  Needs no GPU. */
+/* Compiles (or fetches from the cache) the kernels that calls of this type, these head dims and flags run, whatever their lengths and strides.  Needs no GPU. */
 int fa_prompt_prepare(fa_module* m, const fa_prompt_params* p);
 
 #ifdef __cplusplus
