@@ -208,9 +208,10 @@ __device__ __forceinline__ void read_four(unsigned w, F2 scale, F2* f) {
   f[1] = fma(f2(at(2), at(3)), one, bias) * scale;
 }
 
-// PIECES: 16 bytes of the pages at a time; else value by value
+// PIECES: 16 bytes of the pages at a time; else value by value.  Four blocks per SM; with the registers for three, 45000 tokens in 8 bits (8 heads, D 128) take 4 us more.  (72000
+// tokens: bf16 102 us, 5.8 TB/s, in 8 bits 94.)
 template <int IN, int OUT, bool PIECES>
-__global__ void __launch_bounds__(kReadThreads) fa_read_pages_kernel(const __grid_constant__ FaReadKernelParams P) {
+__global__ void __launch_bounds__(kReadThreads, 4) fa_read_pages_kernel(const __grid_constant__ FaReadKernelParams P) {
   grid_wait();
   constexpr bool EIGHT = IN == kReadEight;
   constexpr int ES = OUT == FA_F32 ? 4 : 2, EI = EIGHT ? 1 : ES, V = PIECES ? 16 / EI : 1, U = 4;
@@ -218,6 +219,11 @@ __global__ void __launch_bounds__(kReadThreads) fa_read_pages_kernel(const __gri
   const int kind = blockIdx.y;  // keys or values
   const int t0 = blockIdx.x << P.token_shift, n = min(1 << P.token_shift, P.tokens - t0), tid = threadIdx.x;
   int before = 0;
+  if (blockIdx.x == 0 && kind == 0 && P.status != nullptr) {  // starts that decrease
+#pragma unroll 1
+    for (int b = tid; b < P.B; b += kReadThreads)
+      if (P.starts[b] > P.starts[b + 1]) atomicOr(P.status, FA_STATUS_BAD_START);
+  }
   for (int b0 = 0; b0 < P.B; b0 += kReadThreads) before += __syncthreads_count(b0 + tid < P.B && P.starts[min(b0 + tid, P.B - 1) + 1] <= t0);
   if (tid < n) {
     const int t = t0 + tid;

@@ -79,7 +79,7 @@ def read_pages(key_pages, value_pages, block_table, starts, num_tokens: int, *, 
     Row ``t`` is token ``t - starts[b]`` of the request ``b`` with ``starts[b] <= t < starts[b + 1]`` (``starts``: int32 ``[B + 1]``, never decreasing; of whole requests
     the sums of their lengths).  ``num_tokens`` is ``starts[B]``, which the host has to know; rows beyond it, or in front of ``starts[0]``, are 0.
     Pages in 8 bits (with their scales) are multiplied out and rounded to ``dtype``, others are copied.  A table entry that is no page, or a token that the table has no
-    room for, leaves the row 0, and the next call raises ``FlaxAttnError`` (``check_status``).
+    room for, leaves the row 0, and the next call raises ``FlaxAttnError`` (``check_status``); so do starts that decrease, with which rows are some tokens or other.
 
     It is what attention over more than a few new tokens takes: the next piece of a prompt (``prompt_attention`` with ``key_starts``), or the
     tokens that requests have in common (``prefix`` of ``paged_attention``).  One launch, no gradient.

@@ -320,7 +320,7 @@ int fa_page_step(const int32_t* lengths, const int32_t* new_tokens, int B, int32
 
 /* The tokens of requests out of their pages, laid end to end: row t of key and value is token t - starts[b] of the request b with
  * starts[b] <= t < starts[b + 1] (starts [B + 1], never decreasing).  Rows of no request, of tokens that the table has no room for and of table entries that are
- * no page are 0; the last two set 4 in the status word.  Pages in 8 bits (scales given) are multiplied out and rounded once; others are copied.  One launch. */
+ * no page are 0; the last two set 4 in the status word, starts that decrease 32 (rows are then some tokens or other, or 0).  Pages in 8 bits (scales given) are multiplied out and rounded once; others are copied.  One launch. */
 typedef struct fa_read_params {
   int32_t dtype;              /* of key and value, and of pages that are not in 8 bits */
   int32_t B, Hkv, D, Dv;
