@@ -131,7 +131,8 @@ __device__ __forceinline__ FaPlace fa_find_item(const FaPackedParams& p, long lo
   return p.B <= 256 ? fa_find_by_level<R>(p, item) : fa_find_by_request<R>(p, item);
 }
 
-// starts that decrease, or lie where there are no tokens: said once, by the threads of one CTA
+// starts that decrease, or lie where there are no tokens: said once, by the threads of one CTA.  (Of such that decrease requests overlap, and may have more items than the grid
+// has CTAs: nothing is read or written out of range, but rows may be left out.  Finding that out in every CTA would take a look at all starts.)
 __device__ __forceinline__ void fa_check_starts(const FaPackedParams& p, int tid, int threads) {
   bool bad = false;
   for (int s = tid; s < p.B; s += threads)

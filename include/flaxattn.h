@@ -388,7 +388,8 @@ typedef struct fa_prompt_params {
   int32_t window;             /* below 0: no window */
   float* lse;                 /* [Hq, tokens] natural-log logsumexp or NULL */
   int32_t flags;              /* FA_FLAG_GENERAL_KERNELS: not the tcgen05 kernel */
-  int32_t* status;            /* optional status word: 32 = starts that decrease or lie beyond the tokens (what lies beyond is left out) */
+  int32_t* status;            /* optional status word: 32 = starts that lie beyond the tokens (what lies there is left out) or decrease (there are no
+                                 results then, and there may be rows that nothing is written to) */
 } fa_prompt_params;
 size_t fa_prompt_workspace_bytes(const fa_prompt_params* p); /* 0, but for few rows over many keys, which are split */
 int fa_prompt(fa_module* m, const fa_prompt_params* p, void* workspace, size_t workspace_bytes, void* stream);
