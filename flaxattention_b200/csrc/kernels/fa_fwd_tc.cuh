@@ -189,16 +189,20 @@ constexpr int BAR_P2 = BAR_S + 10;
 // Work on one 32-column chunk of a score row held in registers (columns C0 .. C0+31 of the kv
 // tile that starts at key n0).  C0 is a template parameter and n0 a multiple of 128, so the low
 // bits of every key index are compile-time constants inside the mods.
+// (Requests of different lengths: the maximum of scores among which one is no number is none, and then the row is.  Its exponential would not say so
+// where it is one of those on the FMA pipe.)
 struct RowMax {
   float a, b, c, d;
 };
+__device__ __forceinline__ float row_max3(float a, float b, float c) { return PACKED ? fa_max_nan(fa_max_nan(a, b), c) : fa_max3(a, b, c); }
+__device__ __forceinline__ float row_max(float a, float b) { return PACKED ? fa_max_nan(a, b) : fmaxf(a, b); }
 __device__ __forceinline__ void max_chunk(const float (&v)[32], RowMax& mx) {
 #pragma unroll
   for (int e = 0; e < 32; e += 8) {
-    mx.a = fa_max3(mx.a, v[e], v[e + 1]);
-    mx.b = fa_max3(mx.b, v[e + 2], v[e + 3]);
-    mx.c = fa_max3(mx.c, v[e + 4], v[e + 5]);
-    mx.d = fa_max3(mx.d, v[e + 6], v[e + 7]);
+    mx.a = row_max3(mx.a, v[e], v[e + 1]);
+    mx.b = row_max3(mx.b, v[e + 2], v[e + 3]);
+    mx.c = row_max3(mx.c, v[e + 4], v[e + 5]);
+    mx.d = row_max3(mx.d, v[e + 6], v[e + 7]);
   }
 }
 // score_mod (and the rounding of the raw scores to the input type, when asked for) in place.  With a score_mod the
@@ -503,15 +507,15 @@ __device__ __forceinline__ bool softmax_step(SoftmaxCtx& c, const int tile, cons
       max_chunk(s3, rm);
     }
   }
-  float mx = fmaxf(fmaxf(rm.a, rm.b), fmaxf(rm.c, rm.d));
+  float mx = row_max(row_max(rm.a, rm.b), row_max(rm.c, rm.d));
   if (!REL) mx *= sc2;
   // running maximum, raised lazily
-  const float m_new = fmaxf(m_ref, REL ? m_base + mx : mx);
+  const float m_new = row_max(m_ref, REL ? m_base + mx : mx);
   bool need = false;
   float corr = 1.f;
   if (m_ref == FA_NEG_INF) {
     m_ref = m_new;  // nothing accumulated yet for this row
-  } else if (m_new - m_ref > RESCALE_THRESHOLD) {
+  } else if (PACKED ? !(m_new - m_ref <= RESCALE_THRESHOLD) : m_new - m_ref > RESCALE_THRESHOLD) {  // (no number is)
     need = true;
     corr = fa_ex2(m_ref - m_new);
     m_ref = m_new;
@@ -1394,7 +1398,7 @@ extern "C" __global__ void __launch_bounds__(fa_tc::NT, fa_tc::NQ == 1 ? 2 : 1) 
       if (D == 64) ok = softmax_step<2>(c, tile, mode, masked);
       else ok = masked ? softmax_step<1>(c, tile, mode, true) : softmax_step<0>(c, tile, mode, false);
     }
-    const float m_ref = c.m_ref, l = c.l;
+    const float m_ref = c.m_ref, l = PACKED && c.m_ref == -FA_NEG_INF ? c.m_ref - c.m_ref : c.l;  // (nothing is a number relative to an infinite score)
     const fa_u32 cnt = warp_active ? c.cnt : idle_cnt;
     // ---- epilogue: O / l and the logsumexp of this thread's row ---------------------------
     if (ok && cnt > 0)

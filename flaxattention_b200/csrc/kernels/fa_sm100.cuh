@@ -312,6 +312,12 @@ __device__ __forceinline__ void fa_ex2_poly2(float x0, float x1, float& p0, floa
 }
 // max of three; written as nested fmaxf so that the compiler may pick the three-input form
 __device__ __forceinline__ float fa_max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// no number if either is none
+__device__ __forceinline__ float fa_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // register re-allocation between warpgroups (all four warps of a warpgroup must execute it)
 template <int N>
 __device__ __forceinline__ void fa_setmaxnreg_inc() {
