@@ -120,10 +120,16 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, score_m
 
     With ``key_scales`` and ``value_scales`` (float32 ``[pages, kv heads, page_size]``) the pages are in 8 bits, as ``rotary_append`` writes them, and queries float16 or
     bfloat16.  A scale that is no number or infinite makes the rows that see its token no numbers, and no others.
+    What else is rounded then: up to 8 query rows per kv head, queries are whole numbers of 23 bits of their row's largest value, and probabilities times the values' scales
+    whole numbers of 16 bits of the largest among 32 keys; with more rows, these products are two bfloat16 parts.  It pays for up to 8 rows per kv head; with more the way from 8 to
+    16 bits takes longer than the smaller pages save.
 
     ``prefix``: keys and values ``[1, kv heads, tokens, D]`` (``bhln=False``: ``[1, tokens, kv heads, D]``) that all requests begin with, in front of those in
     their pages, of the queries' dtype also where the pages are in 8 bits (``read_pages`` takes them out of pages).  They are read once for all requests, not
-    once for each.  ``lengths`` still counts what lies in the pages; a query's token is ``p = tokens + lengths[b] - Sq + i``, for the mods and the window too.
+    once for each.  ``lengths`` still counts what lies in the pages; a query's token is ``p = tokens + lengths[b] - Sq + i``, for the mods and the window too, and a
+    query in front of the request's first token in the pages sees nothing, the prefix neither.  Probabilities over the prefix are rounded to the dtype once (over 16-bit pages up to 16 rows per
+    kv head lose nothing): tokens moved from the pages into the prefix are as exact as in ``prompt_attention``.  Over a prefix and over 8-bit pages a ``score_mod`` takes ``tanh`` of scores to
+    4e-7 in proportion.  A score over the prefix that is no number or ``+inf`` makes the rows that see its key no numbers.
     """
     general = kernel_options is not None and kernel_options.get("kernels") == "general"
     call = native().paged_attention

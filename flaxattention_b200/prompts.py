@@ -31,11 +31,13 @@ def prompt_attention(query, key, value, starts, score_mod: Optional[Callable] = 
     ``kv_idx``.  A query that sees nothing is 0, with a logsumexp of ``-inf``, and so are rows of no request.  Returns the output in the layout of ``query`` and, with
     ``return_lse``, the natural-log logsumexp ``[1, Hq, T]`` in float32.
 
-    Scores, softmax and sums are in fp32; 16-bit probabilities are rounded to the dtype for the product with the values, and a ``score_mod`` over 16-bit inputs divides scores and
-    takes their ``tanh`` as in ``paged_attention``.  A score that is no number or ``+inf`` makes the rows that see its key no numbers.  The values of a request must be finite also where a query does not see them (behind it, or taken out by ``mask_mod``: they are
-    multiplied with 0); other requests' may hold anything.  Starts in front of the rows or beyond them are cut to what is there, and the next call
-    raises ``FlaxAttnError`` (``check_status``); so it does for starts that decrease, with which the call has no results (there may be rows that nothing is written to).  Nothing waits for the GPU or depends on a length on the host.  There is no gradient: training over sequences of
-    several documents is ``flax_attention`` with a mask over their ids.  ``kernel_options``: ``{"kernels": "general"}`` takes the general kernel where the tcgen05 one would do.
+    Scores, softmax and sums are in fp32 (to 2.7e-6 in proportion: some exponentials are a polynomial's); 16-bit probabilities are rounded to the dtype for the product with the values,
+    and a ``score_mod`` over 16-bit inputs divides scores to some 2^-22 and takes their ``tanh`` to 4e-7 in proportion; where a quotient decides something it is exact, as in ``paged_attention``.
+    A score that is no number or ``+inf`` makes the rows that see its key no numbers.  The values of a request must be finite also where a query does not see them (behind it, or taken out by
+    ``mask_mod``: they are multiplied with 0); other requests' may hold anything.  Starts in front of the rows or beyond them are cut to what is there, and the next call raises ``FlaxAttnError``
+    (``check_status``); so it does for starts that decrease, with which the call has no results (there may be rows that nothing is written to).  Nothing waits for the GPU or depends on a
+    length on the host.  There is no gradient: training over sequences of several documents is ``flax_attention`` with a mask over their ids.  ``kernel_options``:
+    ``{"kernels": "general"}`` takes the general kernel where the tcgen05 one would do.
     """
     general = kernel_options is not None and kernel_options.get("kernels") == "general"
     call = native().prompt_attention
