@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(128) fa_merge_kernel(const __grid_constant__ F
 }
 
 PackedShape shape_of(const fa_paged_params* p) { return {p->dtype, p->Hq, p->Hkv, p->D, p->Dv, p->flags, p->scale}; }
-// Rows of an item: 128, one query tile of the tcgen05 kernel; 64, the general kernel, also for short prefixes of few rows, since its CTAs begin sooner (us of the whole
-// call, general / tcgen05, one to eight requests behind 500 tokens, D 64 8.7 / 9.8, D 128 10.3 / 11.2; behind 4000 20.0 / 18.1 and 24.5 / 21.6).
+// Rows of an item: 128, one query tile of the tcgen05 kernel; 64, the general kernel, also for short prefixes of few rows, since its CTAs begin sooner (us on the GPU of the whole
+// call, general / tcgen05, one to eight requests behind 500 tokens, 8 heads, D 64 10.9 / 12.8, D 128 14.1 / 17.1; behind 1000 12.1 / 13.1 and 15.4 / 17.5; behind 2000 14.7 / 13.5 and 18.3 / 17.4).
 int prefix_rows(const fa_paged_params* p) {
   const bool few = p->prefix_length <= 1024 && (long long)p->B * p->Sq * (p->Hq / p->Hkv) <= 64;
   return few || !packed_tc_takes(shape_of(p), p->prefix_length) ? 64 : 128;

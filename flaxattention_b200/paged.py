@@ -121,8 +121,8 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, score_m
     With ``key_scales`` and ``value_scales`` (float32 ``[pages, kv heads, page_size]``) the pages are in 8 bits, as ``rotary_append`` writes them, and queries float16 or
     bfloat16.  A scale that is no number or infinite makes the rows that see its token no numbers, and no others.
     What else is rounded then: up to 8 query rows per kv head, queries are whole numbers of 23 bits of their row's largest value, and probabilities times the values' scales
-    whole numbers of 16 bits of the largest among 32 keys; with more rows, these products are two bfloat16 parts.  It pays for up to 8 rows per kv head; with more the way from 8 to
-    16 bits takes longer than the smaller pages save.
+    whole numbers of 16 bits of the largest among 32 keys; with more rows, these products are two bfloat16 parts.  Pages in 8 bits save time for up to 8 rows per kv head (head
+    dims above 128: 16); with more the way from 8 to 16 bits takes longer than the smaller pages save.
 
     ``prefix``: keys and values ``[1, kv heads, tokens, D]`` (``bhln=False``: ``[1, tokens, kv heads, D]``) that all requests begin with, in front of those in
     their pages, of the queries' dtype also where the pages are in 8 bits (``read_pages`` takes them out of pages).  They are read once for all requests, not
